@@ -31,7 +31,8 @@ enum {
   QA_BF16 = 1,
   QA_F16 = 2,
   QA_I32 = 3,
-  QA_I64 = 4
+  QA_I64 = 4,
+  QA_KV4 = 5 /* a pool of the 4-bit KV cache; its strides are in bytes */
 };
 
 /* Paged KV pool descriptor.
@@ -46,7 +47,9 @@ enum {
  * With per-row pointer arrays and stride_head == 0, row b's head stride is
  * row_blocks[b]*stride_block: contiguous per-request pools
  * (1, heads, P_b, bs, D) of different P_b.
- * Physical ids outside [0, num_blocks) (or row_blocks[b]) are skipped.     */
+ * Physical ids outside [0, num_blocks) (or row_blocks[b]) are skipped.
+ * dtype QA_KV4: a shared pool (P, H_kv, tile) of bytes for the entries named
+ * kv4 and qa_qk_norm_mrope_append; strides in bytes, stride_token unused.    */
 typedef struct qa_paged_kv {
   void* key;
   void* value;
@@ -59,7 +62,7 @@ typedef struct qa_paged_kv {
   int64_t stride_head;
   int64_t stride_token;
   int32_t kv_heads;
-  int32_t dtype;                 /* QA_F32 or QA_BF16 */
+  int32_t dtype;                 /* QA_F32, QA_BF16 or QA_KV4 */
 } qa_paged_kv;
 
 /* ---- library ---------------------------------------------------------- */
@@ -256,6 +259,94 @@ int qa_qk_norm_rope_append(const void* q_proj, int64_t q_stride_t, int64_t q_str
                            int32_t heads, int32_t head_dim, const qa_paged_kv* kv, const void* block_tables,
                            int32_t table_dtype, int64_t table_stride, int64_t max_blocks, int32_t block_size, void* q_out,
                            hipStream_t stream);
+
+/* ---- the 4-bit KV cache of a full-attention layer ------------------------- */
+/* A pool tile (one block of one KV head) is block_size * 17 * head_dim / 32
+ * bytes, 16-byte aligned; head_dim 128 or 256, block_size a power of two from
+ * 16 to 1024.  32 consecutive dims of a token and head are one group: a scale
+ * byte e + 127 and 32 E2M1 codes (sign; 0 0.5 1 1.5 2 3 4 6) of x / 2^e, nearest
+ * with ties to even, saturated at 6; e is the least integer with
+ * max|x| <= 7 * 2^e, within [-125, 125].  A group with an infinity or NaN has
+ * the byte 255 and reads as NaN.  A tile is runs of 16 tokens, each the codes
+ * (8 head_dim bytes, even dim in the low half) and then the scales (head_dim / 2):
+ *   keys    codes [group][token][16], scales [group % 4][token][group / 4]
+ *   values  codes [pair][token / 4][chunk][token in pair][head_dim / 32], a pair
+ *           being 512 / head_dim of a token quad, a chunk head_dim / 16 dims;
+ *           scales [group][token]
+ * A new pool's bytes may be anything: nothing reads a token's bytes before they
+ * are written but masked lanes.  No counterpart in the reference, whose cache
+ * holds the activations' dtype (src/decode_state.py:37-44).                  */
+
+/* The plan of a batched step, on the device: what qa_paged_kv_reserve does, for
+ * any number of new tokens a row, and the step's slot map.  Row b grows from
+ * lengths[b] to lengths[b] + n_b (counts[b] or count_scalar); fresh blocks come
+ * from the front of the ascending free list, rows in order; lengths and
+ * free_state are advanced in place.  Outputs: cu_seqlens (batch + 1), starts
+ * (batch; the old lengths), and per packed token positions and slots
+ * (block id * block_size + position % block_size; -1 where the table has no
+ * block), -1 from the last token up to max_tokens.  status: 0, or as
+ * qa_paged_kv_reserve 1 to 4, or 5 where the step has more than max_tokens
+ * tokens; then cu_seqlens is all 0, every position and slot -1, and tables,
+ * lengths and free_state are left as they were.  tables, lengths int32.
+ * workspace: 4 bytes a row.  Replaces the host-side growth and slot arithmetic
+ * of src/decode_state.py:72-78,271-293,365-374.                              */
+int qa_paged_kv_plan(int32_t* block_tables, int64_t table_stride, int64_t max_blocks, int32_t* lengths,
+                     const void* counts, int32_t counts_dtype, int64_t count_scalar, int64_t batch, int32_t block_size,
+                     const int32_t* free_list, int64_t free_capacity, int32_t* free_state, int32_t* status,
+                     int64_t max_tokens, int32_t* cu_seqlens, int32_t* starts, int32_t* positions, int64_t* slots,
+                     int32_t* workspace, int64_t workspace_bytes, hipStream_t stream);
+
+/* Quantise key/value rows of packed tokens, element (n, h, d) at n*stride_t +
+ * h*stride_h + d, float32 or bfloat16, 16-byte aligned rows, into slots[n] of
+ * the 4-bit pool; slots outside the pool are skipped.  Slots must be distinct:
+ * of tokens that share one, the result is a mixture.                          */
+int qa_paged_kv4_append(const void* key_new, const void* value_new, int32_t dtype, int64_t k_stride_t, int64_t k_stride_h,
+                        int64_t v_stride_t, int64_t v_stride_h, int64_t tokens, int32_t head_dim, const qa_paged_kv* kv,
+                        const void* slots, int32_t slots_dtype, int32_t block_size, hipStream_t stream);
+
+/* qa_paged_kv_gather of a 4-bit pool: the values as bfloat16 (exact).         */
+int qa_paged_kv4_gather(const qa_paged_kv* kv, int32_t head_dim, int64_t batch, const void* block_tables, int32_t table_dtype,
+                        int64_t table_stride, int64_t max_blocks, int64_t valid, int32_t block_size, void* key_out,
+                        void* value_out, hipStream_t stream);
+
+/* qa_paged_attention_decode_batched over a 4-bit pool, with an optional gate
+ * (batch, heads, head_dim) of bfloat16 logits: out *= sigmoid(gate).  query and
+ * output bfloat16, GQA group up to 16.  Rows of length <= 0, and rows that see
+ * only blocks outside the pool, give zeros.  workspace: 16-byte aligned,
+ * qa_paged_attention_decode_kv4_workspace(.., max_blocks * block_size) bytes.  */
+int64_t qa_paged_attention_decode_kv4_workspace(int64_t batch, int32_t heads, int32_t kv_heads, int32_t head_dim, int64_t max_tokens);
+int qa_paged_attention_decode_kv4(const void* query, int32_t q_dtype, int64_t q_stride_b, int64_t q_stride_h, int64_t batch,
+                                  int32_t heads, int32_t head_dim, const qa_paged_kv* kv, const void* block_tables,
+                                  int32_t table_dtype, int64_t table_stride, int64_t max_blocks,
+                                  const void* sequence_lengths, int32_t lengths_dtype, int32_t block_size, float scale,
+                                  const void* gate, int64_t gate_stride_b, int64_t gate_stride_h, void* output,
+                                  void* workspace, int64_t workspace_bytes, hipStream_t stream);
+
+/* qa_paged_attention_prefill over a 4-bit pool: total_new rows of query, GQA
+ * group up to 16; tokens at or past total_new or max_new of their row are not
+ * computed, and output rows past the last sequence are left as they were.     */
+int qa_paged_attention_prefill_kv4(const void* query, int32_t q_dtype, int64_t q_stride_t, int64_t q_stride_h, int64_t total_new,
+                                   const void* cu_seqlens, const void* prefix_lens, int32_t idx_dtype, int64_t batch,
+                                   int64_t max_new, int32_t heads, int32_t head_dim, const qa_paged_kv* kv,
+                                   const void* block_tables, int32_t table_dtype, int64_t table_stride, int64_t max_blocks,
+                                   int32_t block_size, float scale, const void* gate, int64_t gate_stride_t,
+                                   int64_t gate_stride_h, void* output, hipStream_t stream);
+
+/* qa_qk_norm_rope_append with several position axes, through a slot map, into a
+ * bf16 or a 4-bit pool.  positions (axes, tokens), axis a at a*positions_stride;
+ * freq_turns (rotary_dim / 2): base^(-2 j / rotary_dim) / (2 pi) as a fraction of
+ * 2^64; freq_axis (rotary_dim / 2): the axis of each frequency, 1 to 4 axes.
+ * fp32 throughout, rounded to bf16 once (k, then its 4-bit form where the pool
+ * is one).  Tokens whose slot is outside the pool write no k and v; slots must
+ * be distinct.  head_dim 64, 128, 256 (4-bit pool: 128, 256).  For equal
+ * positions the rotation of src/reference_ops.py:203-224.                     */
+int qa_qk_norm_mrope_append(const void* q_proj, int64_t q_stride_t, int64_t q_stride_h, const void* k_proj, int64_t k_stride_t,
+                            int64_t k_stride_h, const void* v_proj, int64_t v_stride_t, int64_t v_stride_h,
+                            const void* q_norm_weight, const void* k_norm_weight, int32_t weight_dtype, float eps,
+                            const uint64_t* freq_turns, const uint8_t* freq_axis, int32_t rotary_dim, const void* positions,
+                            int32_t positions_dtype, int64_t positions_stride, int32_t axes, int64_t tokens, int32_t heads,
+                            int32_t head_dim, const qa_paged_kv* kv, const void* slots, int32_t slots_dtype, int32_t block_size,
+                            void* q_out, hipStream_t stream);
 
 /* ---- gated delta-rule linear attention --------------------------------- */
 /* Depthwise causal conv1d over `seq` tokens (+ optional SiLU), fp32 math.

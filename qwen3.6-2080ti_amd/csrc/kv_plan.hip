@@ -1,0 +1,261 @@
+// The plan of a batched step on the device: block tables grown from the free list, and the slot map of the step's
+// packed tokens, from the requests' lengths and new-token counts.
+//
+// Row b grows from L_b to L_b + n_b tokens.  With need_b = ceil((L_b + n_b) / bs) - ceil(L_b / bs), the exclusive sums
+// over the rows c_b of n and f_b of need give everything: packed token i of row b (i - c_b = x) sits at position
+// L_b + x; its logical block lb is the row's old one while lb < ceil(L_b / bs), else free_list[head + f_b + lb -
+// ceil(L_b / bs)]; its slot is id * bs + position % bs.  A fresh block always holds a new token at its first position,
+// so the token there writes the table entry: no pass of its own over the tables.
+//
+// A few KB move, so latency bounds it: one workgroup makes the sums and the all-or-nothing checks, and with few tokens
+// writes them too; from kInlineTokens on a second launch of one workgroup per kSpanTokens tokens does that, because one
+// CU stores only a few tens of GB/s.
+#include "qa_common.h"
+
+namespace qa {
+namespace kvplan {
+
+struct Params {
+  int32_t* tables;
+  int64_t table_stride, max_blocks;
+  int32_t* lengths;
+  const void* counts;  // null: count_scalar
+  int64_t count_scalar;
+  const int32_t* free_list;
+  int32_t* free_state;
+  int32_t* status;
+  int32_t* cu;         // (B + 1)
+  int32_t* starts;     // (B)
+  int32_t* first;      // (B): where each row's fresh blocks begin in the free list
+  int32_t* positions;  // (max_tokens)
+  int64_t* slots;      // (max_tokens)
+  int64_t max_tokens, capacity;
+  int B, bs, counts_i64;
+  int inline_tokens;   // the planning workgroup writes the tokens too
+};
+
+constexpr int kThreads = 1024;
+constexpr int kSpanTokens = 1024;   // tokens of a workgroup of the second launch
+constexpr int kInlineTokens = 4096;
+constexpr int kRowsInLds = 4096;    // rows whose sums a workgroup looks up in LDS
+
+__device__ __forceinline__ int64_t count_of(const Params& p, int b) {
+  if (p.counts == nullptr) return p.count_scalar;
+  return p.counts_i64 ? reinterpret_cast<const int64_t*>(p.counts)[b] : reinterpret_cast<const int32_t*>(p.counts)[b];
+}
+
+__device__ __forceinline__ int64_t ceil_div_dev(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Writes positions, slots and fresh table entries of tokens lo .. hi - 1.  cu: the row sums (in LDS or in memory).
+__device__ void write_tokens(const Params& p, const int32_t* cu, int64_t lo, int64_t hi) {
+  const int32_t total = cu[p.B];
+  for (int64_t i = lo + threadIdx.x; i < hi; i += blockDim.x) {
+    int32_t position = -1;
+    int64_t slot = -1;
+    if (i < total) {
+      int a = 0, z = p.B;  // cu[a] <= i < cu[z]
+      while (z - a > 1) {
+        const int m = (a + z) >> 1;
+        if (cu[m] <= i)
+          a = m;
+        else
+          z = m;
+      }
+      const int32_t start = p.starts[a];
+      position = start + static_cast<int32_t>(i - cu[a]);
+      const int lb = position / p.bs;
+      const int have = (start + p.bs - 1) / p.bs;
+      const int at = position - lb * p.bs;
+      int32_t id;
+      if (lb < have) {
+        id = p.tables[a * p.table_stride + lb];
+      } else {
+        id = p.free_list[p.first[a] + lb - have];
+        if (at == 0) p.tables[a * p.table_stride + lb] = id;
+      }
+      if (id >= 0) slot = static_cast<int64_t>(id) * p.bs + at;
+    }
+    p.positions[i] = position;
+    p.slots[i] = slot;
+  }
+}
+
+__global__ __launch_bounds__(kThreads) void plan_kernel(Params p) {
+  __shared__ int64_t s_need[kThreads / 64], s_count[kThreads / 64];
+  __shared__ int s_bad[kThreads / 64];
+  __shared__ int32_t s_cu[kRowsInLds + 1];
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = tid >> 6;
+  const int64_t head = p.free_state[0];
+  const int64_t avail = p.free_state[1];
+
+  // every row's length, tokens and blocks: the checks
+  int64_t need = 0, count = 0;
+  int bad = 0;
+  for (int b = tid; b < p.B; b += kThreads) {
+    const int64_t len = p.lengths[b];
+    const int64_t n = count_of(p, b);
+    if (len < 0 || n < 0 || n > 0x7fffffff || len + n > 0x7fffffff - p.bs) {
+      bad |= 4;
+      continue;
+    }
+    const int64_t want = ceil_div_dev(len + n, p.bs);
+    if (want > p.max_blocks) bad |= 2;
+    need += want - ceil_div_dev(len, p.bs);
+    count += n;
+  }
+  for (int off = 32; off > 0; off >>= 1) {
+    need += __shfl_xor(need, off, 64);
+    count += __shfl_xor(count, off, 64);
+    bad |= __shfl_xor(bad, off, 64);
+  }
+  if (lane == 0) {
+    s_need[wave] = need;
+    s_count[wave] = count;
+    s_bad[wave] = bad;
+  }
+  __syncthreads();
+  int64_t total_need = 0, total_count = 0;
+  bad = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 64; ++w) {
+    total_need += s_need[w];
+    total_count += s_count[w];
+    bad |= s_bad[w];
+  }
+  int code = 0;
+  if (head < 0 || avail < 0 || head + avail > p.capacity) code = 3;
+  else if (bad & 4) code = 4;
+  else if (bad & 2) code = 2;
+  else if (total_need > avail) code = 1;
+  else if (total_count > p.max_tokens) code = 5;
+  __syncthreads();  // s_need and s_count are used again
+
+  // the row sums; a step that is refused plans no token and takes nothing
+  int64_t need_before = head, count_before = 0;
+  for (int r0 = 0; r0 < p.B; r0 += kThreads) {
+    const int b = r0 + tid;
+    int64_t len = 0, n = 0, k = 0;
+    if (b < p.B) {
+      len = p.lengths[b];
+      if (code == 0) {
+        n = count_of(p, b);
+        k = ceil_div_dev(len + n, p.bs) - ceil_div_dev(len, p.bs);
+      }
+    }
+    int64_t n_incl = n, k_incl = k;
+    for (int off = 1; off < 64; off <<= 1) {
+      const int64_t nu = __shfl_up(n_incl, off, 64), ku = __shfl_up(k_incl, off, 64);
+      if (lane >= off) {
+        n_incl += nu;
+        k_incl += ku;
+      }
+    }
+    if (lane == 63) {
+      s_count[wave] = n_incl;
+      s_need[wave] = k_incl;
+    }
+    __syncthreads();
+    int64_t n_sum = 0, k_sum = 0;
+#pragma unroll
+    for (int w = 0; w < kThreads / 64; ++w) {
+      if (w == wave) {
+        n_incl += n_sum + count_before;
+        k_incl += k_sum + need_before;
+      }
+      n_sum += s_count[w];
+      k_sum += s_need[w];
+    }
+    if (b < p.B) {
+      const int32_t c = static_cast<int32_t>(n_incl - n);
+      p.cu[b] = c;
+      if (b < kRowsInLds) s_cu[b] = c;
+      p.starts[b] = static_cast<int32_t>(len);
+      p.first[b] = static_cast<int32_t>(k_incl - k);
+      if (code == 0) p.lengths[b] = static_cast<int32_t>(len + n);
+    }
+    count_before += n_sum;
+    need_before += k_sum;
+    __syncthreads();
+  }
+  if (tid == 0) {
+    const int32_t total = static_cast<int32_t>(count_before);
+    p.cu[p.B] = total;
+    if (p.B <= kRowsInLds) s_cu[p.B] = total;
+    if (code == 0) {
+      p.free_state[0] = static_cast<int32_t>(head + total_need);
+      p.free_state[1] = static_cast<int32_t>(avail - total_need);
+    }
+    p.status[0] = code;
+  }
+  if (!p.inline_tokens) return;
+  __syncthreads();  // also orders this workgroup's writes of starts and first before the reads below
+  write_tokens(p, s_cu, 0, p.max_tokens);
+}
+
+__global__ __launch_bounds__(256) void plan_tokens_kernel(Params p) {
+  __shared__ int32_t s_cu[kRowsInLds + 1];
+  const int64_t lo = static_cast<int64_t>(blockIdx.x) * kSpanTokens;
+  const int64_t hi = min64(p.max_tokens, lo + kSpanTokens);
+  if (p.B <= kRowsInLds) {
+    for (int b = threadIdx.x; b <= p.B; b += blockDim.x) s_cu[b] = p.cu[b];
+    __syncthreads();
+    write_tokens(p, s_cu, lo, hi);
+  } else {
+    write_tokens(p, p.cu, lo, hi);
+  }
+}
+
+}  // namespace kvplan
+}  // namespace qa
+
+extern "C" int qa_paged_kv_plan(int32_t* block_tables, int64_t table_stride, int64_t max_blocks, int32_t* lengths, const void* counts, int32_t counts_dtype,
+                                int64_t count_scalar, int64_t batch, int32_t block_size, const int32_t* free_list, int64_t free_capacity, int32_t* free_state,
+                                int32_t* status, int64_t max_tokens, int32_t* cu_seqlens, int32_t* starts, int32_t* positions, int64_t* slots, int32_t* workspace,
+                                int64_t workspace_bytes, hipStream_t stream) {
+  using namespace qa;
+  using namespace qa::kvplan;
+  QA_REQUIRE(batch >= 1 && batch <= 0xffffff, "paged_kv_plan: batch must be in [1, 2^24)");
+  QA_REQUIRE(block_tables && lengths && free_list && free_state && status && cu_seqlens && starts && workspace, "paged_kv_plan: pointers must be non-null");
+  QA_REQUIRE(counts == nullptr || is_index_dtype(counts_dtype), "paged_kv_plan: counts must be int32/int64");
+  QA_REQUIRE(counts != nullptr || (count_scalar >= 0 && count_scalar <= 0x7fffffff), "paged_kv_plan: count must be non-negative");
+  QA_REQUIRE(block_size > 0 && block_size <= 65536 && max_blocks > 0, "paged_kv_plan: block_size must be in [1, 65536] and max_blocks positive");
+  QA_REQUIRE(table_stride >= max_blocks || batch <= 1, "table rows overlap: stride %lld < max_blocks %lld", static_cast<long long>(table_stride),
+             static_cast<long long>(max_blocks));
+  QA_REQUIRE(free_capacity > 0 && free_capacity <= 0x7fffffff, "free list capacity must be in [1, 2^31)");
+  QA_REQUIRE(max_tokens >= 0 && max_tokens <= 0x3fffffff, "paged_kv_plan: max_tokens must be in [0, 2^30)");
+  QA_REQUIRE(max_tokens == 0 || (positions && slots), "paged_kv_plan: pointers must be non-null");
+  QA_REQUIRE(workspace_bytes >= batch * 4, "paged_kv_plan: workspace too small: need %lld bytes", static_cast<long long>(batch * 4));
+  Params p{};
+  p.tables = block_tables;
+  p.table_stride = table_stride;
+  p.max_blocks = max_blocks;
+  p.lengths = lengths;
+  p.counts = counts;
+  p.count_scalar = count_scalar;
+  p.free_list = free_list;
+  p.free_state = free_state;
+  p.status = status;
+  p.cu = cu_seqlens;
+  p.starts = starts;
+  p.first = workspace;
+  p.positions = positions;
+  p.slots = slots;
+  p.max_tokens = max_tokens;
+  p.capacity = free_capacity;
+  p.B = static_cast<int>(batch);
+  p.bs = block_size;
+  p.counts_i64 = counts_dtype == QA_I64;
+  p.inline_tokens = max_tokens <= kInlineTokens && batch <= kRowsInLds;
+  {
+    KernelTimer timer_("kv_plan", stream);
+    hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(kThreads), 0, stream, p);
+  }
+  if (int rc = check_launch("paged_kv_plan")) return rc;
+  if (!p.inline_tokens && max_tokens > 0) {
+    KernelTimer timer_("kv_plan_tokens", stream);
+    hipLaunchKernelGGL(plan_tokens_kernel, dim3(static_cast<unsigned>(ceil_div(max_tokens, kSpanTokens))), dim3(256), 0, stream, p);
+  }
+  return check_launch("paged_kv_plan");
+}

@@ -23,7 +23,7 @@ LIBRARY_PATH = PACKAGE_DIR / "build" / "libqwen36_hip.so"
 
 _LIB: Any | None = None
 
-QA_F32, QA_BF16, QA_F16, QA_I32, QA_I64 = 0, 1, 2, 3, 4
+QA_F32, QA_BF16, QA_F16, QA_I32, QA_I64, QA_KV4 = 0, 1, 2, 3, 4, 5
 
 c_void_p = ctypes.c_void_p
 c_int32 = ctypes.c_int32
@@ -150,6 +150,35 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
         c_int32,
         [c_void_p, c_int32, c_int64, c_int64, c_void_p, c_void_p, c_int32, c_int64, c_int64, c_int32, c_int32, ctypes.POINTER(PagedKV),
          c_void_p, c_int32, c_int64, c_int64, c_int32, c_float, c_void_p, c_int64, c_int64, c_void_p, c_void_p],
+    ),
+    "qa_paged_kv_plan": (
+        c_int32,
+        [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int32, c_int64, c_int64, c_int32, c_void_p, c_int64, c_void_p, c_void_p, c_int64,
+         c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p],
+    ),
+    "qa_paged_kv4_append": (
+        c_int32,
+        [c_void_p, c_void_p, c_int32, c_int64, c_int64, c_int64, c_int64, c_int64, c_int32, ctypes.POINTER(PagedKV), c_void_p, c_int32, c_int32, c_void_p],
+    ),
+    "qa_paged_kv4_gather": (
+        c_int32,
+        [ctypes.POINTER(PagedKV), c_int32, c_int64, c_void_p, c_int32, c_int64, c_int64, c_int64, c_int32, c_void_p, c_void_p, c_void_p],
+    ),
+    "qa_paged_attention_decode_kv4_workspace": (c_int64, [c_int64, c_int32, c_int32, c_int32, c_int64]),
+    "qa_paged_attention_decode_kv4": (
+        c_int32,
+        [c_void_p, c_int32, c_int64, c_int64, c_int64, c_int32, c_int32, ctypes.POINTER(PagedKV), c_void_p, c_int32, c_int64, c_int64, c_void_p, c_int32, c_int32,
+         c_float, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_void_p],
+    ),
+    "qa_paged_attention_prefill_kv4": (
+        c_int32,
+        [c_void_p, c_int32, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int32, c_int64, c_int64, c_int32, c_int32, ctypes.POINTER(PagedKV), c_void_p, c_int32,
+         c_int64, c_int64, c_int32, c_float, c_void_p, c_int64, c_int64, c_void_p, c_void_p],
+    ),
+    "qa_qk_norm_mrope_append": (
+        c_int32,
+        [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int32, c_float, c_void_p, c_void_p, c_int32,
+         c_void_p, c_int32, c_int64, c_int32, c_int64, c_int32, c_int32, ctypes.POINTER(PagedKV), c_void_p, c_int32, c_int32, c_void_p, c_void_p],
     ),
 }
 

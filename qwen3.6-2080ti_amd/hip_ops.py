@@ -21,7 +21,8 @@ torch (its caching allocator owns them); kernels run on torch's current stream.
 from __future__ import annotations
 
 import ctypes
-from typing import Any, Sequence
+import math
+from typing import Any, NamedTuple, Sequence
 
 import torch
 
@@ -1081,3 +1082,400 @@ def qk_norm_rope_kv_append(
     )
     L.check(lib, status, "qk_norm_rope_kv_append")
     return query, q3.narrow(2, head_dim, head_dim)
+
+
+# --------------------------------------------------------------------------- the 4-bit KV cache
+
+
+def _launch(device: torch.device, fn: Any, *args: Any) -> int:
+    """``fn(*args, stream)`` on ``device``'s current stream, with that device current."""
+    if torch._C._cuda_getDevice() == device.index:
+        return fn(*args, _stream(device))
+    with torch.cuda.device(device):
+        return fn(*args, _stream(device))
+
+
+def kv4_tile_bytes(head_dim: int, block_size: int) -> int:
+    """Bytes of one block of one KV head in a 4-bit pool: 4 bits a value and a scale byte per 32 values."""
+    _require(head_dim in (128, 256), "4-bit pools need head_dim 128 or 256")
+    _require(16 <= block_size <= 1024 and block_size & (block_size - 1) == 0, "4-bit pools need a block_size that is a power of two from 16 to 1024")
+    return block_size * 17 * head_dim // 32
+
+
+def _kv4_descriptor(key_pool: torch.Tensor, value_pool: torch.Tensor, block_size: int, device: torch.device) -> tuple[L.PagedKV, int]:
+    """Descriptor and head_dim of a 4-bit pool ``(P, H_kv, kv4_tile_bytes(D, block_size))``."""
+    _require_cuda(key_pool, "key_pool", device)
+    _require_cuda(value_pool, "value_pool", device)
+    if key_pool.dtype != torch.uint8 or value_pool.dtype != torch.uint8 or key_pool.dim() != 3 or value_pool.shape != key_pool.shape:
+        raise RuntimeError("4-bit pools must be uint8 (blocks, kv_heads, tile bytes) and alike")
+    strides = key_pool.stride()
+    if strides[2] != 1 or value_pool.stride() != strides:
+        raise RuntimeError("key/value pools must share strides with contiguous tiles")
+    blocks, kv_heads, tile = key_pool.shape
+    for head_dim in (256, 128):
+        if tile == kv4_tile_bytes(head_dim, block_size):
+            return L.PagedKV(key_pool.data_ptr(), value_pool.data_ptr(), None, None, None, blocks, 0, strides[0], strides[1], 0, kv_heads, L.QA_KV4), head_dim
+    raise RuntimeError(f"a tile of {tile} bytes is no block of {block_size} tokens of 128 or 256 dims in 4 bits")
+
+
+def _rows(tensor: torch.Tensor, multiple: int) -> torch.Tensor:
+    """``tensor`` (.., .., D) as it is where its rows can be read in aligned pieces of ``multiple`` elements, else a copy."""
+    strides = tensor.stride()
+    if strides[-1] == 1 and strides[0] % multiple == 0 and strides[1] % multiple == 0 and tensor.data_ptr() % (multiple * tensor.element_size()) == 0:
+        return tensor
+    return tensor.contiguous()
+
+
+def _kv4_gate(gate: torch.Tensor | None, rows: int, heads: int, head_dim: int, device: torch.device) -> torch.Tensor | None:
+    if gate is None:
+        return None
+    _require_cuda(gate, "gate", device)
+    _require(gate.dtype == torch.bfloat16, "gate must be bfloat16")
+    if gate.dim() == 2 and gate.shape == (rows, heads * head_dim):
+        gate = gate.reshape(rows, heads, head_dim)
+    _require(gate.shape == (rows, heads, head_dim), "gate must be (tokens, heads*head_dim) or (tokens, heads, head_dim)")
+    return _rows(gate, 4)
+
+
+def _kv4_out(out: torch.Tensor | None, like: torch.Tensor) -> torch.Tensor:
+    if out is None:
+        return torch.empty(like.shape, dtype=torch.bfloat16, device=like.device)
+    _require_cuda(out, "out", like.device)
+    _require(out.dtype == torch.bfloat16 and out.shape == like.shape and out.is_contiguous(), "out must be contiguous bfloat16 of query's shape")
+    return out
+
+
+class PagedPlan(NamedTuple):
+    """A step of packed new tokens on the device (:func:`paged_kv_plan`): ``cu_seqlens`` ``(B + 1,)`` and ``starts``
+    ``(B,)`` int32 (each row's tokens and its length before the step), ``positions`` int32 and ``slots`` int64
+    ``(max_tokens,)``, -1 past the step's last token."""
+
+    cu_seqlens: torch.Tensor
+    starts: torch.Tensor
+    positions: torch.Tensor
+    slots: torch.Tensor
+
+
+def paged_kv_plan(
+    block_tables: torch.Tensor,
+    lengths: torch.Tensor,
+    counts: torch.Tensor | int,
+    free_list: torch.Tensor,
+    free_state: torch.Tensor,
+    status: torch.Tensor,
+    block_size: int,
+    *,
+    max_tokens: int,
+) -> PagedPlan:
+    """Block tables and slot map of a batched step, built on the device from the requests' lengths.
+
+    Row ``b`` grows from ``lengths[b]`` to ``lengths[b] + counts_b`` tokens: fresh logical blocks get ids from the
+    front of the ascending ``free_list``, rows in order (:func:`paged_kv_reserve`'s policy), and ``block_tables``
+    ``(B, max_blocks)`` int32, ``lengths`` ``(B,)`` int32 and ``free_state`` are advanced in place.  The returned
+    plan holds the packed step for :func:`qk_norm_mrope_kv_append`, :func:`paged_kv4_append` and
+    :func:`paged_attention_prefill_kv4`.  ``max_tokens`` bounds the step (the host need not know its size), and the
+    token arrays are that long.  ``status`` (int32 ``[1]``) becomes 0, or 1 (pool exhausted), 2 (a table row too
+    short), 3 (corrupt free state), 4 (negative or overflowing length or count), 5 (more than ``max_tokens``
+    tokens): then nothing is taken and the plan is empty, so that the operators fed by it do nothing.  Nothing is
+    read back, so the call can be captured in a HIP graph.
+    """
+    lib = L.load_library()
+    _require_cuda(block_tables, "block_tables")
+    device = block_tables.device
+    for tensor, name in ((lengths, "lengths"), (free_list, "free_list"), (free_state, "free_state"), (status, "status")):
+        _require_cuda(tensor, name, device)
+    _require(block_tables.dtype == torch.int32 and block_tables.dim() == 2 and block_tables.stride(1) == 1, "block_tables must be int32 [batch, max_blocks] with contiguous rows")
+    batch, max_blocks = block_tables.shape
+    _require(batch > 0 and max_blocks > 0, "block_tables must have shape [batch, max_blocks]")
+    _require(lengths.dtype == torch.int32 and lengths.shape == (batch,) and lengths.is_contiguous(), "lengths must be a contiguous int32 [batch] tensor")
+    _require(free_list.dtype == torch.int32 and free_list.dim() == 1 and free_list.is_contiguous(), "free_list must be a contiguous int32 vector")
+    _require(free_state.dtype == torch.int32 and free_state.numel() == 2 and free_state.is_contiguous(), "free_state must be int32 [head, count]")
+    _require(status.dtype == torch.int32 and status.numel() >= 1, "status must be an int32 tensor")
+    max_tokens = int(max_tokens)
+    _require(max_tokens >= 0, "max_tokens must be non-negative")
+    count_ptr, count_code, count_scalar = 0, L.QA_I32, 0
+    if isinstance(counts, torch.Tensor):
+        _require_cuda(counts, "counts", device)
+        _index_dtype(counts, "counts")
+        _require(counts.shape == (batch,) and counts.is_contiguous(), "counts must be a contiguous [batch] tensor")
+        count_ptr, count_code = _ptr(counts), _code(counts)
+    else:
+        count_scalar = int(counts)
+        _require(count_scalar >= 0, "counts must be non-negative")
+    # one allocation: cu_seqlens, starts, the kernel's scratch row sums, positions
+    ints = torch.empty(3 * batch + 1 + max_tokens, dtype=torch.int32, device=device)
+    slots = torch.empty(max_tokens, dtype=torch.int64, device=device)
+    at = ints.data_ptr()
+    code = _launch(
+        device, lib.qa_paged_kv_plan, _ptr(block_tables), block_tables.stride(0), max_blocks, _ptr(lengths), count_ptr, count_code, count_scalar, batch,
+        int(block_size), _ptr(free_list), free_list.numel(), _ptr(free_state), _ptr(status), max_tokens, at, at + 4 * (batch + 1), at + 4 * (3 * batch + 1),
+        _ptr(slots), at + 4 * (2 * batch + 1), 4 * batch,
+    )
+    L.check(lib, code, "paged_kv_plan")
+    return PagedPlan(ints[: batch + 1], ints[batch + 1 : 2 * batch + 1], ints[3 * batch + 1 :], slots)
+
+
+def paged_kv4_append(key: torch.Tensor, value: torch.Tensor, key_pool: torch.Tensor, value_pool: torch.Tensor, slots: torch.Tensor, block_size: int) -> None:
+    """Quantise packed K/V rows ``(tokens, H_kv, D)`` (bf16 or fp32) into ``slots`` of a 4-bit pool, in place.
+
+    The pools are uint8 ``(P, H_kv, kv4_tile_bytes(D, block_size))``; per 32 dims of a token a power-of-two scale and
+    E2M1 codes (the format and layout stand in ``qwen36_hip.h``).  ``slots`` ``(tokens,)`` hold ``block id *
+    block_size + position % block_size`` (:func:`paged_kv_plan`); those outside the pool, such as -1, are skipped.
+    They have to be distinct.
+    """
+    lib = L.load_library()
+    _require_cuda(key, "key")
+    device = key.device
+    _require_cuda(value, "value", device)
+    _require_cuda(slots, "slots", device)
+    _index_dtype(slots, "slots")
+    desc, head_dim = _kv4_descriptor(key_pool, value_pool, block_size, device)
+    _require(key.dim() == 3 and key.shape[1:] == (desc.kv_heads, head_dim) and value.shape == key.shape, "key/value must be (tokens, kv_heads, head_dim) of the pool's heads")
+    _float_dtype(key, "key")
+    _require(value.dtype == key.dtype, "key and value must share a dtype")
+    _require(slots.dim() == 1 and slots.shape[0] == key.shape[0], "slots must have one entry per token")
+    multiple = 8 if key.dtype == torch.bfloat16 else 4
+    k, v, s = _rows(key, multiple), _rows(value, multiple), slots.contiguous()
+    code = _launch(
+        device, lib.qa_paged_kv4_append, _ptr(k), _ptr(v), _code(k), k.stride(0), k.stride(1), v.stride(0), v.stride(1), k.shape[0], head_dim, ctypes.byref(desc),
+        _ptr(s), _code(s), int(block_size),
+    )
+    L.check(lib, code, "paged_kv4_append")
+
+
+def paged_kv4_gather(key_pool: torch.Tensor, value_pool: torch.Tensor, block_tables: torch.Tensor, valid: int, block_size: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """Dense ``(B, H_kv, valid, D)`` bf16 K/V of a 4-bit pool in logical order (:func:`paged_kv_gather`'s counterpart).
+
+    Every value the cache holds is exact in bf16.  Tokens whose block id is outside the pool, or past the table, are
+    zeros; a group stored from an infinity or a NaN reads as NaN.
+    """
+    lib = L.load_library()
+    _require_cuda(key_pool, "key_pool")
+    device = key_pool.device
+    _require_cuda(block_tables, "block_tables", device)
+    _index_dtype(block_tables, "block_tables")
+    desc, head_dim = _kv4_descriptor(key_pool, value_pool, block_size, device)
+    tables = block_tables.contiguous()
+    if tables.dim() == 1:
+        tables = tables.unsqueeze(0)
+    _require(tables.dim() == 2 and tables.shape[1] > 0, "block_tables must have shape [batch, max_blocks]")
+    batch = tables.shape[0]
+    _require(int(valid) >= 0, "valid must be non-negative")
+    key_out = torch.empty((batch, desc.kv_heads, int(valid), head_dim), dtype=torch.bfloat16, device=device)
+    value_out = torch.empty_like(key_out)
+    code = _launch(
+        device, lib.qa_paged_kv4_gather, ctypes.byref(desc), head_dim, batch, _ptr(tables), _code(tables), tables.stride(0), tables.shape[1], int(valid),
+        int(block_size), _ptr(key_out), _ptr(value_out),
+    )
+    L.check(lib, code, "paged_kv4_gather")
+    return key_out, value_out
+
+
+def paged_attention_decode_kv4(
+    query: torch.Tensor,
+    block_tables: torch.Tensor,
+    key_pool: torch.Tensor,
+    value_pool: torch.Tensor,
+    sequence_lengths: torch.Tensor,
+    block_size: int,
+    *,
+    gate: torch.Tensor | None = None,
+    scale: float | None = None,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """``paged_attention_decode_batched`` over a 4-bit pool: one token per row, ``query`` ``(B, H, 1, D)`` bf16.
+
+    ``gate`` ``(B, H*D)`` or ``(B, H, D)`` bf16 logits (a view of ``q_proj`` is read in place) give ``out *
+    sigmoid(gate)``.  Rows of length <= 0, and rows that see only blocks outside the pool, give zeros.  Returns
+    ``(B, H, 1, D)`` bf16, in ``out`` where it is given.
+    """
+    lib = L.load_library()
+    _require_cuda(query, "query")
+    device = query.device
+    _require_cuda(block_tables, "block_tables", device)
+    _require_cuda(sequence_lengths, "sequence_lengths", device)
+    _require(query.dtype == torch.bfloat16, "query must be bfloat16")
+    _index_dtype(block_tables, "block_tables")
+    _index_dtype(sequence_lengths, "sequence_lengths")
+    _require(query.dim() == 4 and query.shape[2] == 1, "query must have shape [batch, heads, 1, head_dim]")
+    desc, head_dim = _kv4_descriptor(key_pool, value_pool, block_size, device)
+    batch, heads = query.shape[:2]
+    _require(query.shape[3] == head_dim, "KV head_dim must match query")
+    _require(block_tables.dim() == 2 and block_tables.shape[0] == batch and block_tables.shape[1] > 0, "block_tables must have shape [batch, max_blocks]")
+    _require(sequence_lengths.shape == (batch,), "sequence_lengths batch must match query")
+    _require(heads % desc.kv_heads == 0, "KV heads must divide query heads")
+    q = _rows(query.squeeze(2), 8)
+    g = _kv4_gate(gate, batch, heads, head_dim, device)
+    tables, lens = block_tables.contiguous(), sequence_lengths.contiguous()
+    max_blocks = tables.shape[1]
+    result = _kv4_out(out, query)
+    nbytes = lib.qa_paged_attention_decode_kv4_workspace(batch, heads, desc.kv_heads, head_dim, max_blocks * block_size)
+    ws = torch.empty(max(nbytes, 4), dtype=torch.uint8, device=device)
+    code = _launch(
+        device, lib.qa_paged_attention_decode_kv4, _ptr(q), _code(q), q.stride(0), q.stride(1), batch, heads, head_dim, ctypes.byref(desc), _ptr(tables),
+        _code(tables), tables.stride(0), max_blocks, _ptr(lens), _code(lens), int(block_size), float(scale or 0.0), _ptr(g), 0 if g is None else g.stride(0),
+        0 if g is None else g.stride(1), _ptr(result), _ptr(ws), ws.numel(),
+    )
+    L.check(lib, code, "paged_attention_decode_kv4")
+    return result
+
+
+def paged_attention_prefill_kv4(
+    query: torch.Tensor,
+    cu_seqlens: torch.Tensor,
+    prefix_lens: torch.Tensor,
+    key_pool: torch.Tensor,
+    value_pool: torch.Tensor,
+    block_tables: torch.Tensor,
+    block_size: int,
+    *,
+    max_new: int,
+    gate: torch.Tensor | None = None,
+    scale: float | None = None,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """:func:`paged_attention_prefill` over a 4-bit pool: causal attention of packed new tokens.
+
+    ``query`` ``(tokens, H, D)`` bf16; the new tokens' K/V are in the pool already, so a new token sees itself and
+    its neighbours in 4 bits, as every later step will.  ``max_new`` is at least the longest row of ``cu_seqlens``
+    (tokens past it are not computed).  Returns ``(tokens, H, D)`` bf16, in ``out`` where it is given; rows past the
+    last sequence are not written.
+    """
+    lib = L.load_library()
+    _require_cuda(query, "query")
+    device = query.device
+    _require(query.dtype == torch.bfloat16 and query.dim() == 3, "query must be (tokens, heads, head_dim) bfloat16")
+    for tensor, name in ((cu_seqlens, "cu_seqlens"), (prefix_lens, "prefix_lens"), (block_tables, "block_tables")):
+        _require_cuda(tensor, name, device)
+        _index_dtype(tensor, name)
+    _require(cu_seqlens.dtype == prefix_lens.dtype, "cu_seqlens and prefix_lens must share a dtype")
+    desc, head_dim = _kv4_descriptor(key_pool, value_pool, block_size, device)
+    tokens, heads = query.shape[:2]
+    _require(query.shape[2] == head_dim, "KV head_dim must match query")
+    _require(heads % desc.kv_heads == 0, "KV heads must divide query heads")
+    _require(prefix_lens.dim() == 1 and cu_seqlens.shape == (prefix_lens.shape[0] + 1,), "cu_seqlens must have batch + 1 entries")
+    batch = prefix_lens.shape[0]
+    _require(block_tables.dim() == 2 and block_tables.shape[0] == batch and block_tables.shape[1] > 0, "block_tables must have shape [batch, max_blocks]")
+    q = _rows(query, 8)
+    g = _kv4_gate(gate, tokens, heads, head_dim, device)
+    cu, prefix, tables = cu_seqlens.contiguous(), prefix_lens.contiguous(), block_tables.contiguous()
+    result = _kv4_out(out, query)
+    code = _launch(
+        device, lib.qa_paged_attention_prefill_kv4, _ptr(q), _code(q), q.stride(0), q.stride(1), tokens, _ptr(cu), _ptr(prefix), _code(cu), batch, int(max_new),
+        heads, head_dim, ctypes.byref(desc), _ptr(tables), _code(tables), tables.stride(0), tables.shape[1], int(block_size), float(scale or 0.0), _ptr(g),
+        0 if g is None else g.stride(0), 0 if g is None else g.stride(1), _ptr(result),
+    )
+    L.check(lib, code, "paged_attention_prefill_kv4")
+    return result
+
+
+def mrope_axes(sections: Sequence[int], interleaved: bool) -> list[int]:
+    """The position axis of each of the ``sum(sections)`` frequencies.
+
+    Section ``a`` counts the frequencies of axis ``a``.  In order: the first ``sections[0]`` are axis 0's, the next
+    axis 1's, and so on.  Interleaved: with ``n`` axes, axis ``a > 0`` has frequencies ``a, a + n, ..`` below
+    ``n * sections[a]``, and axis 0 all others.
+    """
+    sections = [int(s) for s in sections]
+    _require(1 <= len(sections) <= 4 and min(sections) >= 0 and sum(sections) > 0, "sections must be 1 to 4 counts of frequencies")
+    if not interleaved:
+        return [a for a, n in enumerate(sections) for _ in range(n)]
+    axes = [0] * sum(sections)
+    for a in range(1, len(sections)):
+        for j in range(a, min(len(sections) * sections[a], len(axes)), len(sections)):
+            axes[j] = a
+    return axes
+
+
+_MROPE: dict[tuple[Any, ...], tuple[torch.Tensor, torch.Tensor]] = {}
+
+
+def _mrope_tables(sections: tuple[int, ...], interleaved: bool, rope_theta: float, device: torch.device) -> tuple[torch.Tensor, torch.Tensor]:
+    """The frequencies ``theta^(-j / half) / (2 pi)`` as fractions of 2^64 (int64) and their axes (uint8), cached: they
+    depend on the model's configuration alone."""
+    key = (sections, interleaved, rope_theta, device)
+    cached = _MROPE.get(key)
+    if cached is None:
+        axes = mrope_axes(sections, interleaved)
+        turns = [round(math.ldexp(rope_theta ** (-j / len(axes)) / (2 * math.pi), 64)) for j in range(len(axes))]
+        _require(rope_theta >= 1.0, "rope_theta must be at least 1")
+        cached = (torch.tensor(turns, dtype=torch.int64, device=device), torch.tensor(axes, dtype=torch.uint8, device=device))
+        _MROPE[key] = cached
+    return cached
+
+
+def qk_norm_mrope_kv_append(
+    q_proj: torch.Tensor,
+    k_proj: torch.Tensor,
+    v_proj: torch.Tensor,
+    q_norm_weight: torch.Tensor,
+    k_norm_weight: torch.Tensor,
+    positions: torch.Tensor,
+    sections: Sequence[int],
+    key_pool: torch.Tensor,
+    value_pool: torch.Tensor,
+    slots: torch.Tensor,
+    block_size: int,
+    *,
+    eps: float,
+    rope_theta: float,
+    interleaved: bool = False,
+) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """Prologue of a full-attention layer with rotary positions of several axes, in one launch.
+
+    :func:`qk_norm_rope_kv_append` for tokens that have a time, a row and a column (pictures, video) rather than one
+    position: ``positions`` ``(axes, tokens)`` (or ``(tokens,)``), ``sections`` and ``interleaved`` say which axis
+    turns which frequency (:func:`mrope_axes`); the first ``2 * sum(sections)`` dims of a head are rotated, in pairs
+    ``(j, j + sum(sections))`` by ``positions[axis(j)] * rope_theta^(-j / sum(sections))``.  fp32 throughout, rounded
+    to bf16 once; angles are exact at any position.  ``sum(sections)`` is a multiple of ``D / 64``.
+
+    ``q_proj`` ``(tokens, H, 2D)`` (query and gate halves) or ``(tokens, H, D)``, ``k_proj``/``v_proj`` ``(tokens,
+    H_kv, D)``, or flat in their last two dims, bf16.  k and v go to ``slots`` (:func:`paged_kv_plan`; those outside the
+    pool are skipped, the others have to be distinct) of a bf16 pool ``(P, H_kv, bs, D)`` or a 4-bit one ``(P, H_kv,
+    kv4_tile_bytes(D, bs))``; the latter then holds what :func:`paged_kv4_append` makes of the bf16 k and v.  Returns
+    ``(query (tokens, H, D) bf16, gate (tokens, H, D) view of q_proj or None)``.
+    """
+    lib = L.load_library()
+    _require_cuda(q_proj, "q_proj")
+    device = q_proj.device
+    for tensor, name in ((k_proj, "k_proj"), (v_proj, "v_proj"), (q_norm_weight, "q_norm_weight"), (k_norm_weight, "k_norm_weight"), (positions, "positions"),
+                         (key_pool, "key_pool"), (value_pool, "value_pool"), (slots, "slots")):
+        _require_cuda(tensor, name, device)
+    if key_pool.dtype == torch.uint8:
+        desc, head_dim = _kv4_descriptor(key_pool, value_pool, block_size, device)
+    else:
+        _require(key_pool.dtype == torch.bfloat16 and key_pool.dim() == 4 and key_pool.shape[2] == block_size, "the pool must be bfloat16 (blocks, kv_heads, block_size, head_dim) or 4-bit")
+        desc, head_dim = _pool_descriptor(key_pool, value_pool, "shared"), key_pool.shape[3]
+    kv_heads = desc.kv_heads
+    tokens = q_proj.shape[0]
+    k3 = k_proj.view(tokens, kv_heads, head_dim) if k_proj.dim() == 2 else k_proj
+    v3 = v_proj.view(tokens, kv_heads, head_dim) if v_proj.dim() == 2 else v_proj
+    _require(q_proj.dim() == 3 or q_proj.dim() == 2 and q_proj.shape[1] % (2 * head_dim) == 0, "q_proj must be (tokens, heads, head_dim or 2*head_dim) or (tokens, heads*2*head_dim)")
+    q3 = q_proj.view(tokens, -1, 2 * head_dim) if q_proj.dim() == 2 else q_proj
+    heads = q3.shape[1]
+    _require(q3.shape[2] in (head_dim, 2 * head_dim), "q_proj must be (tokens, heads, head_dim or 2*head_dim) or (tokens, heads*2*head_dim)")
+    _require(k3.shape == (tokens, kv_heads, head_dim) and v3.shape == (tokens, kv_heads, head_dim), "k_proj/v_proj must be (tokens, kv_heads, head_dim)")
+    for tensor, name in ((q3, "q_proj"), (k3, "k_proj"), (v3, "v_proj")):
+        if tensor.dtype != torch.bfloat16 or tensor.stride(-1) != 1:
+            raise RuntimeError(f"{name} must be bfloat16 with a contiguous last dimension")
+    _float_dtype(q_norm_weight, "q_norm_weight")
+    _require(q_norm_weight.dtype == k_norm_weight.dtype and q_norm_weight.shape == (head_dim,) and k_norm_weight.shape == (head_dim,),
+             "norm weights must be (head_dim,) of one dtype")
+    _index_dtype(positions, "positions")
+    _index_dtype(slots, "slots")
+    sections = tuple(sections)
+    pos = positions.unsqueeze(0) if positions.dim() == 1 else positions
+    _require(pos.shape == (len(sections), tokens), "positions must be (axes, tokens), one axis per section")
+    _require(slots.shape == (tokens,), "slots must have one entry per token")
+    freq, axis = _mrope_tables(sections, bool(interleaved), float(rope_theta), device)
+    if pos.stride(1) != 1:
+        pos = pos.contiguous()
+    s, qw, kw = slots.contiguous(), q_norm_weight.contiguous(), k_norm_weight.contiguous()
+    query = torch.empty((tokens, heads, head_dim), dtype=torch.bfloat16, device=device)
+    code = _launch(
+        device, lib.qa_qk_norm_mrope_append, _ptr(q3), q3.stride(0), q3.stride(1), _ptr(k3), k3.stride(0), k3.stride(1), _ptr(v3), v3.stride(0), v3.stride(1), _ptr(qw),
+        _ptr(kw), _code(qw), float(eps), _ptr(freq), _ptr(axis), 2 * axis.numel(), _ptr(pos), _code(pos), pos.stride(0), len(sections), tokens, heads, head_dim,
+        ctypes.byref(desc), _ptr(s), _code(s), int(block_size), _ptr(query),
+    )
+    L.check(lib, code, "qk_norm_mrope_kv_append")
+    return query, q3.narrow(2, head_dim, head_dim) if q3.shape[2] == 2 * head_dim else None
