@@ -10,7 +10,7 @@
 #include "kv4.h"
 
 namespace qa {
-namespace attn4 {
+namespace simple4 {
 
 struct Params {
   const bf16_t* q;
@@ -188,30 +188,8 @@ static int launch(const Params& p, int D, int64_t x, int64_t y, const char* what
   return check_launch(what);
 }
 
-}  // namespace attn4
+}  // namespace simple4
 }  // namespace qa
-
-extern "C" int64_t qa_paged_attention_decode_kv4_workspace(int64_t batch, int32_t heads, int32_t kv_heads, int32_t head_dim, int64_t max_tokens) {
-  if (batch <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0 || max_tokens < 0) return 0;
-  return 16;
-}
-
-extern "C" int qa_paged_attention_decode_kv4(const void* query, int32_t q_dtype, int64_t q_stride_b, int64_t q_stride_h, int64_t batch, int32_t heads,
-                                             int32_t head_dim, const qa_paged_kv* kv, const void* block_tables, int32_t table_dtype, int64_t table_stride,
-                                             int64_t max_blocks, const void* sequence_lengths, int32_t lengths_dtype, int32_t block_size, float scale,
-                                             const void* gate, int64_t gate_stride_b, int64_t gate_stride_h, void* output, void* workspace,
-                                             int64_t workspace_bytes, hipStream_t stream) {
-  using namespace qa;
-  using namespace qa::attn4;
-  Params p{};
-  const Args a{"paged_attention_decode_kv4", query, q_dtype, q_stride_b, q_stride_h, batch, heads, head_dim, kv, block_tables, table_dtype, table_stride, max_blocks,
-               lengths_dtype, block_size, scale, gate, gate_stride_b, gate_stride_h, output};
-  if (int rc = fill(p, a)) return rc;
-  if (batch == 0) return 0;
-  QA_REQUIRE(sequence_lengths != nullptr, "sequence_lengths must be a device array");
-  p.lens = sequence_lengths;
-  return launch(p, head_dim, 1, batch * heads, a.what, stream);
-}
 
 extern "C" int qa_paged_attention_prefill_kv4(const void* query, int32_t q_dtype, int64_t q_stride_t, int64_t q_stride_h, int64_t total_new, const void* cu_seqlens,
                                               const void* prefix_lens, int32_t idx_dtype, int64_t batch, int64_t max_new, int32_t heads, int32_t head_dim,
@@ -219,7 +197,7 @@ extern "C" int qa_paged_attention_prefill_kv4(const void* query, int32_t q_dtype
                                               int32_t block_size, float scale, const void* gate, int64_t gate_stride_t, int64_t gate_stride_h, void* output,
                                               hipStream_t stream) {
   using namespace qa;
-  using namespace qa::attn4;
+  using namespace qa::simple4;
   Params p{};
   const Args a{"paged_attention_prefill_kv4", query, q_dtype, q_stride_t, q_stride_h, batch, heads, head_dim, kv, block_tables, table_dtype, table_stride, max_blocks,
                idx_dtype, block_size, scale, gate, gate_stride_t, gate_stride_h, output};
