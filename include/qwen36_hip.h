@@ -324,13 +324,19 @@ int qa_paged_attention_decode_kv4(const void* query, int32_t q_dtype, int64_t q_
 
 /* qa_paged_attention_prefill over a 4-bit pool: total_new rows of query, GQA
  * group up to 16; tokens at or past total_new or max_new of their row are not
- * computed, and output rows past the last sequence are left as they were.     */
+ * computed, and output rows past the last sequence are left as they were.
+ * workspace: 16-byte aligned, qa_paged_attention_prefill_kv4_workspace(..,
+ * max_blocks * block_size) bytes (0 for steps that fill the GPU by themselves;
+ * then it may be NULL): the parts of a split of the keys.                      */
+int64_t qa_paged_attention_prefill_kv4_workspace(int64_t total_new, int64_t batch, int64_t max_new, int32_t heads, int32_t kv_heads,
+                                                 int32_t head_dim, int64_t max_tokens);
 int qa_paged_attention_prefill_kv4(const void* query, int32_t q_dtype, int64_t q_stride_t, int64_t q_stride_h, int64_t total_new,
                                    const void* cu_seqlens, const void* prefix_lens, int32_t idx_dtype, int64_t batch,
                                    int64_t max_new, int32_t heads, int32_t head_dim, const qa_paged_kv* kv,
                                    const void* block_tables, int32_t table_dtype, int64_t table_stride, int64_t max_blocks,
                                    int32_t block_size, float scale, const void* gate, int64_t gate_stride_t,
-                                   int64_t gate_stride_h, void* output, hipStream_t stream);
+                                   int64_t gate_stride_h, void* output, void* workspace, int64_t workspace_bytes,
+                                   hipStream_t stream);
 
 /* qa_qk_norm_rope_append with several position axes, through a slot map, into a
  * bf16 or a 4-bit pool.  positions (axes, tokens), axis a at a*positions_stride;

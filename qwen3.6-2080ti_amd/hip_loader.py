@@ -173,8 +173,9 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
     "qa_paged_attention_prefill_kv4": (
         c_int32,
         [c_void_p, c_int32, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int32, c_int64, c_int64, c_int32, c_int32, ctypes.POINTER(PagedKV), c_void_p, c_int32,
-         c_int64, c_int64, c_int32, c_float, c_void_p, c_int64, c_int64, c_void_p, c_void_p],
+         c_int64, c_int64, c_int32, c_float, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_void_p],
     ),
+    "qa_paged_attention_prefill_kv4_workspace": (c_int64, [c_int64, c_int64, c_int64, c_int32, c_int32, c_int32, c_int64]),
     "qa_qk_norm_mrope_append": (
         c_int32,
         [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int32, c_float, c_void_p, c_void_p, c_int32,

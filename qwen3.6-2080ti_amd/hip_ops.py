@@ -1360,10 +1360,12 @@ def paged_attention_prefill_kv4(
     g = _kv4_gate(gate, tokens, heads, head_dim, device)
     cu, prefix, tables = cu_seqlens.contiguous(), prefix_lens.contiguous(), block_tables.contiguous()
     result = _kv4_out(out, query)
+    nbytes = lib.qa_paged_attention_prefill_kv4_workspace(tokens, batch, int(max_new), heads, desc.kv_heads, head_dim, tables.shape[1] * block_size)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
     code = _launch(
         device, lib.qa_paged_attention_prefill_kv4, _ptr(q), _code(q), q.stride(0), q.stride(1), tokens, _ptr(cu), _ptr(prefix), _code(cu), batch, int(max_new),
         heads, head_dim, ctypes.byref(desc), _ptr(tables), _code(tables), tables.stride(0), tables.shape[1], int(block_size), float(scale or 0.0), _ptr(g),
-        0 if g is None else g.stride(0), 0 if g is None else g.stride(1), _ptr(result),
+        0 if g is None else g.stride(0), 0 if g is None else g.stride(1), _ptr(result), _ptr(ws), nbytes,
     )
     L.check(lib, code, "paged_attention_prefill_kv4")
     return result

@@ -296,3 +296,58 @@ def test_refusals_of_tensors() -> None:
                  (q1, tables, *pools, p.repeat(2), 16), (q1, tables.float(), *pools, p, 16), (q1, tables.cpu(), *pools, p, 16), (q1, tables, pools[0], pools[1][:1], p, 16)):
         with pytest.raises(RuntimeError):
             hip_ops.paged_attention_decode_kv4(*args)
+
+
+@pytest.mark.parametrize("dim,heads", [(256, 16), (128, 6)])
+def test_prefill_keeps_a_nan_to_the_tokens_that_see_it(dim, heads) -> None:
+    gen = torch.Generator().manual_seed(29)
+    new, prefix, block = 150, 70, 16
+    tables, pools = _cache(gen, [new + prefix], 2, dim, block)
+    query = torch.randn(new, heads, dim, generator=gen).to(torch.bfloat16).to(DEV)
+    cu = torch.tensor([0, new], device=DEV)
+    run = lambda: hip_ops.paged_attention_prefill_kv4(query, cu, torch.tensor([prefix], device=DEV), *pools, tables, block, max_new=new)  # noqa: E731
+    want = run()
+    group = heads // 2
+    one = torch.ones(1, 2, dim, dtype=torch.bfloat16, device=DEV)
+    for at in (219, 195, 130, 70, 30):
+        saved = [p.clone() for p in pools]
+        k, v = (x[:, :, at].clone() for x in hip_ops.paged_kv4_gather(*pools, tables, new + prefix, block))
+        v[0, 1, 40] = float("nan")
+        hip_ops.paged_kv4_append(k, v, *pools, (tables[0, at // block].long() * block + at % block).reshape(1), block)
+        got = run()
+        first = max(at - prefix, 0)
+        assert torch.equal(got[:first], want[:first])
+        assert torch.equal(got[:, :group], want[:, :group])  # the other KV head
+        assert got[first:, group:, 32:64].isnan().all()
+        assert torch.equal(got[first:, group:, :32], want[first:, group:, :32]) and torch.equal(got[first:, group:, 64:], want[first:, group:, 64:])
+        for p, q in zip(pools, saved):
+            p.copy_(q)
+        k[0, 1, 3] = float("inf")  # a key: every dim of the tokens that see it
+        hip_ops.paged_kv4_append(k, one * 0, *pools, (tables[0, at // block].long() * block + at % block).reshape(1), block)
+        got = run()
+        assert torch.equal(got[:first], want[:first]) and got[first:, group:].isnan().all() and torch.isfinite(got[:, :group]).all()
+        for p, q in zip(pools, saved):
+            p.copy_(q)
+
+
+def test_captured_prefill_replays_as_eager_runs() -> None:
+    query, cu, tables, pools, _, gate = _check_prefill(30, [30, 9], [400, 60], 16, 2, 256, 16)
+    prefix = torch.tensor([400, 60], dtype=torch.int32, device=DEV)
+    call = lambda: hip_ops.paged_attention_prefill_kv4(query, cu, prefix, *pools, tables, 16, max_new=30, gate=gate)  # noqa: E731
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for _ in range(4):
+        query.mul_(-1.01)
+        prefix.sub_(torch.tensor([7, 1], device=DEV, dtype=torch.int32))
+        want = call()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("new,prefix,heads,kv_heads,dim", [([7], [9000], 16, 2, 256), ([40, 3], [3000, 20_000], 8, 2, 128), ([1, 0, 5], [0, 50, 12_000], 16, 1, 256)])
+def test_prefill_of_few_tokens_splits_the_keys(new, prefix, heads, kv_heads, dim) -> None:
+    _check_prefill(sum(new) + dim, new, prefix, heads, kv_heads, dim, 32, gated=True, holes=dim == 128)

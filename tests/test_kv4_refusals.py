@@ -55,7 +55,7 @@ def test_every_entry_refuses_a_bad_pool(changes, message) -> None:
                                              1 << 30, P(0)) == 1
     assert message in L.last_error(lib)
     assert lib.qa_paged_attention_prefill_kv4(SOME, L.QA_BF16, 4096, 256, 3, SOME, SOME, L.QA_I32, 1, 3, 16, 256, ctypes.byref(desc), SOME, L.QA_I32, 4, 4, 16, 0.0, P(0), 0, 0,
-                                              SOME, P(0)) == 1
+                                              SOME, SOME, 1 << 30, P(0)) == 1
     assert message in L.last_error(lib)
 
 
@@ -99,14 +99,16 @@ def test_decode_refuses(changes, message) -> None:
     assert message in L.last_error(lib)
 
 
-@pytest.mark.parametrize("changes,message", BAD_ATTENTION + [(dict(cu=P(0)), "non-null"), (dict(total=-1), "out of range"), (dict(max_new=-1), "out of range")])
+@pytest.mark.parametrize("changes,message", BAD_ATTENTION + [(dict(cu=P(0)), "non-null"), (dict(total=-1), "out of range"), (dict(max_new=-1), "out of range"),
+                                                             (dict(width=4000, wsb=4), "workspace too small")])
 def test_prefill_refuses(changes, message) -> None:
     lib = _lib()
     a = dict(q=SOME, dtype=L.QA_BF16, qb=4096, qh=256, total=3, cu=SOME, prefix=SOME, batch=1, max_new=3, heads=16, dim=256, tables=SOME, tdtype=L.QA_I32, stride=4, width=4,
              block=16, gate=P(0), gb=0, out=SOME)
     a.update(changes)
     assert lib.qa_paged_attention_prefill_kv4(a["q"], a["dtype"], a["qb"], a["qh"], a["total"], a["cu"], a["prefix"], L.QA_I32, a["batch"], a["max_new"], a["heads"], a["dim"],
-                                              ctypes.byref(_desc()), a["tables"], a["tdtype"], a["stride"], a["width"], a["block"], 0.0, a["gate"], a["gb"], 0, a["out"], P(0)) == 1
+                                              ctypes.byref(_desc()), a["tables"], a["tdtype"], a["stride"], a["width"], a["block"], 0.0, a["gate"], a["gb"], 0, a["out"],
+                                              SOME, a.get("wsb", 1 << 30), P(0)) == 1
     assert message in L.last_error(lib)
 
 
