@@ -63,12 +63,17 @@ __device__ __forceinline__ int64_t uniform64(int64_t v) {
   return static_cast<int64_t>((static_cast<uint64_t>(hi) << 32) | lo);
 }
 
-// Physical block of a run of 16 tokens of row b, -1 where there is none.  Wave-uniform.
+// Physical block of a run of 16 tokens of row b, -1 where there is none.  Wave-uniform and without a branch (scalar
+// loads under branches are waited for at each join): a run past the row reads a clamped entry, and an entry of either
+// width is read as words.
 __device__ __forceinline__ int32_t block_of_run(const Params& p, int64_t b, int64_t run, int64_t runs) {
+  typedef const __attribute__((address_space(4))) int32_t c32;
   const int64_t lb = run >> (p.bs_shift - 4);
-  if (run >= runs || lb >= p.max_blocks) return -1;
-  const int64_t e = read_index(p.tables, p.table_i64, b * p.table_stride + lb);
-  return e >= 0 && e < p.num_blocks ? static_cast<int32_t>(e) : -1;
+  const int64_t at = (b * p.table_stride + max64(0, min64(lb, p.max_blocks - 1))) << p.table_i64;
+  const int32_t lo = ((c32*)p.tables)[at];
+  const int32_t hi = ((c32*)p.tables)[at + p.table_i64];  // the entry itself where it has one word
+  const bool ok = (run < runs) & (lb < p.max_blocks) & (static_cast<uint32_t>(lo) < static_cast<uint32_t>(p.num_blocks)) & ((hi == 0) | (p.table_i64 == 0));
+  return ok ? lo : -1;
 }
 
 // Buffer resource over one run; a skipped one has no records, so that its loads read zeros, touch no memory, and every
@@ -247,7 +252,10 @@ __device__ __forceinline__ float column_sum(float v) {
 }
 
 // o / l: zeros where a query saw nothing; a NaN stays one.
-__device__ __forceinline__ float normalised(float o, float l) { return l > 0.f ? o / l : l == 0.f ? 0.f : l; }
+__device__ __forceinline__ float normalised(float o, float l) {
+  const float r = o * (1.f / l);
+  return l == 0.f ? 0.f : r;
+}
 
 __device__ __forceinline__ float sigmoid(float x) { return 1.f / (1.f + __expf(-x)); }
 

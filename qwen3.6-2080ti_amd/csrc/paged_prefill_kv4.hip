@@ -1,19 +1,26 @@
 // Chunked causal prefill attention over the 4-bit paged KV cache (attention_kv4.h, kv4.h), gfx950.
 //
 // Columns of the products are (new position, query head of the KV head's group), position-major, so any group size
-// fills them.  A workgroup owns kCols of one row and KV head, a wave 16 NCT of them, and walks the keys in tiles of 64.
-// Keys go from memory straight into each wave's registers as the scores' A operand, one tile ahead (1/4 of a bf16
-// tile's bytes, so the waves' repeated reads are cheap).  Values are unpacked once a workgroup: every wave turns its
-// share of the next tile into bf16 operand fragments in LDS, [unit of 32 keys][dims][lane][16 bytes], which all waves
-// read back without bank conflicts.  One barrier a tile.
+// fills them.  A workgroup owns 128 of one row and KV head and walks the keys in tiles of 64.  Its eight waves are four
+// pairs of 32 columns.  A wave takes the scores and the softmax of 16 of them, then the products with the values of all
+// 32 for half of the dims, with its partner's probabilities through LDS: so that each operand of values read from LDS
+// feeds two products (with 16 columns and all dims a wave, LDS would be as busy as the matrix units), and the
+// accumulators of a wave stay at 64 registers, two waves to a SIMD (with 32 columns and all dims in one wave a SIMD,
+// accumulators and query took 512 registers, 300 moves a tile between the two halves of the file: 1571 us where this
+// form takes 966, 2048 tokens behind 32000).
 //
-// Iteration t: the scores of tile t + 1 (matrix unit) next to the softmax of tile t (vector unit), then the products of
-// tile t's values next to the unpacking of tile t + 1's.
+// Keys go from memory into LDS as they are, one tile ahead, one 1 KB copy a wave (with each wave loading them into its
+// registers the vector memory path was busy longer than the matrix units: 1328 us).  Values are unpacked once a workgroup: waves 0 to 3, one a
+// SIMD, turn a run of the next tile each into bf16 operand fragments in LDS, [unit of 32 keys][dim tile][run][lane][8
+// bytes], read back without bank conflicts.
+//
+// Iteration t, one barrier: scores and softmax of tile t + 1, products of tile t's values, unpacking of tile t + 1's.
 //
 // With few columns the keys are split over gridDim.z and a second launch joins the parts.
 #include "attention_kv4.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace qa {
 namespace prefill4 {
@@ -29,36 +36,56 @@ struct PrefillParams {
 
 constexpr int kTile = 64;      // keys
 constexpr int kRuns = kTile / kv4::kRun;
-constexpr int kWaves = 4;
-constexpr int kColTiles = 2;   // 16-column tiles of a wave
-constexpr int kCols = kWaves * kColTiles * 16;
+constexpr int kWaves = 8;
+constexpr int kCols = kWaves * 16;
 constexpr int kRankRows = 64;  // batches up to this many rows start with the longest row
 
 template <int D>
 struct Smem {
   static constexpr int kTileBytes = kTile * D * 2;
-  static constexpr int kBytes = 2 * kTileBytes + 16;  // two tiles of values; for each, the last tile that had a NaN group
+  static constexpr int kP = 2 * kTileBytes;                    // probabilities: [buffer][wave][unit][lane][16 bytes]
+  static constexpr int kCorr = kP + 2 * kWaves * 2 * 1024;     // [buffer][wave][16] floats
+  static constexpr int kFlag = kCorr + 2 * kWaves * 16 * 4;    // [buffer]: the last tile that had a NaN group
+  static constexpr int kKeys = kFlag + 16;                     // [buffer][run]: codes; then [buffer][run]: scales
+  static constexpr int kRunCodes = kv4::Run<D>::kCodes;
+  static constexpr int kRunScales = kv4::Run<D>::kBytes - kRunCodes;
+  static constexpr int kScales = kKeys + 2 * kRuns * kRunCodes;
+  static constexpr int kBytes = kScales + 2 * kRuns * kRunScales;
 };
 
-template <int N>
-__device__ __forceinline__ uint32_t load_bytes(__amdgpu_buffer_rsrc_t r, int off) {
-  if constexpr (N == 4)
-    return __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0);
-  else
-    return __builtin_amdgcn_raw_buffer_load_b16(r, off, 0, 0);
+// Four bytes per lane from memory to LDS bytes lds + 4 l, as lds_copy16.
+__device__ __forceinline__ void lds_copy4(const void* src, uint32_t lds) {
+  uint32_t saved;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\t"
+      "s_mov_b32 m0, %1\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dword %2, off\n\t"
+      "s_mov_b32 m0, %0"
+      : "=&s"(saved)
+      : "s"(lds), "v"(src)
+      : "memory");
 }
 
+// Every vector memory operation of the wave has completed, the copies to LDS among them (which the compiler does not count).
+__device__ __forceinline__ void wait_vm0() { __builtin_amdgcn_s_waitcnt(0x0F70); }
+
+// The products stay where they are written: the compiler would move them to where their sums are used.
+__device__ __forceinline__ void keep(floatx4_v (&s)[kRuns]) { asm volatile("" : "+v"(s[0]), "+v"(s[1]), "+v"(s[2]), "+v"(s[3])); }
+
 template <int D>
-__global__ __launch_bounds__(64 * kWaves, 1) void prefill_kernel(PrefillParams pp) {
+__global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams pp) {
   const Params& p = pp.c;
   constexpr int MT = D / 16;
-  constexpr int HB = D / 64;        // bytes of a token's value chunk that a wave unpacks: half of the chunk
-  constexpr int NCT = kColTiles;
+  constexpr int MH = MT / 2;        // dim tiles of a wave
+  using S = Smem<D>;
   extern __shared__ __align__(16) unsigned char smem[];
-  int* s_flag = reinterpret_cast<int*>(smem + 2 * Smem<D>::kTileBytes);
+  float* s_corr = reinterpret_cast<float*>(smem + S::kCorr);
+  int* s_flag = reinterpret_cast<int*>(smem + S::kFlag);
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int half = wave & 1;
   const int col = lane & 15;
   const int quad = lane >> 4;
 
@@ -102,255 +129,365 @@ __global__ __launch_bounds__(64 * kWaves, 1) void prefill_kernel(PrefillParams p
   const uint8_t* kb = p.kpool + g * p.sG;
   const uint8_t* vb = p.vpool + g * p.sG;
 
-  int64_t pos[NCT], tok[NCT];
-  int head[NCT];
-  bool live[NCT];
+  // columns: [0] the wave's own 16, [1] its partner's; their position past first_pos
+  const int n_cols = static_cast<int>(last - x0) + 1;
+  const int x_head = static_cast<int>(x0 % p.G);  // head of the workgroup's first column
+  int ahead[2];
 #pragma unroll
-  for (int c = 0; c < NCT; ++c) {
-    const int64_t x = x0 + (wave * NCT + c) * 16 + col;
-    live[c] = x <= last;
-    const int64_t n = (live[c] ? x : last) / p.G;
-    head[c] = static_cast<int>((live[c] ? x : last) - n * p.G) + g * p.G;
-    pos[c] = prefix + n;
-    tok[c] = tok0 + n;
-  }
+  for (int c = 0; c < 2; ++c) ahead[c] = (min((wave ^ c) * 16 + col, n_cols - 1) + x_head) / p.G;
 
   // ---- the tiles' loads
-  KeyRun<D> kr[kRuns];
-  uint32_t vcode[2][4], vscale[2];  // this wave's share: unit wave / 2, half (wave & 1) of each chunk
-  const int vunit = wave >> 1, vhalf = wave & 1;
-  int32_t phys[kRuns];
-  auto entries = [&](int64_t kt) {
-#pragma unroll
-    for (int j = 0; j < kRuns; ++j) phys[j] = kt < kt1 ? block_of_run(p, b, kRuns * kt + j, runs) : -1;
+  // Lane l of `cur` holds the offset in the head's pool of run 64 c + l (-1: not there), of `nxt` that of the next 64:
+  // one vector load each 16 tiles (scalar loads of the table share their wait counter with LDS, and every tile stalled
+  // about 1000 cycles for them).
+  int64_t cur, nxt;
+  auto chunk = [&](int64_t c) -> int64_t {
+    const int64_t run = 64 * c + lane;
+    const int64_t lb = run >> (p.bs_shift - 4);
+    const int64_t at = (b * p.table_stride + min64(lb, p.max_blocks - 1)) << p.table_i64;
+    const int32_t lo = reinterpret_cast<const int32_t*>(p.tables)[at];
+    const int32_t hi = reinterpret_cast<const int32_t*>(p.tables)[at + p.table_i64];  // the entry itself where it has one word
+    const bool ok = (run < runs) & (static_cast<uint32_t>(lo) < static_cast<uint32_t>(p.num_blocks)) & ((hi == 0) | (p.table_i64 == 0));
+    const int64_t o = static_cast<int64_t>(ok ? lo : 0) * p.sP + (run & ((1 << (p.bs_shift - 4)) - 1)) * kv4::Run<D>::kBytes;
+    return ok ? o : -1;
   };
-  auto there = [&]() { return (phys[0] >= 0 ? 1 : 0) | (phys[1] >= 0 ? 2 : 0) | (phys[2] >= 0 ? 4 : 0) | (phys[3] >= 0 ? 8 : 0); };
-  auto fetch_keys = [&](int64_t kt) {
+  int64_t off[kRuns];  // of the runs of a tile
+  auto offsets = [&](int64_t kt) {
+    const int at = static_cast<int>(kt & 15) * kRuns;
+    if (at == 0 && kt != kt0) {
+      cur = nxt;
+      nxt = chunk((kt >> 4) + 1);
+    }
 #pragma unroll
-    for (int j = 0; j < kRuns; ++j) load_keys<D>(kr[j], run_rsrc<D>(p, kb, phys[j], kRuns * kt + j), lane);
-  };
-  auto fetch_values = [&](int64_t kt) {
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int32_t ph = vunit == 0 ? phys[j] : phys[2 + j];
-      const __amdgpu_buffer_rsrc_t r = run_rsrc<D>(p, vb, ph, kRuns * kt + 2 * vunit + j);
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const int off = D == 256 ? 1024 * (t >> 1) + 16 * lane + 8 * (t & 1) + HB * vhalf : 16 * lane + 4 * t + HB * vhalf;
-        vcode[j][t] = load_bytes<HB>(r, off);
-      }
-      vscale[j] = __builtin_amdgcn_raw_buffer_load_b32(r, kv4::Run<D>::kCodes + 16 * (col / (512 / D)) + 4 * quad, 0, 0);
+    for (int j = 0; j < kRuns; ++j) {
+      const uint32_t lo = __builtin_amdgcn_readlane(static_cast<uint32_t>(cur), at + j);
+      const uint32_t hi = __builtin_amdgcn_readlane(static_cast<uint32_t>(cur >> 32), at + j);
+      off[j] = static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
     }
   };
-  // unpacks the share of tile kt that is in vcode / vscale into buffer buf
-  auto unpack = [&](int64_t kt, int buf) {
-    if (kt * kTile + kTile > first_pos + 1) {  // some column does not see all of the tile
+  auto there = [&]() { return (off[0] >= 0 ? 1 : 0) | (off[1] >= 0 ? 2 : 0) | (off[2] >= 0 ? 4 : 0) | (off[3] >= 0 ? 8 : 0); };
+  // run `wave % 4` of the tile whose offsets are in off: waves 0 to 3 unpack its values, waves 4 to 7 copy its key scales
+  auto own_run = [&]() -> int64_t {
+    int64_t r = 0;  // with masks: a choice between the elements would put the array into memory
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        // keys that no column sees may hold anything, and 0 times a NaN is one
-        const int64_t left = kv_end - kt * kTile - kv4::kRun * (2 * vunit + j) - 4 * quad;
-        vscale[j] &= left >= 4 ? 0xffffffffu : left <= 0 ? 0u : (1u << (8 * static_cast<int>(left))) - 1u;
-        // a NaN group reaches only the columns that see its token: out of the product, and nan_groups adds it
-        uint32_t drop = 0;
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-          if ((vscale[j] >> (8 * t) & 255u) == 255u) drop |= 255u << (8 * t);
-        vscale[j] &= ~drop;
-        if (drop != 0) s_flag[buf] = static_cast<int>(kt - kt0) + 1;
-      }
-    }
-    float s[8];
-#pragma unroll
-    for (int t = 0; t < 8; ++t) s[t] = value_scale(vscale[t >> 2], t & 3);
-    uint4* dst = reinterpret_cast<uint4*>(smem + buf * Smem<D>::kTileBytes) + (vunit * MT + 2 * HB * vhalf) * 64 + lane;
-#pragma unroll
-    for (int e = 0; e < HB; ++e) {
-      uint32_t pair[8];
-#pragma unroll
-      for (int t = 0; t < 8; ++t) {
-        const uint32_t c = vcode[t >> 2][t & 3];
-        switch (e) {
-          case 0: pair[t] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s[t], 0)); break;
-          case 1: pair[t] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s[t], 1)); break;
-          case 2: pair[t] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s[t], 2)); break;
-          default: pair[t] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s[t], 3)); break;
-        }
-      }
-      uint4 even, odd;
-      even.x = __builtin_amdgcn_perm(pair[1], pair[0], 0x05040100u);
-      even.y = __builtin_amdgcn_perm(pair[3], pair[2], 0x05040100u);
-      even.z = __builtin_amdgcn_perm(pair[5], pair[4], 0x05040100u);
-      even.w = __builtin_amdgcn_perm(pair[7], pair[6], 0x05040100u);
-      odd.x = __builtin_amdgcn_perm(pair[1], pair[0], 0x07060302u);
-      odd.y = __builtin_amdgcn_perm(pair[3], pair[2], 0x07060302u);
-      odd.z = __builtin_amdgcn_perm(pair[5], pair[4], 0x07060302u);
-      odd.w = __builtin_amdgcn_perm(pair[7], pair[6], 0x07060302u);
-      dst[(2 * e) * 64] = even;
-      dst[(2 * e + 1) * 64] = odd;
-    }
+    for (int j = 0; j < kRuns; ++j) r |= off[j] & -static_cast<int64_t>(j == (wave & 3));
+    return r;
   };
+  const uint32_t smem_lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(smem));
+  // Copies the keys of the tile whose offsets are in off to buffer buf, a wave 1 KB of codes, the waves that do not
+  // unpack a run's scales too.  Of runs that are not there nothing is read; what the buffer held gives scores that are
+  // masked.
+  auto copy_keys = [&](int buf) {
+    constexpr int PER = D / 128;  // copies of a run
+    const int64_t o = own_run();
+    if (o < 0) return;
+    const uint8_t* src = kb + o;
+    if (PER == 2 || wave < 4) {
+      const int part = PER == 2 ? wave >> 2 : 0;
+      lds_copy16(src + 1024 * part + 16 * lane, smem_lds + S::kKeys + (buf * kRuns + (wave & 3)) * S::kRunCodes + 1024 * part);
+    }
+    if (wave >= 4 && lane < S::kRunScales / 4) lds_copy4(src + S::kRunCodes + 4 * lane, smem_lds + S::kScales + (buf * kRuns + (wave & 3)) * S::kRunScales);
+  };
+  const bool unpacks = wave < 4;
+  ValueRun<D> vr;
+  auto fetch_values = [&]() {
+    const int64_t o = own_run();
+    load_values<D>(vr, __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(vb + (o < 0 ? 0 : o)), 0, o < 0 ? 0 : kv4::Run<D>::kBytes, 0x00020000), lane);
+  };
+  // what of vr no column sees, or not every column where it is NaN, leaves the product
+  auto trim = [&](int64_t kt, int buf) {
+    if (kt * kTile + kTile <= first_pos + 1) return;  // every column sees all of the tile
+    // keys that no column sees may hold anything, and 0 times a NaN is one
+    const int64_t left = kv_end - kt * kTile - kv4::kRun * wave - 4 * quad;
+    vr.scale &= left >= 4 ? 0xffffffffu : left <= 0 ? 0u : (1u << (8 * static_cast<int>(left))) - 1u;
+    // a NaN group reaches only the columns that see its token: marked for them below
+    uint32_t drop = 0;
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+      if ((vr.scale >> (8 * t) & 255u) == 255u) drop |= 255u << (8 * t);
+    vr.scale &= ~drop;
+    if (drop != 0) s_flag[buf] = static_cast<int>(kt - kt0) + 1;
+  };
+  // Byte e of the lane's chunk of vr's four tokens: dims 2 e and 2 e + 1, converted and written to buffer buf.  A
+  // fragment is two planes of 512 bytes, one a run, so that neither the writes nor the reads conflict on banks.
+  float vs[4];
+  auto unpack_byte = [&](int e, int buf) {
+    uint32_t pair[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      if (e == 0) vs[t] = value_scale(vr.scale, t);
+      const int at = t * (D / 128) + (e >> 2);  // dword of the lane's chunk of token t
+      const uint4& c = vr.code[at >> 2];
+      const uint32_t w = (at & 3) == 0 ? c.x : (at & 3) == 1 ? c.y : (at & 3) == 2 ? c.z : c.w;
+      switch (e & 3) {
+        case 0: pair[t] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, vs[t], 0)); break;
+        case 1: pair[t] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, vs[t], 1)); break;
+        case 2: pair[t] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, vs[t], 2)); break;
+        default: pair[t] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, vs[t], 3)); break;
+      }
+    }
+    uint2* dst = reinterpret_cast<uint2*>(smem + buf * S::kTileBytes) + ((wave >> 1) * MT + 2 * e) * 128 + 64 * (wave & 1) + lane;
+    dst[0] = make_uint2(__builtin_amdgcn_perm(pair[1], pair[0], 0x05040100u), __builtin_amdgcn_perm(pair[3], pair[2], 0x05040100u));
+    dst[128] = make_uint2(__builtin_amdgcn_perm(pair[1], pair[0], 0x07060302u), __builtin_amdgcn_perm(pair[3], pair[2], 0x07060302u));
+  };
+  constexpr int kBytesOfChunk = D / 32;
 
-  float m_run[NCT], l_run[NCT];
-  floatx4_v o[NCT][MT];
+  float m_run = -INFINITY, l_run = 0.f;  // of the own column
+  floatx4_v o[2][MH];
 #pragma unroll
-  for (int c = 0; c < NCT; ++c) {
-    m_run[c] = -INFINITY;
-    l_run[c] = 0.f;
+  for (int c = 0; c < 2; ++c)
 #pragma unroll
-    for (int i = 0; i < MT; ++i) o[c][i] = floatx4_v{0.f, 0.f, 0.f, 0.f};
-  }
+    for (int i = 0; i < MH; ++i) o[c][i] = floatx4_v{0.f, 0.f, 0.f, 0.f};
+  uint32_t nan_rows = 0;  // bit 4 c + r: column c saw a NaN group at the dims of accumulator row r
 
   if (kt0 < kt1) {
     if (tid < 2) s_flag[tid] = 0;
-    entries(kt0);
+    cur = chunk(kt0 >> 4);
+    nxt = chunk((kt0 >> 4) + 1);
+    offsets(kt0);
     int there_cur = there();
-    fetch_keys(kt0);
-    fetch_values(kt0);
-    QueryCols<D> qh[NCT], ql[NCT];
-#pragma unroll
-    for (int c = 0; c < NCT; ++c) {
+    copy_keys(0);
+    if (unpacks) fetch_values();
+    QueryCols<D> qh, ql;
+    {
       QueryRow<D> row;
-      row.load(live[c] ? p.q + tok[c] * p.q_st + static_cast<int64_t>(head[c]) * p.q_sh : nullptr, quad);
-      row.template split<false>(qh[c]);
-      row.template split<true>(ql[c]);
+      const int x = wave * 16 + col;
+      const int64_t tok = tok0 + (x0 + x) / p.G;
+      const int64_t head = (x0 + x) % p.G + g * p.G;
+      row.load(x < n_cols ? p.q + tok * p.q_st + head * p.q_sh : nullptr, quad);
+      row.template split<false>(qh);
+      row.template split<true>(ql);
     }
-    floatx4_v sc[NCT][kRuns];
-    auto scores = [&]() {
-#pragma unroll
-      for (int c = 0; c < NCT; ++c)
-#pragma unroll
-        for (int j = 0; j < kRuns; ++j) sc[c][j] = floatx4_v{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int j = 0; j < kRuns; ++j) {
-#pragma unroll
-        for (int c = 0; c < NCT; ++c) sc[c][j] = score<D>(kr[j], qh[c], sc[c][j]);
-#pragma unroll
-        for (int c = 0; c < NCT; ++c) sc[c][j] = score<D>(kr[j], ql[c], sc[c][j]);
+    const float qk_scale = p.scale * kLog2e;
+    floatx4_v sc[kRuns];
+    float use = 0.f;
+    bf16x8_v pb[2];  // the own probabilities of the two units
+    // The scores: operand f of a tile is slice f / kRuns of run f % kRuns and feeds the products of both pieces; runs
+    // innermost, so that products of one accumulator are eight apart.
+    constexpr int kOperands = kRuns * (D / 128);
+    auto kread = [&](int f, int buf) {
+      const int j = f % kRuns, i = f / kRuns;
+      const uint4 u = *reinterpret_cast<const uint4*>(smem + S::kKeys + (buf * kRuns + j) * S::kRunCodes + 1024 * i + 16 * lane);
+      return int8_v{static_cast<int>(u.x), static_cast<int>(u.y), static_cast<int>(u.z), static_cast<int>(u.w), 0, 0, 0, 0};
+    };
+    auto sread = [&](int j, int buf) {
+      const unsigned char* at = smem + S::kScales + (buf * kRuns + j) * S::kRunScales + lane * (D / 128);
+      return D == 256 ? static_cast<int>(*reinterpret_cast<const uint16_t*>(at)) : static_cast<int>(*at);
+    };
+    auto products = [&](int f, const int8_v& a, int scale) {
+      const int j = f % kRuns, i = f / kRuns;
+      const floatx4_v acc = i == 0 ? floatx4_v{0.f, 0.f, 0.f, 0.f} : sc[j];
+      if (i == 0) {
+        sc[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, qh.code[0], acc, 4, 0, 0, scale, 0, static_cast<int>(qh.scale));
+        sc[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, ql.code[0], sc[j], 4, 0, 0, scale, 0, static_cast<int>(ql.scale));
+      } else {
+        sc[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, qh.code[D / 128 - 1], acc, 4, 0, 1, scale, 0, static_cast<int>(qh.scale));
+        sc[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, ql.code[D / 128 - 1], sc[j], 4, 0, 1, scale, 0, static_cast<int>(ql.scale));
       }
     };
-    scores();
-    __syncthreads();  // the flags
-    unpack(kt0, 0);
-    entries(kt0 + 1);
-    int there_next = there();
-    fetch_keys(kt0 + 1);
-    fetch_values(kt0 + 1);
-    __syncthreads();
-
-    const float qk_scale = p.scale * kLog2e;
-    for (int64_t kt = kt0; kt < kt1; ++kt) {
-      const int buf = static_cast<int>((kt - kt0) & 1);
-      const int64_t key0 = kt * kTile;
-      // ---- mask
-      if (!(key0 + kTile <= first_pos + 1 && there_cur == 15)) {
+    static_assert(kOperands == kBytesOfChunk, "a byte of the chunk goes with each operand");
+    constexpr int kAheadK = 2;
+    auto scores = [&](int buf, auto slice) {
+      int scale[kRuns];
 #pragma unroll
-        for (int c = 0; c < NCT; ++c) {
-          const int lim = static_cast<int>(max64(-1, min64(kTile - 1, min64(pos[c], kv_end - 1) - key0)));  // the last key the column sees
+      for (int j = 0; j < kRuns; ++j) scale[j] = sread(j, buf);
+      int8_v ka[kAheadK];
 #pragma unroll
-          for (int j = 0; j < kRuns; ++j)
+      for (int f = 0; f < kAheadK; ++f) ka[f] = kread(f, buf);
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (16 * j + 4 * quad + r > lim || !(there_cur >> j & 1)) sc[c][j][r] = -INFINITY;
-        }
+      for (int f = 0; f < kOperands; ++f) {
+        const int8_v a = ka[f % kAheadK];
+        if (f + kAheadK < kOperands) ka[f % kAheadK] = kread(f + kAheadK, buf);
+        products(f, a, scale[f % kRuns]);
+        slice(f);
+        __builtin_amdgcn_sched_barrier(0);
       }
-      // ---- softmax of tile kt
-      bf16x8_v pb[NCT][2];
-#pragma unroll
-      for (int c = 0; c < NCT; ++c) {
-        float mx = -INFINITY;
-#pragma unroll
-        for (int j = 0; j < kRuns; ++j) mx = fmaxf(mx, fmaxf(fmaxf(sc[c][j][0], sc[c][j][1]), fmaxf(sc[c][j][2], sc[c][j][3])));
-        mx *= qk_scale;
-        if (__ballot(mx > m_run[c] + kLazy) != 0) {
-          const float m_new = fmaxf(m_run[c], column_max(mx));
-          const float corr = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run[c] - m_new);
-          m_run[c] = m_new;
-          l_run[c] *= corr;
-#pragma unroll
-          for (int i = 0; i < MT; ++i) o[c][i] *= corr;
-        }
-        const float use = m_run[c] == -INFINITY ? 0.f : m_run[c];
+      keep(sc);
+    };
+    // masks the scores of tile kt and moves the own column's reference point where they ask for it
+    auto reference = [&](int64_t kt, int have, int buf) {
+      const int64_t key0 = kt * kTile;
+      if (!(key0 + kTile <= first_pos + 1 && have == 15)) {
+        const int lim = static_cast<int>(max64(-1, min64(kTile - 1, min64(first_pos + ahead[0], kv_end - 1) - key0)));  // the last key the column sees
 #pragma unroll
         for (int j = 0; j < kRuns; ++j)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[c][j][r], qk_scale, -use));
-            l_run[c] += pr;
-            pb[c][j >> 1][4 * (j & 1) + r] = static_cast<__bf16>(pr);
-          }
+          for (int r = 0; r < 4; ++r)
+            if (16 * j + 4 * quad + r > lim || !(have >> j & 1)) sc[j][r] = -INFINITY;
       }
-      // ---- scores of tile kt + 1, keys of kt + 2
-      scores();
-      entries(kt + 2);
-      fetch_keys(kt + 2);
-      // ---- values of tile kt
-      const uint4* vt = reinterpret_cast<const uint4*>(smem + buf * Smem<D>::kTileBytes) + lane;
+      float mx = -INFINITY;
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int j = 0; j < kRuns; ++j) mx = fmaxf(mx, fmaxf(fmaxf(sc[j][0], sc[j][1]), fmaxf(sc[j][2], sc[j][3])));
+      mx *= qk_scale;
+      float corr = 1.f;
+      if (__ballot(mx > m_run + kLazy) != 0) {
+        const float m_new = fmaxf(m_run, column_max(mx));
+        corr = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run - m_new);
+        m_run = m_new;
+        l_run *= corr;
+        use = m_run == -INFINITY ? 0.f : m_run;
+      }
+      if (quad == 0) s_corr[(buf * kWaves + wave) * 16 + col] = corr;
+    };
+    // the probability of score k of the lane's 16
+    auto prob = [&](int k) {
+      const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[k >> 2][k & 3], qk_scale, -use));
+      l_run += pr;
+      pb[k >> 3][k & 7] = static_cast<__bf16>(pr);
+    };
+    auto publish = [&](int buf) {
+      uint4* dst = reinterpret_cast<uint4*>(smem + S::kP) + (buf * kWaves + wave) * 128 + lane;
+      dst[0] = __builtin_bit_cast(uint4, pb[0]);
+      dst[64] = __builtin_bit_cast(uint4, pb[1]);
+    };
+    wait_vm0();
+    __syncthreads();  // the flags and the first tile's keys
+    scores(0, [](int) {});
+    reference(kt0, there_cur, 0);
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          const bf16x8_v a = __builtin_bit_cast(bf16x8_v, vt[(u * MT + i) * 64]);
+    for (int k = 0; k < 16; ++k) prob(k);
+    publish(0);
+    if (unpacks) {
+      trim(kt0, 0);
 #pragma unroll
-          for (int c = 0; c < NCT; ++c) o[c][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, pb[c][u], o[c][i], 0, 0, 0);
+      for (int e = 0; e < kBytesOfChunk; ++e) unpack_byte(e, 0);
+    }
+    offsets(kt0 + 1);
+    int there_next = there();
+    copy_keys(1);
+    if (unpacks) fetch_values();
+    wait_vm0();
+    __syncthreads();
+
+    // Iteration kt.  The products are laid between slices of the vector work that does not depend on them, with fences
+    // that keep the order: the scores of tile kt + 1 with its unpacking, the values of tile kt with the exponentials.
+    auto iterate = [&](int64_t kt, auto unpacking, auto more) {
+      const int buf = static_cast<int>((kt - kt0) & 1);
+      if constexpr (more) {
+        if constexpr (unpacking) trim(kt + 1, buf ^ 1);
+        scores(buf ^ 1, [&](int f) {
+          if constexpr (unpacking) {
+            unpack_byte(f, buf ^ 1);
+          }
+        });
+        offsets(kt + 2);
+        copy_keys(buf);
+        if constexpr (unpacking) fetch_values();
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      bf16x8_v pv[2][2];
+      pv[0][0] = pb[0];
+      pv[0][1] = pb[1];
+      const uint4* src = reinterpret_cast<const uint4*>(smem + S::kP) + (buf * kWaves + (wave ^ 1)) * 128 + lane;
+      pv[1][0] = __builtin_bit_cast(bf16x8_v, src[0]);
+      pv[1][1] = __builtin_bit_cast(bf16x8_v, src[64]);
+      const int flag = s_flag[buf];
+      const float c0 = s_corr[(buf * kWaves + wave) * 16 + col], c1 = s_corr[(buf * kWaves + (wave ^ 1)) * 16 + col];
+      if (__ballot(c0 != 1.f || c1 != 1.f) != 0) {  // columns whose reference point moved at this tile
+#pragma unroll
+        for (int i = 0; i < MH; ++i) {
+          o[0][i] *= c0;
+          o[1][i] *= c1;
         }
+      }
+      if constexpr (more) reference(kt + 1, there_next, buf ^ 1);
+      // ---- values of this tile, exponentials of the next
+      const uint2* vt = reinterpret_cast<const uint2*>(smem + buf * S::kTileBytes) + half * MH * 128 + lane;
+      constexpr int kAhead = 4;
+      auto vread = [&](int f) {
+        const uint2 a = vt[(f / MH * MT + f % MH) * 128], c = vt[(f / MH * MT + f % MH) * 128 + 64];
+        return __builtin_bit_cast(bf16x8_v, make_uint4(a.x, a.y, c.x, c.y));
+      };
+      bf16x8_v va[kAhead];
+#pragma unroll
+      for (int f = 0; f < kAhead; ++f) va[f] = vread(f);
+#pragma unroll
+      for (int f = 0; f < 2 * MH; ++f) {
+        const bf16x8_v a = va[f % kAhead];
+        const int u = f / MH, i = f % MH;
+        o[0][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, pv[0][u], o[0][i], 0, 0, 0);
+        if constexpr (more) prob(f * (16 / (2 * MH)));
+        o[1][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, pv[1][u], o[1][i], 0, 0, 0);
+        if constexpr (more && MH == 4) prob(f * 2 + 1);
+        if (f + kAhead < 2 * MH) va[f % kAhead] = vread(f + kAhead);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if constexpr (more) publish(buf ^ 1);
       // ---- NaN groups among keys that not every column sees
-      if (s_flag[buf] == static_cast<int>(kt - kt0) + 1) {
+      if (flag == static_cast<int>(kt - kt0) + 1) {
         for (int t = 0; t < kTile; ++t) {
-          const int64_t key = key0 + t;
+          const int64_t key = kt * kTile + t;
           if (!(there_cur >> (t >> 4) & 1) || key >= kv_end) continue;
           const int32_t ph = block_of_run(p, b, key >> 4, runs);
           const uint8_t* run = vb + static_cast<int64_t>(ph) * p.sP + ((key >> 4) & ((1 << (p.bs_shift - 4)) - 1)) * kv4::Run<D>::kBytes;
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const bool nan = run[kv4::Run<D>::value_scale(t & 15, (4 * quad + r) / (512 / D))] == 255;
-#pragma unroll
-            for (int c = 0; c < NCT; ++c)
-              if (nan && key <= pos[c]) {
-#pragma unroll
-                for (int i = 0; i < MT; ++i) o[c][i][r] = __uint_as_float(0x7fc00000u);
-              }
-          }
+          for (int r = 0; r < 4; ++r)
+            if (run[kv4::Run<D>::value_scale(t & 15, (4 * quad + r) / (512 / D))] == 255) nan_rows |= (key <= first_pos + ahead[0] ? 1u : 0u) << r | (key <= first_pos + ahead[1] ? 16u : 0u) << r;
         }
       }
-      // ---- the next tile's values
-      unpack(kt + 1, buf ^ 1);
-      fetch_values(kt + 2);
       there_cur = there_next;
       there_next = there();
+      wait_vm0();
       lds_barrier();
+    };
+    using yes = std::integral_constant<bool, true>;
+    using no = std::integral_constant<bool, false>;
+    if (unpacks) {
+      for (int64_t kt = kt0; kt + 1 < kt1; ++kt) iterate(kt, yes{}, yes{});
+    } else {
+      for (int64_t kt = kt0; kt + 1 < kt1; ++kt) iterate(kt, no{}, yes{});
     }
+    iterate(kt1 - 1, no{}, no{});
   }
 
-  // ---- out
+  // ---- out: this wave's dims of both column tiles
+  __syncthreads();
+  float* s_l = s_corr;  // [wave][16]; then the reference points
+  const float l_own = column_sum(l_run);
+  if (quad == 0) {
+    s_l[wave * 16 + col] = l_own;
+    s_l[(kWaves + wave) * 16 + col] = m_run;
+  }
+  __syncthreads();
 #pragma unroll
-  for (int c = 0; c < NCT; ++c) {
-    const float l = column_sum(l_run[c]);
-    if (!live[c]) continue;
-    const int64_t row = tok[c] * p.H + head[c];
+  for (int c = 0; c < 2; ++c) {
+    const int x = (wave ^ c) * 16 + col;
+    if (x >= n_cols) continue;
+    const float l = s_l[(wave ^ c) * 16 + col];
+    const int64_t tok = tok0 + (x0 + x) / p.G;
+    const int64_t head = (x0 + x) % p.G + g * p.G;
+    const int64_t row = tok * p.H + head;
+    const int d0 = half * MH;  // dims (4 quad + r) MT + d0 + i
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (nan_rows >> (4 * c + r) & 1) {
+#pragma unroll
+        for (int i = 0; i < MH; ++i) o[c][i][r] = __uint_as_float(0x7fc00000u);
+      }
     if (pp.splits > 1) {
       const int64_t at = blockIdx.z * p.total * p.H + row;
-      if (quad == 0) *reinterpret_cast<float2*>(pp.part_ml + at * 2) = make_float2(m_run[c], l);
+      if (quad == 0 && half == 0) *reinterpret_cast<float2*>(pp.part_ml + at * 2) = make_float2(s_l[(kWaves + (wave ^ c)) * 16 + col], l);
       if (kt0 < kt1) {
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
-          for (int i = 0; i < MT; i += 4)
-            *reinterpret_cast<floatx4_v*>(pp.part_o + at * D + (4 * quad + r) * MT + i) = floatx4_v{o[c][i][r], o[c][i + 1][r], o[c][i + 2][r], o[c][i + 3][r]};
+          for (int i = 0; i < MH; i += 4)
+            *reinterpret_cast<floatx4_v*>(pp.part_o + at * D + (4 * quad + r) * MT + d0 + i) = floatx4_v{o[c][i][r], o[c][i + 1][r], o[c][i + 2][r], o[c][i + 3][r]};
       }
       continue;
     }
-    const bf16_t* gate = p.gate != nullptr ? p.gate + tok[c] * p.gate_st + static_cast<int64_t>(head[c]) * p.gate_sh : nullptr;
-    uint2 graw[4][MT / 4];
+    const bf16_t* gate = p.gate != nullptr ? p.gate + tok * p.gate_st + head * p.gate_sh : nullptr;
+    uint2 graw[4][MH / 4];
     if (gate != nullptr) {
 #pragma unroll
       for (int r = 0; r < 4; ++r)
 #pragma unroll
-        for (int i = 0; i < MT / 4; ++i) graw[r][i] = *reinterpret_cast<const uint2*>(gate + (4 * quad + r) * MT + 4 * i);
+        for (int i = 0; i < MH / 4; ++i) graw[r][i] = *reinterpret_cast<const uint2*>(gate + (4 * quad + r) * MT + d0 + 4 * i);
     }
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
-      for (int i = 0; i < MT; i += 4) {
+      for (int i = 0; i < MH; i += 4) {
         float v[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -363,7 +500,7 @@ __global__ __launch_bounds__(64 * kWaves, 1) void prefill_kernel(PrefillParams p
         uint2 packed;
         packed.x = static_cast<uint32_t>(f32_to_bf16(v[0])) | static_cast<uint32_t>(f32_to_bf16(v[1])) << 16;
         packed.y = static_cast<uint32_t>(f32_to_bf16(v[2])) | static_cast<uint32_t>(f32_to_bf16(v[3])) << 16;
-        *reinterpret_cast<uint2*>(p.out + row * D + (4 * quad + r) * MT + i) = packed;
+        *reinterpret_cast<uint2*>(p.out + row * D + (4 * quad + r) * MT + d0 + i) = packed;
       }
   }
 }
