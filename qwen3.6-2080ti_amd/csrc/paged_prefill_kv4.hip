@@ -7,10 +7,11 @@
 // feeds two products (with 16 columns and all dims a wave, LDS would be as busy as the matrix units), and the
 // accumulators of a wave stay at 64 registers, two waves to a SIMD (with 32 columns and all dims in one wave a SIMD,
 // accumulators and query took 512 registers, 300 moves a tile between the two halves of the file: 1571 us where this
-// form takes 966, 2048 tokens behind 32000).
+// form takes 895, 2048 tokens behind 32000).
 //
-// Keys go from memory into LDS as they are, one tile ahead, one 1 KB copy a wave (with each wave loading them into its
-// registers the vector memory path was busy longer than the matrix units: 1328 us).  Values are unpacked once a workgroup: waves 0 to 3, one a
+// Keys go from memory into LDS as they are, two tiles ahead, 1 KB a wave through its registers (with each wave loading
+// all of them the vector memory path was busy longer than the matrix units: 1328 us; copies straight to LDS each held
+// their wave for about 450 cycles).  Values are unpacked once a workgroup: waves 0 to 3, one a
 // SIMD, turn a run of the next tile each into bf16 operand fragments in LDS, [unit of 32 keys][dim tile][run][lane][8
 // bytes], read back without bank conflicts.
 //
@@ -52,23 +53,6 @@ struct Smem {
   static constexpr int kScales = kKeys + 2 * kRuns * kRunCodes;
   static constexpr int kBytes = kScales + 2 * kRuns * kRunScales;
 };
-
-// Four bytes per lane from memory to LDS bytes lds + 4 l, as lds_copy16.
-__device__ __forceinline__ void lds_copy4(const void* src, uint32_t lds) {
-  uint32_t saved;
-  asm volatile(
-      "s_mov_b32 %0, m0\n\t"
-      "s_mov_b32 m0, %1\n\t"
-      "s_nop 0\n\t"
-      "global_load_lds_dword %2, off\n\t"
-      "s_mov_b32 m0, %0"
-      : "=&s"(saved)
-      : "s"(lds), "v"(src)
-      : "memory");
-}
-
-// Every vector memory operation of the wave has completed, the copies to LDS among them (which the compiler does not count).
-__device__ __forceinline__ void wait_vm0() { __builtin_amdgcn_s_waitcnt(0x0F70); }
 
 // The products stay where they are written: the compiler would move them to where their sums are used.
 __device__ __forceinline__ void keep(floatx4_v (&s)[kRuns]) { asm volatile("" : "+v"(s[0]), "+v"(s[1]), "+v"(s[2]), "+v"(s[3])); }
@@ -137,10 +121,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams p
   for (int c = 0; c < 2; ++c) ahead[c] = (min((wave ^ c) * 16 + col, n_cols - 1) + x_head) / p.G;
 
   // ---- the tiles' loads
-  // Lane l of `cur` holds the offset in the head's pool of run 64 c + l (-1: not there), of `nxt` that of the next 64:
+  // Lane l of `cur` holds the offset in the head's pool of run 64 c + l (-1: not there), of `nxt` that of the next 64,
   // one vector load each 16 tiles (scalar loads of the table share their wait counter with LDS, and every tile stalled
-  // about 1000 cycles for them).
+  // about 1000 cycles for them); the masks say which runs are there.
   int64_t cur, nxt;
+  uint64_t cur_mask, nxt_mask;
   auto chunk = [&](int64_t c) -> int64_t {
     const int64_t run = 64 * c + lane;
     const int64_t lb = run >> (p.bs_shift - 4);
@@ -151,49 +136,46 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams p
     const int64_t o = static_cast<int64_t>(ok ? lo : 0) * p.sP + (run & ((1 << (p.bs_shift - 4)) - 1)) * kv4::Run<D>::kBytes;
     return ok ? o : -1;
   };
-  int64_t off[kRuns];  // of the runs of a tile
+  // A wave loads only run `wave % 4` of a tile: waves 0 to 3 its values and half of its keys' codes, waves 4 to 7 the
+  // rest of its keys.
+  int64_t own;  // offset of that run of the tile last asked for, -1: not there
+  int there;    // which runs of that tile are there
   auto offsets = [&](int64_t kt) {
     const int at = static_cast<int>(kt & 15) * kRuns;
     if (at == 0 && kt != kt0) {
       cur = nxt;
+      cur_mask = nxt_mask;
       nxt = chunk((kt >> 4) + 1);
+      nxt_mask = __ballot(nxt >= 0);
     }
-#pragma unroll
-    for (int j = 0; j < kRuns; ++j) {
-      const uint32_t lo = __builtin_amdgcn_readlane(static_cast<uint32_t>(cur), at + j);
-      const uint32_t hi = __builtin_amdgcn_readlane(static_cast<uint32_t>(cur >> 32), at + j);
-      off[j] = static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
-    }
+    const uint32_t lo = __builtin_amdgcn_readlane(static_cast<uint32_t>(cur), at + (wave & 3));
+    const uint32_t hi = __builtin_amdgcn_readlane(static_cast<uint32_t>(cur >> 32), at + (wave & 3));
+    own = static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
+    there = static_cast<int>(cur_mask >> at) & 15;
   };
-  auto there = [&]() { return (off[0] >= 0 ? 1 : 0) | (off[1] >= 0 ? 2 : 0) | (off[2] >= 0 ? 4 : 0) | (off[3] >= 0 ? 8 : 0); };
-  // run `wave % 4` of the tile whose offsets are in off: waves 0 to 3 unpack its values, waves 4 to 7 copy its key scales
-  auto own_run = [&]() -> int64_t {
-    int64_t r = 0;  // with masks: a choice between the elements would put the array into memory
-#pragma unroll
-    for (int j = 0; j < kRuns; ++j) r |= off[j] & -static_cast<int64_t>(j == (wave & 3));
-    return r;
+  // That run as a buffer; one that is not there has no records and reads zeros.
+  auto rsrc = [&](const uint8_t* base) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base + (own < 0 ? 0 : own)), 0, own < 0 ? 0 : kv4::Run<D>::kBytes, 0x00020000);
   };
-  const uint32_t smem_lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(smem));
-  // Copies the keys of the tile whose offsets are in off to buffer buf, a wave 1 KB of codes, the waves that do not
-  // unpack a run's scales too.  Of runs that are not there nothing is read; what the buffer held gives scores that are
-  // masked.
-  auto copy_keys = [&](int buf) {
-    constexpr int PER = D / 128;  // copies of a run
-    const int64_t o = own_run();
-    if (o < 0) return;
-    const uint8_t* src = kb + o;
-    if (PER == 2 || wave < 4) {
-      const int part = PER == 2 ? wave >> 2 : 0;
-      lds_copy16(src + 1024 * part + 16 * lane, smem_lds + S::kKeys + (buf * kRuns + (wave & 3)) * S::kRunCodes + 1024 * part);
-    }
-    if (wave >= 4 && lane < S::kRunScales / 4) lds_copy4(src + S::kRunCodes + 4 * lane, smem_lds + S::kScales + (buf * kRuns + (wave & 3)) * S::kRunScales);
+  // The wave's part of a tile's keys on its way to LDS: 1 KB of codes (at D = 128 only waves 4 to 7), the waves that do
+  // not unpack a run's scales too.
+  constexpr int PER = D / 128;  // KB of codes of a run
+  uint4 kcode = make_uint4(0, 0, 0, 0);
+  uint32_t kscale = 0;
+  auto fetch_keys = [&]() {
+    const __amdgpu_buffer_rsrc_t r = rsrc(kb);
+    const int part = PER == 2 ? wave >> 2 : 0;
+    if (PER == 2 || wave >= 4) kcode = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, 1024 * part + 16 * lane, 0, 0));
+    if (wave >= 4) kscale = __builtin_amdgcn_raw_buffer_load_b32(r, S::kRunCodes + 4 * (lane % (S::kRunScales / 4)), 0, 0);
+  };
+  auto store_keys = [&](int buf) {
+    const int part = PER == 2 ? wave >> 2 : 0;
+    if (PER == 2 || wave >= 4) *reinterpret_cast<uint4*>(smem + S::kKeys + (buf * kRuns + (wave & 3)) * S::kRunCodes + 1024 * part + 16 * lane) = kcode;
+    if (wave >= 4 && lane < S::kRunScales / 4) *reinterpret_cast<uint32_t*>(smem + S::kScales + (buf * kRuns + (wave & 3)) * S::kRunScales + 4 * lane) = kscale;
   };
   const bool unpacks = wave < 4;
   ValueRun<D> vr;
-  auto fetch_values = [&]() {
-    const int64_t o = own_run();
-    load_values<D>(vr, __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(vb + (o < 0 ? 0 : o)), 0, o < 0 ? 0 : kv4::Run<D>::kBytes, 0x00020000), lane);
-  };
+  auto fetch_values = [&]() { load_values<D>(vr, rsrc(vb), lane); };
   // what of vr no column sees, or not every column where it is NaN, leaves the product
   auto trim = [&](int64_t kt, int buf) {
     if (kt * kTile + kTile <= first_pos + 1) return;  // every column sees all of the tile
@@ -244,9 +226,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams p
     if (tid < 2) s_flag[tid] = 0;
     cur = chunk(kt0 >> 4);
     nxt = chunk((kt0 >> 4) + 1);
+    cur_mask = __ballot(cur >= 0);
+    nxt_mask = __ballot(nxt >= 0);
     offsets(kt0);
-    int there_cur = there();
-    copy_keys(0);
+    int there_cur = there;
+    fetch_keys();
     if (unpacks) fetch_values();
     QueryCols<D> qh, ql;
     {
@@ -262,8 +246,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams p
     floatx4_v sc[kRuns];
     float use = 0.f;
     bf16x8_v pb[2];  // the own probabilities of the two units
-    // The scores: operand f of a tile is slice f / kRuns of run f % kRuns and feeds the products of both pieces; runs
-    // innermost, so that products of one accumulator are eight apart.
+    // The scores: operand f of a tile is slice f / kRuns of run f % kRuns and feeds the products of both pieces; two
+    // operands go together, so that products of one accumulator do not follow each other.
     constexpr int kOperands = kRuns * (D / 128);
     auto kread = [&](int f, int buf) {
       const int j = f % kRuns, i = f / kRuns;
@@ -274,19 +258,18 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams p
       const unsigned char* at = smem + S::kScales + (buf * kRuns + j) * S::kRunScales + lane * (D / 128);
       return D == 256 ? static_cast<int>(*reinterpret_cast<const uint16_t*>(at)) : static_cast<int>(*at);
     };
-    auto products = [&](int f, const int8_v& a, int scale) {
+    auto product = [&](int f, const int8_v& a, int scale, bool lo) {
       const int j = f % kRuns, i = f / kRuns;
-      const floatx4_v acc = i == 0 ? floatx4_v{0.f, 0.f, 0.f, 0.f} : sc[j];
-      if (i == 0) {
-        sc[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, qh.code[0], acc, 4, 0, 0, scale, 0, static_cast<int>(qh.scale));
-        sc[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, ql.code[0], sc[j], 4, 0, 0, scale, 0, static_cast<int>(ql.scale));
-      } else {
-        sc[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, qh.code[D / 128 - 1], acc, 4, 0, 1, scale, 0, static_cast<int>(qh.scale));
-        sc[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, ql.code[D / 128 - 1], sc[j], 4, 0, 1, scale, 0, static_cast<int>(ql.scale));
-      }
+      const floatx4_v acc = i == 0 && !lo ? floatx4_v{0.f, 0.f, 0.f, 0.f} : sc[j];
+      const int8_v& code = lo ? ql.code[i] : qh.code[i];
+      const int qs = static_cast<int>(lo ? ql.scale : qh.scale);
+      if (i == 0)
+        sc[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, code, acc, 4, 0, 0, scale, 0, qs);
+      else
+        sc[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, code, acc, 4, 0, 1, scale, 0, qs);
     };
     static_assert(kOperands == kBytesOfChunk, "a byte of the chunk goes with each operand");
-    constexpr int kAheadK = 2;
+    constexpr int kAheadK = 4;
     auto scores = [&](int buf, auto slice) {
       int scale[kRuns];
 #pragma unroll
@@ -295,11 +278,18 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams p
 #pragma unroll
       for (int f = 0; f < kAheadK; ++f) ka[f] = kread(f, buf);
 #pragma unroll
-      for (int f = 0; f < kOperands; ++f) {
-        const int8_v a = ka[f % kAheadK];
-        if (f + kAheadK < kOperands) ka[f % kAheadK] = kread(f + kAheadK, buf);
-        products(f, a, scale[f % kRuns]);
+      for (int f = 0; f < kOperands; f += 2) {
+        const int8_v a0 = ka[f % kAheadK], a1 = ka[(f + 1) % kAheadK];
+        product(f, a0, scale[f % kRuns], false);
         slice(f);
+        __builtin_amdgcn_sched_barrier(0);
+        product(f + 1, a1, scale[(f + 1) % kRuns], false);
+        product(f, a0, scale[f % kRuns], true);
+        if (f + kAheadK < kOperands) ka[f % kAheadK] = kread(f + kAheadK, buf);
+        slice(f + 1);
+        __builtin_amdgcn_sched_barrier(0);
+        product(f + 1, a1, scale[(f + 1) % kRuns], true);
+        if (f + 1 + kAheadK < kOperands) ka[(f + 1) % kAheadK] = kread(f + 1 + kAheadK, buf);
         __builtin_amdgcn_sched_barrier(0);
       }
       keep(sc);
@@ -340,7 +330,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams p
       dst[0] = __builtin_bit_cast(uint4, pb[0]);
       dst[64] = __builtin_bit_cast(uint4, pb[1]);
     };
-    wait_vm0();
+    store_keys(0);
     __syncthreads();  // the flags and the first tile's keys
     scores(0, [](int) {});
     reference(kt0, there_cur, 0);
@@ -353,36 +343,38 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams p
       for (int e = 0; e < kBytesOfChunk; ++e) unpack_byte(e, 0);
     }
     offsets(kt0 + 1);
-    int there_next = there();
-    copy_keys(1);
+    int there_next = there;
+    fetch_keys();
     if (unpacks) fetch_values();
-    wait_vm0();
+    store_keys(1);
     __syncthreads();
 
     // Iteration kt.  The products are laid between slices of the vector work that does not depend on them, with fences
     // that keep the order: the scores of tile kt + 1 with its unpacking, the values of tile kt with the exponentials.
+    // (Waves 4 to 7 with the values first, half an iteration apart from the waves they share SIMDs with: no faster, 901
+    // us against 895, 2048 tokens behind 32000.)
     auto iterate = [&](int64_t kt, auto unpacking, auto more) {
       const int buf = static_cast<int>((kt - kt0) & 1);
+      const int flag = s_flag[buf];
+      const float c0 = s_corr[(buf * kWaves + wave) * 16 + col], c1 = s_corr[(buf * kWaves + (wave ^ 1)) * 16 + col];
+      if constexpr (more) {
+        offsets(kt + 2);
+        fetch_keys();
+      }
       if constexpr (more) {
         if constexpr (unpacking) trim(kt + 1, buf ^ 1);
         scores(buf ^ 1, [&](int f) {
-          if constexpr (unpacking) {
-            unpack_byte(f, buf ^ 1);
-          }
+          if constexpr (unpacking) unpack_byte(f, buf ^ 1);
         });
-        offsets(kt + 2);
-        copy_keys(buf);
         if constexpr (unpacking) fetch_values();
+        __builtin_amdgcn_sched_barrier(0);
       }
-      __builtin_amdgcn_sched_barrier(0);
       bf16x8_v pv[2][2];
       pv[0][0] = pb[0];
       pv[0][1] = pb[1];
       const uint4* src = reinterpret_cast<const uint4*>(smem + S::kP) + (buf * kWaves + (wave ^ 1)) * 128 + lane;
       pv[1][0] = __builtin_bit_cast(bf16x8_v, src[0]);
       pv[1][1] = __builtin_bit_cast(bf16x8_v, src[64]);
-      const int flag = s_flag[buf];
-      const float c0 = s_corr[(buf * kWaves + wave) * 16 + col], c1 = s_corr[(buf * kWaves + (wave ^ 1)) * 16 + col];
       if (__ballot(c0 != 1.f || c1 != 1.f) != 0) {  // columns whose reference point moved at this tile
 #pragma unroll
         for (int i = 0; i < MH; ++i) {
@@ -391,7 +383,6 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams p
         }
       }
       if constexpr (more) reference(kt + 1, there_next, buf ^ 1);
-      // ---- values of this tile, exponentials of the next
       const uint2* vt = reinterpret_cast<const uint2*>(smem + buf * S::kTileBytes) + half * MH * 128 + lane;
       constexpr int kAhead = 4;
       auto vread = [&](int f) {
@@ -422,12 +413,13 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams p
           const uint8_t* run = vb + static_cast<int64_t>(ph) * p.sP + ((key >> 4) & ((1 << (p.bs_shift - 4)) - 1)) * kv4::Run<D>::kBytes;
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            if (run[kv4::Run<D>::value_scale(t & 15, (4 * quad + r) / (512 / D))] == 255) nan_rows |= (key <= first_pos + ahead[0] ? 1u : 0u) << r | (key <= first_pos + ahead[1] ? 16u : 0u) << r;
+            if (run[kv4::Run<D>::value_scale(t & 15, (4 * quad + r) / (512 / D))] == 255)
+              nan_rows |= (key <= first_pos + ahead[0] ? 1u : 0u) << r | (key <= first_pos + ahead[1] ? 16u : 0u) << r;
         }
       }
       there_cur = there_next;
-      there_next = there();
-      wait_vm0();
+      there_next = there;
+      if constexpr (more) store_keys(buf);
       lds_barrier();
     };
     using yes = std::integral_constant<bool, true>;
