@@ -76,15 +76,6 @@ __device__ __forceinline__ int32_t block_of_run(const Params& p, int64_t b, int6
   return ok ? lo : -1;
 }
 
-// Buffer resource over one run; a skipped one has no records, so that its loads read zeros, touch no memory, and every
-// step of a load stream issues the same instructions.
-template <int D>
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t run_rsrc(const Params& p, const uint8_t* head, int32_t phys, int64_t run) {
-  const int64_t sub = run & ((1 << (p.bs_shift - 4)) - 1);
-  const uint8_t* at = head + static_cast<int64_t>(phys < 0 ? 0 : phys) * p.sP + sub * kv4::Run<D>::kBytes;
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(at), 0, phys < 0 ? 0 : kv4::Run<D>::kBytes, 0x00020000);
-}
-
 // A run of keys in registers: lane 16 q + t holds token t, dims 32 q .. 32 q + 31 of each slice of 128.
 template <int D>
 struct KeyRun {
@@ -126,6 +117,10 @@ struct QueryCols {
   uint32_t scale;
 };
 
+// The scale byte of a row's hi piece: the row's largest element, of bits top, lands in [128, 256), the lo piece's scale is
+// 2^-4 of it.  A row with an infinity or a NaN becomes NaN.
+__device__ __forceinline__ uint32_t query_scale(uint32_t top) { return static_cast<uint32_t>(min(max(static_cast<int>(top >> 23) - 7, 5), 247)); }
+
 // Loads row qrow (null: zeros) of this lane's column and splits it.  LO: the second piece.  Both need the same row.
 template <int D>
 struct QueryRow {
@@ -150,8 +145,7 @@ struct QueryRow {
       }
     top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 16, 64)));
     top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 32, 64)));
-    // the row's largest element lands in [128, 256); a row with an infinity or a NaN becomes NaN
-    byte = static_cast<uint32_t>(min(max(static_cast<int>(top >> 23) - 7, 5), 247));
+    byte = query_scale(top);
   }
 
   template <bool LO>

@@ -2,15 +2,18 @@
 //
 // Bound by memory: 17 D / 32 bytes a cached token, KV head and K or V, each read once for the G query heads that share
 // it.  All (row, KV head, unit of 32 tokens) are laid end to end, T units, and workgroup w of W takes the range
-// [T w / W, T (w + 1) / W): equal shares whatever the lengths.  Inside a row group the workgroup's eight waves take its
-// units in turn, so that neighbouring waves read neighbouring tiles, each with an online softmax of its own and no
-// barrier; where the range leaves the row group they merge in LDS and write one partial (m, l, o) of the G heads.  A
-// workgroup that had the whole row group writes the result; the other groups' partials are merged by combine_kernel.
+// [T w / W, T (w + 1) / W): equal shares whatever the lengths.  The workgroup's eight waves take its units in turn, so
+// that neighbouring waves read neighbouring tiles, each with an online softmax of its own and no barrier; where the
+// range leaves a row group they merge in LDS and write one partial (m, l, o) of the G heads.  A workgroup that had the
+// whole row group writes the result; the other groups' partials are merged by combine_kernel.
 //
-// A wave loads a unit's keys and values two units ahead into registers (buffer loads of zero records for what is
-// skipped, so every step issues the same loads and the wait counts are fixed).  Columns of the scores' product: with up
-// to eight heads the first eight are the heads' hi pieces and the last eight their lo pieces, one product a slice, and a
-// row rotation adds the two; with more the pieces take two products.
+// A wave keeps two units of keys and values in flight in registers (buffer loads of zero records for what is skipped, so
+// every step issues the same loads and the wait counts are fixed), across row groups: the merge of one and the query of
+// the next run while the next one's tiles arrive.  Lane j of a wave holds where unit j of its next 64 lies; one search and
+// one vector load of the tables serve them all, and a step reads its lane.  Columns of the scores' product: with up to
+// eight heads the first eight are the heads' hi pieces and the last eight their lo pieces, one product a slice, and a
+// row rotation adds the two; with more the pieces take two products.  The query is split once a workgroup, a head a wave,
+// through LDS.
 #include "attention_kv4.h"
 
 #include <algorithm>
@@ -30,61 +33,59 @@ constexpr int kWaves = 8;
 constexpr int kUnit = 32;  // tokens
 constexpr int kMaxWgs = 256;  // one per CU: eight waves of up to 256 registers fill it
 
-// Units of row b (0 for rows of length <= 0); lengths past the table stop at it.
+// Tokens and units of row b (0 for rows of length <= 0); lengths past the table stop at it.
 __device__ __forceinline__ int64_t row_tokens(const Params& p, int b) {
   const int64_t len = p.idx_i64 ? reinterpret_cast<const int64_t*>(p.lens)[b] : reinterpret_cast<const int32_t*>(p.lens)[b];
   return max64(0, min64(len, p.max_blocks << p.bs_shift));
 }
-__device__ __forceinline__ int64_t row_units(const Params& p, int b) { return (row_tokens(p, b) + kUnit - 1) / kUnit; }
+__device__ __forceinline__ int units_of(int64_t tokens) { return static_cast<int>((tokens + kUnit - 1) / kUnit); }
 
+// A row group: row b, KV head g, the units before it, its units.
 struct Cursor {
-  int b, g;
-  int64_t cum, nu;  // units before the row group, units of it
+  int b, g, cum, nu;
 };
 
-// Units of all row groups.
-__device__ int64_t total_units(const Params& p, int lane) {
-  int64_t sum = 0;
-  for (int b0 = 0; b0 < p.B; b0 += 64) sum += b0 + lane < p.B ? row_units(p, b0 + lane) : 0;
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
-  return sum * p.Hkv;
+__device__ __forceinline__ void next_row_group(const Params& p, Cursor& c) {
+  c.cum += c.nu;
+  if (++c.g < p.Hkv) return;
+  c.g = 0;
+  do {
+    ++c.b;
+    c.nu = c.b < p.B ? __builtin_amdgcn_readfirstlane(units_of(row_tokens(p, c.b))) : 0;
+  } while (c.nu == 0 && c.b < p.B);
 }
 
-// The row group that holds unit t < T.
-__device__ Cursor locate(const Params& p, int64_t t, int lane) {
-  int64_t base = 0;
-  for (int b0 = 0; b0 < p.B; b0 += 64) {
-    const int64_t nu = b0 + lane < p.B ? row_units(p, b0 + lane) : 0;
-    int64_t incl = nu * p.Hkv;
+// Inclusive sum over the lanes.
+__device__ __forceinline__ int lane_scan(int v, int lane) {
 #pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const int64_t up = __shfl_up(incl, off, 64);
-      if (lane >= off) incl += up;
-    }
-    const int64_t chunk = __shfl(incl, 63, 64);
-    if (t < base + chunk) {
-      const int first = __ffsll(static_cast<unsigned long long>(__ballot(base + incl > t))) - 1;
-      const int64_t n = __shfl(nu, first, 64);
-      const int64_t before = base + __shfl(incl, first, 64) - n * p.Hkv;
-      Cursor c;
-      c.b = b0 + first;
-      c.g = static_cast<int>((t - before) / n);
-      c.cum = before + c.g * n;
-      c.nu = n;
-      return c;
-    }
-    base += chunk;
+  for (int off = 1; off < 64; off <<= 1) {
+    const int up = __shfl_up(v, off, 64);
+    if (lane >= off) v += up;
   }
-  return Cursor{p.B, 0, base, 0};
+  return v;
+}
+
+// Max over the wave of non-negative floats' bits.
+__device__ __forceinline__ uint32_t wave_max_bits(uint32_t v) {
+  v = kv4::quad_max(v);
+  v = max(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x124, 0xF, 0xF, false)));  // row_ror:4
+  v = max(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x128, 0xF, 0xF, false)));  // row_ror:8
+  const uint32_t a = max(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16));
+  const uint32_t b = max(__builtin_amdgcn_readlane(v, 32), __builtin_amdgcn_readlane(v, 48));
+  return max(a, b);
 }
 
 template <int D, bool WIDE>
 struct Smem {
   static constexpr int kHeads = WIDE ? 16 : 8;
-  static constexpr int kRow = D + 4;  // floats: neighbouring heads start four banks apart
-  static constexpr int kO = kWaves * kHeads * kRow;
-  static constexpr int kBytes = (kO + 2 * kWaves * 16) * 4;
+  static constexpr int kRow = D + 4;                      // floats: neighbouring heads start four banks apart
+  static constexpr int kM = kWaves * kHeads * kRow * 4;   // after the waves' sums: (kWaves, 16) reference points,
+  static constexpr int kL = kM + kWaves * 16 * 4;         // (kWaves, 16) denominators,
+  static constexpr int kTotal = kL + kWaves * 16 * 4;     // the merged ones (2, 16),
+  static constexpr int kQ = kTotal + 2 * 16 * 4;          // the query's pieces, 32 rows of D bytes,
+  static constexpr int kQRow = D + 16;
+  static constexpr int kQScale = kQ + 32 * kQRow;         // and their scales
+  static constexpr int kBytes = kQScale + 32 * 4;
 };
 
 // WIDE: more than eight heads a group.
@@ -93,81 +94,220 @@ __global__ __launch_bounds__(64 * kWaves, 2) void decode_kernel(DecodeParams dp)
   const Params& p = dp.c;
   using S = Smem<D, WIDE>;
   constexpr int MT = D / 16;
-  extern __shared__ __align__(16) float smem[];
-  float* s_m = smem + S::kO;              // (kWaves, 16)
-  float* s_l = s_m + kWaves * 16;
+  extern __shared__ __align__(16) unsigned char smem[];
+  float* s_o = reinterpret_cast<float*>(smem);
+  float* s_m = reinterpret_cast<float*>(smem + S::kM);
+  float* s_l = reinterpret_cast<float*>(smem + S::kL);
+  float* s_total = reinterpret_cast<float*>(smem + S::kTotal);
+  uint32_t* s_qscale = reinterpret_cast<uint32_t*>(smem + S::kQScale);
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15;
   const int quad = lane >> 4;
-  const int head = WIDE ? col : col & 7;
 
-  const int64_t T = uniform64(total_units(p, lane));
+  // ---- this workgroup's share
+  int T = 0;
+  int64_t len_first = 0;  // of row `lane`, kept for the search
+  for (int b0 = 0; b0 < p.B; b0 += 64) {
+    const int64_t len = b0 + lane < p.B ? row_tokens(p, b0 + lane) : 0;
+    if (b0 == 0) len_first = len;
+    T += units_of(len);
+  }
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) T += __shfl_xor(T, off, 64);
+  T = __builtin_amdgcn_readfirstlane(T) * p.Hkv;
   // a workgroup has a unit for each wave before another one starts
-  const int64_t W = min64(dp.n_wgs, (T + kWaves - 1) / kWaves);
-  const int64_t wg = blockIdx.x;
+  const int W = min(dp.n_wgs, (T + kWaves - 1) / kWaves);
+  const int wg = blockIdx.x;
   if (wg >= W) return;
-  const int64_t lo = T * wg / W;
-  const int64_t hi = T * (wg + 1) / W;
-  Cursor cur = locate(p, lo, lane);
-  cur.b = __builtin_amdgcn_readfirstlane(cur.b);
-  cur.g = __builtin_amdgcn_readfirstlane(cur.g);
-  cur.cum = uniform64(cur.cum);
-  cur.nu = uniform64(cur.nu);
-  const float qk_scale = p.scale * kLog2e;
+  const int lo = static_cast<int>(static_cast<int64_t>(T) * wg / W);
+  const int hi = static_cast<int>(static_cast<int64_t>(T) * (wg + 1) / W);
 
-  for (int64_t at = lo; at < hi;) {
-    const int64_t seg_end = min64(hi, cur.cum + cur.nu);
-    const int64_t len = uniform64(row_tokens(p, cur.b));
-    const int64_t runs = (len + kv4::kRun - 1) / kv4::kRun;
-    const uint8_t* kb = p.kpool + cur.g * p.sG;
-    const uint8_t* vb = p.vpool + cur.g * p.sG;
-    const int64_t u1 = seg_end - cur.cum;  // end of the segment in the row group's units
-    int64_t u = at - cur.cum + wave;
-
-    KeyRun<D> kr[2][2];
-    ValueRun<D> vr[2][2];
-    int32_t phys[2][2];    // of the units in kr / vr
-    int32_t ahead[2];      // of the unit after those
-    auto entries = [&](int64_t unit, int32_t (&e)[2]) {
+  // ---- where the wave's units lie: lane j holds unit 64 c + j, that is unit lo + wave + kWaves (64 c + j) of all
+  int64_t at0, at1;  // offsets of its two runs in the pools, -1: not there
+  int left;          // its tokens
+  Cursor cur{0, 0, 0, 0};
+  auto locate = [&](int c, bool begin) {
+    const int gu = lo + wave + kWaves * (64 * c + lane);
+    int row = -1, g = 0, u = 0;
+    int64_t tokens = 0;
+    int base = 0;
+    for (int b0 = 0; b0 < p.B; b0 += 64) {
+      const int64_t len = b0 == 0 ? len_first : b0 + lane < p.B ? row_tokens(p, b0 + lane) : 0;
+      const int nu = units_of(len);
+      const int incl = lane_scan(nu * p.Hkv, lane);
+      const int chunk = __builtin_amdgcn_readlane(incl, 63);
+      if (begin && lo >= base && lo < base + chunk) {
+        const int first = __ffsll(static_cast<unsigned long long>(__ballot(base + incl > lo))) - 1;
+        cur.b = b0 + first;
+        cur.nu = __builtin_amdgcn_readlane(nu, first);
+        const int before = base + __builtin_amdgcn_readlane(incl, first) - cur.nu * p.Hkv;
+        cur.g = (lo - before) / cur.nu;
+        cur.cum = before + cur.g * cur.nu;
+      }
+      int pos = 0;  // rows of the block that end at or before gu
 #pragma unroll
-      for (int j = 0; j < 2; ++j) e[j] = unit < u1 ? block_of_run(p, cur.b, 2 * unit + j, runs) : -1;
-    };
-    auto fetch_keys = [&](int s, int64_t unit) {
-#pragma unroll
-      for (int j = 0; j < 2; ++j) load_keys<D>(kr[s][j], run_rsrc<D>(p, kb, phys[s][j], 2 * unit + j), lane);
-    };
-    auto fetch_values = [&](int s, int64_t unit) {
-#pragma unroll
-      for (int j = 0; j < 2; ++j) load_values<D>(vr[s][j], run_rsrc<D>(p, vb, phys[s][j], 2 * unit + j), lane);
-    };
-#pragma unroll
-    for (int s = 0; s < 2; ++s) entries(u + s * kWaves, phys[s]);
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      fetch_keys(s, u + s * kWaves);
-      fetch_values(s, u + s * kWaves);
+      for (int step = 32; step > 0; step >>= 1) {
+        const int end = __shfl(incl, pos + step - 1, 64);
+        if (base + end <= gu) pos += step;
+      }
+      const int n = __shfl(nu, pos, 64);
+      const int before = base + __shfl(incl, pos, 64) - n * p.Hkv;
+      const int64_t t = (static_cast<int64_t>(__shfl(static_cast<int>(len >> 32), pos, 64)) << 32) | static_cast<uint32_t>(__shfl(static_cast<int>(len), pos, 64));
+      if (gu >= base && gu < base + chunk) {
+        row = b0 + pos;
+        g = (gu - before) / n;
+        u = gu - before - g * n;
+        tokens = t;
+      }
+      base += chunk;
+      if (base >= hi) break;
     }
-    entries(u + 2 * kWaves, ahead);
+    at0 = at1 = -1;
+    left = 0;
+    if (gu < hi && row >= 0) {
+      left = static_cast<int>(min64(kUnit, tokens - static_cast<int64_t>(u) * kUnit));
+      const int sub_shift = p.bs_shift - 4;
+      auto offset = [&](int64_t run) -> int64_t {
+        const int64_t e = (static_cast<int64_t>(row) * p.table_stride + (run >> sub_shift)) << p.table_i64;
+        const int32_t id = reinterpret_cast<const int32_t*>(p.tables)[e];
+        const int32_t high = reinterpret_cast<const int32_t*>(p.tables)[e + p.table_i64];  // the entry itself where it has one word
+        const bool ok = (static_cast<uint32_t>(id) < static_cast<uint32_t>(p.num_blocks)) & ((high == 0) | (p.table_i64 == 0));
+        return ok ? static_cast<int64_t>(id) * p.sP + (run & ((1 << sub_shift) - 1)) * kv4::Run<D>::kBytes + g * p.sG : -1;
+      };
+      at0 = offset(2 * static_cast<int64_t>(u));
+      if (left > kv4::kRun) at1 = offset(2 * static_cast<int64_t>(u) + 1);
+    }
+  };
+  locate(0, true);
 
-    QueryCols<D> qa_, qb_;
-    {
-      QueryRow<D> row;
-      row.load(head < p.G ? p.q + static_cast<int64_t>(cur.b) * p.q_st + static_cast<int64_t>(cur.g * p.G + head) * p.q_sh : nullptr, quad);
-      row.template split<false>(qa_);
-      row.template split<true>(qb_);
-      if constexpr (!WIDE) {
-        if (col >= 8) qa_ = qb_;
+  KeyRun<D> kr[2][2];
+  ValueRun<D> vr[2][2];
+  int64_t where[2];  // of the unit being asked for
+  int have[2];       // tokens of the units in kr / vr, and 256 / 512 where the first / second run is not there
+  auto look = [&](int i, int s) {
+    const int j = i & 63;
+    auto read = [&](int64_t v) {
+      const uint32_t l = __builtin_amdgcn_readlane(static_cast<uint32_t>(v), j), h = __builtin_amdgcn_readlane(static_cast<uint32_t>(v >> 32), j);
+      return static_cast<int64_t>(static_cast<uint64_t>(h) << 32 | l);
+    };
+    where[0] = read(at0);
+    where[1] = read(at1);
+    have[s] = __builtin_amdgcn_readlane(left, j) | (where[0] < 0 ? 256 : 0) | (where[1] < 0 ? 512 : 0);
+  };
+  auto rsrc = [&](const uint8_t* base, int64_t o) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base + (o < 0 ? 0 : o)), 0, o < 0 ? 0 : kv4::Run<D>::kBytes, 0x00020000);
+  };
+  auto fetch_keys = [&](int s) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) load_keys<D>(kr[s][j], rsrc(p.kpool, where[j]), lane);
+  };
+  auto fetch_values = [&](int s) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) load_values<D>(vr[s][j], rsrc(p.vpool, where[j]), lane);
+  };
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    look(s, s);
+    fetch_keys(s);
+    fetch_values(s);
+  }
+
+  // ---- the query of a row group: wave w takes heads w and w + 8, lane l dims E l ..
+  constexpr int E = D / 64;
+  uint32_t qraw[WIDE ? 2 : 1][E / 2];
+  auto fetch_query = [&](const Cursor& c) {
+#pragma unroll
+    for (int k = 0; k < (WIDE ? 2 : 1); ++k) {
+      const int h = wave + 8 * k;
+#pragma unroll
+      for (int e = 0; e < E / 2; ++e) qraw[k][e] = 0;
+      if (h < p.G && c.b < p.B) {
+        const bf16_t* row = p.q + static_cast<int64_t>(c.b) * p.q_st + static_cast<int64_t>(c.g * p.G + h) * p.q_sh + E * lane;
+        if constexpr (E == 4) {
+          const uint2 u = *reinterpret_cast<const uint2*>(row);
+          qraw[k][0] = u.x, qraw[k][1] = u.y;
+        } else {
+          qraw[k][0] = *reinterpret_cast<const uint32_t*>(row);
+        }
       }
     }
+  };
+  // rows of s_q: head h's hi piece at h, its lo piece at h + (WIDE ? 16 : 8)
+  auto split_query = [&]() {
+#pragma unroll
+    for (int k = 0; k < (WIDE ? 2 : 1); ++k) {
+      const int h = wave + 8 * k;
+      uint32_t top = 0;
+      float x[E];
+#pragma unroll
+      for (int e = 0; e < E / 2; ++e) {
+        const uint32_t w = qraw[k][e];
+        x[2 * e] = __uint_as_float(w << 16);
+        x[2 * e + 1] = __uint_as_float(w & 0xffff0000u);
+        top = max(top, max(w << 16 & 0x7fffffffu, w & 0x7fff0000u));
+      }
+      const uint32_t byte = query_scale(wave_max_bits(top));
+      const float inv = __uint_as_float((254u - byte) << 23);
+      uint32_t hi8 = 0, lo8 = 0;
+#pragma unroll
+      for (int e = 0; e < E; e += 2) {
+        const float y0 = x[e] * inv, y1 = x[e + 1] * inv;
+        const uint32_t h2 = __builtin_amdgcn_cvt_pk_fp8_f32(y0, y1, 0, false);
+        const floatx2_v a = __builtin_amdgcn_cvt_pk_f32_fp8(h2, false);
+        const uint32_t l2 = __builtin_amdgcn_cvt_pk_fp8_f32((y0 - a[0]) * 16.f, (y1 - a[1]) * 16.f, 0, false);
+        hi8 |= (h2 & 0xffffu) << (8 * e);
+        lo8 |= (l2 & 0xffffu) << (8 * e);
+      }
+      unsigned char* hi_row = smem + S::kQ + h * S::kQRow + E * lane;
+      unsigned char* lo_row = hi_row + S::kHeads * S::kQRow;
+      if constexpr (E == 4) {
+        *reinterpret_cast<uint32_t*>(hi_row) = hi8;
+        *reinterpret_cast<uint32_t*>(lo_row) = lo8;
+      } else {
+        *reinterpret_cast<uint16_t*>(hi_row) = static_cast<uint16_t>(hi8);
+        *reinterpret_cast<uint16_t*>(lo_row) = static_cast<uint16_t>(lo8);
+      }
+      if (lane == 0) {
+        s_qscale[h] = byte;
+        s_qscale[h + S::kHeads] = byte - 4u;
+      }
+    }
+  };
+  auto read_query = [&](QueryCols<D>& q, int row) {
+    const unsigned char* at = smem + S::kQ + row * S::kQRow + 16 * quad;
+#pragma unroll
+    for (int i = 0; i < D / 128; ++i) {
+      const uint4 a = *reinterpret_cast<const uint4*>(at + 128 * i), b = *reinterpret_cast<const uint4*>(at + 128 * i + 64);
+      q.code[i] = int8_v{static_cast<int>(a.x), static_cast<int>(a.y), static_cast<int>(a.z), static_cast<int>(a.w),
+                         static_cast<int>(b.x), static_cast<int>(b.y), static_cast<int>(b.z), static_cast<int>(b.w)};
+    }
+    q.scale = s_qscale[row];
+  };
+  fetch_query(cur);
+  const float qk_scale = p.scale * kLog2e;
+
+  int i = 0;                // the wave's next unit, in slot i & 1
+  int gu = lo + wave;       // that unit among all
+  for (int at = lo; at < hi;) {
+    const int seg_end = min(hi, cur.cum + cur.nu);
+    split_query();
+    __syncthreads();  // the query is there; the waves are done with the last merge
+    QueryCols<D> qa_, qb_;
+    read_query(qa_, col);
+    if constexpr (WIDE) read_query(qb_, 16 + col);
+    Cursor nxt = cur;
+    next_row_group(p, nxt);
+    if (seg_end < hi) fetch_query(nxt);
+
     float m_run = -INFINITY, l_run = 0.f;
     floatx4_v o[MT];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) o[i] = floatx4_v{0.f, 0.f, 0.f, 0.f};
+    for (int k = 0; k < MT; ++k) o[k] = floatx4_v{0.f, 0.f, 0.f, 0.f};
 
     auto step = [&](int s) {
-      // ---- scores: this lane's are tokens 4 quad + r of both runs, of head `head`
+      // ---- scores: this lane's are tokens 4 quad + r of both runs, of head col & 7 (WIDE: col)
       float sc[8];
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
@@ -181,23 +321,20 @@ __global__ __launch_bounds__(64 * kWaves, 2) void decode_kernel(DecodeParams dp)
         }
       }
       // ---- what is not there: the last unit of a row, and blocks outside the pool
-      const int64_t t0 = u * kUnit;
-      if (!(t0 + kUnit <= len && phys[s][0] >= 0 && phys[s][1] >= 0)) {
+      if (have[s] != kUnit) {
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const int64_t left = phys[s][j] < 0 ? 0 : len - t0 - kv4::kRun * j - 4 * quad;  // this lane's tokens that are there
+          const int mine = (have[s] >> (8 + j) & 1) ? 0 : (have[s] & 255) - kv4::kRun * j - 4 * quad;  // this lane's tokens that are there
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            if (r >= left) sc[4 * j + r] = -INFINITY;
+            if (r >= mine) sc[4 * j + r] = -INFINITY;
           // their values may be anything, and 0 times a NaN is one
-          vr[s][j].scale &= left >= 4 ? 0xffffffffu : left <= 0 ? 0u : (1u << (8 * static_cast<int>(left))) - 1u;
+          vr[s][j].scale &= mine >= 4 ? 0xffffffffu : mine <= 0 ? 0u : (1u << (8 * mine)) - 1u;
         }
       }
-      const int64_t next = u + 2 * kWaves;
-#pragma unroll
-      for (int j = 0; j < 2; ++j) phys[s][j] = ahead[j];
-      fetch_keys(s, next);
-      entries(next + kWaves, ahead);
+      if (((i + 2) & 63) == 0) locate((i + 2) >> 6, false);
+      look(i + 2, s);
+      fetch_keys(s);
 
       // ---- online softmax
       float mx = fmaxf(fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3])), fmaxf(fmaxf(sc[4], sc[5]), fmaxf(sc[6], sc[7])));
@@ -207,24 +344,27 @@ __global__ __launch_bounds__(64 * kWaves, 2) void decode_kernel(DecodeParams dp)
         m_run = m_new;
         l_run *= corr;
 #pragma unroll
-        for (int i = 0; i < MT; ++i) o[i] *= corr;
+        for (int k = 0; k < MT; ++k) o[k] *= corr;
       }
       const float use = m_run == -INFINITY ? 0.f : m_run;
       bf16x8_v pb;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float pr = __builtin_amdgcn_exp2f(sc[i] - use);
+      for (int k = 0; k < 8; ++k) {
+        const float pr = __builtin_amdgcn_exp2f(sc[k] - use);
         l_run += pr;
-        pb[i] = static_cast<__bf16>(pr);
+        pb[k] = static_cast<__bf16>(pr);
       }
       // ---- values
       accumulate<D>(vr[s], pb, o);
-      fetch_values(s, next);
-      u += kWaves;
+      fetch_values(s);
+      ++i;
+      gu += kWaves;
     };
-    while (u < u1) {
-      step(0);
-      if (u >= u1) break;
+    while (gu < seg_end) {
+      if ((i & 1) == 0) {
+        step(0);
+        if (gu >= seg_end) break;
+      }
       step(1);
     }
 
@@ -236,60 +376,67 @@ __global__ __launch_bounds__(64 * kWaves, 2) void decode_kernel(DecodeParams dp)
     }
     __syncthreads();
     float big = -INFINITY;
+    float wm[kWaves];
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) big = fmaxf(big, s_m[w * 16 + col]);
+    for (int w = 0; w < kWaves; ++w) {
+      wm[w] = s_m[w * 16 + col];
+      big = fmaxf(big, wm[w]);
+    }
     const float use = big == -INFINITY ? 0.f : big;
+    if (wave == 0 && quad == 0) {
+      float l = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) l += s_l[w * 16 + col] * __builtin_amdgcn_exp2f(wm[w] - use);
+      s_total[col] = big;
+      s_total[16 + col] = l;
+    }
     const float f = __builtin_amdgcn_exp2f(m_run - use);
     if (col < S::kHeads && col < p.G) {
-      float* so = smem + (wave * S::kHeads + col) * S::kRow;
+      float* so = s_o + (wave * S::kHeads + col) * S::kRow;
 #pragma unroll
       for (int r = 0; r < 4; ++r)
 #pragma unroll
-        for (int i = 0; i < MT; i += 4)
-          *reinterpret_cast<floatx4_v*>(so + (4 * quad + r) * MT + i) = floatx4_v{o[i][r], o[i + 1][r], o[i + 2][r], o[i + 3][r]} * f;
+        for (int k = 0; k < MT; k += 4)
+          *reinterpret_cast<floatx4_v*>(so + (4 * quad + r) * MT + k) = floatx4_v{o[k][r], o[k + 1][r], o[k + 2][r], o[k + 3][r]} * f;
     }
     __syncthreads();
     const int64_t rg = static_cast<int64_t>(cur.b) * p.Hkv + cur.g;
     const bool whole = at == cur.cum && seg_end == cur.cum + cur.nu;
     const int64_t slot = wg + rg;
-    for (int e = tid; e < p.G * D; e += 64 * kWaves) {
+    for (int e = 4 * tid; e < p.G * D; e += 4 * 64 * kWaves) {
       const int h = e / D, d = e % D;
-      float m = -INFINITY;
+      const float l = s_total[16 + h];
+      const int64_t hq = cur.g * p.G + h;
+      uint2 gate = make_uint2(0, 0);
+      if (whole && p.gate != nullptr) gate = *reinterpret_cast<const uint2*>(p.gate + cur.b * p.gate_st + hq * p.gate_sh + d);
+      floatx4_v sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) m = fmaxf(m, s_m[w * 16 + h]);
-      const float mu = m == -INFINITY ? 0.f : m;
-      float sum = 0.f, l = 0.f;
-#pragma unroll
-      for (int w = 0; w < kWaves; ++w) {
-        sum += smem[(w * S::kHeads + h) * S::kRow + d];
-        l += s_l[w * 16 + h] * __builtin_amdgcn_exp2f(s_m[w * 16 + h] - mu);
-      }
+      for (int w = 0; w < kWaves; ++w) sum += *reinterpret_cast<const floatx4_v*>(s_o + (w * S::kHeads + h) * S::kRow + d);
       if (whole) {
-        const int64_t hq = cur.g * p.G + h;
-        float r = normalised(sum, l);
-        if (p.gate != nullptr) r *= sigmoid(bf16_to_f32(p.gate[cur.b * p.gate_st + hq * p.gate_sh + d]));
-        p.out[(static_cast<int64_t>(cur.b) * p.H + hq) * D + d] = f32_to_bf16(r);
+        float r[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          r[k] = normalised(sum[k], l);
+          if (p.gate != nullptr) {
+            const uint32_t w = k < 2 ? gate.x : gate.y;
+            r[k] *= sigmoid(__uint_as_float(k & 1 ? w & 0xffff0000u : w << 16));
+          }
+        }
+        uint2 packed;
+        packed.x = static_cast<uint32_t>(f32_to_bf16(r[0])) | static_cast<uint32_t>(f32_to_bf16(r[1])) << 16;
+        packed.y = static_cast<uint32_t>(f32_to_bf16(r[2])) | static_cast<uint32_t>(f32_to_bf16(r[3])) << 16;
+        *reinterpret_cast<uint2*>(p.out + (static_cast<int64_t>(cur.b) * p.H + hq) * D + d) = packed;
       } else {
-        dp.part_o[(slot * p.G + h) * D + d] = sum;
-        if (d == 0) *reinterpret_cast<float2*>(dp.part_ml + (slot * p.G + h) * 2) = make_float2(m, l);
+        *reinterpret_cast<floatx4_v*>(dp.part_o + (slot * p.G + h) * D + d) = sum;
+        if (d == 0) *reinterpret_cast<float2*>(dp.part_ml + (slot * p.G + h) * 2) = make_float2(s_total[h], l);
       }
     }
     if (tid == 0) {
-      if (at == cur.cum) dp.rg_wgs[2 * rg] = whole ? -1 : static_cast<int32_t>(wg);
-      if (seg_end == cur.cum + cur.nu) dp.rg_wgs[2 * rg + 1] = static_cast<int32_t>(wg);
+      if (at == cur.cum) dp.rg_wgs[2 * rg] = whole ? -1 : wg;
+      if (seg_end == cur.cum + cur.nu) dp.rg_wgs[2 * rg + 1] = wg;
     }
     at = seg_end;
-    if (at < hi) {
-      __syncthreads();  // smem is written again
-      cur.cum += cur.nu;
-      if (++cur.g == p.Hkv) {
-        cur.g = 0;
-        do {
-          ++cur.b;
-          cur.nu = cur.b < p.B ? uniform64(row_units(p, cur.b)) : 0;
-        } while (cur.nu == 0 && cur.b < p.B);
-      }
-    }
+    cur = nxt;
   }
 }
 
@@ -425,6 +572,8 @@ extern "C" int qa_paged_attention_decode_kv4(const void* query, int32_t q_dtype,
   p.c.lens = sequence_lengths;
   const int64_t groups = batch * kv->kv_heads;
   const int64_t max_tokens = max_blocks * block_size;
+  QA_REQUIRE(groups * ceil_div(max_tokens, kUnit) <= 0x7fffffff, "%s: the tables cover too many tokens: %lld row groups of up to %lld", a.what, static_cast<long long>(groups),
+             static_cast<long long>(max_tokens));
   const int64_t need = workspace_bytes_of(batch, heads, kv->kv_heads, head_dim, max_tokens);
   QA_REQUIRE(workspace != nullptr && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 15u) == 0,
              "paged decode workspace too small or not 16-byte aligned: need %lld bytes, have %lld", static_cast<long long>(need), static_cast<long long>(workspace_bytes));
