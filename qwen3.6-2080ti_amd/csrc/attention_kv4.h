@@ -83,14 +83,17 @@ struct KeyRun {
   uint32_t scale;  // byte i: slice i
 };
 
-template <int D>
+// Cache policy of a load: kOnce (non-temporal) for tiles that one workgroup reads once.
+constexpr int kShared = 0, kOnce = 2;
+
+template <int D, int POLICY>
 __device__ __forceinline__ void load_keys(KeyRun<D>& k, __amdgpu_buffer_rsrc_t r, int lane) {
 #pragma unroll
-  for (int i = 0; i < D / 128; ++i) k.code[i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, 16 * lane + 1024 * i, 0, 0));
+  for (int i = 0; i < D / 128; ++i) k.code[i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, 16 * lane + 1024 * i, 0, POLICY));
   if constexpr (D == 256)
-    k.scale = __builtin_amdgcn_raw_buffer_load_b16(r, kv4::Run<D>::kCodes + 2 * lane, 0, 0);
+    k.scale = __builtin_amdgcn_raw_buffer_load_b16(r, kv4::Run<D>::kCodes + 2 * lane, 0, POLICY);
   else
-    k.scale = __builtin_amdgcn_raw_buffer_load_b8(r, kv4::Run<D>::kCodes + lane, 0, 0);
+    k.scale = __builtin_amdgcn_raw_buffer_load_b8(r, kv4::Run<D>::kCodes + lane, 0, POLICY);
 }
 
 // A run of values: lane 16 q + c holds tokens 4 q .. 4 q + 3, dims c D/16 ..
@@ -100,12 +103,12 @@ struct ValueRun {
   uint32_t scale;  // byte r: token 4 q + r
 };
 
-template <int D>
+template <int D, int POLICY>
 __device__ __forceinline__ void load_values(ValueRun<D>& v, __amdgpu_buffer_rsrc_t r, int lane) {
 #pragma unroll
-  for (int i = 0; i < D / 128; ++i) v.code[i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, 16 * lane + 1024 * i, 0, 0));
+  for (int i = 0; i < D / 128; ++i) v.code[i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, 16 * lane + 1024 * i, 0, POLICY));
   const int group = (lane & 15) / (512 / D);
-  v.scale = __builtin_amdgcn_raw_buffer_load_b32(r, kv4::Run<D>::kCodes + 16 * group + 4 * (lane >> 4), 0, 0);
+  v.scale = __builtin_amdgcn_raw_buffer_load_b32(r, kv4::Run<D>::kCodes + 16 * group + 4 * (lane >> 4), 0, POLICY);
 }
 
 // The query columns of a wave in fp8.  Byte order of the B operand: lane 16 q + n holds of column n and each slice of

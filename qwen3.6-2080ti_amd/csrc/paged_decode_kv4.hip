@@ -55,13 +55,14 @@ __device__ __forceinline__ void next_row_group(const Params& p, Cursor& c) {
   } while (c.nu == 0 && c.b < p.B);
 }
 
-// Inclusive sum over the lanes.
-__device__ __forceinline__ int lane_scan(int v, int lane) {
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int up = __shfl_up(v, off, 64);
-    if (lane >= off) v += up;
-  }
+// Inclusive sum over the lanes: shifts within rows of 16, then the rows' last sums passed on (DPP, no LDS).
+__device__ __forceinline__ int lane_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // row_shr:1
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);  // row_shr:2
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);  // row_shr:4
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);  // row_shr:8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row_bcast:15 into rows 1 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // row_bcast:31 into rows 2 and 3
   return v;
 }
 
@@ -107,16 +108,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void decode_kernel(DecodeParams dp)
   const int quad = lane >> 4;
 
   // ---- this workgroup's share
-  int T = 0;
-  int64_t len_first = 0;  // of row `lane`, kept for the search
-  for (int b0 = 0; b0 < p.B; b0 += 64) {
-    const int64_t len = b0 + lane < p.B ? row_tokens(p, b0 + lane) : 0;
-    if (b0 == 0) len_first = len;
-    T += units_of(len);
-  }
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) T += __shfl_xor(T, off, 64);
-  T = __builtin_amdgcn_readfirstlane(T) * p.Hkv;
+  // rows of up to 64 are loaded and summed once, for the total and for the search below
+  const int64_t len_first = lane < p.B ? row_tokens(p, lane) : 0;
+  const int incl_first = lane_scan(units_of(len_first) * p.Hkv);
+  int T = __builtin_amdgcn_readlane(incl_first, 63);
+  for (int b0 = 64; b0 < p.B; b0 += 64) T += __builtin_amdgcn_readlane(lane_scan((b0 + lane < p.B ? units_of(row_tokens(p, b0 + lane)) : 0) * p.Hkv), 63);
   // a workgroup has a unit for each wave before another one starts
   const int W = min(dp.n_wgs, (T + kWaves - 1) / kWaves);
   const int wg = blockIdx.x;
@@ -136,7 +132,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void decode_kernel(DecodeParams dp)
     for (int b0 = 0; b0 < p.B; b0 += 64) {
       const int64_t len = b0 == 0 ? len_first : b0 + lane < p.B ? row_tokens(p, b0 + lane) : 0;
       const int nu = units_of(len);
-      const int incl = lane_scan(nu * p.Hkv, lane);
+      const int incl = b0 == 0 ? incl_first : lane_scan(nu * p.Hkv);
       const int chunk = __builtin_amdgcn_readlane(incl, 63);
       if (begin && lo >= base && lo < base + chunk) {
         const int first = __ffsll(static_cast<unsigned long long>(__ballot(base + incl > lo))) - 1;
@@ -147,11 +143,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void decode_kernel(DecodeParams dp)
         cur.cum = before + cur.g * cur.nu;
       }
       int pos = 0;  // rows of the block that end at or before gu
-#pragma unroll
-      for (int step = 32; step > 0; step >>= 1) {
-        const int end = __shfl(incl, pos + step - 1, 64);
-        if (base + end <= gu) pos += step;
-      }
+      const int rows = min(63, p.B - b0);
+      for (int r = 0; r < rows; ++r) pos += base + __builtin_amdgcn_readlane(incl, r) <= gu;
       const int n = __shfl(nu, pos, 64);
       const int before = base + __shfl(incl, pos, 64) - n * p.Hkv;
       const int64_t t = (static_cast<int64_t>(__shfl(static_cast<int>(len >> 32), pos, 64)) << 32) | static_cast<uint32_t>(__shfl(static_cast<int>(len), pos, 64));
@@ -201,18 +194,12 @@ __global__ __launch_bounds__(64 * kWaves, 2) void decode_kernel(DecodeParams dp)
   };
   auto fetch_keys = [&](int s) {
 #pragma unroll
-    for (int j = 0; j < 2; ++j) load_keys<D>(kr[s][j], rsrc(p.kpool, where[j]), lane);
+    for (int j = 0; j < 2; ++j) load_keys<D, kOnce>(kr[s][j], rsrc(p.kpool, where[j]), lane);
   };
   auto fetch_values = [&](int s) {
 #pragma unroll
-    for (int j = 0; j < 2; ++j) load_values<D>(vr[s][j], rsrc(p.vpool, where[j]), lane);
+    for (int j = 0; j < 2; ++j) load_values<D, kOnce>(vr[s][j], rsrc(p.vpool, where[j]), lane);
   };
-#pragma unroll
-  for (int s = 0; s < 2; ++s) {
-    look(s, s);
-    fetch_keys(s);
-    fetch_values(s);
-  }
 
   // ---- the query of a row group: wave w takes heads w and w + 8, lane l dims E l ..
   constexpr int E = D / 64;
@@ -285,7 +272,13 @@ __global__ __launch_bounds__(64 * kWaves, 2) void decode_kernel(DecodeParams dp)
     }
     q.scale = s_qscale[row];
   };
-  fetch_query(cur);
+  fetch_query(cur);  // before the tiles: loads are waited for in their order
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    look(s, s);
+    fetch_keys(s);
+    fetch_values(s);
+  }
   const float qk_scale = p.scale * kLog2e;
 
   int i = 0;                // the wave's next unit, in slot i & 1

@@ -175,7 +175,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams p
   };
   const bool unpacks = wave < 4;
   ValueRun<D> vr;
-  auto fetch_values = [&]() { load_values<D>(vr, rsrc(vb), lane); };
+  auto fetch_values = [&]() { load_values<D, kShared>(vr, rsrc(vb), lane); };
   // what of vr no column sees, or not every column where it is NaN, leaves the product
   auto trim = [&](int64_t kt, int buf) {
     if (kt * kTile + kTile <= first_pos + 1) return;  // every column sees all of the tile
