@@ -17,6 +17,8 @@
 
 #include "kv4.h"
 
+#include <atomic>
+
 namespace qa {
 namespace attn4 {
 
@@ -257,6 +259,21 @@ __device__ __forceinline__ float normalised(float o, float l) {
 __device__ __forceinline__ float sigmoid(float x) { return 1.f / (1.f + __expf(-x)); }
 
 // ---- host ------------------------------------------------------------------
+// Lets a kernel have `bytes` of dynamic LDS, once per device: the call costs the host about a microsecond.
+template <auto KERNEL>
+inline int reserve_lds(const char* what, int bytes) {
+  static std::atomic<uint64_t> done{0};
+  int device = 0;
+  hipError_t err = hipGetDevice(&device);
+  if (err != hipSuccess) return fail("%s: hipGetDevice failed: %s", what, hipGetErrorString(err));
+  const uint64_t bit = uint64_t{1} << (device & 63);
+  if (device < 64 && (done.load(std::memory_order_relaxed) & bit)) return 0;
+  err = hipFuncSetAttribute(reinterpret_cast<const void*>(KERNEL), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (err != hipSuccess) return fail("%s: cannot reserve %d bytes of LDS: %s", what, bytes, hipGetErrorString(err));
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return 0;
+}
+
 struct Args {
   const char* what;
   const void* query;

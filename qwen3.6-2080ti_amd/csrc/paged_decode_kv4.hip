@@ -520,8 +520,7 @@ static int64_t workspace_bytes_of(int64_t batch, int heads, int kv_heads, int he
 template <int D, bool WIDE>
 static int launch(const DecodeParams& p, hipStream_t stream) {
   using S = Smem<D, WIDE>;
-  const hipError_t err = hipFuncSetAttribute(reinterpret_cast<const void*>(&decode_kernel<D, WIDE>), hipFuncAttributeMaxDynamicSharedMemorySize, S::kBytes);
-  if (err != hipSuccess) return fail("paged_attention_decode_kv4: cannot reserve %d bytes of LDS: %s", S::kBytes, hipGetErrorString(err));
+  if (int rc = reserve_lds<&decode_kernel<D, WIDE>>("paged_attention_decode_kv4", S::kBytes)) return rc;
   {
     KernelTimer timer_("decode_kv4", stream);
     hipLaunchKernelGGL((decode_kernel<D, WIDE>), dim3(p.n_wgs), dim3(64 * kWaves), S::kBytes, stream, p);

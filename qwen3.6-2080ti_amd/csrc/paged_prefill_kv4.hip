@@ -546,8 +546,7 @@ static int64_t workspace_of(int splits, int64_t total, int heads, int head_dim) 
 
 template <int D>
 static int launch(const PrefillParams& p, dim3 grid, int64_t max_new, hipStream_t stream) {
-  const hipError_t err = hipFuncSetAttribute(reinterpret_cast<const void*>(&prefill_kernel<D>), hipFuncAttributeMaxDynamicSharedMemorySize, Smem<D>::kBytes);
-  if (err != hipSuccess) return fail("paged_attention_prefill_kv4: cannot reserve %d bytes of LDS: %s", Smem<D>::kBytes, hipGetErrorString(err));
+  if (int rc = reserve_lds<&prefill_kernel<D>>("paged_attention_prefill_kv4", Smem<D>::kBytes)) return rc;
   {
     KernelTimer timer_("prefill_kv4", stream);
     hipLaunchKernelGGL(prefill_kernel<D>, grid, dim3(64 * kWaves), Smem<D>::kBytes, stream, p);

@@ -1089,10 +1089,17 @@ def qk_norm_rope_kv_append(
 
 def _launch(device: torch.device, fn: Any, *args: Any) -> int:
     """``fn(*args, stream)`` on ``device``'s current stream, with that device current."""
-    if torch._C._cuda_getDevice() == device.index:
-        return fn(*args, _stream(device))
+    index = device.index
+    if torch._C._cuda_getDevice() == index:
+        return fn(*args, torch._C._cuda_getCurrentRawStream(index))
     with torch.cuda.device(device):
-        return fn(*args, _stream(device))
+        return fn(*args, torch._C._cuda_getCurrentRawStream(index))
+
+
+def _same_device(device: torch.device, **tensors: Any) -> None:
+    """Names the tensor that is not on ``device`` (called where a cheaper check has found one)."""
+    for name, tensor in tensors.items():
+        _require_cuda(tensor, name, device)
 
 
 def kv4_tile_bytes(head_dim: int, block_size: int) -> int:
@@ -1104,42 +1111,48 @@ def kv4_tile_bytes(head_dim: int, block_size: int) -> int:
 
 def _kv4_descriptor(key_pool: torch.Tensor, value_pool: torch.Tensor, block_size: int, device: torch.device) -> tuple[L.PagedKV, int]:
     """Descriptor and head_dim of a 4-bit pool ``(P, H_kv, kv4_tile_bytes(D, block_size))``."""
-    _require_cuda(key_pool, "key_pool", device)
-    _require_cuda(value_pool, "value_pool", device)
-    if key_pool.dtype != torch.uint8 or value_pool.dtype != torch.uint8 or key_pool.dim() != 3 or value_pool.shape != key_pool.shape:
+    if key_pool.device != device or value_pool.device != device:
+        _same_device(device, key_pool=key_pool, value_pool=value_pool)
+    shape, strides = key_pool.shape, key_pool.stride()
+    if key_pool.dtype is not torch.uint8 or value_pool.dtype is not torch.uint8 or len(shape) != 3 or value_pool.shape != shape:
         raise RuntimeError("4-bit pools must be uint8 (blocks, kv_heads, tile bytes) and alike")
-    strides = key_pool.stride()
     if strides[2] != 1 or value_pool.stride() != strides:
         raise RuntimeError("key/value pools must share strides with contiguous tiles")
-    blocks, kv_heads, tile = key_pool.shape
+    blocks, kv_heads, tile = shape
     for head_dim in (256, 128):
-        if tile == kv4_tile_bytes(head_dim, block_size):
+        if tile * 32 == block_size * 17 * head_dim:
             return L.PagedKV(key_pool.data_ptr(), value_pool.data_ptr(), None, None, None, blocks, 0, strides[0], strides[1], 0, kv_heads, L.QA_KV4), head_dim
     raise RuntimeError(f"a tile of {tile} bytes is no block of {block_size} tokens of 128 or 256 dims in 4 bits")
 
 
-def _rows(tensor: torch.Tensor, multiple: int) -> torch.Tensor:
-    """``tensor`` (.., .., D) as it is where its rows can be read in aligned pieces of ``multiple`` elements, else a copy."""
+def _rows(tensor: torch.Tensor, multiple: int) -> tuple[torch.Tensor, int, int]:
+    """``tensor`` (.., .., D) as it is where its rows can be read in aligned pieces of ``multiple`` elements, else a
+    copy; and its row strides."""
     strides = tensor.stride()
     if strides[-1] == 1 and strides[0] % multiple == 0 and strides[1] % multiple == 0 and tensor.data_ptr() % (multiple * tensor.element_size()) == 0:
-        return tensor
-    return tensor.contiguous()
+        return tensor, strides[0], strides[1]
+    tensor = tensor.contiguous()
+    strides = tensor.stride()
+    return tensor, strides[0], strides[1]
 
 
-def _kv4_gate(gate: torch.Tensor | None, rows: int, heads: int, head_dim: int, device: torch.device) -> torch.Tensor | None:
+def _kv4_gate(gate: torch.Tensor | None, rows: int, heads: int, head_dim: int, device: torch.device) -> tuple[torch.Tensor | None, int, int, int]:
+    """The gate as ``(tensor to keep, pointer, token stride, head stride)``."""
     if gate is None:
-        return None
-    _require_cuda(gate, "gate", device)
-    _require(gate.dtype == torch.bfloat16, "gate must be bfloat16")
+        return None, 0, 0, 0
+    if gate.device != device:
+        _require_cuda(gate, "gate", device)
+    _require(gate.dtype is torch.bfloat16, "gate must be bfloat16")
     if gate.dim() == 2 and gate.shape == (rows, heads * head_dim):
         gate = gate.reshape(rows, heads, head_dim)
     _require(gate.shape == (rows, heads, head_dim), "gate must be (tokens, heads*head_dim) or (tokens, heads, head_dim)")
-    return _rows(gate, 4)
+    gate, stride_t, stride_h = _rows(gate, 4)
+    return gate, gate.data_ptr(), stride_t, stride_h
 
 
 def _kv4_out(out: torch.Tensor | None, like: torch.Tensor) -> torch.Tensor:
     if out is None:
-        return torch.empty(like.shape, dtype=torch.bfloat16, device=like.device)
+        return torch.empty_like(like) if like.is_contiguous() else like.new_empty(like.shape)
     _require_cuda(out, "out", like.device)
     _require(out.dtype == torch.bfloat16 and out.shape == like.shape and out.is_contiguous(), "out must be contiguous bfloat16 of query's shape")
     return out
@@ -1180,39 +1193,41 @@ def paged_kv_plan(
     read back, so the call can be captured in a HIP graph.
     """
     lib = L.load_library()
-    _require_cuda(block_tables, "block_tables")
     device = block_tables.device
-    for tensor, name in ((lengths, "lengths"), (free_list, "free_list"), (free_state, "free_state"), (status, "status")):
-        _require_cuda(tensor, name, device)
-    _require(block_tables.dtype == torch.int32 and block_tables.dim() == 2 and block_tables.stride(1) == 1, "block_tables must be int32 [batch, max_blocks] with contiguous rows")
+    if device.type != "cuda" or not (lengths.device == free_list.device == free_state.device == status.device == device):
+        _same_device(device, block_tables=block_tables, lengths=lengths, free_list=free_list, free_state=free_state, status=status)
+    i32 = torch.int32
+    _require(block_tables.dtype is i32 and block_tables.dim() == 2 and block_tables.stride(1) == 1, "block_tables must be int32 [batch, max_blocks] with contiguous rows")
     batch, max_blocks = block_tables.shape
     _require(batch > 0 and max_blocks > 0, "block_tables must have shape [batch, max_blocks]")
-    _require(lengths.dtype == torch.int32 and lengths.shape == (batch,) and lengths.is_contiguous(), "lengths must be a contiguous int32 [batch] tensor")
-    _require(free_list.dtype == torch.int32 and free_list.dim() == 1 and free_list.is_contiguous(), "free_list must be a contiguous int32 vector")
-    _require(free_state.dtype == torch.int32 and free_state.numel() == 2 and free_state.is_contiguous(), "free_state must be int32 [head, count]")
-    _require(status.dtype == torch.int32 and status.numel() >= 1, "status must be an int32 tensor")
+    _require(lengths.dtype is i32 and lengths.shape == (batch,) and lengths.is_contiguous(), "lengths must be a contiguous int32 [batch] tensor")
+    _require(free_list.dtype is i32 and free_list.dim() == 1 and free_list.is_contiguous(), "free_list must be a contiguous int32 vector")
+    _require(free_state.dtype is i32 and free_state.numel() == 2 and free_state.is_contiguous(), "free_state must be int32 [head, count]")
+    _require(status.dtype is i32 and status.numel() >= 1, "status must be an int32 tensor")
     max_tokens = int(max_tokens)
     _require(max_tokens >= 0, "max_tokens must be non-negative")
     count_ptr, count_code, count_scalar = 0, L.QA_I32, 0
     if isinstance(counts, torch.Tensor):
-        _require_cuda(counts, "counts", device)
+        if counts.device != device:
+            _require_cuda(counts, "counts", device)
         _index_dtype(counts, "counts")
         _require(counts.shape == (batch,) and counts.is_contiguous(), "counts must be a contiguous [batch] tensor")
-        count_ptr, count_code = _ptr(counts), _code(counts)
+        count_ptr, count_code = counts.data_ptr(), _code(counts)
     else:
         count_scalar = int(counts)
         _require(count_scalar >= 0, "counts must be non-negative")
-    # one allocation: cu_seqlens, starts, the kernel's scratch row sums, positions
-    ints = torch.empty(3 * batch + 1 + max_tokens, dtype=torch.int32, device=device)
     slots = torch.empty(max_tokens, dtype=torch.int64, device=device)
+    # one allocation: cu_seqlens, starts, the kernel's scratch row sums, positions
+    ints = lengths.new_empty(3 * batch + 1 + max_tokens)
     at = ints.data_ptr()
     code = _launch(
-        device, lib.qa_paged_kv_plan, _ptr(block_tables), block_tables.stride(0), max_blocks, _ptr(lengths), count_ptr, count_code, count_scalar, batch,
-        int(block_size), _ptr(free_list), free_list.numel(), _ptr(free_state), _ptr(status), max_tokens, at, at + 4 * (batch + 1), at + 4 * (3 * batch + 1),
-        _ptr(slots), at + 4 * (2 * batch + 1), 4 * batch,
+        device, lib.qa_paged_kv_plan, block_tables.data_ptr(), block_tables.stride(0), max_blocks, lengths.data_ptr(), count_ptr, count_code, count_scalar, batch,
+        int(block_size), free_list.data_ptr(), free_list.numel(), free_state.data_ptr(), status.data_ptr(), max_tokens, at, at + 4 * (batch + 1), at + 4 * (3 * batch + 1),
+        slots.data_ptr(), at + 4 * (2 * batch + 1), 4 * batch,
     )
     L.check(lib, code, "paged_kv_plan")
-    return PagedPlan(ints[: batch + 1], ints[batch + 1 : 2 * batch + 1], ints[3 * batch + 1 :], slots)
+    cu_seqlens, starts, _, positions = ints.split_with_sizes((batch + 1, batch, batch, max_tokens))
+    return PagedPlan(cu_seqlens, starts, positions, slots)
 
 
 def paged_kv4_append(key: torch.Tensor, value: torch.Tensor, key_pool: torch.Tensor, value_pool: torch.Tensor, slots: torch.Tensor, block_size: int) -> None:
@@ -1224,21 +1239,23 @@ def paged_kv4_append(key: torch.Tensor, value: torch.Tensor, key_pool: torch.Ten
     They have to be distinct.
     """
     lib = L.load_library()
-    _require_cuda(key, "key")
     device = key.device
-    _require_cuda(value, "value", device)
-    _require_cuda(slots, "slots", device)
+    if device.type != "cuda" or not (value.device == slots.device == device):
+        _same_device(device, key=key, value=value, slots=slots)
     _index_dtype(slots, "slots")
     desc, head_dim = _kv4_descriptor(key_pool, value_pool, block_size, device)
-    _require(key.dim() == 3 and key.shape[1:] == (desc.kv_heads, head_dim) and value.shape == key.shape, "key/value must be (tokens, kv_heads, head_dim) of the pool's heads")
+    shape = key.shape
+    _require(len(shape) == 3 and shape[1] == desc.kv_heads and shape[2] == head_dim and value.shape == shape, "key/value must be (tokens, kv_heads, head_dim) of the pool's heads")
     _float_dtype(key, "key")
-    _require(value.dtype == key.dtype, "key and value must share a dtype")
-    _require(slots.dim() == 1 and slots.shape[0] == key.shape[0], "slots must have one entry per token")
-    multiple = 8 if key.dtype == torch.bfloat16 else 4
-    k, v, s = _rows(key, multiple), _rows(value, multiple), slots.contiguous()
+    _require(value.dtype is key.dtype, "key and value must share a dtype")
+    _require(slots.shape == shape[:1], "slots must have one entry per token")
+    multiple = 8 if key.dtype is torch.bfloat16 else 4
+    k, k_st, k_sh = _rows(key, multiple)
+    v, v_st, v_sh = _rows(value, multiple)
+    s = slots.contiguous()
     code = _launch(
-        device, lib.qa_paged_kv4_append, _ptr(k), _ptr(v), _code(k), k.stride(0), k.stride(1), v.stride(0), v.stride(1), k.shape[0], head_dim, ctypes.byref(desc),
-        _ptr(s), _code(s), int(block_size),
+        device, lib.qa_paged_kv4_append, k.data_ptr(), v.data_ptr(), _code(k), k_st, k_sh, v_st, v_sh, shape[0], head_dim, ctypes.byref(desc), s.data_ptr(), _code(s),
+        int(block_size),
     )
     L.check(lib, code, "paged_kv4_append")
 
@@ -1250,22 +1267,23 @@ def paged_kv4_gather(key_pool: torch.Tensor, value_pool: torch.Tensor, block_tab
     zeros; a group stored from an infinity or a NaN reads as NaN.
     """
     lib = L.load_library()
-    _require_cuda(key_pool, "key_pool")
     device = key_pool.device
-    _require_cuda(block_tables, "block_tables", device)
+    if device.type != "cuda" or block_tables.device != device:
+        _same_device(device, key_pool=key_pool, block_tables=block_tables)
     _index_dtype(block_tables, "block_tables")
     desc, head_dim = _kv4_descriptor(key_pool, value_pool, block_size, device)
     tables = block_tables.contiguous()
     if tables.dim() == 1:
         tables = tables.unsqueeze(0)
     _require(tables.dim() == 2 and tables.shape[1] > 0, "block_tables must have shape [batch, max_blocks]")
-    batch = tables.shape[0]
-    _require(int(valid) >= 0, "valid must be non-negative")
-    key_out = torch.empty((batch, desc.kv_heads, int(valid), head_dim), dtype=torch.bfloat16, device=device)
+    batch, max_blocks = tables.shape
+    valid = int(valid)
+    _require(valid >= 0, "valid must be non-negative")
+    key_out = torch.empty((batch, desc.kv_heads, valid, head_dim), dtype=torch.bfloat16, device=device)
     value_out = torch.empty_like(key_out)
     code = _launch(
-        device, lib.qa_paged_kv4_gather, ctypes.byref(desc), head_dim, batch, _ptr(tables), _code(tables), tables.stride(0), tables.shape[1], int(valid),
-        int(block_size), _ptr(key_out), _ptr(value_out),
+        device, lib.qa_paged_kv4_gather, ctypes.byref(desc), head_dim, batch, tables.data_ptr(), _code(tables), max_blocks, max_blocks, valid, int(block_size),
+        key_out.data_ptr(), value_out.data_ptr(),
     )
     L.check(lib, code, "paged_kv4_gather")
     return key_out, value_out
@@ -1290,31 +1308,30 @@ def paged_attention_decode_kv4(
     ``(B, H, 1, D)`` bf16, in ``out`` where it is given.
     """
     lib = L.load_library()
-    _require_cuda(query, "query")
     device = query.device
-    _require_cuda(block_tables, "block_tables", device)
-    _require_cuda(sequence_lengths, "sequence_lengths", device)
-    _require(query.dtype == torch.bfloat16, "query must be bfloat16")
+    if device.type != "cuda" or not (block_tables.device == sequence_lengths.device == device):
+        _same_device(device, query=query, block_tables=block_tables, sequence_lengths=sequence_lengths)
+    _require(query.dtype is torch.bfloat16, "query must be bfloat16")
     _index_dtype(block_tables, "block_tables")
     _index_dtype(sequence_lengths, "sequence_lengths")
-    _require(query.dim() == 4 and query.shape[2] == 1, "query must have shape [batch, heads, 1, head_dim]")
+    shape = query.shape
+    _require(len(shape) == 4 and shape[2] == 1, "query must have shape [batch, heads, 1, head_dim]")
     desc, head_dim = _kv4_descriptor(key_pool, value_pool, block_size, device)
-    batch, heads = query.shape[:2]
-    _require(query.shape[3] == head_dim, "KV head_dim must match query")
+    batch, heads = shape[0], shape[1]
+    _require(shape[3] == head_dim, "KV head_dim must match query")
     _require(block_tables.dim() == 2 and block_tables.shape[0] == batch and block_tables.shape[1] > 0, "block_tables must have shape [batch, max_blocks]")
-    _require(sequence_lengths.shape == (batch,), "sequence_lengths batch must match query")
+    _require(sequence_lengths.shape == shape[:1], "sequence_lengths batch must match query")
     _require(heads % desc.kv_heads == 0, "KV heads must divide query heads")
-    q = _rows(query.squeeze(2), 8)
-    g = _kv4_gate(gate, batch, heads, head_dim, device)
+    q, q_sb, q_sh = _rows(query, 8)
+    g, g_ptr, g_sb, g_sh = _kv4_gate(gate, batch, heads, head_dim, device)
     tables, lens = block_tables.contiguous(), sequence_lengths.contiguous()
     max_blocks = tables.shape[1]
     result = _kv4_out(out, query)
     nbytes = lib.qa_paged_attention_decode_kv4_workspace(batch, heads, desc.kv_heads, head_dim, max_blocks * block_size)
-    ws = torch.empty(max(nbytes, 4), dtype=torch.uint8, device=device)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
     code = _launch(
-        device, lib.qa_paged_attention_decode_kv4, _ptr(q), _code(q), q.stride(0), q.stride(1), batch, heads, head_dim, ctypes.byref(desc), _ptr(tables),
-        _code(tables), tables.stride(0), max_blocks, _ptr(lens), _code(lens), int(block_size), float(scale or 0.0), _ptr(g), 0 if g is None else g.stride(0),
-        0 if g is None else g.stride(1), _ptr(result), _ptr(ws), ws.numel(),
+        device, lib.qa_paged_attention_decode_kv4, q.data_ptr(), L.QA_BF16, q_sb, q_sh, batch, heads, head_dim, ctypes.byref(desc), tables.data_ptr(), _code(tables),
+        max_blocks, max_blocks, lens.data_ptr(), _code(lens), int(block_size), float(scale or 0.0), g_ptr, g_sb, g_sh, result.data_ptr(), ws.data_ptr(), nbytes,
     )
     L.check(lib, code, "paged_attention_decode_kv4")
     return result
@@ -1342,30 +1359,32 @@ def paged_attention_prefill_kv4(
     last sequence are not written.
     """
     lib = L.load_library()
-    _require_cuda(query, "query")
     device = query.device
-    _require(query.dtype == torch.bfloat16 and query.dim() == 3, "query must be (tokens, heads, head_dim) bfloat16")
-    for tensor, name in ((cu_seqlens, "cu_seqlens"), (prefix_lens, "prefix_lens"), (block_tables, "block_tables")):
-        _require_cuda(tensor, name, device)
-        _index_dtype(tensor, name)
-    _require(cu_seqlens.dtype == prefix_lens.dtype, "cu_seqlens and prefix_lens must share a dtype")
+    if device.type != "cuda" or not (cu_seqlens.device == prefix_lens.device == block_tables.device == device):
+        _same_device(device, query=query, cu_seqlens=cu_seqlens, prefix_lens=prefix_lens, block_tables=block_tables)
+    shape = query.shape
+    _require(query.dtype is torch.bfloat16 and len(shape) == 3, "query must be (tokens, heads, head_dim) bfloat16")
+    _index_dtype(cu_seqlens, "cu_seqlens")
+    _index_dtype(block_tables, "block_tables")
+    _require(cu_seqlens.dtype is prefix_lens.dtype, "cu_seqlens and prefix_lens must share a dtype")
     desc, head_dim = _kv4_descriptor(key_pool, value_pool, block_size, device)
-    tokens, heads = query.shape[:2]
-    _require(query.shape[2] == head_dim, "KV head_dim must match query")
+    tokens, heads = shape[0], shape[1]
+    _require(shape[2] == head_dim, "KV head_dim must match query")
     _require(heads % desc.kv_heads == 0, "KV heads must divide query heads")
     _require(prefix_lens.dim() == 1 and cu_seqlens.shape == (prefix_lens.shape[0] + 1,), "cu_seqlens must have batch + 1 entries")
     batch = prefix_lens.shape[0]
     _require(block_tables.dim() == 2 and block_tables.shape[0] == batch and block_tables.shape[1] > 0, "block_tables must have shape [batch, max_blocks]")
-    q = _rows(query, 8)
-    g = _kv4_gate(gate, tokens, heads, head_dim, device)
+    q, q_st, q_sh = _rows(query, 8)
+    g, g_ptr, g_st, g_sh = _kv4_gate(gate, tokens, heads, head_dim, device)
     cu, prefix, tables = cu_seqlens.contiguous(), prefix_lens.contiguous(), block_tables.contiguous()
+    max_blocks = tables.shape[1]
     result = _kv4_out(out, query)
-    nbytes = lib.qa_paged_attention_prefill_kv4_workspace(tokens, batch, int(max_new), heads, desc.kv_heads, head_dim, tables.shape[1] * block_size)
+    nbytes = lib.qa_paged_attention_prefill_kv4_workspace(tokens, batch, int(max_new), heads, desc.kv_heads, head_dim, max_blocks * block_size)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
     code = _launch(
-        device, lib.qa_paged_attention_prefill_kv4, _ptr(q), _code(q), q.stride(0), q.stride(1), tokens, _ptr(cu), _ptr(prefix), _code(cu), batch, int(max_new),
-        heads, head_dim, ctypes.byref(desc), _ptr(tables), _code(tables), tables.stride(0), tables.shape[1], int(block_size), float(scale or 0.0), _ptr(g),
-        0 if g is None else g.stride(0), 0 if g is None else g.stride(1), _ptr(result), _ptr(ws), nbytes,
+        device, lib.qa_paged_attention_prefill_kv4, q.data_ptr(), L.QA_BF16, q_st, q_sh, tokens, cu.data_ptr(), prefix.data_ptr(), _code(cu), batch, int(max_new),
+        heads, head_dim, ctypes.byref(desc), tables.data_ptr(), _code(tables), max_blocks, max_blocks, int(block_size), float(scale or 0.0), g_ptr, g_st, g_sh,
+        result.data_ptr(), _ptr(ws), nbytes,
     )
     L.check(lib, code, "paged_attention_prefill_kv4")
     return result
@@ -1438,30 +1457,36 @@ def qk_norm_mrope_kv_append(
     ``(query (tokens, H, D) bf16, gate (tokens, H, D) view of q_proj or None)``.
     """
     lib = L.load_library()
-    _require_cuda(q_proj, "q_proj")
     device = q_proj.device
-    for tensor, name in ((k_proj, "k_proj"), (v_proj, "v_proj"), (q_norm_weight, "q_norm_weight"), (k_norm_weight, "k_norm_weight"), (positions, "positions"),
-                         (key_pool, "key_pool"), (value_pool, "value_pool"), (slots, "slots")):
-        _require_cuda(tensor, name, device)
-    if key_pool.dtype == torch.uint8:
+    if device.type != "cuda" or not (k_proj.device == v_proj.device == q_norm_weight.device == k_norm_weight.device == positions.device == slots.device == key_pool.device == device):
+        _same_device(device, q_proj=q_proj, k_proj=k_proj, v_proj=v_proj, q_norm_weight=q_norm_weight, k_norm_weight=k_norm_weight, positions=positions, key_pool=key_pool,
+                     value_pool=value_pool, slots=slots)
+    bf16 = torch.bfloat16
+    if key_pool.dtype is torch.uint8:
         desc, head_dim = _kv4_descriptor(key_pool, value_pool, block_size, device)
     else:
-        _require(key_pool.dtype == torch.bfloat16 and key_pool.dim() == 4 and key_pool.shape[2] == block_size, "the pool must be bfloat16 (blocks, kv_heads, block_size, head_dim) or 4-bit")
+        _require_cuda(value_pool, "value_pool", device)
+        _require(key_pool.dtype is bf16 and key_pool.dim() == 4 and key_pool.shape[2] == block_size, "the pool must be bfloat16 (blocks, kv_heads, block_size, head_dim) or 4-bit")
         desc, head_dim = _pool_descriptor(key_pool, value_pool, "shared"), key_pool.shape[3]
     kv_heads = desc.kv_heads
-    tokens = q_proj.shape[0]
+    q_shape = q_proj.shape
+    tokens = q_shape[0]
     k3 = k_proj.view(tokens, kv_heads, head_dim) if k_proj.dim() == 2 else k_proj
     v3 = v_proj.view(tokens, kv_heads, head_dim) if v_proj.dim() == 2 else v_proj
-    _require(q_proj.dim() == 3 or q_proj.dim() == 2 and q_proj.shape[1] % (2 * head_dim) == 0, "q_proj must be (tokens, heads, head_dim or 2*head_dim) or (tokens, heads*2*head_dim)")
-    q3 = q_proj.view(tokens, -1, 2 * head_dim) if q_proj.dim() == 2 else q_proj
-    heads = q3.shape[1]
-    _require(q3.shape[2] in (head_dim, 2 * head_dim), "q_proj must be (tokens, heads, head_dim or 2*head_dim) or (tokens, heads*2*head_dim)")
-    _require(k3.shape == (tokens, kv_heads, head_dim) and v3.shape == (tokens, kv_heads, head_dim), "k_proj/v_proj must be (tokens, kv_heads, head_dim)")
-    for tensor, name in ((q3, "q_proj"), (k3, "k_proj"), (v3, "v_proj")):
-        if tensor.dtype != torch.bfloat16 or tensor.stride(-1) != 1:
-            raise RuntimeError(f"{name} must be bfloat16 with a contiguous last dimension")
+    q3 = q_proj
+    if len(q_shape) == 2 and q_shape[1] % (2 * head_dim) == 0:
+        q3 = q_proj.view(tokens, -1, 2 * head_dim)
+        q_shape = q3.shape
+    _require(len(q_shape) == 3 and q_shape[2] in (head_dim, 2 * head_dim), "q_proj must be (tokens, heads, head_dim or 2*head_dim) or (tokens, heads*2*head_dim)")
+    heads = q_shape[1]
+    _require(k3.shape == (tokens, kv_heads, head_dim) and v3.shape == k3.shape, "k_proj/v_proj must be (tokens, kv_heads, head_dim)")
+    q_st, q_sh, q_sd = q3.stride()
+    k_st, k_sh, k_sd = k3.stride()
+    v_st, v_sh, v_sd = v3.stride()
+    if not (q3.dtype is bf16 and k3.dtype is bf16 and v3.dtype is bf16 and q_sd == k_sd == v_sd == 1):
+        raise RuntimeError("q_proj, k_proj and v_proj must be bfloat16 with a contiguous last dimension")
     _float_dtype(q_norm_weight, "q_norm_weight")
-    _require(q_norm_weight.dtype == k_norm_weight.dtype and q_norm_weight.shape == (head_dim,) and k_norm_weight.shape == (head_dim,),
+    _require(q_norm_weight.dtype is k_norm_weight.dtype and q_norm_weight.shape == (head_dim,) and k_norm_weight.shape == (head_dim,),
              "norm weights must be (head_dim,) of one dtype")
     _index_dtype(positions, "positions")
     _index_dtype(slots, "slots")
@@ -1470,14 +1495,16 @@ def qk_norm_mrope_kv_append(
     _require(pos.shape == (len(sections), tokens), "positions must be (axes, tokens), one axis per section")
     _require(slots.shape == (tokens,), "slots must have one entry per token")
     freq, axis = _mrope_tables(sections, bool(interleaved), float(rope_theta), device)
-    if pos.stride(1) != 1:
+    pos_stride, pos_unit = pos.stride()
+    if pos_unit != 1:
         pos = pos.contiguous()
+        pos_stride = tokens
     s, qw, kw = slots.contiguous(), q_norm_weight.contiguous(), k_norm_weight.contiguous()
-    query = torch.empty((tokens, heads, head_dim), dtype=torch.bfloat16, device=device)
+    query = torch.empty((tokens, heads, head_dim), dtype=bf16, device=device)
     code = _launch(
-        device, lib.qa_qk_norm_mrope_append, _ptr(q3), q3.stride(0), q3.stride(1), _ptr(k3), k3.stride(0), k3.stride(1), _ptr(v3), v3.stride(0), v3.stride(1), _ptr(qw),
-        _ptr(kw), _code(qw), float(eps), _ptr(freq), _ptr(axis), 2 * axis.numel(), _ptr(pos), _code(pos), pos.stride(0), len(sections), tokens, heads, head_dim,
-        ctypes.byref(desc), _ptr(s), _code(s), int(block_size), _ptr(query),
+        device, lib.qa_qk_norm_mrope_append, q3.data_ptr(), q_st, q_sh, k3.data_ptr(), k_st, k_sh, v3.data_ptr(), v_st, v_sh, qw.data_ptr(), kw.data_ptr(), _code(qw),
+        float(eps), freq.data_ptr(), axis.data_ptr(), 2 * axis.numel(), pos.data_ptr(), _code(pos), pos_stride, len(sections), tokens, heads, head_dim, ctypes.byref(desc),
+        s.data_ptr(), _code(s), int(block_size), query.data_ptr(),
     )
     L.check(lib, code, "qk_norm_mrope_kv_append")
-    return query, q3.narrow(2, head_dim, head_dim) if q3.shape[2] == 2 * head_dim else None
+    return query, q3.narrow(2, head_dim, head_dim) if q_shape[2] == 2 * head_dim else None
