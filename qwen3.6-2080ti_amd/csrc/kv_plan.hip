@@ -7,9 +7,10 @@
 // ceil(L_b / bs)]; its slot is id * bs + position % bs.  A fresh block always holds a new token at its first position,
 // so the token there writes the table entry: no pass of its own over the tables.
 //
-// A few KB move, so latency bounds it: one workgroup makes the sums and the all-or-nothing checks, and with few tokens
-// writes them too; from kInlineTokens on a second launch of one workgroup per kSpanTokens tokens does that, because one
-// CU stores only a few tens of GB/s.
+// A few KB move, so latency bounds it: a launch of one workgroup reads lengths, counts and state at once (with a thread a
+// row the scan that plans is also the sum that is checked), looks the tokens' rows up in LDS and writes them.  128 rows of
+// one token: 5.5 us.  From kInlineTokens on a second launch of one workgroup per kSpanTokens tokens writes them, because
+// one CU stores only a few tens of GB/s; 61 rows of up to 8192 tokens: 4.4 + 5.5 us.
 #include "qa_common.h"
 
 namespace qa {
@@ -35,20 +36,30 @@ struct Params {
 };
 
 constexpr int kThreads = 1024;
-constexpr int kSpanTokens = 1024;   // tokens of a workgroup of the second launch
+constexpr int kSpanTokens = 256;    // tokens of a workgroup of the second launch; with 1024, four dependent chains one after the other, 7.9 us in place of 5.5 for 61 rows of 8192
+// Tokens that the planning workgroup writes itself.  us there, and with a second launch (whose gap comes on top): 128 tokens
+// 5.5 and 4.2 + 2.3, 1024 tokens 5.8 and 4.4 + 3.4, 4096 tokens 8.8 and 4.3 + 3.8, 8192 tokens 12.6 and 4.3 + 3.6.
 constexpr int kInlineTokens = 4096;
-constexpr int kRowsInLds = 4096;    // rows whose sums a workgroup looks up in LDS
+constexpr int kRowsInLds = 4096;    // rows whose sums a workgroup looks up in LDS: what 48 KB hold of the three arrays
 
 __device__ __forceinline__ int64_t count_of(const Params& p, int b) {
   if (p.counts == nullptr) return p.count_scalar;
   return p.counts_i64 ? reinterpret_cast<const int64_t*>(p.counts)[b] : reinterpret_cast<const int32_t*>(p.counts)[b];
 }
 
-__device__ __forceinline__ int64_t ceil_div_dev(int64_t a, int64_t b) { return (a + b - 1) / b; }
+// Blocks of n tokens.  In 32 bits: a row that is planned has n + bs below 2^31.
+__device__ __forceinline__ uint32_t blocks_of(const Params& p, int64_t n) { return (static_cast<uint32_t>(n) + p.bs - 1) / p.bs; }
 
-// Writes positions, slots and fresh table entries of tokens lo .. hi - 1.  cu: the row sums (in LDS or in memory).
-__device__ void write_tokens(const Params& p, const int32_t* cu, int64_t lo, int64_t hi) {
-  const int32_t total = cu[p.B];
+// What the writing of tokens reads of the rows: in LDS, or in memory where they are too many.
+struct Rows {
+  const int32_t* cu;
+  const int32_t* starts;
+  const int32_t* first;
+};
+
+// Writes positions, slots and fresh table entries of tokens lo .. hi - 1.
+__device__ void write_tokens(const Params& p, const Rows& rows, int64_t lo, int64_t hi) {
+  const int32_t total = rows.cu[p.B];
   for (int64_t i = lo + threadIdx.x; i < hi; i += blockDim.x) {
     int32_t position = -1;
     int64_t slot = -1;
@@ -56,21 +67,21 @@ __device__ void write_tokens(const Params& p, const int32_t* cu, int64_t lo, int
       int a = 0, z = p.B;  // cu[a] <= i < cu[z]
       while (z - a > 1) {
         const int m = (a + z) >> 1;
-        if (cu[m] <= i)
+        if (rows.cu[m] <= i)
           a = m;
         else
           z = m;
       }
-      const int32_t start = p.starts[a];
-      position = start + static_cast<int32_t>(i - cu[a]);
-      const int lb = position / p.bs;
-      const int have = (start + p.bs - 1) / p.bs;
-      const int at = position - lb * p.bs;
+      const int32_t start = rows.starts[a];
+      position = start + static_cast<int32_t>(i - rows.cu[a]);
+      const uint32_t lb = static_cast<uint32_t>(position) / p.bs;
+      const uint32_t have = blocks_of(p, start);
+      const uint32_t at = position - lb * p.bs;
       int32_t id;
       if (lb < have) {
         id = p.tables[a * p.table_stride + lb];
       } else {
-        id = p.free_list[p.first[a] + lb - have];
+        id = p.free_list[rows.first[a] + static_cast<int64_t>(lb - have)];
         if (at == 0) p.tables[a * p.table_stride + lb] = id;
       }
       if (id >= 0) slot = static_cast<int64_t>(id) * p.bs + at;
@@ -83,46 +94,79 @@ __device__ void write_tokens(const Params& p, const int32_t* cu, int64_t lo, int
 __global__ __launch_bounds__(kThreads) void plan_kernel(Params p) {
   __shared__ int64_t s_need[kThreads / 64], s_count[kThreads / 64];
   __shared__ int s_bad[kThreads / 64];
-  __shared__ int32_t s_cu[kRowsInLds + 1];
+  __shared__ int32_t s_cu[kRowsInLds + 1], s_starts[kRowsInLds], s_first[kRowsInLds];
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wave = tid >> 6;
   const int64_t head = p.free_state[0];
   const int64_t avail = p.free_state[1];
 
-  // every row's length, tokens and blocks: the checks
-  int64_t need = 0, count = 0;
+  // a row's length, tokens and blocks; what it asks for if that can be counted at all
+  int64_t len, n, need;
   int bad = 0;
-  for (int b = tid; b < p.B; b += kThreads) {
-    const int64_t len = p.lengths[b];
-    const int64_t n = count_of(p, b);
+  auto row = [&](int b) {
+    len = n = need = 0;
+    if (b >= p.B) return;
+    len = p.lengths[b];
+    n = count_of(p, b);
     if (len < 0 || n < 0 || n > 0x7fffffff || len + n > 0x7fffffff - p.bs) {
       bad |= 4;
-      continue;
+      n = 0;
+      return;
     }
-    const int64_t want = ceil_div_dev(len + n, p.bs);
+    const uint32_t want = blocks_of(p, len + n);
     if (want > p.max_blocks) bad |= 2;
-    need += want - ceil_div_dev(len, p.bs);
-    count += n;
-  }
-  for (int off = 32; off > 0; off >>= 1) {
-    need += __shfl_xor(need, off, 64);
-    count += __shfl_xor(count, off, 64);
-    bad |= __shfl_xor(bad, off, 64);
-  }
-  if (lane == 0) {
-    s_need[wave] = need;
-    s_count[wave] = count;
-    s_bad[wave] = bad;
-  }
-  __syncthreads();
+    need = want - blocks_of(p, len);
+  };
+  // sums over the workgroup: of all rows, or up to and with a thread's own
   int64_t total_need = 0, total_count = 0;
-  bad = 0;
+  auto totals = [&](int64_t of_need, int64_t of_count) {  // of_*: a wave's sums, in its last lane
+    for (int off = 32; off > 0; off >>= 1) bad |= __shfl_xor(bad, off, 64);
+    if (lane == 63) {
+      s_need[wave] = of_need;
+      s_count[wave] = of_count;
+      s_bad[wave] = bad;
+    }
+    __syncthreads();
+    total_need = total_count = 0;
 #pragma unroll
-  for (int w = 0; w < kThreads / 64; ++w) {
-    total_need += s_need[w];
-    total_count += s_count[w];
-    bad |= s_bad[w];
+    for (int w = 0; w < kThreads / 64; ++w) {
+      total_need += s_need[w];
+      total_count += s_count[w];
+      bad |= s_bad[w];
+    }
+  };
+  int64_t need_incl, n_incl;
+  auto scan_wave = [&]() {
+    need_incl = need;
+    n_incl = n;
+    for (int off = 1; off < 64; off <<= 1) {
+      const int64_t nu = __shfl_up(n_incl, off, 64), ku = __shfl_up(need_incl, off, 64);
+      if (lane >= off) {
+        n_incl += nu;
+        need_incl += ku;
+      }
+    }
+  };
+
+  // the checks; with a thread for every row the sums they need are the ones the plan needs
+  const bool one = p.B <= kThreads;
+  if (one) {
+    row(tid);
+    scan_wave();
+    totals(need_incl, n_incl);
+  } else {
+    int64_t my_need = 0, my_count = 0;
+    for (int b = tid; b < p.B; b += kThreads) {
+      row(b);
+      my_need += need;
+      my_count += n;
+    }
+    for (int off = 32; off > 0; off >>= 1) {
+      my_need += __shfl_xor(my_need, off, 64);
+      my_count += __shfl_xor(my_count, off, 64);
+    }
+    totals(my_need, my_count);
   }
   int code = 0;
   if (head < 0 || avail < 0 || head + avail > p.capacity) code = 3;
@@ -130,68 +174,52 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(Params p) {
   else if (bad & 2) code = 2;
   else if (total_need > avail) code = 1;
   else if (total_count > p.max_tokens) code = 5;
-  __syncthreads();  // s_need and s_count are used again
+  const int64_t taken = total_need;
 
   // the row sums; a step that is refused plans no token and takes nothing
   int64_t need_before = head, count_before = 0;
   for (int r0 = 0; r0 < p.B; r0 += kThreads) {
     const int b = r0 + tid;
-    int64_t len = 0, n = 0, k = 0;
-    if (b < p.B) {
-      len = p.lengths[b];
-      if (code == 0) {
-        n = count_of(p, b);
-        k = ceil_div_dev(len + n, p.bs) - ceil_div_dev(len, p.bs);
-      }
+    if (!one) {
+      __syncthreads();  // s_need and s_count are used again
+      row(b);
+      scan_wave();
+      totals(need_incl, n_incl);
     }
-    int64_t n_incl = n, k_incl = k;
-    for (int off = 1; off < 64; off <<= 1) {
-      const int64_t nu = __shfl_up(n_incl, off, 64), ku = __shfl_up(k_incl, off, 64);
-      if (lane >= off) {
-        n_incl += nu;
-        k_incl += ku;
-      }
-    }
-    if (lane == 63) {
-      s_count[wave] = n_incl;
-      s_need[wave] = k_incl;
-    }
-    __syncthreads();
-    int64_t n_sum = 0, k_sum = 0;
-#pragma unroll
-    for (int w = 0; w < kThreads / 64; ++w) {
-      if (w == wave) {
-        n_incl += n_sum + count_before;
-        k_incl += k_sum + need_before;
-      }
-      n_sum += s_count[w];
-      k_sum += s_need[w];
+    int64_t need_at = need_before, n_at = count_before;
+    for (int w = 0; w < wave; ++w) {
+      need_at += s_need[w];
+      n_at += s_count[w];
     }
     if (b < p.B) {
-      const int32_t c = static_cast<int32_t>(n_incl - n);
+      const int32_t c = code ? 0 : static_cast<int32_t>(n_at + n_incl - n);
+      const int32_t f = code ? 0 : static_cast<int32_t>(need_at + need_incl - need);
       p.cu[b] = c;
-      if (b < kRowsInLds) s_cu[b] = c;
       p.starts[b] = static_cast<int32_t>(len);
-      p.first[b] = static_cast<int32_t>(k_incl - k);
+      if (b < kRowsInLds) {
+        s_cu[b] = c;
+        s_starts[b] = static_cast<int32_t>(len);
+        s_first[b] = f;
+      }
+      if (!p.inline_tokens) p.first[b] = f;
       if (code == 0) p.lengths[b] = static_cast<int32_t>(len + n);
     }
-    count_before += n_sum;
-    need_before += k_sum;
-    __syncthreads();
+    need_before += total_need;
+    count_before += total_count;
   }
   if (tid == 0) {
-    const int32_t total = static_cast<int32_t>(count_before);
+    const int32_t total = code ? 0 : static_cast<int32_t>(count_before);
     p.cu[p.B] = total;
     if (p.B <= kRowsInLds) s_cu[p.B] = total;
     if (code == 0) {
-      p.free_state[0] = static_cast<int32_t>(head + total_need);
-      p.free_state[1] = static_cast<int32_t>(avail - total_need);
+      p.free_state[0] = static_cast<int32_t>(head + taken);
+      p.free_state[1] = static_cast<int32_t>(avail - taken);
     }
     p.status[0] = code;
   }
   if (!p.inline_tokens) return;
-  __syncthreads();  // also orders this workgroup's writes of starts and first before the reads below
-  write_tokens(p, s_cu, 0, p.max_tokens);
+  lds_barrier();
+  write_tokens(p, {s_cu, s_starts, s_first}, 0, p.max_tokens);
 }
 
 __global__ __launch_bounds__(256) void plan_tokens_kernel(Params p) {
@@ -201,10 +229,8 @@ __global__ __launch_bounds__(256) void plan_tokens_kernel(Params p) {
   if (p.B <= kRowsInLds) {
     for (int b = threadIdx.x; b <= p.B; b += blockDim.x) s_cu[b] = p.cu[b];
     __syncthreads();
-    write_tokens(p, s_cu, lo, hi);
-  } else {
-    write_tokens(p, p.cu, lo, hi);
   }
+  write_tokens(p, {p.B <= kRowsInLds ? s_cu : p.cu, p.starts, p.first}, lo, hi);
 }
 
 }  // namespace kvplan

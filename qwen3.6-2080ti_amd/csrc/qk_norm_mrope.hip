@@ -12,9 +12,14 @@
 // k goes to the pool rounded to bf16; a 4-bit pool holds the 4-bit form (kv4.h) of that bf16 value, so that both pools
 // and paged_kv4_append agree bit for bit.
 //
-// Bound by memory: 2 D (H + 2 H_kv) bytes of bf16 read and written per token.  One workgroup per token; its four waves
-// walk the H + 2 H_kv heads and each loads the rows of all its heads before it reduces any of them.  Lane l holds
-// elements E l .. E l + E - 1 (D = 64 E); the partner of an element is rd / (2 E) lanes away.
+// Bound by memory, 2 D (H + 2 H_kv) bytes of bf16 read and written per token, with the arithmetic close behind.  Two
+// kernels.  rows_kernel gives a lane eight dims, 16-byte accesses, and a head D / 8 lanes: a wave takes 2 or 4 heads at a
+// time, the norm is a sum over one or two rows of lanes, the partner comes by DPP on packed values, and weight times
+// cosine is formed once a token.  It needs rd / 2 a multiple of 8 and rows on 16 bytes.  heads_kernel gives a lane D / 64
+// dims and a head the whole wave, and takes what is left (head_dim 64 among it).  5003 tokens of 16 + 2 x 4 heads of 128:
+// 26.5 us there, 17.0 us here (3.6 TB/s; a copy runs at 4.8); 128 tokens of 16 + 2 x 2 heads of 256: 7.3 and 5.5 us.
+#include <algorithm>
+
 #include "kv4.h"
 
 namespace qa {
@@ -132,7 +137,7 @@ __device__ __forceinline__ void store_kv4(uint8_t* run, int t, int lane, const R
 }
 
 template <int E, bool KV4>
-__global__ __launch_bounds__(256) void qk_norm_mrope_kernel(Params p) {
+__global__ __launch_bounds__(256) void heads_kernel(Params p) {
   constexpr int D = 64 * E;
   const int64_t n = blockIdx.x;
   const int lane = threadIdx.x & 63;
@@ -221,6 +226,176 @@ __global__ __launch_bounds__(256) void qk_norm_mrope_kernel(Params p) {
   }
 }
 
+// ---- a lane eight dims ---------------------------------------------------------
+constexpr int kStepsInFlight = 2;  // steps whose loads a wave issues before it works on the first; 6 are 3 to 20 % slower at 5003 tokens
+// Waves to aim at: with fewer tokens than this the heads of a token are shared among waves, at the price of the angles in
+// each.  us at 1, 2, 4 and 10 waves a token, D = 256: 128 tokens 10.6 7.6 6.4 5.5, 512 tokens 11.3 8.7 7.9 7.8, 1024 tokens
+// 11.9 9.8 9.5 12.0, 2000 tokens 15.8 14.3 16.0 19.7, 5003 tokens 22.8 25.8 29.3 40.9.
+constexpr int kWaves = 4096;
+
+// The dword that the lane `distance` lanes on (lanes of the first half of the rotated dims) or back holds.
+__device__ __forceinline__ uint32_t partner_of(uint32_t x, int distance, bool first, int lane) {
+  const int v = static_cast<int>(x);
+  if (distance == 8) return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, v, 0x128, 0xF, 0xF, false));  // row_ror:8
+  if (distance == 4) {
+    const int up = __builtin_amdgcn_update_dpp(0, v, 0x104, 0xF, 0xF, false);    // row_shl:4
+    const int down = __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);  // row_shr:4
+    return static_cast<uint32_t>(first ? up : down);
+  }
+  return static_cast<uint32_t>(__shfl(v, first ? lane + distance : lane - distance, 64));
+}
+
+__device__ __forceinline__ void widen8(const uint4& u, float (&x)[8]) {
+  const uint32_t d[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(e & 1 ? d[e / 2] & 0xffff0000u : d[e / 2] << 16);
+}
+
+__device__ __forceinline__ void load_weights(const void* base, int f32, int j, float (&w)[8]) {
+  if (f32) {
+    const float4 a = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(base) + j);
+    const float4 b = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(base) + j + 4);
+    w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w, w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
+  } else {
+    widen8(*reinterpret_cast<const uint4*>(reinterpret_cast<const bf16_t*>(base) + j), w);
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) w[e] += 1.f;
+}
+
+template <int D, bool KV4>
+__global__ __launch_bounds__(256) void rows_kernel(Params p, int waves_per_token) {
+  constexpr int LANES = D / 8;       // of a head
+  constexpr int SLOTS = 64 / LANES;  // heads of a step
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t all = static_cast<uint32_t>(blockIdx.x) * 4u + static_cast<uint32_t>(wave);
+  const int64_t n = all / static_cast<uint32_t>(waves_per_token);
+  const int part = static_cast<int>(all - static_cast<uint32_t>(n) * static_cast<uint32_t>(waves_per_token));
+  if (n >= p.tokens) return;
+  const int in_head = lane % LANES;
+  const int sub = lane / LANES;
+  const int j0 = 8 * in_head;
+  const int half = p.rd / 2;
+  const bool rot = j0 < p.rd;
+  const bool first = j0 < half;
+  const int jh = rot ? (first ? j0 : j0 - half) : 0;
+
+  // steps of one kind each, so that no lane chooses between kinds: the queries' heads, then the keys', then the values'
+  const int nq = (p.H + SLOTS - 1) / SLOTS, nk = (p.Hkv + SLOTS - 1) / SLOTS;
+  const int steps = nq + 2 * nk;
+  auto source = [&](int step) -> const bf16_t* {  // lanes past the last head read it again
+    if (step < nq) return p.q + n * p.q_st + static_cast<int64_t>(min(step * SLOTS + sub, p.H - 1)) * p.q_sh;
+    if (step < nq + nk) return p.k + n * p.k_st + static_cast<int64_t>(min((step - nq) * SLOTS + sub, p.Hkv - 1)) * p.k_sh;
+    return p.v + n * p.v_st + static_cast<int64_t>(min((step - nq - nk) * SLOTS + sub, p.Hkv - 1)) * p.v_sh;
+  };
+  uint4 raw[kStepsInFlight];
+  auto load_pass = [&](int from) {
+#pragma unroll
+    for (int i = 0; i < kStepsInFlight; ++i) {
+      if (from + i * waves_per_token < steps) raw[i] = *reinterpret_cast<const uint4*>(source(from + i * waves_per_token) + j0);
+    }
+  };
+  load_pass(part);
+  const int64_t slot = read_index(p.slots, p.slots_i64, n);
+
+  // a lane an angle or two, then every lane its eight through LDS: eight a lane cost 0.4 us a wave more
+  __shared__ __align__(16) float s_cos[4][D / 2], s_sin[4][D / 2];
+  for (int j = lane; j < half; j += 64) {
+    const int64_t at = read_index(p.positions, p.pos_i64, min(static_cast<int>(p.axis[j]), p.axes - 1) * p.pos_stride + n);
+    const uint64_t turn = static_cast<uint64_t>(at) * p.freq[j];
+    const float f = static_cast<float>(static_cast<uint32_t>(turn >> 40)) * 0x1p-24f;  // as in heads_kernel
+    s_cos[wave][j] = __builtin_amdgcn_cosf(f);
+    s_sin[wave][j] = __builtin_amdgcn_sinf(f);
+  }
+  // out = rs (x A + x' B), x' the dim's partner: A = (1 + w) cos, B = (1 + w') (-+ sin)
+  float qa[8], qb[8], ka[8], kb[8];
+  load_weights(p.qw, p.w_f32, j0, qa);
+  load_weights(p.kw, p.w_f32, j0, ka);
+  const int jp = !rot ? j0 : first ? j0 + half : j0 - half;
+  load_weights(p.qw, p.w_f32, jp, qb);
+  load_weights(p.kw, p.w_f32, jp, kb);
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");  // the wave reads only what it wrote
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float c = rot ? s_cos[wave][jh + e] : 1.f;
+    const float s = !rot ? 0.f : first ? -s_sin[wave][jh + e] : s_sin[wave][jh + e];
+    qa[e] *= c;
+    ka[e] *= c;
+    qb[e] *= s;
+    kb[e] *= s;
+  }
+  const uint32_t turns = rot ? ~0u : 0u;  // a lane that does not turn would get anyone's value, a NaN perhaps
+  const bool live = slot >= 0 && slot < p.num_slots;
+  // a 32-bit division where the pool allows it: a fifth of a 64-bit one
+  const int64_t block = !live ? 0 : p.num_slots <= 0xffffffffll ? static_cast<uint32_t>(slot) / static_cast<uint32_t>(p.bs) : slot / p.bs;
+  const int at = live ? static_cast<int>(slot - block * p.bs) : 0;
+
+  auto normalised = [&](const uint4& u, const float (&A)[8], const float (&B)[8]) {
+    float x[8], y[8];
+    widen8(u, x);
+    widen8(make_uint4(partner_of(u.x, half / 8, first, lane) & turns, partner_of(u.y, half / 8, first, lane) & turns, partner_of(u.z, half / 8, first, lane) & turns,
+                      partner_of(u.w, half / 8, first, lane) & turns), y);
+    float ss = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) ss += x[e] * x[e];
+    ss = row16_sum(ss);
+    if constexpr (D == 256) {
+      const auto both = __builtin_amdgcn_permlane16_swap(__float_as_uint(ss), __float_as_uint(ss), false, false);
+      ss = __uint_as_float(both[0]) + __uint_as_float(both[1]);
+    }
+    const float rs = rsqrtf(ss * (1.f / D) + p.eps);
+    uint32_t out[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float lo = (x[2 * e] * A[2 * e] + y[2 * e] * B[2 * e]) * rs;
+      const float hi = (x[2 * e + 1] * A[2 * e + 1] + y[2 * e + 1] * B[2 * e + 1]) * rs;
+      out[e] = static_cast<uint32_t>(f32_to_bf16(lo)) | static_cast<uint32_t>(f32_to_bf16(hi)) << 16;
+    }
+    return make_uint4(out[0], out[1], out[2], out[3]);
+  };
+  auto append = [&](const uint4& u, int h, bool value) {
+    if (!live || h >= p.Hkv) return;
+    if constexpr (KV4) {
+      using R = kv4::Run<D>;
+      uint8_t* run = reinterpret_cast<uint8_t*>(value ? p.vpool : p.kpool) + block * p.sP + h * p.sG + static_cast<int64_t>(at >> 4) * R::kBytes;
+      float z[8];
+      widen8(u, z);
+      uint32_t top = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(z[e]) & 0x7fffffffu);
+      const uint32_t byte = kv4::scale_byte(__uint_as_float(kv4::quad_max(top)));
+      const uint32_t codes = kv4::pack_codes(z, byte);
+      const int t = at & 15, group = in_head / 4;
+      const int to = value ? R::value_code(t, j0 / (D / 16)) + j0 % (D / 16) / 2 : R::key_code(t, group) + 4 * (in_head & 3);
+      *reinterpret_cast<uint32_t*>(run + to) = codes;
+      if ((in_head & 3) == 0) run[value ? R::value_scale(t, group) : R::key_scale(t, group)] = static_cast<uint8_t>(byte);
+    } else {
+      *reinterpret_cast<uint4*>(reinterpret_cast<bf16_t*>(value ? p.vpool : p.kpool) + block * p.sP + h * p.sG + at * p.sT + j0) = u;
+    }
+  };
+
+  for (int from = part; from < steps; from += kStepsInFlight * waves_per_token) {
+    if (from != part) load_pass(from);
+#pragma unroll
+    for (int i = 0; i < kStepsInFlight; ++i) {
+      const int step = from + i * waves_per_token;
+      if (step >= steps) break;
+      if (step < nq) {
+        const uint4 out = normalised(raw[i], qa, qb);
+        const int h = step * SLOTS + sub;
+        if (h < p.H) *reinterpret_cast<uint4*>(p.q_out + (n * p.H + h) * D + j0) = out;
+      } else if (step < nq + nk) {
+        append(normalised(raw[i], ka, kb), (step - nq) * SLOTS + sub, false);
+      } else {
+        append(raw[i], (step - nq - nk) * SLOTS + sub, true);
+      }
+    }
+  }
+}
+
 }  // namespace mrope
 }  // namespace qa
 
@@ -292,21 +467,41 @@ extern "C" int qa_qk_norm_mrope_append(const void* q_proj, int64_t q_stride_t, i
   p.rd = rotary_dim;
   p.bs = block_size;
   p.q_out = reinterpret_cast<bf16_t*>(q_out);
-  const dim3 grid(static_cast<unsigned>(tokens));
-  {
-    KernelTimer timer_("qk_norm_mrope", stream);
+  auto rows16 = [](const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15u) == 0; };
+  const bool rows = E >= 2 && rotary_dim % 16 == 0 && rows16(q_proj) && rows16(k_proj) && rows16(v_proj) && rows16(q_out) && rows16(q_norm_weight) && rows16(k_norm_weight) &&
+                    q_stride_t % 8 == 0 && q_stride_h % 8 == 0 && k_stride_t % 8 == 0 && k_stride_h % 8 == 0 && v_stride_t % 8 == 0 && v_stride_h % 8 == 0 &&
+                    (kv4_pool || (rows16(kv->key) && rows16(kv->value) && kv->stride_block % 8 == 0 && kv->stride_head % 8 == 0 && kv->stride_token % 8 == 0));
+  KernelTimer timer_("qk_norm_mrope", stream);
+  if (rows) {
+    const int at_once = E == 4 ? 2 : 4;
+    const int64_t steps = ceil_div(p.H, at_once) + 2 * ceil_div(p.Hkv, at_once);
+    const int waves = static_cast<int>(std::min(steps, std::max<int64_t>(1, kWaves / tokens)));
+    const dim3 grid(static_cast<unsigned>(ceil_div(tokens * waves, 4)));
+    if (E == 4) {
+      if (kv4_pool)
+        hipLaunchKernelGGL((rows_kernel<256, true>), grid, dim3(256), 0, stream, p, waves);
+      else
+        hipLaunchKernelGGL((rows_kernel<256, false>), grid, dim3(256), 0, stream, p, waves);
+    } else {
+      if (kv4_pool)
+        hipLaunchKernelGGL((rows_kernel<128, true>), grid, dim3(256), 0, stream, p, waves);
+      else
+        hipLaunchKernelGGL((rows_kernel<128, false>), grid, dim3(256), 0, stream, p, waves);
+    }
+  } else {
+    const dim3 grid(static_cast<unsigned>(tokens));
     if (kv4_pool) {
       if (E == 4)
-        hipLaunchKernelGGL((qk_norm_mrope_kernel<4, true>), grid, dim3(256), 0, stream, p);
+        hipLaunchKernelGGL((heads_kernel<4, true>), grid, dim3(256), 0, stream, p);
       else
-        hipLaunchKernelGGL((qk_norm_mrope_kernel<2, true>), grid, dim3(256), 0, stream, p);
+        hipLaunchKernelGGL((heads_kernel<2, true>), grid, dim3(256), 0, stream, p);
     } else {
       if (E == 4)
-        hipLaunchKernelGGL((qk_norm_mrope_kernel<4, false>), grid, dim3(256), 0, stream, p);
+        hipLaunchKernelGGL((heads_kernel<4, false>), grid, dim3(256), 0, stream, p);
       else if (E == 2)
-        hipLaunchKernelGGL((qk_norm_mrope_kernel<2, false>), grid, dim3(256), 0, stream, p);
+        hipLaunchKernelGGL((heads_kernel<2, false>), grid, dim3(256), 0, stream, p);
       else
-        hipLaunchKernelGGL((qk_norm_mrope_kernel<1, false>), grid, dim3(256), 0, stream, p);
+        hipLaunchKernelGGL((heads_kernel<1, false>), grid, dim3(256), 0, stream, p);
     }
   }
   return check_launch("qk_norm_mrope_append");

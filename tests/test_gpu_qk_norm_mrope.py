@@ -128,3 +128,42 @@ def test_rotary_dims_that_lanes_would_share_are_refused() -> None:
     pools = [torch.zeros(1, 1, 16, 128, dtype=torch.bfloat16, device=DEV) for _ in range(2)]
     with pytest.raises(RuntimeError, match="multiple of 4"):
         hip_ops.qk_norm_mrope_kv_append(q, k, v, qw, kw, positions, (7,), *pools, torch.arange(3, device=DEV), 16, eps=EPS, rope_theta=1e6)
+
+
+@pytest.mark.parametrize("dim,sections,tokens", [(256, (11, 11, 10), 33), (128, (16, 24, 24), 33), (128, (4, 4), 2050), (256, (16,), 2047), (256, (40, 56), 5)])
+def test_rows_of_any_alignment_and_count_agree(dim, sections, tokens) -> None:
+    """The same call with every row on 16 bytes and with rows 4 elements off: to a rounding, as the sums run in other orders."""
+    heads, kv_heads, block = 6, 2, 16
+    q, k, v, qw, kw, positions = (x.to(DEV) for x in _inputs(13, tokens, heads, kv_heads, dim, len(sections), 4000))
+    wide = torch.zeros(tokens, (2 * heads + 2 * kv_heads) * dim + 4, dtype=torch.bfloat16, device=DEV)
+    parts = [wide[:, 4 + a * dim:4 + b * dim] for a, b in ((0, 2 * heads), (2 * heads, 2 * heads + kv_heads), (2 * heads + kv_heads, 2 * heads + 2 * kv_heads))]
+    for part, x in zip(parts, (q, k, v)):
+        part.copy_(x.reshape(tokens, -1))
+    blocks = tokens // block + 1
+    slots = torch.randperm(blocks * block, device=DEV)[:tokens]
+    runs = []
+    for rows in ((q, k, v), parts):
+        pools = [torch.zeros(blocks, kv_heads, block, dim, dtype=torch.bfloat16, device=DEV) for _ in range(2)]
+        query, _ = hip_ops.qk_norm_mrope_kv_append(*rows, qw, kw, positions, sections, *pools, slots, block, eps=EPS, rope_theta=1e6)
+        runs.append((query, *pools))
+    form = kv4.norm_mrope(q[..., :dim].double().cpu().numpy(), qw.double().cpu().numpy(), positions.cpu().numpy(), sections, False, 1e6, EPS)
+    for query, keys, values in runs:
+        _close(query, form)
+        assert torch.equal(values, runs[0][2])
+        top = runs[0][1].float().abs().amax(-1, keepdim=True)
+        assert ((keys.float() - runs[0][1].float()).abs() <= 2.0**-7 * runs[0][1].float().abs() + 2.0**-17 * top).all()
+
+
+@pytest.mark.parametrize("shift", [0, 4])
+def test_an_infinity_stays_in_its_pair(shift) -> None:
+    """x rsqrt(inf) is 0 at every finite x and NaN at the infinity; the rotation mixes a dim with its pair only."""
+    dim, sections = 256, (11, 11, 10)
+    q, k, v, qw, kw, positions = (x.to(DEV) for x in _inputs(15, 3, 2, 1, dim, 3, 50))
+    wide = torch.zeros(3, 4 * dim + shift, dtype=torch.bfloat16, device=DEV)
+    rows = wide[:, shift:]
+    rows.copy_(q.reshape(3, -1))
+    rows[1, 33], rows[2, 2 * dim + 200] = float("inf"), float("inf")  # head 0's dim 33 turns with dim 1; head 1's dim 200 does not turn
+    pools = [torch.zeros(1, 1, 16, dim, dtype=torch.bfloat16, device=DEV) for _ in range(2)]
+    query, _ = hip_ops.qk_norm_mrope_kv_append(rows, k, v, qw, kw, positions, sections, *pools, torch.arange(3, device=DEV), 16, eps=EPS, rope_theta=1e6, interleaved=True)
+    assert query[1, 0].isnan().nonzero().flatten().tolist() == [1, 33] and query[2, 1].isnan().nonzero().flatten().tolist() == [200]
+    assert (query[1, 0].nan_to_num() == 0).all() and (query[2, 1].nan_to_num() == 0).all() and query.isnan().sum() == 3
