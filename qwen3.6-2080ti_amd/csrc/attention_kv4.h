@@ -49,14 +49,16 @@ struct Params {
   int64_t gate_st, gate_sh;
   bf16_t* out;
   int B, H, Hkv, G, bs_shift, table_i64, idx_i64;
+  uint32_t g_mul, g_shift;  // x / G = x g_mul >> 32 >> g_shift for x below 2^31, where G > 1
   float scale;
 };
 
 // Index arrays that no kernel here writes, read through the constant address space: uniform reads are scalar loads.
+// Entry i of an int32 or int64 array.  Without a branch, so that several are on their way at once.
 __device__ __forceinline__ int64_t read_index(const void* base, int is64, int64_t i) {
-  typedef const __attribute__((address_space(4))) int64_t c64;
-  typedef const __attribute__((address_space(4))) int32_t c32;
-  return is64 ? ((c64*)base)[i] : static_cast<int64_t>(((c32*)base)[i]);
+  const int32_t* at = reinterpret_cast<const int32_t*>(base) + (i << is64);
+  const int32_t lo = at[0], hi = at[is64];
+  return is64 ? static_cast<int64_t>(hi) << 32 | static_cast<uint32_t>(lo) : lo;
 }
 
 __device__ __forceinline__ int64_t uniform64(int64_t v) {
@@ -129,18 +131,27 @@ __device__ __forceinline__ uint32_t query_scale(uint32_t top) { return static_ca
 // Loads row qrow (null: zeros) of this lane's column and splits it.  LO: the second piece.  Both need the same row.
 template <int D>
 struct QueryRow {
+  uint4 raw[D / 128][4];
   float x[D / 128][32];
   uint32_t byte;  // scale of hi
 
-  __device__ __forceinline__ void load(const bf16_t* qrow, int quad) {
+  __device__ __forceinline__ void ask(const bf16_t* qrow, int quad) {
+#pragma unroll
+    for (int i = 0; i < D / 128; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        raw[i][j] = make_uint4(0, 0, 0, 0);
+        if (qrow != nullptr) raw[i][j] = *reinterpret_cast<const uint4*>(qrow + 128 * i + 64 * (j >> 1) + 16 * quad + 8 * (j & 1));
+      }
+  }
+
+  __device__ __forceinline__ void widen() {
     uint32_t top = 0;
 #pragma unroll
     for (int i = 0; i < D / 128; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        uint4 u = make_uint4(0, 0, 0, 0);
-        if (qrow != nullptr) u = *reinterpret_cast<const uint4*>(qrow + 128 * i + 64 * (j >> 1) + 16 * quad + 8 * (j & 1));
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+        const uint32_t w[4] = {raw[i][j].x, raw[i][j].y, raw[i][j].z, raw[i][j].w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           x[i][8 * j + 2 * e] = __uint_as_float(w[e] << 16);
@@ -250,13 +261,17 @@ __device__ __forceinline__ float column_sum(float v) {
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
+// x / G, by a product with its reciprocal rounded up: with 2^s >= G the error of x ceil(2^(31 + s) / G) is below 2^(31 + s) / G.
+__device__ __forceinline__ uint32_t over_group(const Params& p, uint32_t x) { return p.G == 1 ? x : __umulhi(x, p.g_mul) >> p.g_shift; }
+
 // o / l: zeros where a query saw nothing; a NaN stays one.
 __device__ __forceinline__ float normalised(float o, float l) {
   const float r = o * (1.f / l);
   return l == 0.f ? 0.f : r;
 }
 
-__device__ __forceinline__ float sigmoid(float x) { return 1.f / (1.f + __expf(-x)); }
+// v_rcp_f32 is within an ulp and a division ten instructions: a prefill workgroup spent 4 us on those of its outputs.
+__device__ __forceinline__ float sigmoid(float x) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * -kLog2e)); }
 
 // ---- host ------------------------------------------------------------------
 // Lets a kernel have `bytes` of dynamic LDS, once per device: the call costs the host about a microsecond.
@@ -323,6 +338,9 @@ inline int fill(Params& p, const Args& a) {
   p.H = a.heads;
   p.Hkv = a.kv->kv_heads;
   p.G = a.heads / a.kv->kv_heads;
+  p.g_shift = 0;
+  while ((2 << p.g_shift) < p.G) ++p.g_shift;  // ceil(log2 G) - 1
+  p.g_mul = static_cast<uint32_t>(((1ull << (32 + p.g_shift)) + p.G - 1) / p.G);
   p.bs_shift = __builtin_ctz(static_cast<unsigned>(a.block_size));
   p.table_i64 = a.table_dtype == QA_I64;
   p.idx_i64 = a.idx_dtype == QA_I64;

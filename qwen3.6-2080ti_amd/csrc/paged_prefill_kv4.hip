@@ -21,6 +21,7 @@
 #include "attention_kv4.h"
 
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 namespace qa {
@@ -77,48 +78,63 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams p
   const int rr = blockIdx.y / p.Hkv;
   const int g = blockIdx.y - rr * p.Hkv;
   int b = rr;
+  int64_t tok0, tok1, prefix;
   if (p.B <= kRankRows && p.B > 1) {
     int64_t* s_len = reinterpret_cast<int64_t*>(smem);
-    int* s_order = reinterpret_cast<int*>(smem + 8 * kRankRows);
+    int64_t* s_row = s_len + kRankRows;  // of the row of each rank: itself, its first token, the next row's, its prefix
+    int64_t c0 = 0, c1 = 0, before = 0;
     if (tid < p.B) {
-      const int64_t c0 = p.idx_i64 ? reinterpret_cast<const int64_t*>(p.cu)[tid] : reinterpret_cast<const int32_t*>(p.cu)[tid];
-      const int64_t c1 = p.idx_i64 ? reinterpret_cast<const int64_t*>(p.cu)[tid + 1] : reinterpret_cast<const int32_t*>(p.cu)[tid + 1];
-      s_len[tid] = c1 - c0 + (p.idx_i64 ? reinterpret_cast<const int64_t*>(p.prefix)[tid] : reinterpret_cast<const int32_t*>(p.prefix)[tid]);
+      c0 = read_index(p.cu, p.idx_i64, tid);
+      c1 = read_index(p.cu, p.idx_i64, tid + 1);
+      before = read_index(p.prefix, p.idx_i64, tid);
+      s_len[tid] = c1 - c0 + before;
     }
     __syncthreads();
     if (tid < p.B) {
-      const int64_t mine = s_len[tid];
+      const int64_t mine = c1 - c0 + before;
       int rank = 0;
       for (int u = 0; u < p.B; ++u) rank += s_len[u] > mine || (s_len[u] == mine && u < tid);
-      s_order[rank] = tid;
+      s_row[4 * rank] = tid;
+      s_row[4 * rank + 1] = c0;
+      s_row[4 * rank + 2] = c1;
+      s_row[4 * rank + 3] = before;
     }
     __syncthreads();
-    b = __builtin_amdgcn_readfirstlane(s_order[rr]);
+    b = __builtin_amdgcn_readfirstlane(static_cast<int>(s_row[4 * rr]));
+    tok0 = uniform64(s_row[4 * rr + 1]);
+    tok1 = uniform64(s_row[4 * rr + 2]);
+    prefix = uniform64(s_row[4 * rr + 3]);
     __syncthreads();
+  } else {
+    tok0 = read_index(p.cu, p.idx_i64, b);
+    tok1 = read_index(p.cu, p.idx_i64, b + 1);
+    prefix = read_index(p.prefix, p.idx_i64, b);
   }
-  const int64_t tok0 = read_index(p.cu, p.idx_i64, b);
-  const int64_t n_new = min64(read_index(p.cu, p.idx_i64, b + 1), p.total) - tok0;
+  const int64_t n_new = min64(tok1, p.total) - tok0;
   const int64_t ct0 = static_cast<int64_t>(gridDim.x) - 1 - blockIdx.x;
   const int64_t x0 = ct0 * kCols;  // first column of the workgroup
   if (tok0 < 0 || x0 >= n_new * p.G) return;
-  const int64_t prefix = read_index(p.prefix, p.idx_i64, b);
+  auto token_of = [&](int64_t x) { return over_group(p, static_cast<uint32_t>(x)); };  // columns fit 31 bits
   const int64_t last = min64(n_new * p.G, x0 + kCols) - 1;
   // keys that any column sees: not past the table
-  const int64_t kv_end = max64(0, min64(prefix + last / p.G + 1, p.max_blocks << p.bs_shift));
-  const int64_t first_pos = prefix + x0 / p.G;  // every column sees the keys up to here
+  const int64_t kv_end = max64(0, min64(prefix + token_of(last) + 1, p.max_blocks << p.bs_shift));
+  const int64_t first_pos = prefix + token_of(x0);  // every column sees the keys up to here
   const int64_t runs = (kv_end + kv4::kRun - 1) / kv4::kRun;
   const int64_t all_tiles = (kv_end + kTile - 1) / kTile;
-  const int64_t kt0 = all_tiles * blockIdx.z / pp.splits;
-  const int64_t kt1 = all_tiles * (blockIdx.z + 1) / pp.splits;
+  int64_t kt0 = 0, kt1 = all_tiles;
+  if (pp.splits > 1) {
+    kt0 = all_tiles * blockIdx.z / pp.splits;
+    kt1 = all_tiles * (blockIdx.z + 1) / pp.splits;
+  }
   const uint8_t* kb = p.kpool + g * p.sG;
   const uint8_t* vb = p.vpool + g * p.sG;
 
   // columns: [0] the wave's own 16, [1] its partner's; their position past first_pos
   const int n_cols = static_cast<int>(last - x0) + 1;
-  const int x_head = static_cast<int>(x0 % p.G);  // head of the workgroup's first column
+  const int x_head = static_cast<int>(x0 - static_cast<int64_t>(token_of(x0)) * p.G);  // head of the workgroup's first column
   int ahead[2];
 #pragma unroll
-  for (int c = 0; c < 2; ++c) ahead[c] = (min((wave ^ c) * 16 + col, n_cols - 1) + x_head) / p.G;
+  for (int c = 0; c < 2; ++c) ahead[c] = static_cast<int>(over_group(p, min((wave ^ c) * 16 + col, n_cols - 1) + x_head));
 
   // ---- the tiles' loads
   // Lane l of `cur` holds the offset in the head's pool of run 64 c + l (-1: not there), of `nxt` that of the next 64,
@@ -224,6 +240,14 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams p
 
   if (kt0 < kt1) {
     if (tid < 2) s_flag[tid] = 0;
+    // what the first tiles need is asked for before any of it is waited for: the query, the table, then two tiles' keys
+    QueryRow<D> row;
+    {
+      const int x = wave * 16 + col;
+      const int64_t tok = tok0 + token_of(x0 + x);
+      const int64_t head = x0 + x - (tok - tok0) * p.G + g * p.G;
+      row.ask(x < n_cols ? p.q + tok * p.q_st + head * p.q_sh : nullptr, quad);
+    }
     cur = chunk(kt0 >> 4);
     nxt = chunk((kt0 >> 4) + 1);
     cur_mask = __ballot(cur >= 0);
@@ -231,17 +255,20 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams p
     offsets(kt0);
     int there_cur = there;
     fetch_keys();
+    const uint4 kcode0 = kcode;
+    const uint32_t kscale0 = kscale;
     if (unpacks) fetch_values();
+    offsets(kt0 + 1);
+    int there_next = there;
+    fetch_keys();
+    const uint4 kcode1 = kcode;
+    const uint32_t kscale1 = kscale;
+    kcode = kcode0;
+    kscale = kscale0;
     QueryCols<D> qh, ql;
-    {
-      QueryRow<D> row;
-      const int x = wave * 16 + col;
-      const int64_t tok = tok0 + (x0 + x) / p.G;
-      const int64_t head = (x0 + x) % p.G + g * p.G;
-      row.load(x < n_cols ? p.q + tok * p.q_st + head * p.q_sh : nullptr, quad);
-      row.template split<false>(qh);
-      row.template split<true>(ql);
-    }
+    row.widen();
+    row.template split<false>(qh);
+    row.template split<true>(ql);
     const float qk_scale = p.scale * kLog2e;
     floatx4_v sc[kRuns];
     float use = 0.f;
@@ -342,10 +369,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams p
 #pragma unroll
       for (int e = 0; e < kBytesOfChunk; ++e) unpack_byte(e, 0);
     }
-    offsets(kt0 + 1);
-    int there_next = there;
-    fetch_keys();
     if (unpacks) fetch_values();
+    kcode = kcode1;
+    kscale = kscale1;
     store_keys(1);
     __syncthreads();
 
@@ -353,7 +379,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams p
     // that keep the order: the scores of tile kt + 1 with its unpacking, the values of tile kt with the exponentials.
     // (Waves 4 to 7 with the values first, half an iteration apart from the waves they share SIMDs with: no faster, 901
     // us against 895, 2048 tokens behind 32000.)
-    auto iterate = [&](int64_t kt, auto unpacking, auto more) {
+    auto iterate = [&](int64_t kt, auto more) {
       const int buf = static_cast<int>((kt - kt0) & 1);
       const int flag = s_flag[buf];
       const float c0 = s_corr[(buf * kWaves + wave) * 16 + col], c1 = s_corr[(buf * kWaves + (wave ^ 1)) * 16 + col];
@@ -362,11 +388,13 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams p
         fetch_keys();
       }
       if constexpr (more) {
-        if constexpr (unpacking) trim(kt + 1, buf ^ 1);
-        scores(buf ^ 1, [&](int f) {
-          if constexpr (unpacking) unpack_byte(f, buf ^ 1);
-        });
-        if constexpr (unpacking) fetch_values();
+        if (unpacks) {
+          trim(kt + 1, buf ^ 1);
+          scores(buf ^ 1, [&](int f) { unpack_byte(f, buf ^ 1); });
+          fetch_values();
+        } else {
+          scores(buf ^ 1, [](int) {});
+        }
         __builtin_amdgcn_sched_barrier(0);
       }
       bf16x8_v pv[2][2];
@@ -424,12 +452,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams p
     };
     using yes = std::integral_constant<bool, true>;
     using no = std::integral_constant<bool, false>;
-    if (unpacks) {
-      for (int64_t kt = kt0; kt + 1 < kt1; ++kt) iterate(kt, yes{}, yes{});
-    } else {
-      for (int64_t kt = kt0; kt + 1 < kt1; ++kt) iterate(kt, no{}, yes{});
+    for (int64_t kt = kt0; kt + 1 < kt1; ++kt) {
+      asm volatile(".p2align 6");  // the loop on a cache line: 875 us, unaligned 883
+      iterate(kt, yes{});
     }
-    iterate(kt1 - 1, no{}, no{});
+    iterate(kt1 - 1, no{});
   }
 
   // ---- out: this wave's dims of both column tiles
@@ -446,8 +473,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams p
     const int x = (wave ^ c) * 16 + col;
     if (x >= n_cols) continue;
     const float l = s_l[(wave ^ c) * 16 + col];
-    const int64_t tok = tok0 + (x0 + x) / p.G;
-    const int64_t head = (x0 + x) % p.G + g * p.G;
+    const float over = l == 0.f ? 0.f : 1.f / l;
+    const int64_t tok = tok0 + token_of(x0 + x);
+    const int64_t head = x0 + x - (tok - tok0) * p.G + g * p.G;
     const int64_t row = tok * p.H + head;
     const int d0 = half * MH;  // dims (4 quad + r) MT + d0 + i
 #pragma unroll
@@ -483,7 +511,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams p
         float v[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          v[e] = normalised(o[c][i + e][r], l);
+          v[e] = o[c][i + e][r] * over;
           if (gate != nullptr) {
             const uint32_t w = e < 2 ? graw[r][i / 4].x : graw[r][i / 4].y;
             v[e] *= sigmoid(__uint_as_float(e & 1 ? w & 0xffff0000u : w << 16));
@@ -496,6 +524,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams p
       }
   }
 }
+
+constexpr int kJoinAhead = 8;  // parts asked for at a time
 
 // Joins the parts of one (token, head): a wave each, lane l dims l D/64 ..
 template <int D>
@@ -516,28 +546,48 @@ __global__ __launch_bounds__(256) void join_kernel(PrefillParams pp, int64_t max
   const float f = __builtin_amdgcn_exp2f(ml.x - (m == -INFINITY ? 0.f : m));
   const float l = wave_sum(f * ml.y);
   vec_t acc = vec_t(0.f);
-  for (int s = 0; s < pp.splits; ++s) {
-    const float fs = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f), s));
-    const float ls = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(ml.y), s));
-    if (ls != 0.f) acc += fs * *reinterpret_cast<const vec_t*>(pp.part_o + (s * stride + row) * D + E * lane);  // a part that saw nothing wrote nothing
-  }
-  const int64_t n = x / p.H, h = x - n * p.H;
+  for (int s0 = 0; s0 < pp.splits; s0 += kJoinAhead) {
+    vec_t part[kJoinAhead];
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    float r = normalised(acc[e], l);
-    if (p.gate != nullptr) r *= sigmoid(bf16_to_f32(p.gate[(tok0 + n) * p.gate_st + h * p.gate_sh + E * lane + e]));
-    p.out[row * D + E * lane + e] = f32_to_bf16(r);
+    for (int i = 0; i < kJoinAhead; ++i)  // past the end: the last part again
+      part[i] = *reinterpret_cast<const vec_t*>(pp.part_o + (min(s0 + i, pp.splits - 1) * stride + row) * D + E * lane);
+#pragma unroll
+    for (int i = 0; i < kJoinAhead; ++i) {
+      const int s = min(s0 + i, pp.splits - 1);
+      const float fs = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f), s));
+      const float ls = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(ml.y), s));
+      if (s0 + i < pp.splits && ls != 0.f) acc += fs * part[i];  // a part that saw nothing wrote nothing
+    }
   }
+  const uint32_t n = static_cast<uint32_t>(x) / static_cast<uint32_t>(p.H), h = static_cast<uint32_t>(x) - n * static_cast<uint32_t>(p.H);
+  typedef uint32_t packed_t __attribute__((ext_vector_type(E / 2)));
+  packed_t gate = packed_t(0u), out;
+  if (p.gate != nullptr) gate = *reinterpret_cast<const packed_t*>(p.gate + (tok0 + n) * p.gate_st + h * p.gate_sh + E * lane);
+#pragma unroll
+  for (int e = 0; e < E; e += 2) {
+    float lo = normalised(acc[e], l), hi = normalised(acc[e + 1], l);
+    if (p.gate != nullptr) {
+      lo *= sigmoid(__uint_as_float(gate[e / 2] << 16));
+      hi *= sigmoid(__uint_as_float(gate[e / 2] & 0xffff0000u));
+    }
+    out[e / 2] = static_cast<uint32_t>(f32_to_bf16(lo)) | static_cast<uint32_t>(f32_to_bf16(hi)) << 16;
+  }
+  *reinterpret_cast<packed_t*>(p.out + row * D + E * lane) = out;
 }
 
 constexpr int kMaxSplits = 64;
 
-// Parts the keys are split into: as many as fill the chip, of at least four tiles each where every row is as long as its table.
+// Parts the keys are split into where the workgroups leave CUs free.  A part saves a share of 1.5 us a tile and costs its
+// piece of the partial results, in time like parts times workgroups, which puts the best number at a root; the 30 is from
+// us with 1, 2, 4, 8, 16 parts, D = 256, one row: 16 tokens (2 workgroups) over 32 tiles 65.6 41.9 29.2 23.3 22.1, 128 tokens
+// (16) over 17 tiles 42.3 31.9 27.7 30.8 35.4, 512 tokens (64) over 8 tiles 28.6 33.6 35.4 51.4 64.5, over 32 tiles 67.2
+// 52.8 45.3 64.9 105.
 static int splits_of(int64_t batch, int kv_heads, int group, int64_t max_new, int64_t max_tokens) {
   const int64_t wgs = batch * kv_heads * ceil_div(max_new * group, kCols);
   const int64_t tiles = ceil_div(std::max<int64_t>(max_tokens, 1), kTile);
   if (wgs >= 256) return 1;
-  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({kMaxSplits, 256 / wgs, tiles / 4})));
+  const int64_t best = static_cast<int64_t>(std::sqrt(30.0 * static_cast<double>(tiles) / static_cast<double>(wgs)));
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({kMaxSplits, 256 / wgs, tiles, best})));
 }
 
 static int64_t workspace_of(int splits, int64_t total, int heads, int head_dim) {
