@@ -288,13 +288,16 @@ int qa_qk_norm_rope_append(const void* q_proj, int64_t q_stride_t, int64_t q_str
  * qa_paged_kv_reserve 1 to 4, or 5 where the step has more than max_tokens
  * tokens; then cu_seqlens is all 0, every position and slot -1, and tables,
  * lengths and free_state are left as they were.  tables, lengths int32.
+ * per_row: 0, or the entries that positions and slots hold for each row (then
+ * max_tokens is batch * per_row, a row's tokens are the first of its entries,
+ * and a row with more is status 5).
  * workspace: 4 bytes a row.  Replaces the host-side growth and slot arithmetic
  * of src/decode_state.py:72-78,271-293,365-374.                              */
 int qa_paged_kv_plan(int32_t* block_tables, int64_t table_stride, int64_t max_blocks, int32_t* lengths,
                      const void* counts, int32_t counts_dtype, int64_t count_scalar, int64_t batch, int32_t block_size,
                      const int32_t* free_list, int64_t free_capacity, int32_t* free_state, int32_t* status,
-                     int64_t max_tokens, int32_t* cu_seqlens, int32_t* starts, int32_t* positions, int64_t* slots,
-                     int32_t* workspace, int64_t workspace_bytes, hipStream_t stream);
+                     int64_t max_tokens, int64_t per_row, int32_t* cu_seqlens, int32_t* starts, int32_t* positions,
+                     int64_t* slots, int32_t* workspace, int64_t workspace_bytes, hipStream_t stream);
 
 /* Quantise key/value rows of packed tokens, element (n, h, d) at n*stride_t +
  * h*stride_h + d, float32 or bfloat16, 16-byte aligned rows, into slots[n] of

@@ -24,7 +24,9 @@ engine and scheduler above it keep their calls:
   kernel.
 
 Host-side tensor preparation (L2 norm, transposes) is PyTorch on the same
-device; every hot loop is a HIP kernel.  There is no CPU or dense fallback in
+device; every hot loop is a HIP kernel.  Pools may hold bf16 or 4 bits
+(``decode_state.SharedKV4BlockPool``): the entry points choose by the pool's
+type, and ``RopeConfig.mrope_section`` adds rotary positions of several axes.  There is no CPU or dense fallback in
 this module.
 """
 
@@ -34,7 +36,7 @@ import contextlib
 from dataclasses import dataclass, field
 from typing import Any, Iterator, Sequence
 
-from decode_state import DeviceBatchPageTables, FullAttentionCache, LinearStatePool, PrefillStep, batch_page_tables
+from decode_state import DeviceBatchPageTables, FullAttentionCache, LinearStatePool, PrefillStep, batch_page_tables, is_kv4, kv4_head_dim
 
 # --------------------------------------------------------------------------- config
 
@@ -166,6 +168,8 @@ def paged_attention_fallback_reason(config: AttentionConfig, query: Any, key: An
     q_shape = tuple(getattr(query, "shape", ()))
     k_shape = tuple(getattr(key, "shape", ()))
     v_shape = tuple(getattr(value, "shape", ()))
+    if is_kv4(key):
+        return _kv4_reason(query, key, value)
     if len(q_shape) != 4 or len(k_shape) not in (4, 5) or len(v_shape) != len(k_shape):
         return "shape"
     if len(k_shape) == 5:
@@ -185,6 +189,19 @@ def paged_attention_fallback_reason(config: AttentionConfig, query: Any, key: An
         if str(q_dtype) not in _FLOAT_DTYPES or str(k_dtype) not in _FLOAT_DTYPES or str(k_dtype) != str(v_dtype):
             return "shape"
     return "no_kernel"
+
+
+def _kv4_reason(query: Any, key: Any, value: Any, block_size: int | None = None) -> str:
+    """The ladder's last rung for a 4-bit pool ``(P, H_kv, tile)``, which the reference does not have: a bf16 query
+    ``(B, H, 1, D)`` of a group of up to 16 heads, over tiles of its head_dim (and of ``block_size`` tokens)."""
+    q_shape = tuple(query.shape)
+    if len(q_shape) != 4 or str(query.dtype) != "torch.bfloat16" or not is_kv4(value) or key.dim() != 3 or tuple(value.shape) != tuple(key.shape):
+        return "shape"
+    if q_shape[1] % int(key.shape[1]) or q_shape[1] // int(key.shape[1]) > 16 or q_shape[3] not in (128, 256):
+        return "shape"
+    if block_size is None:
+        return "no_kernel" if int(key.shape[2]) * 32 % (17 * q_shape[3]) == 0 else "shape"
+    return "no_kernel" if kv4_head_dim(key, value, block_size) == q_shape[3] else "shape"
 
 
 def batched_paged_attention_fallback_reason(config: AttentionConfig, query: Any, caches: Sequence[FullAttentionCache], page_tables: Any, *, seq_len: int) -> str:
@@ -258,9 +275,14 @@ def full_attention_paged(query: Any, gate: Any | None, cache: FullAttentionCache
 
     try:
         with runtime.profile_scope("full_attention.native_paged"):
-            heads = hip_ops.paged_attention_decode(
-                query, page_table.block_table, page_table.key_blocks, page_table.value_blocks, page_table.sequence_length, page_table.block_size
-            )
+            if is_kv4(page_table.key_blocks):
+                table = page_table.block_table.unsqueeze(0)
+                lengths = table.new_full((1,), page_table.sequence_length)
+                heads = hip_ops.paged_attention_decode_kv4(query, table, page_table.key_blocks, page_table.value_blocks, lengths, page_table.block_size)
+            else:
+                heads = hip_ops.paged_attention_decode(
+                    query, page_table.block_table, page_table.key_blocks, page_table.value_blocks, page_table.sequence_length, page_table.block_size
+                )
     except hip_loader.NativeLibraryMissing:
         raise
     except RuntimeError:
@@ -276,10 +298,14 @@ def full_attention_paged_batch(query: Any, gate: Any | None, caches: Sequence[Fu
     """Native branch of ``_tp_full_attention_batch_paged_or_dense`` (``src/tp_runtime.py:2498-2555``).
 
     Caches may each own a reference-layout pool or share one
-    ``SharedKVBlockPool``; either way one kernel launch serves the batch.
+    ``SharedKVBlockPool``; either way one kernel launch serves the batch.  Caches
+    on 4-bit pools must share one.
     """
     page_tables = batch_page_tables(caches) if config.full_attention.paged_kv_metadata else None
     reason = batched_paged_attention_fallback_reason(config, query, caches, page_tables, seq_len=int(query.shape[2]))
+    kv4 = any(is_kv4(cache.key_blocks) for cache in caches)
+    if reason == "no_kernel" and kv4 and any(cache.key_blocks is not caches[0].key_blocks for cache in caches):
+        reason = "per_request_pools"
     if reason != "no_kernel" or page_tables is None:
         record_native_paged_dispatch(runtime, reason, native=False)
         return None
@@ -288,10 +314,15 @@ def full_attention_paged_batch(query: Any, gate: Any | None, caches: Sequence[Fu
 
     try:
         with runtime.profile_scope("batch.full_attention.native_paged"):
-            heads = hip_ops.paged_attention_decode_batched(
-                query, page_tables.block_tables, list(page_tables.key_blocks), list(page_tables.value_blocks), page_tables.sequence_lengths,
-                page_tables.block_size,
-            )
+            if kv4:
+                heads = hip_ops.paged_attention_decode_kv4(
+                    query, page_tables.block_tables, page_tables.key_blocks[0], page_tables.value_blocks[0], page_tables.sequence_lengths, page_tables.block_size
+                )
+            else:
+                heads = hip_ops.paged_attention_decode_batched(
+                    query, page_tables.block_tables, list(page_tables.key_blocks), list(page_tables.value_blocks), page_tables.sequence_lengths,
+                    page_tables.block_size,
+                )
     except hip_loader.NativeLibraryMissing:
         raise
     except RuntimeError:
@@ -305,7 +336,7 @@ def full_attention_paged_batch(query: Any, gate: Any | None, caches: Sequence[Fu
 
 def full_attention_decode_device(
     query: Any, gate: Any | None, key: Any, value: Any, key_blocks: Any, value_blocks: Any, tables: DeviceBatchPageTables,
-    config: AttentionConfig, runtime: HotPathRuntime, *, no_alloc: bool = False,
+    config: AttentionConfig, runtime: HotPathRuntime, *, no_alloc: bool = False, plan: Any | None = None,
 ) -> Any | None:
     """One decode token of a full-attention layer for every row of a running batch, on
     device-resident page tables: the batched native branch of
@@ -321,8 +352,14 @@ def full_attention_decode_device(
     ``None`` means the caller runs its dense path.  With ``no_alloc`` the attention runs on the
     library's static scratch (``qa_paged_attention_decode_batched_noalloc``) instead of a
     workspace.  Nothing here reads back to the host or copies host to device.
+
+    On a 4-bit pool the step is reserved by ``plan = tables.plan_step()`` in place of
+    ``reserve_step``, and its K/V are written to the plan's slots; ``no_alloc`` is for bf16 pools.
     """
     reason = _device_pool_reason(config, query, key_blocks, value_blocks, tables)
+    kv4 = is_kv4(key_blocks)
+    if reason == "no_kernel":
+        _check_step(kv4, plan, no_alloc, tables)
     if reason != "no_kernel":
         record_native_paged_dispatch(runtime, reason, native=False)
         return None
@@ -332,8 +369,12 @@ def full_attention_decode_device(
     # later kernel error propagates: a dense fallback would attend over a cache that already
     # holds the step (and under graph capture would record a step without attention).
     with runtime.profile_scope("batch.full_attention.native_paged_device"):
-        tables.append(key, value, key_blocks, value_blocks)
-        decode = hip_ops.paged_attention_decode_batched_noalloc if no_alloc else hip_ops.paged_attention_decode_batched
+        if kv4:
+            hip_ops.paged_kv4_append(key[:, :, 0], value[:, :, 0], key_blocks, value_blocks, plan.slots, tables.block_size)
+            decode = hip_ops.paged_attention_decode_kv4
+        else:
+            tables.append(key, value, key_blocks, value_blocks)
+            decode = hip_ops.paged_attention_decode_batched_noalloc if no_alloc else hip_ops.paged_attention_decode_batched
         heads = decode(query, tables.block_tables, key_blocks, value_blocks, tables.sequence_lengths, tables.block_size)
     record_native_paged_dispatch(runtime, reason, native=True)
     return heads if gate is None else _gate_heads(heads, gate)
@@ -342,16 +383,29 @@ def full_attention_decode_device(
 def _device_pool_reason(config: AttentionConfig, query: Any, key_blocks: Any, value_blocks: Any, tables: DeviceBatchPageTables) -> str:
     """The dispatch ladder for a step on device page tables, checked before anything is written:
     the reference's reasons (one token per row), then what the native kernels need of the pool
-    (a shared ``(P, H_kv, bs, D)`` bf16 pool with the tables' block size and block count)."""
+    (a shared ``(P, H_kv, bs, D)`` bf16 pool with the tables' block size and block count, or such
+    a pool of 4-bit tiles)."""
     seq_len = int(query.shape[2]) if len(tuple(getattr(query, "shape", ()))) == 4 else 1
     reason = paged_attention_fallback_reason(config, query, key_blocks, value_blocks, seq_len=seq_len, batched=False)
     if reason != "no_kernel":
         return reason
+    if is_kv4(key_blocks):
+        return _kv4_reason(query, key_blocks, value_blocks, tables.block_size) if int(key_blocks.shape[0]) == tables.num_blocks else "shape"
     if key_blocks.dim() != 4 or tuple(value_blocks.shape) != tuple(key_blocks.shape):
         return "shape"
     if int(key_blocks.shape[2]) != tables.block_size or int(key_blocks.shape[0]) != tables.num_blocks:
         return "shape"
     return "no_kernel"
+
+
+def _check_step(by_slots: bool, plan: Any | None, no_alloc: bool, tables: DeviceBatchPageTables) -> None:
+    """Calls that would be wrong whatever the tensors hold, refused before anything is written."""
+    if not by_slots:
+        return
+    if plan is None or tuple(plan.slots.shape) != (tables.rows,):
+        raise ValueError("a 4-bit pool or mrope_section needs the step's plan (tables.plan_step())")
+    if no_alloc:
+        raise ValueError("no_alloc is for bf16 pools: the 4-bit decode takes its workspace per call")
 
 
 def _qk_norm_rope(q_proj: Any, k_proj: Any, v_proj: Any, q_norm_weight: Any, k_norm_weight: Any, key_blocks: Any, value_blocks: Any,
@@ -372,12 +426,33 @@ class RopeConfig:
     rms_norm_eps: float = 1e-6
     rope_theta: float = 10_000_000.0
     partial_rotary_factor: float = 0.25
+    # rotary positions of several axes (time, row, column of a picture's tokens): how many of the frequencies each axis
+    # turns, and whether the axes take turns (hip_ops.mrope_axes).  None: one position a token.
+    mrope_section: tuple[int, ...] | None = None
+    mrope_interleaved: bool = False
+
+    def sections(self, head_dim: int) -> tuple[int, ...]:
+        return self.mrope_section or (int(head_dim * self.partial_rotary_factor) // 2,)
+
+
+def _qk_norm_mrope(q_proj: Any, k_proj: Any, v_proj: Any, q_norm_weight: Any, k_norm_weight: Any, key_blocks: Any, value_blocks: Any, plan: Any, block_size: int,
+                   rope: RopeConfig, head_dim: int, positions: Any | None) -> tuple[Any, Any]:
+    """The prologue by slots; without ``positions`` a token has its place in its row on every axis, as text does."""
+    import hip_ops
+
+    sections = rope.sections(head_dim)
+    if positions is None:
+        positions = plan.positions.expand(len(sections), -1)
+    return hip_ops.qk_norm_mrope_kv_append(
+        q_proj, k_proj, v_proj, q_norm_weight, k_norm_weight, positions, sections, key_blocks, value_blocks, plan.slots, block_size,
+        eps=rope.rms_norm_eps, rope_theta=rope.rope_theta, interleaved=rope.mrope_interleaved,
+    )
 
 
 def full_attention_decode_step_device(
     q_proj: Any, k_proj: Any, v_proj: Any, q_norm_weight: Any, k_norm_weight: Any, key_blocks: Any, value_blocks: Any,
     tables: DeviceBatchPageTables, config: AttentionConfig, runtime: HotPathRuntime, rope: RopeConfig = RopeConfig(), *,
-    no_alloc: bool = False,
+    no_alloc: bool = False, plan: Any | None = None, positions: Any | None = None,
 ) -> Any | None:
     """One decode token of a full-attention layer for every row of a running batch, from the
     projection outputs: ``tp_full_attention``'s norm/RoPE/append (``src/tp_runtime.py:511-525``)
@@ -394,24 +469,42 @@ def full_attention_decode_step_device(
     appended, errors raise instead of returning ``None``: with ``no_alloc`` a batch whose partials
     exceed the library's 32 MiB scratch raises ``RuntimeError`` with the token already in the
     cache, so the caller must not append it again.
+
+    With a 4-bit pool (``SharedKV4BlockPool``) or ``rope.mrope_section`` the step is reserved by
+    ``plan = tables.plan_step()`` in place of ``reserve_step``; ``positions`` ``(axes, rows)`` then
+    gives each row's rotary positions (its place in the row on every axis where omitted: text).
+    On a 4-bit pool the gate is applied inside the decode and ``no_alloc`` is refused.
     """
     rows = int(q_proj.shape[0])
     full = config.full_attention
     heads, head_dim, kv_heads = full.num_heads, full.head_dim, full.num_key_value_heads
     probe = _query_probe(q_proj, heads, head_dim)
     reason = _device_pool_reason(config, probe, key_blocks, value_blocks, tables)
-    if reason == "no_kernel" and (rows != tables.rows or int(key_blocks.shape[1]) != kv_heads or int(key_blocks.shape[3]) != head_dim
-                                  or str(key_blocks.dtype) != "torch.bfloat16" or str(q_proj.dtype) != "torch.bfloat16"):
+    kv4 = is_kv4(key_blocks)
+    if reason == "no_kernel" and (rows != tables.rows or int(key_blocks.shape[1]) != kv_heads or str(q_proj.dtype) != "torch.bfloat16"):
         reason = "shape"
+    if reason == "no_kernel" and not kv4 and (int(key_blocks.shape[3]) != head_dim or str(key_blocks.dtype) != "torch.bfloat16"):
+        reason = "shape"
+    by_slots = kv4 or rope.mrope_section is not None
+    if reason == "no_kernel":
+        _check_step(by_slots, plan, no_alloc and kv4, tables)
     if reason != "no_kernel":
         record_native_paged_dispatch(runtime, reason, native=False)
         return None
     import hip_ops
 
-    cu = _row_offsets(rows, q_proj.device)
     with runtime.profile_scope("batch.full_attention.native_paged_device"):
-        query, gate = _qk_norm_rope(q_proj, k_proj, v_proj, q_norm_weight, k_norm_weight, key_blocks, value_blocks, tables.block_tables,
-                                    cu, tables.positions, tables.block_size, 1, rope)
+        if by_slots:
+            query, gate = _qk_norm_mrope(q_proj, k_proj, v_proj, q_norm_weight, k_norm_weight, key_blocks, value_blocks, plan, tables.block_size, rope, head_dim, positions)
+        else:
+            cu = _row_offsets(rows, q_proj.device)
+            query, gate = _qk_norm_rope(q_proj, k_proj, v_proj, q_norm_weight, k_norm_weight, key_blocks, value_blocks, tables.block_tables,
+                                        cu, tables.positions, tables.block_size, 1, rope)
+        if kv4:
+            out = hip_ops.paged_attention_decode_kv4(query.view(rows, heads, 1, head_dim), tables.block_tables, key_blocks, value_blocks, tables.sequence_lengths,
+                                                     tables.block_size, gate=gate if full.output_gate else None)
+            record_native_paged_dispatch(runtime, reason, native=True)
+            return out.view(rows, 1, heads * head_dim)
         decode = hip_ops.paged_attention_decode_batched_noalloc if no_alloc else hip_ops.paged_attention_decode_batched
         heads_out = decode(query.view(rows, heads, 1, head_dim), tables.block_tables, key_blocks, value_blocks, tables.sequence_lengths,
                            tables.block_size)
@@ -449,7 +542,8 @@ def _query_probe(q_proj: Any, heads: int, head_dim: int) -> Any:
 
 def full_attention_prefill_device(
     q_proj: Any, k_proj: Any, v_proj: Any, q_norm_weight: Any, k_norm_weight: Any, key_blocks: Any, value_blocks: Any,
-    step: PrefillStep, config: AttentionConfig, runtime: HotPathRuntime, rope: RopeConfig = RopeConfig(),
+    step: PrefillStep, config: AttentionConfig, runtime: HotPathRuntime, rope: RopeConfig = RopeConfig(), *,
+    positions: Any | None = None,
 ) -> Any | None:
     """A multi-token step (a prompt or one chunk of it) of a full-attention layer, from the
     projection outputs, on the native chunked prefill: ``tp_full_attention``
@@ -470,18 +564,28 @@ def full_attention_prefill_device(
     call that does not qualify returns ``None`` and counts as ``"prefill_or_multitoken"`` (the
     reference's reason for every multi-token call) or ``"shape"``, so the caller's dense path
     runs; nothing has been written by then.  Native calls count in ``native_prefill_hits``.
+
+    A 4-bit pool or ``rope.mrope_section`` needs the ``step`` of ``DeviceBatchPageTables.plan_prefill``;
+    ``positions`` ``(axes, tokens)`` are the tokens' rotary positions, by default their places in
+    their rows on every axis.
     """
     import torch
 
     tokens = int(q_proj.shape[0])
     full = config.full_attention
     heads, head_dim, kv_heads = full.num_heads, full.head_dim, full.num_key_value_heads
+    kv4 = is_kv4(key_blocks)
+    by_slots = kv4 or rope.mrope_section is not None
     probe = _query_probe(q_proj, heads, head_dim)
     if probe.dim() == 4:
         probe = probe[:1]  # one token stands for the step: the ladder reads heads and widths, not rows
     reason = paged_attention_fallback_reason(config, probe, key_blocks, value_blocks, seq_len=1, batched=False)
     if reason == "no_kernel":
-        if key_blocks.dim() != 4:
+        if kv4:
+            if (int(key_blocks.shape[1]) != kv_heads or tokens != step.total_tokens or q_proj.dtype != torch.bfloat16
+                    or kv4_head_dim(key_blocks, value_blocks, step.block_size) != head_dim):
+                reason = "shape"
+        elif key_blocks.dim() != 4:
             reason = "prefill_or_multitoken"  # per-request (reference-layout) pools: the dense path
         elif (tuple(value_blocks.shape) != tuple(key_blocks.shape) or int(key_blocks.shape[2]) != step.block_size
               or int(key_blocks.shape[1]) != kv_heads or int(key_blocks.shape[3]) != head_dim or tokens != step.total_tokens
@@ -492,11 +596,17 @@ def full_attention_prefill_device(
         return None
     import hip_ops
 
+    if by_slots and step.plan is None:
+        raise ValueError("a 4-bit pool or mrope_section needs a step of plan_prefill")
     with runtime.profile_scope("full_attention.native_paged_prefill"):
-        query, gate = _qk_norm_rope(q_proj, k_proj, v_proj, q_norm_weight, k_norm_weight, key_blocks, value_blocks, step.block_tables,
-                                    step.cu_seqlens, step.starts, step.block_size, step.max_new, rope)
-        out = hip_ops.paged_attention_prefill(query, step.cu_seqlens, step.starts, key_blocks, value_blocks, step.block_tables,
-                                              step.block_size, max_new=step.max_new, gate=gate if full.output_gate else None)
+        if by_slots:
+            query, gate = _qk_norm_mrope(q_proj, k_proj, v_proj, q_norm_weight, k_norm_weight, key_blocks, value_blocks, step.plan, step.block_size, rope, head_dim, positions)
+        else:
+            query, gate = _qk_norm_rope(q_proj, k_proj, v_proj, q_norm_weight, k_norm_weight, key_blocks, value_blocks, step.block_tables,
+                                        step.cu_seqlens, step.starts, step.block_size, step.max_new, rope)
+        prefill = hip_ops.paged_attention_prefill_kv4 if kv4 else hip_ops.paged_attention_prefill
+        out = prefill(query, step.cu_seqlens, step.starts, key_blocks, value_blocks, step.block_tables,
+                      step.block_size, max_new=step.max_new, gate=gate if full.output_gate else None)
     stats = runtime.paged_attention_stats
     stats.calls += 1
     stats.eligible += 1

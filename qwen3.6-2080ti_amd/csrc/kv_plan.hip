@@ -5,7 +5,8 @@
 // over the rows c_b of n and f_b of need give everything: packed token i of row b (i - c_b = x) sits at position
 // L_b + x; its logical block lb is the row's old one while lb < ceil(L_b / bs), else free_list[head + f_b + lb -
 // ceil(L_b / bs)]; its slot is id * bs + position % bs.  A fresh block always holds a new token at its first position,
-// so the token there writes the table entry: no pass of its own over the tables.
+// so the token there writes the table entry: no pass of its own over the tables.  Where every row has per_row entries of
+// the token arrays instead, the row of an entry is a division and the rest the same.
 //
 // A few KB move, so latency bounds it: a launch of one workgroup reads lengths, counts and state at once (with a thread a
 // row the scan that plans is also the sum that is checked), looks the tokens' rows up in LDS and writes them.  128 rows of
@@ -31,6 +32,7 @@ struct Params {
   int32_t* positions;  // (max_tokens)
   int64_t* slots;      // (max_tokens)
   int64_t max_tokens, capacity;
+  uint32_t per_row;    // 0: the tokens are packed; else row b's are entries b per_row ..
   int B, bs, counts_i64;
   int inline_tokens;   // the planning workgroup writes the tokens too
 };
@@ -63,8 +65,15 @@ __device__ void write_tokens(const Params& p, const Rows& rows, int64_t lo, int6
   for (int64_t i = lo + threadIdx.x; i < hi; i += blockDim.x) {
     int32_t position = -1;
     int64_t slot = -1;
-    if (i < total) {
-      int a = 0, z = p.B;  // cu[a] <= i < cu[z]
+    int a = 0;
+    int32_t nth = 0;
+    bool token = i < total;
+    if (p.per_row != 0) {
+      a = static_cast<int>(static_cast<uint32_t>(i) / p.per_row);
+      nth = static_cast<int32_t>(i - static_cast<int64_t>(a) * p.per_row);
+      token = nth < rows.cu[a + 1] - rows.cu[a];
+    } else if (token) {
+      int z = p.B;  // cu[a] <= i < cu[z]
       while (z - a > 1) {
         const int m = (a + z) >> 1;
         if (rows.cu[m] <= i)
@@ -72,8 +81,11 @@ __device__ void write_tokens(const Params& p, const Rows& rows, int64_t lo, int6
         else
           z = m;
       }
+      nth = static_cast<int32_t>(i - rows.cu[a]);
+    }
+    if (token) {
       const int32_t start = rows.starts[a];
-      position = start + static_cast<int32_t>(i - rows.cu[a]);
+      position = start + nth;
       const uint32_t lb = static_cast<uint32_t>(position) / p.bs;
       const uint32_t have = blocks_of(p, start);
       const uint32_t at = position - lb * p.bs;
@@ -116,6 +128,7 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(Params p) {
     }
     const uint32_t want = blocks_of(p, len + n);
     if (want > p.max_blocks) bad |= 2;
+    if (p.per_row != 0 && n > p.per_row) bad |= 8;
     need = want - blocks_of(p, len);
   };
   // sums over the workgroup: of all rows, or up to and with a thread's own
@@ -173,7 +186,7 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(Params p) {
   else if (bad & 4) code = 4;
   else if (bad & 2) code = 2;
   else if (total_need > avail) code = 1;
-  else if (total_count > p.max_tokens) code = 5;
+  else if (total_count > p.max_tokens || (bad & 8)) code = 5;
   const int64_t taken = total_need;
 
   // the row sums; a step that is refused plans no token and takes nothing
@@ -238,7 +251,7 @@ __global__ __launch_bounds__(256) void plan_tokens_kernel(Params p) {
 
 extern "C" int qa_paged_kv_plan(int32_t* block_tables, int64_t table_stride, int64_t max_blocks, int32_t* lengths, const void* counts, int32_t counts_dtype,
                                 int64_t count_scalar, int64_t batch, int32_t block_size, const int32_t* free_list, int64_t free_capacity, int32_t* free_state,
-                                int32_t* status, int64_t max_tokens, int32_t* cu_seqlens, int32_t* starts, int32_t* positions, int64_t* slots, int32_t* workspace,
+                                int32_t* status, int64_t max_tokens, int64_t per_row, int32_t* cu_seqlens, int32_t* starts, int32_t* positions, int64_t* slots, int32_t* workspace,
                                 int64_t workspace_bytes, hipStream_t stream) {
   using namespace qa;
   using namespace qa::kvplan;
@@ -251,6 +264,8 @@ extern "C" int qa_paged_kv_plan(int32_t* block_tables, int64_t table_stride, int
              static_cast<long long>(max_blocks));
   QA_REQUIRE(free_capacity > 0 && free_capacity <= 0x7fffffff, "free list capacity must be in [1, 2^31)");
   QA_REQUIRE(max_tokens >= 0 && max_tokens <= 0x3fffffff, "paged_kv_plan: max_tokens must be in [0, 2^30)");
+  QA_REQUIRE(per_row >= 0 && per_row <= 0x3fffffff && (per_row == 0 || per_row * batch == max_tokens), "paged_kv_plan: with %lld entries a row max_tokens must be %lld", static_cast<long long>(per_row),
+             static_cast<long long>(per_row * batch));
   QA_REQUIRE(max_tokens == 0 || (positions && slots), "paged_kv_plan: pointers must be non-null");
   QA_REQUIRE(workspace_bytes >= batch * 4, "paged_kv_plan: workspace too small: need %lld bytes", static_cast<long long>(batch * 4));
   Params p{};
@@ -269,6 +284,7 @@ extern "C" int qa_paged_kv_plan(int32_t* block_tables, int64_t table_stride, int
   p.positions = positions;
   p.slots = slots;
   p.max_tokens = max_tokens;
+  p.per_row = static_cast<uint32_t>(per_row);
   p.capacity = free_capacity;
   p.B = static_cast<int>(batch);
   p.bs = block_size;

@@ -20,6 +20,8 @@ What changes underneath:
   every request; caches created with ``shared_pool=`` draw blocks from it, so
   growth never reallocates and ``batch_page_tables`` hands the decode kernel a
   single pool.
+* ``SharedKV4BlockPool`` is the same pool in 4 bits (17 bytes per 32 values in
+  place of 64): the reference has no quantised cache.
 * ``LinearStatePool`` keeps recurrent and conv states of many requests in
   slot-indexed device tensors updated in place (the reference stacks and
   scatters per-request states each step, ``src/tp_runtime.py:2678-2707``).
@@ -188,6 +190,67 @@ class SharedKVBlockPool:
         return self.allocator
 
 
+class SharedKV4BlockPool(SharedKVBlockPool):
+    """:class:`SharedKVBlockPool` in 4 bits: uint8 tensors ``(num_blocks, kv_heads, kv4_tile_bytes(head_dim, block_size))``.
+
+    E2M1 codes with a power-of-two scale per 32 dims of a token (``qwen36_hip.h``), 17 bytes per 32 values where bf16
+    takes 64, so a pool holds 3.8 times the tokens.  ``head_dim`` is 128 or 256, ``block_size`` a power of two from 16 to
+    1024.  It is written and read by the 4-bit operators of ``hip_ops`` and takes the place of a bf16 pool in
+    :class:`FullAttentionCache`, :class:`DeviceBatchPageTables` and the entry points of ``attention_runtime``.
+    """
+
+    def __init__(self, num_blocks: int, kv_heads: int, head_dim: int, *, block_size: int = DEFAULT_KV_BLOCK_SIZE, device: Any = None) -> None:
+        import torch
+
+        import hip_ops
+
+        if num_blocks <= 0 or kv_heads <= 0:
+            raise ValueError("num_blocks and kv_heads must be positive")
+        self.block_size = block_size
+        self.kv_heads = kv_heads
+        self.head_dim = head_dim
+        self.key_blocks = torch.zeros((num_blocks, kv_heads, hip_ops.kv4_tile_bytes(head_dim, block_size)), dtype=torch.uint8, device=device)
+        self.value_blocks = torch.zeros_like(self.key_blocks)
+        self.free_blocks = list(range(num_blocks))
+        self.allocator = None
+
+    @classmethod
+    def from_tensors(cls, key_blocks: Any, value_blocks: Any, *, block_size: int = DEFAULT_KV_BLOCK_SIZE, free_blocks: Sequence[int] | None = None) -> "SharedKV4BlockPool":
+        """A pool over existing tiles; ``block_size`` says how many tokens one holds."""
+        head_dim = kv4_head_dim(key_blocks, value_blocks, block_size)
+        if head_dim is None:
+            raise ValueError("pool tensors must be uint8 (num_blocks, kv_heads, tile bytes of the block size) and alike")
+        pool = cls.__new__(cls)
+        pool.block_size = block_size
+        pool.kv_heads = int(key_blocks.shape[1])
+        pool.head_dim = head_dim
+        pool.key_blocks = key_blocks
+        pool.value_blocks = value_blocks
+        pool.free_blocks = list(range(int(key_blocks.shape[0]))) if free_blocks is None else sorted(int(b) for b in free_blocks)
+        pool.allocator = None
+        return pool
+
+
+def is_kv4(blocks: Any) -> bool:
+    """Whether a pool tensor is one of 4-bit tiles."""
+    return str(getattr(blocks, "dtype", "")) == "torch.uint8"
+
+
+def kv4_head_dim(key_blocks: Any, value_blocks: Any, block_size: int) -> int | None:
+    """The head_dim of a 4-bit pool whose tiles hold ``block_size`` tokens, or ``None`` where they do not."""
+    import hip_ops
+
+    if not is_kv4(key_blocks) or not is_kv4(value_blocks) or key_blocks.dim() != 3 or tuple(value_blocks.shape) != tuple(key_blocks.shape):
+        return None
+    for head_dim in (128, 256):
+        try:
+            if hip_ops.kv4_tile_bytes(head_dim, block_size) == int(key_blocks.shape[2]):
+                return head_dim
+        except RuntimeError:
+            return None
+    return None
+
+
 class DeviceBlockAllocator:
     """Device-resident free list of a shared KV pool.
 
@@ -217,25 +280,35 @@ class DeviceBlockAllocator:
             self.free_list[: len(ids)] = torch.tensor(ids, dtype=torch.int32, device=self.device)
         self.free_state = torch.tensor([0, len(ids)], dtype=torch.int32, device=self.device)
         self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
+        self._last = "paged_kv_reserve"
 
     _STATUS = {
         1: "shared KV pool exhausted",
         2: "block table too short for the reserved blocks",
         3: "device free list state is corrupt",
         4: "negative or overflowing length/count",
+        5: "more new tokens than the step has room for",
     }
 
     def reserve(self, block_tables: Any, lengths: Any, block_size: int, *, counts: Any = 1, positions: Any = None) -> None:
         """Reserve blocks for ``counts`` new tokens per row; advances ``lengths`` in place."""
         import hip_ops
 
+        self._last = "paged_kv_reserve"
         hip_ops.paged_kv_reserve(block_tables, lengths, self.free_list, self.free_state, self.status, block_size, counts=counts, positions=positions)
+
+    def plan(self, block_tables: Any, lengths: Any, block_size: int, *, counts: Any = 1, max_tokens: int, per_row: int = 0) -> Any:
+        """:meth:`reserve` together with the step's slot map (``hip_ops.paged_kv_plan``): a ``PagedPlan``."""
+        import hip_ops
+
+        self._last = "paged_kv_plan"
+        return hip_ops.paged_kv_plan(block_tables, lengths, counts, self.free_list, self.free_state, self.status, block_size, max_tokens=max_tokens, per_row=per_row)
 
     def check(self) -> None:
         """Raise ``RuntimeError`` if the last reservation failed (reads the status: a sync)."""
         code = int(self.status.item())
         if code != 0:
-            raise RuntimeError(f"paged_kv_reserve failed: {self._STATUS.get(code, f'status {code}')}")
+            raise RuntimeError(f"{self._last} failed: {self._STATUS.get(code, f'status {code}')}")
 
     def free_blocks(self) -> list[int]:
         head, count = (int(v) for v in self.free_state.tolist())
@@ -324,6 +397,51 @@ class DeviceBatchPageTables:
         self.step_counts[row] = 1
         return row
 
+    def plan_step(self) -> Any:
+        """:meth:`reserve_step` with the slot map of the step's tokens, for the layers that write by slot (4-bit pools,
+        rotary positions of several axes): a ``hip_ops.PagedPlan`` whose ``positions`` and ``slots`` have one entry for
+        every row (-1 where it holds no request).  Leaves the append positions in ``positions`` and is device only, like
+        ``reserve_step``."""
+        plan = self.allocator.plan(self.block_tables, self.sequence_lengths, self.block_size, counts=self.step_counts, max_tokens=self.rows, per_row=1)
+        self.positions.copy_(plan.starts)
+        return plan
+
+    def plan_prefill(self, rows: Sequence[int], counts: Sequence[int]) -> "PrefillStep":
+        """:meth:`reserve_prefill` with the slot map, for the layers that write by slot.  The step's tokens are packed in
+        row order, so ``rows`` must be ascending.  ``cu_seqlens``, ``starts`` and ``block_tables`` of the record have an
+        entry for every row of the tables, the ones not in the step without tokens; ``block_tables`` is the running
+        batch's own, so the step's layers run before the next reservation."""
+        import torch
+
+        rows, counts = self._step_rows(rows, counts, "plan_prefill")
+        if rows != sorted(rows):
+            raise ValueError("plan_prefill rows must be ascending: the step is packed in row order")
+        full = [0] * self.rows
+        for r, c in zip(rows, counts):
+            full[r] = c
+        device = self.block_tables.device
+        plan = self.allocator.plan(self.block_tables, self.sequence_lengths, self.block_size, counts=torch.tensor(full, dtype=torch.int32, device=device), max_tokens=sum(counts))
+        self.allocator.check()
+        return PrefillStep(
+            rows=tuple(rows), counts=tuple(counts), index=torch.tensor(rows, dtype=torch.int64, device=device),
+            cu_seqlens=plan.cu_seqlens, starts=plan.starts, block_tables=self.block_tables,
+            max_new=max(counts), total_tokens=sum(counts), block_size=self.block_size, plan=plan,
+        )
+
+    def _step_rows(self, rows: Sequence[int], counts: Sequence[int], what: str) -> tuple[list[int], list[int]]:
+        rows = [int(r) for r in rows]
+        counts = [int(c) for c in counts]
+        if not rows or len(rows) != len(counts):
+            raise ValueError(f"{what} needs one count per row")
+        if len(set(rows)) != len(rows) or min(rows) < 0 or max(rows) >= self.rows:
+            raise ValueError(f"{what} rows must be distinct table rows")
+        if min(counts) <= 0:
+            raise ValueError(f"{what} counts must be positive")
+        for r in rows:
+            if not self.active[r]:
+                raise ValueError(f"row {r} holds no request")
+        return rows, counts
+
     def reserve_prefill(self, rows: Sequence[int], counts: Sequence[int]) -> "PrefillStep":
         """Reserve blocks for a multi-token step (a prompt, or one chunk of it) of some rows.
 
@@ -335,17 +453,7 @@ class DeviceBatchPageTables:
         status back (one sync), so a failed reservation raises here rather than in a layer."""
         import torch
 
-        rows = [int(r) for r in rows]
-        counts = [int(c) for c in counts]
-        if not rows or len(rows) != len(counts):
-            raise ValueError("reserve_prefill needs one count per row")
-        if len(set(rows)) != len(rows) or min(rows) < 0 or max(rows) >= self.rows:
-            raise ValueError("reserve_prefill rows must be distinct table rows")
-        if min(counts) <= 0:
-            raise ValueError("reserve_prefill counts must be positive")
-        for r in rows:
-            if not self.active[r]:
-                raise ValueError(f"row {r} holds no request")
+        rows, counts = self._step_rows(rows, counts, "reserve_prefill")
         device = self.block_tables.device
         index = torch.tensor(rows, dtype=torch.int64, device=device)
         full = torch.zeros_like(self.step_counts)
@@ -384,7 +492,7 @@ class DeviceBatchPageTables:
         self.allocator.reserve(self.block_tables, self.sequence_lengths, self.block_size, counts=self.step_counts, positions=self.positions)
 
     def append(self, key: Any, value: Any, key_blocks: Any, value_blocks: Any, *, counts: Any = None) -> None:
-        """Write a layer's new K/V ``(rows, H_kv, S, D)`` at the reserved positions of its pool."""
+        """Write a layer's new K/V ``(rows, H_kv, S, D)`` at the reserved positions of its (bf16 or fp32) pool."""
         import hip_ops
 
         hip_ops.paged_kv_append(key, value, key_blocks, value_blocks, self.block_tables, self.positions, self.block_size,
@@ -412,7 +520,8 @@ class PrefillStep:
     """The reservation of one multi-token step (``DeviceBatchPageTables.reserve_prefill``):
     rows in packing order, their new token counts, ``cu_seqlens`` ``(n + 1,)`` and the first
     new position ``starts`` ``(n,)`` of each row (its length before the step), and the rows'
-    block tables ``(n, max_blocks)`` after the reservation, all int32 on the device."""
+    block tables ``(n, max_blocks)`` after the reservation, all int32 on the device.  ``plan`` is
+    the step's ``hip_ops.PagedPlan`` where ``plan_prefill`` made the record."""
 
     rows: tuple[int, ...]
     counts: tuple[int, ...]
@@ -423,6 +532,7 @@ class PrefillStep:
     max_new: int
     total_tokens: int
     block_size: int
+    plan: Any = None
 
 
 # --------------------------------------------------------------------------- records
@@ -520,7 +630,9 @@ class FullAttentionCache:
     ``append`` / ``append_blocks`` take post-rotary K/V ``(1 or batch, heads,
     seq, head_dim)``; ``block_table`` maps logical blocks to physical ones.
     With ``shared_pool`` set, ``heads`` is the KV head count of the shared
-    GQA-native pool and the cache's batch dimension must be 1.
+    GQA-native pool and the cache's batch dimension must be 1.  On a
+    ``SharedKV4BlockPool`` (GPU tensors only) ``append_blocks`` quantises and
+    ``as_tensors`` gives the values the cache holds, in bf16.
     """
 
     capacity_hint: int | None = None
@@ -576,6 +688,8 @@ class FullAttentionCache:
     def append_blocks(self, key: Any, value: Any) -> None:
         """Write new K/V into slots ``(table[pos // bs], pos % bs)`` (``src/decode_state.py:271-293``)."""
         seq = int(key.shape[2])
+        if is_kv4(self.pool.key_blocks) and not _on_gpu(key):
+            raise RuntimeError("a 4-bit pool is written from GPU tensors only")
         self.append_calls += 1
         self.appended_tokens += seq
         target = self.valid + seq
@@ -615,6 +729,11 @@ class FullAttentionCache:
         if self.shared_pool is not None:
             if key.shape[0] != 1:
                 raise ValueError("caches on a shared pool hold one request (batch 1)")
+            if is_kv4(self.pool.key_blocks):
+                at = torch.arange(self.valid, self.valid + int(key.shape[2]), device=key.device)
+                slots = table.long()[at // self.block_size] * self.block_size + at % self.block_size
+                hip_ops.paged_kv4_append(key[0].transpose(0, 1), value[0].transpose(0, 1), self.pool.key_blocks, self.pool.value_blocks, slots, self.block_size)
+                return
             hip_ops.paged_kv_append(key, value, self.pool.key_blocks, self.pool.value_blocks, table, self.valid, self.block_size)
             return
         # reference-layout pool (batch, heads, P, bs, D): every batch row shares the table
@@ -733,10 +852,12 @@ class FullAttentionCache:
         import torch
 
         keys, values = self.pool.key_blocks, self.pool.value_blocks
-        if _on_gpu(keys):
+        if _on_gpu(keys) or is_kv4(keys):
             import hip_ops
 
             table = torch.tensor(self.block_table, dtype=torch.int32, device=keys.device)
+            if is_kv4(keys):
+                return hip_ops.paged_kv4_gather(keys, values, table, self.valid, self.block_size)
             if self.shared_pool is not None:
                 return hip_ops.paged_kv_gather(keys, values, table, self.valid, self.block_size)
             return hip_ops.paged_kv_gather(keys, values, table, self.valid, self.block_size)

@@ -154,7 +154,7 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
     "qa_paged_kv_plan": (
         c_int32,
         [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int32, c_int64, c_int64, c_int32, c_void_p, c_int64, c_void_p, c_void_p, c_int64,
-         c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p],
+         c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p],
     ),
     "qa_paged_kv4_append": (
         c_int32,

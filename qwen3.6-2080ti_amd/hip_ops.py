@@ -1179,6 +1179,7 @@ def paged_kv_plan(
     block_size: int,
     *,
     max_tokens: int,
+    per_row: int = 0,
 ) -> PagedPlan:
     """Block tables and slot map of a batched step, built on the device from the requests' lengths.
 
@@ -1191,6 +1192,10 @@ def paged_kv_plan(
     short), 3 (corrupt free state), 4 (negative or overflowing length or count), 5 (more than ``max_tokens``
     tokens): then nothing is taken and the plan is empty, so that the operators fed by it do nothing.  Nothing is
     read back, so the call can be captured in a HIP graph.
+
+    With ``per_row`` the token arrays are not packed but hold ``per_row`` entries for each row (``max_tokens`` is
+    ``B * per_row``), a row's tokens first and -1 behind them: the form of a decode step, whose operators take one
+    token of every row whether it holds a request or not.
     """
     lib = L.load_library()
     device = block_tables.device
@@ -1205,7 +1210,9 @@ def paged_kv_plan(
     _require(free_state.dtype is i32 and free_state.numel() == 2 and free_state.is_contiguous(), "free_state must be int32 [head, count]")
     _require(status.dtype is i32 and status.numel() >= 1, "status must be an int32 tensor")
     max_tokens = int(max_tokens)
+    per_row = int(per_row)
     _require(max_tokens >= 0, "max_tokens must be non-negative")
+    _require(per_row == 0 or per_row * batch == max_tokens, "with per_row entries a row max_tokens must be batch * per_row")
     count_ptr, count_code, count_scalar = 0, L.QA_I32, 0
     if isinstance(counts, torch.Tensor):
         if counts.device != device:
@@ -1222,7 +1229,7 @@ def paged_kv_plan(
     at = ints.data_ptr()
     code = _launch(
         device, lib.qa_paged_kv_plan, block_tables.data_ptr(), block_tables.stride(0), max_blocks, lengths.data_ptr(), count_ptr, count_code, count_scalar, batch,
-        int(block_size), free_list.data_ptr(), free_list.numel(), free_state.data_ptr(), status.data_ptr(), max_tokens, at, at + 4 * (batch + 1), at + 4 * (3 * batch + 1),
+        int(block_size), free_list.data_ptr(), free_list.numel(), free_state.data_ptr(), status.data_ptr(), max_tokens, per_row, at, at + 4 * (batch + 1), at + 4 * (3 * batch + 1),
         slots.data_ptr(), at + 4 * (2 * batch + 1), 4 * batch,
     )
     L.check(lib, code, "paged_kv_plan")
@@ -1417,9 +1424,11 @@ def _mrope_tables(sections: tuple[int, ...], interleaved: bool, rope_theta: floa
     key = (sections, interleaved, rope_theta, device)
     cached = _MROPE.get(key)
     if cached is None:
+        # made by a copy from the host that waits: not while a graph records
+        _require(not torch.cuda.is_current_stream_capturing(), "the first prologue with these sections and rope_theta must run outside a graph capture")
+        _require(rope_theta >= 1.0, "rope_theta must be at least 1")
         axes = mrope_axes(sections, interleaved)
         turns = [round(math.ldexp(rope_theta ** (-j / len(axes)) / (2 * math.pi), 64)) for j in range(len(axes))]
-        _require(rope_theta >= 1.0, "rope_theta must be at least 1")
         cached = (torch.tensor(turns, dtype=torch.int64, device=device), torch.tensor(axes, dtype=torch.uint8, device=device))
         _MROPE[key] = cached
     return cached

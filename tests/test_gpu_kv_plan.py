@@ -130,3 +130,27 @@ def test_captured_plan_replays_step_after_step() -> None:
         assert tables.tolist() == want[0] and lengths.tolist() == want[1] and state.tolist() == want[2:]
         assert [x.tolist() for x in plan] == [cu, starts, positions, slots]
         (torch.ones(64, device=DEV) * 2).sum().item()
+
+
+@pytest.mark.parametrize("batch,per_row,block", [(1, 1, 16), (128, 1, 16), (9, 4, 16), (1030, 5, 32), (5000, 1, 16), (70, 100, 16)])
+def test_entries_for_every_row(batch, per_row, block) -> None:
+    """Rows without a new token keep their entries, at -1; the rest of the plan is the packed one's."""
+    lengths, counts, tables, free, head, count = _case(batch + per_row, batch, per_row, 60, block)
+    code, *want = kv4.plan(tables, lengths, counts, free, head, count, block, sum(counts), len(free))
+    dev = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    t, n, state, status = dev(tables), dev(lengths), dev([head, count]), dev([99])
+    plan = hip_ops.paged_kv_plan(t, n, dev(counts), dev(free), state, status, block, max_tokens=batch * per_row, per_row=per_row)
+    assert int(status) == code == 0
+    assert [t.tolist(), n.tolist(), *state.tolist(), plan.cu_seqlens.tolist(), plan.starts.tolist()] == want[:6]
+    cu = want[4]
+    for got, packed in ((plan.positions, want[6]), (plan.slots, want[7])):
+        assert got.tolist() == [packed[cu[b] + x] if x < counts[b] else -1 for b in range(batch) for x in range(per_row)]
+
+
+def test_a_row_with_more_tokens_than_entries_takes_nothing() -> None:
+    dev = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    t, n, state, status = dev([[-1], [3]]), dev([0, 5]), dev([0, 2]), dev([0])
+    plan = hip_ops.paged_kv_plan(t, n, dev([0, 3]), dev([1, 2]), state, status, 16, max_tokens=4, per_row=2)
+    assert int(status) == 5 and n.tolist() == [0, 5] and state.tolist() == [0, 2] and plan.slots.tolist() == [-1] * 4 and plan.cu_seqlens.tolist() == [0, 0, 0]
+    with pytest.raises(RuntimeError, match="batch"):
+        hip_ops.paged_kv_plan(t, n, 1, dev([1, 2]), state, status, 16, max_tokens=4, per_row=3)

@@ -115,13 +115,14 @@ def test_prefill_refuses(changes, message) -> None:
 @pytest.mark.parametrize("changes,message", [
     (dict(batch=0), "batch"), (dict(tables=P(0)), "non-null"), (dict(counts_dtype=L.QA_F32, counts=SOME), "counts"), (dict(scalar=-1), "non-negative"), (dict(block=0), "block_size"),
     (dict(stride=3), "overlap"), (dict(capacity=0), "capacity"), (dict(max_tokens=-1), "max_tokens"), (dict(positions=P(0)), "non-null"), (dict(wsb=4), "workspace too small"),
+    (dict(per_row=-1), "entries a row"), (dict(per_row=3), "max_tokens must be 6"),
 ])
 def test_plan_refuses(changes, message) -> None:
     lib = _lib()
-    a = dict(tables=SOME, stride=4, width=4, counts=P(0), counts_dtype=L.QA_I32, scalar=1, batch=2, block=16, capacity=8, max_tokens=4, positions=SOME, wsb=8)
+    a = dict(tables=SOME, stride=4, width=4, counts=P(0), counts_dtype=L.QA_I32, scalar=1, batch=2, block=16, capacity=8, max_tokens=4, positions=SOME, wsb=8, per_row=0)
     a.update(changes)
     assert lib.qa_paged_kv_plan(a["tables"], a["stride"], a["width"], SOME, a["counts"], a["counts_dtype"], a["scalar"], a["batch"], a["block"], SOME, a["capacity"], SOME, SOME,
-                                a["max_tokens"], SOME, SOME, a["positions"], SOME, SOME, a["wsb"], P(0)) == 1
+                                a["max_tokens"], a["per_row"], SOME, SOME, a["positions"], SOME, SOME, a["wsb"], P(0)) == 1
     assert message in L.last_error(lib)
 
 
