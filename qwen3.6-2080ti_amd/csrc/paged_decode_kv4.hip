@@ -5,7 +5,8 @@
 // [T w / W, T (w + 1) / W): equal shares whatever the lengths.  The workgroup's eight waves take its units in turn, so
 // that neighbouring waves read neighbouring tiles, each with an online softmax of its own and no barrier; where the
 // range leaves a row group they merge in LDS and write one partial (m, l, o) of the G heads.  A workgroup that had the
-// whole row group writes the result; the other groups' partials are merged by combine_kernel.
+// whole row group writes the result; the other groups' partials are merged by combine_kernel.  Where all rows are short a
+// workgroup takes a row group as it is.
 //
 // A wave keeps two units of keys and values in flight in registers (buffer loads of zero records for what is skipped, so
 // every step issues the same loads and the wait counts are fixed), across row groups: the merge of one and the query of
@@ -24,6 +25,7 @@ namespace attn4 {
 struct DecodeParams {
   Params c;
   int n_wgs;
+  int short_rows;     // the tables hold no row that is split: no partials, no workspace
   float* part_o;      // (n_wgs + B Hkv, G, D)
   float* part_ml;     // (n_wgs + B Hkv, G, 2)
   int32_t* rg_wgs;    // (B Hkv, 2): first and last workgroup of a row group; -1: the result is written
@@ -31,6 +33,10 @@ struct DecodeParams {
 
 constexpr int kWaves = 8;
 constexpr int kUnit = 32;  // tokens
+// Where no row is longer than this, a workgroup takes a row group and nothing is merged; where the tables cannot hold a
+// longer one, the second launch is left out.  us split / by row, 2 KV heads of 256: 4 rows of 512 12.1 / 9.1, of 1024 12.4 /
+// 13.3, of 2048 12.2 / 19.4; 64 rows of up to 1024 25.5 / 14.1, of up to 4096 34.5 / 36.3; 200 rows of 500 37.7 / 22.0.
+constexpr int kByRowTokens = 1024;
 constexpr int kMaxWgs = 256;  // one per CU: eight waves of up to 256 registers fill it
 
 // Tokens and units of row b (0 for rows of length <= 0); lengths past the table stop at it.
@@ -107,29 +113,56 @@ __global__ __launch_bounds__(64 * kWaves, 2) void decode_kernel(DecodeParams dp)
   const int col = lane & 15;
   const int quad = lane >> 4;
 
-  // ---- this workgroup's share
-  // rows of up to 64 are loaded and summed once, for the total and for the search below
-  const int64_t len_first = lane < p.B ? row_tokens(p, lane) : 0;
-  const int incl_first = lane_scan(units_of(len_first) * p.Hkv);
-  int T = __builtin_amdgcn_readlane(incl_first, 63);
-  for (int b0 = 64; b0 < p.B; b0 += 64) T += __builtin_amdgcn_readlane(lane_scan((b0 + lane < p.B ? units_of(row_tokens(p, b0 + lane)) : 0) * p.Hkv), 63);
-  // a workgroup has a unit for each wave before another one starts
-  const int W = min(dp.n_wgs, (T + kWaves - 1) / kWaves);
+  // ---- this workgroup's share: units lo .. hi - 1
   const int wg = blockIdx.x;
-  if (wg >= W) return;
-  const int lo = static_cast<int>(static_cast<int64_t>(T) * wg / W);
-  const int hi = static_cast<int>(static_cast<int64_t>(T) * (wg + 1) / W);
+  Cursor cur{0, 0, 0, 0};
+  int lo = 0, hi;
+  // rows of up to 64 are loaded and summed once, for the total and for the search below
+  int64_t len_first = lane < p.B ? row_tokens(p, lane) : 0;
+  const int nu_first = units_of(len_first);
+  const int incl_first = lane_scan(nu_first * p.Hkv);
+  int T = __builtin_amdgcn_readlane(incl_first, 63);
+  uint32_t longest = wave_max_bits(nu_first);
+  for (int b0 = 64; b0 < p.B; b0 += 64) {
+    const int nu = b0 + lane < p.B ? units_of(row_tokens(p, b0 + lane)) : 0;
+    T += __builtin_amdgcn_readlane(lane_scan(nu * p.Hkv), 63);
+    longest = max(longest, wave_max_bits(nu));
+  }
+  const bool by_row = longest <= kByRowTokens / kUnit;
+  if (by_row) {
+    cur.b = wg / p.Hkv;
+    cur.g = wg - cur.b * p.Hkv;
+    if (cur.b >= p.B) return;
+    len_first = row_tokens(p, cur.b);
+    cur.nu = __builtin_amdgcn_readfirstlane(units_of(len_first));
+    hi = cur.nu;
+    if (hi == 0) {
+      for (int e = 4 * tid; e < p.G * D; e += 4 * 64 * kWaves) *reinterpret_cast<uint2*>(p.out + (static_cast<int64_t>(cur.b) * p.H + cur.g * p.G) * D + e) = make_uint2(0, 0);
+      return;
+    }
+  } else {
+    // a workgroup has a unit for each wave before another one starts
+    const int W = min(dp.n_wgs, (T + kWaves - 1) / kWaves);
+    if (wg >= W) return;
+    lo = static_cast<int>(static_cast<int64_t>(T) * wg / W);
+    hi = static_cast<int>(static_cast<int64_t>(T) * (wg + 1) / W);
+  }
 
   // ---- where the wave's units lie: lane j holds unit 64 c + j, that is unit lo + wave + kWaves (64 c + j) of all
   int64_t at0, at1;  // offsets of its two runs in the pools, -1: not there
   int left;          // its tokens
-  Cursor cur{0, 0, 0, 0};
   auto locate = [&](int c, bool begin) {
     const int gu = lo + wave + kWaves * (64 * c + lane);
     int row = -1, g = 0, u = 0;
     int64_t tokens = 0;
     int base = 0;
-    for (int b0 = 0; b0 < p.B; b0 += 64) {
+    if (by_row) {
+      row = cur.b;
+      g = cur.g;
+      u = gu;
+      tokens = len_first;
+    }
+    for (int b0 = 0; b0 < p.B && !by_row; b0 += 64) {
       const int64_t len = b0 == 0 ? len_first : b0 + lane < p.B ? row_tokens(p, b0 + lane) : 0;
       const int nu = units_of(len);
       const int incl = b0 == 0 ? incl_first : lane_scan(nu * p.Hkv);
@@ -291,8 +324,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void decode_kernel(DecodeParams dp)
     read_query(qa_, col);
     if constexpr (WIDE) read_query(qb_, 16 + col);
     Cursor nxt = cur;
-    next_row_group(p, nxt);
-    if (seg_end < hi) fetch_query(nxt);
+    if (seg_end < hi) {
+      next_row_group(p, nxt);
+      fetch_query(nxt);
+    }
 
     float m_run = -INFINITY, l_run = 0.f;
     floatx4_v o[MT];
@@ -424,7 +459,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void decode_kernel(DecodeParams dp)
         if (d == 0) *reinterpret_cast<float2*>(dp.part_ml + (slot * p.G + h) * 2) = make_float2(s_total[h], l);
       }
     }
-    if (tid == 0) {
+    if (tid == 0 && !dp.short_rows) {
       if (at == cur.cum) dp.rg_wgs[2 * rg] = whole ? -1 : wg;
       if (seg_end == cur.cum + cur.nu) dp.rg_wgs[2 * rg + 1] = wg;
     }
@@ -433,87 +468,89 @@ __global__ __launch_bounds__(64 * kWaves, 2) void decode_kernel(DecodeParams dp)
   }
 }
 
-// Merges the partials of one (row, head): slots first + rg .. last + rg.  A workgroup of THREADS, each thread a dim of
-// every (THREADS / D)-th partial with up to kRowsInFlight loads in flight.
-constexpr int kRowsInFlight = 16;
+// Merges the partials of one (row, head): slots first + rg .. last + rg.  A thread has four of a workgroup's CHUNK dims of
+// every SHARE-th partial, kPartsInFlight of them on their way at once.
+constexpr int kPartsInFlight = 8;
+constexpr int kCombineThreads = kMaxWgs;  // a thread for each partial's m and l
 
-template <int D, int THREADS>
-__global__ __launch_bounds__(THREADS) void combine_kernel(DecodeParams dp) {
+template <int D, int CHUNK>
+__global__ __launch_bounds__(kCombineThreads) void combine_kernel(DecodeParams dp) {
   const Params& p = dp.c;
-  constexpr int SHARE = THREADS / D;
+  constexpr int ACROSS = CHUNK / 4;
+  constexpr int SHARE = kCombineThreads / ACROSS;
   __shared__ float s_f[kMaxWgs];
-  __shared__ float s_red[2][THREADS / 64];
-  __shared__ float s_o[SHARE][D];
+  __shared__ float s_red[2][kCombineThreads / 64];
+  __shared__ __align__(16) float s_o[SHARE][CHUNK];
   const int tid = threadIdx.x;
   const int64_t bh = blockIdx.x;
-  const int b = static_cast<int>(bh / p.H);
-  const int h = static_cast<int>(bh - static_cast<int64_t>(b) * p.H);
-  const int g = h / p.G;
+  const int b = static_cast<int>(static_cast<uint32_t>(bh) / static_cast<uint32_t>(p.H));
+  const int h = static_cast<int>(bh) - b * p.H;
+  const int g = static_cast<int>(over_group(p, h));
   const int hh = h - g * p.G;
   const int64_t rg = static_cast<int64_t>(b) * p.Hkv + g;
   const int first = dp.rg_wgs[2 * rg], last = dp.rg_wgs[2 * rg + 1];
-  bf16_t* out = p.out + bh * D;
+  const int d0 = static_cast<int>(blockIdx.y) * CHUNK;
+  bf16_t* out = p.out + bh * D + d0;
   if (row_tokens(p, b) == 0) {  // its record was never written
-    if (tid < D) out[tid] = 0;
+    if (tid < CHUNK) out[tid] = 0;
     return;
   }
   if (first < 0) return;
   const int n = last - first + 1;
   const int64_t row0 = (first + rg) * p.G + hh;
-  const int d = tid % D, share = tid / D;
-  const float* po = dp.part_o + row0 * D + d;
+  const int share = tid / ACROSS, d = 4 * (tid % ACROSS);
+  const float* po = dp.part_o + row0 * D + d0 + d;
   const int64_t so = static_cast<int64_t>(p.G) * D;
-  float pre[kRowsInFlight];
+  floatx4_v part[kPartsInFlight];
+  auto ask = [&](int s0) {
 #pragma unroll
-  for (int i = 0; i < kRowsInFlight; ++i) pre[i] = share + i * SHARE < n ? po[(share + i * SHARE) * so] : 0.f;
+    for (int i = 0; i < kPartsInFlight; ++i) part[i] = *reinterpret_cast<const floatx4_v*>(po + min(s0 + i * SHARE, n - 1) * so);  // past the end: the last one again
+  };
+  ask(share);
   float2 ml = make_float2(-INFINITY, 0.f);
   if (tid < n) ml = *reinterpret_cast<const float2*>(dp.part_ml + (row0 + static_cast<int64_t>(tid) * p.G) * 2);
+  float gate = 0.f;
+  if (p.gate != nullptr && tid < CHUNK) gate = bf16_to_f32(p.gate[b * p.gate_st + h * p.gate_sh + d0 + tid]);
   const float wm = wave_max(ml.x);
   if ((tid & 63) == 0) s_red[0][tid >> 6] = wm;
   __syncthreads();
   float m = s_red[0][0];
 #pragma unroll
-  for (int w = 1; w < THREADS / 64; ++w) m = fmaxf(m, s_red[0][w]);
+  for (int w = 1; w < kCombineThreads / 64; ++w) m = fmaxf(m, s_red[0][w]);
   const float use = m == -INFINITY ? 0.f : m;
   const float f = tid < n ? __builtin_amdgcn_exp2f(ml.x - use) : 0.f;
-  if (tid < n) s_f[tid] = f;
+  s_f[tid] = f;
   const float wl = wave_sum(tid < n ? f * ml.y : 0.f);
   if ((tid & 63) == 0) s_red[1][tid >> 6] = wl;
   __syncthreads();
-  float acc = 0.f;
+  floatx4_v acc = {0.f, 0.f, 0.f, 0.f};
+  for (int s0 = share; s0 < n; s0 += kPartsInFlight * SHARE) {
+    if (s0 != share) ask(s0);
 #pragma unroll
-  for (int i = 0; i < kRowsInFlight; ++i)
-    if (share + i * SHARE < n) acc += s_f[share + i * SHARE] * pre[i];
-  for (int s0 = share + kRowsInFlight * SHARE; s0 < n; s0 += kRowsInFlight * SHARE) {
-    float row[kRowsInFlight];
-#pragma unroll
-    for (int i = 0; i < kRowsInFlight; ++i) row[i] = s0 + i * SHARE < n ? po[(s0 + i * SHARE) * so] : 0.f;
-#pragma unroll
-    for (int i = 0; i < kRowsInFlight; ++i)
-      if (s0 + i * SHARE < n) acc += s_f[s0 + i * SHARE] * row[i];
+    for (int i = 0; i < kPartsInFlight; ++i)
+      if (s0 + i * SHARE < n) acc += s_f[s0 + i * SHARE] * part[i];
   }
-  if constexpr (SHARE > 1) {
-    s_o[share][d] = acc;
-    __syncthreads();
-    if (share != 0) return;
+  *reinterpret_cast<floatx4_v*>(&s_o[share][d]) = acc;
+  __syncthreads();
+  if (tid >= CHUNK) return;
+  float sum = 0.f;
 #pragma unroll
-    for (int i = 1; i < SHARE; ++i) acc += s_o[i][d];
-  }
+  for (int i = 0; i < SHARE; ++i) sum += s_o[i][tid];
   float l = 0.f;
 #pragma unroll
-  for (int w = 0; w < THREADS / 64; ++w) l += s_red[1][w];
-  float r = normalised(acc, l);
-  if (p.gate != nullptr) r *= sigmoid(bf16_to_f32(p.gate[b * p.gate_st + h * p.gate_sh + d]));
-  out[d] = f32_to_bf16(r);
+  for (int w = 0; w < kCombineThreads / 64; ++w) l += s_red[1][w];
+  float r = normalised(sum, l);
+  if (p.gate != nullptr) r *= sigmoid(gate);
+  out[tid] = f32_to_bf16(r);
 }
 
-// Workgroups of a launch: as many as there could be units for, up to one a CU.
 static int64_t decode_wgs(int64_t row_groups, int64_t max_tokens) {
   return std::min<int64_t>(kMaxWgs, std::max<int64_t>(1, ceil_div(row_groups * ceil_div(std::max<int64_t>(max_tokens, 1), kUnit), kWaves)));
 }
 
 static int64_t workspace_bytes_of(int64_t batch, int heads, int kv_heads, int head_dim, int64_t max_tokens) {
   const int64_t groups = batch * kv_heads;
+  if (max_tokens <= kByRowTokens) return 0;
   return (decode_wgs(groups, max_tokens) + groups) * (heads / kv_heads) * (head_dim + 2) * 4 + groups * 8;
 }
 
@@ -523,18 +560,20 @@ static int launch(const DecodeParams& p, hipStream_t stream) {
   if (int rc = reserve_lds<&decode_kernel<D, WIDE>>("paged_attention_decode_kv4", S::kBytes)) return rc;
   {
     KernelTimer timer_("decode_kv4", stream);
-    hipLaunchKernelGGL((decode_kernel<D, WIDE>), dim3(p.n_wgs), dim3(64 * kWaves), S::kBytes, stream, p);
+    hipLaunchKernelGGL((decode_kernel<D, WIDE>), dim3(static_cast<unsigned>(std::max<int64_t>(p.n_wgs, static_cast<int64_t>(p.c.B) * p.c.Hkv))), dim3(64 * kWaves), S::kBytes, stream, p);
   }
   if (int rc = check_launch("paged_attention_decode_kv4")) return rc;
-  const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(p.c.B) * p.c.H));
-  // many partials a row group: 1024 threads share them, so that fewer rounds of loads follow one another
+  if (p.short_rows) return 0;
+  const unsigned rows = static_cast<unsigned>(static_cast<int64_t>(p.c.B) * p.c.H);
+  // many partials a row group: more workgroups share its dims.  us of the whole call, not shared / shared: 1 row of 20000 16.9 /
+  // 14.9, of 200000 30.8 / 28.0; 8 rows of 30000 31.4 / 32.0, 64 of up to 1024 25.5 / 34.3
   const bool many = p.n_wgs > 16 * static_cast<int64_t>(p.c.B) * p.c.Hkv;
   {
     KernelTimer timer_("decode_kv4_combine", stream);
     if (many)
-      hipLaunchKernelGGL((combine_kernel<D, 1024>), grid, dim3(1024), 0, stream, p);
+      hipLaunchKernelGGL((combine_kernel<D, 32>), dim3(rows, D / 32), dim3(kCombineThreads), 0, stream, p);
     else
-      hipLaunchKernelGGL((combine_kernel<D, 256>), grid, dim3(256), 0, stream, p);
+      hipLaunchKernelGGL((combine_kernel<D, D>), dim3(rows), dim3(kCombineThreads), 0, stream, p);
   }
   return check_launch("paged_attention_decode_kv4");
 }
@@ -567,8 +606,9 @@ extern "C" int qa_paged_attention_decode_kv4(const void* query, int32_t q_dtype,
   QA_REQUIRE(groups * ceil_div(max_tokens, kUnit) <= 0x7fffffff, "%s: the tables cover too many tokens: %lld row groups of up to %lld", a.what, static_cast<long long>(groups),
              static_cast<long long>(max_tokens));
   const int64_t need = workspace_bytes_of(batch, heads, kv->kv_heads, head_dim, max_tokens);
-  QA_REQUIRE(workspace != nullptr && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 15u) == 0,
+  QA_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 15u) == 0),
              "paged decode workspace too small or not 16-byte aligned: need %lld bytes, have %lld", static_cast<long long>(need), static_cast<long long>(workspace_bytes));
+  p.short_rows = max_tokens <= kByRowTokens;
   p.n_wgs = static_cast<int>(decode_wgs(groups, max_tokens));
   const int64_t rows = (p.n_wgs + groups) * p.c.G;
   p.part_o = reinterpret_cast<float*>(workspace);

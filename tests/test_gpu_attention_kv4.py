@@ -351,3 +351,19 @@ def test_captured_prefill_replays_as_eager_runs() -> None:
 @pytest.mark.parametrize("new,prefix,heads,kv_heads,dim", [([7], [9000], 16, 2, 256), ([40, 3], [3000, 20_000], 8, 2, 128), ([1, 0, 5], [0, 50, 12_000], 16, 1, 256)])
 def test_prefill_of_few_tokens_splits_the_keys(new, prefix, heads, kv_heads, dim) -> None:
     _check_prefill(sum(new) + dim, new, prefix, heads, kv_heads, dim, 32, gated=True, holes=dim == 128)
+
+
+@pytest.mark.parametrize("longest", [1024, 1025, 700])
+@pytest.mark.parametrize("rows,heads,kv_heads,dim", [(4, 16, 2, 256), (70, 12, 4, 128), (5, 16, 1, 256)])
+@pytest.mark.parametrize("width", [None, 300])
+def test_decode_of_short_rows(longest, rows, heads, kv_heads, dim, width) -> None:
+    """A workgroup a row group where no row is longer than 1024 tokens, with tables that could hold longer ones and without."""
+    rng = random.Random(rows + longest)
+    lens = [longest, 0, 1, 33] + [rng.choice((0, 17, rng.randint(1, 300))) for _ in range(rows - 4)]
+    _check_decode(21, lens, heads, kv_heads, dim, 16, gated=rows == 4, width=width, holes=rows == 70)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", GROUPS)
+def test_decode_of_every_group_size_beside_long_rows(heads, kv_heads, dim) -> None:
+    _check_decode(22, [1, 15, 0, 2000, 31, 32, -3, 33, 1100, 16], heads, kv_heads, dim, 16, gated=True)
+    _check_decode(23, [3] * 63 + [0, 1500] + [7] * 70, heads, kv_heads, dim, 16)
