@@ -53,7 +53,6 @@ struct Params {
   float scale;
 };
 
-// Index arrays that no kernel here writes, read through the constant address space: uniform reads are scalar loads.
 // Entry i of an int32 or int64 array.  Without a branch, so that several are on their way at once.
 __device__ __forceinline__ int64_t read_index(const void* base, int is64, int64_t i) {
   const int32_t* at = reinterpret_cast<const int32_t*>(base) + (i << is64);
@@ -285,7 +284,7 @@ inline int reserve_lds(const char* what, int bytes) {
   if (device < 64 && (done.load(std::memory_order_relaxed) & bit)) return 0;
   err = hipFuncSetAttribute(reinterpret_cast<const void*>(KERNEL), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (err != hipSuccess) return fail("%s: cannot reserve %d bytes of LDS: %s", what, bytes, hipGetErrorString(err));
-  done.fetch_or(bit, std::memory_order_relaxed);
+  if (device < 64) done.fetch_or(bit, std::memory_order_relaxed);
   return 0;
 }
 

@@ -37,6 +37,8 @@ constexpr int kUnit = 32;  // tokens
 // longer one, the second launch is left out.  us split / by row, 2 KV heads of 256: 4 rows of 512 12.1 / 9.1, of 1024 12.4 /
 // 13.3, of 2048 12.2 / 19.4; 64 rows of up to 1024 25.5 / 14.1, of up to 4096 34.5 / 36.3; 200 rows of 500 37.7 / 22.0.
 constexpr int kByRowTokens = 1024;
+// Row groups up to which a call of long tables has the workgroups for that; each of them reads all the lengths first.
+constexpr int kByRowGroups = 4096;
 constexpr int kMaxWgs = 256;  // one per CU: eight waves of up to 256 registers fill it
 
 // Tokens and units of row b (0 for rows of length <= 0); lengths past the table stop at it.
@@ -117,18 +119,24 @@ __global__ __launch_bounds__(64 * kWaves, 2) void decode_kernel(DecodeParams dp)
   const int wg = blockIdx.x;
   Cursor cur{0, 0, 0, 0};
   int lo = 0, hi;
-  // rows of up to 64 are loaded and summed once, for the total and for the search below
-  int64_t len_first = lane < p.B ? row_tokens(p, lane) : 0;
-  const int nu_first = units_of(len_first);
-  const int incl_first = lane_scan(nu_first * p.Hkv);
-  int T = __builtin_amdgcn_readlane(incl_first, 63);
-  uint32_t longest = wave_max_bits(nu_first);
-  for (int b0 = 64; b0 < p.B; b0 += 64) {
-    const int nu = b0 + lane < p.B ? units_of(row_tokens(p, b0 + lane)) : 0;
-    T += __builtin_amdgcn_readlane(lane_scan(nu * p.Hkv), 63);
-    longest = max(longest, wave_max_bits(nu));
+  int64_t len_first = 0;  // rows of up to 64 are loaded and summed once, for the total and for the search below
+  int incl_first = 0, T = 0;
+  bool by_row = dp.short_rows != 0;
+  if (!by_row) {
+    uint32_t longest = 0;
+    for (int b0 = 0; b0 < p.B; b0 += 64) {
+      const int64_t len = b0 + lane < p.B ? row_tokens(p, b0 + lane) : 0;
+      const int nu = units_of(len);
+      const int incl = lane_scan(nu * p.Hkv);
+      T += __builtin_amdgcn_readlane(incl, 63);
+      longest = max(longest, wave_max_bits(nu));
+      if (b0 == 0) {
+        len_first = len;
+        incl_first = incl;
+      }
+    }
+    by_row = longest <= kByRowTokens / kUnit && static_cast<int64_t>(p.B) * p.Hkv <= kByRowGroups;
   }
-  const bool by_row = longest <= kByRowTokens / kUnit;
   if (by_row) {
     cur.b = wg / p.Hkv;
     cur.g = wg - cur.b * p.Hkv;
@@ -559,8 +567,10 @@ static int launch(const DecodeParams& p, hipStream_t stream) {
   using S = Smem<D, WIDE>;
   if (int rc = reserve_lds<&decode_kernel<D, WIDE>>("paged_attention_decode_kv4", S::kBytes)) return rc;
   {
+    const int64_t groups = static_cast<int64_t>(p.c.B) * p.c.Hkv;
+    const unsigned wgs = static_cast<unsigned>(p.short_rows ? groups : groups <= kByRowGroups ? std::max<int64_t>(p.n_wgs, groups) : p.n_wgs);
     KernelTimer timer_("decode_kv4", stream);
-    hipLaunchKernelGGL((decode_kernel<D, WIDE>), dim3(static_cast<unsigned>(std::max<int64_t>(p.n_wgs, static_cast<int64_t>(p.c.B) * p.c.Hkv))), dim3(64 * kWaves), S::kBytes, stream, p);
+    hipLaunchKernelGGL((decode_kernel<D, WIDE>), dim3(wgs), dim3(64 * kWaves), S::kBytes, stream, p);
   }
   if (int rc = check_launch("paged_attention_decode_kv4")) return rc;
   if (p.short_rows) return 0;

@@ -367,3 +367,11 @@ def test_decode_of_short_rows(longest, rows, heads, kv_heads, dim, width) -> Non
 def test_decode_of_every_group_size_beside_long_rows(heads, kv_heads, dim) -> None:
     _check_decode(22, [1, 15, 0, 2000, 31, 32, -3, 33, 1100, 16], heads, kv_heads, dim, 16, gated=True)
     _check_decode(23, [3] * 63 + [0, 1500] + [7] * 70, heads, kv_heads, dim, 16)
+
+
+def test_decode_of_more_row_groups_than_take_a_workgroup_each() -> None:
+    """2100 rows of two KV heads: with tables that could hold longer rows they are split over the usual workgroups."""
+    rng = random.Random(5)
+    lens = [rng.choice((0, 1, 16, 40)) for _ in range(2100)]
+    for width in (None, 70):
+        _check_decode(24, lens, 4, 2, 128, 16, width=width)
