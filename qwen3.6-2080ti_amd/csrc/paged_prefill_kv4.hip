@@ -7,7 +7,7 @@
 // feeds two products (with 16 columns and all dims a wave, LDS would be as busy as the matrix units), and the
 // accumulators of a wave stay at 64 registers, two waves to a SIMD (with 32 columns and all dims in one wave a SIMD,
 // accumulators and query took 512 registers, 300 moves a tile between the two halves of the file: 1571 us where this
-// form takes 895, 2048 tokens behind 32000).
+// form took 895, 2048 tokens behind 32000).
 //
 // Keys go from memory into LDS as they are, two tiles ahead, 1 KB a wave through its registers (with each wave loading
 // all of them the vector memory path was busy longer than the matrix units: 1328 us; copies straight to LDS each held
@@ -18,6 +18,10 @@
 // Iteration t, one barrier: scores and softmax of tile t + 1, products of tile t's values, unpacking of tile t + 1's.
 //
 // With few columns the keys are split over gridDim.z and a second launch joins the parts.
+//
+// Bound by the matrix and vector units together.  16 heads of 256 over 2: 2048 tokens behind 32000 875 us, 1270 TFLOP/s of
+// the two products (a large bf16 library product runs at 1210), eight chunks of 512 behind up to 8k 291 us, 1060; five
+// prompts of up to 700, 20 heads of 128 over 4, 32 us: a workgroup's start and end are 11 of them and its longest row 13.
 #include "attention_kv4.h"
 
 #include <algorithm>
@@ -40,7 +44,9 @@ constexpr int kTile = 64;      // keys
 constexpr int kRuns = kTile / kv4::kRun;
 constexpr int kWaves = 8;
 constexpr int kCols = kWaves * 16;
-constexpr int kRankRows = 64;  // batches up to this many rows start with the longest row
+// Batches up to this many rows start with the longest row, so that the launch ends on short ones: 60 rows of up to 300 new
+// tokens behind up to 4000 439 -> 403 us, 12 of up to 1500 behind up to 8000 738 -> 677; 64 equal rows of 16 64.5 -> 65.8.
+constexpr int kRankRows = 64;
 
 template <int D>
 struct Smem {
