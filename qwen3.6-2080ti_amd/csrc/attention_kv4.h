@@ -69,7 +69,8 @@ __device__ __forceinline__ int64_t uniform64(int64_t v) {
 // Physical block of a run of 16 tokens of row b, -1 where there is none.  Wave-uniform and without a branch (scalar
 // loads under branches are waited for at each join): a run past the row reads a clamped entry, and an entry of either
 // width is read as words.
-__device__ __forceinline__ int32_t block_of_run(const Params& p, int64_t b, int64_t run, int64_t runs) {
+template <typename P>  // Params, wherever they lie
+__device__ __forceinline__ int32_t block_of_run(const P& p, int64_t b, int64_t run, int64_t runs) {
   typedef const __attribute__((address_space(4))) int32_t c32;
   const int64_t lb = run >> (p.bs_shift - 4);
   const int64_t at = (b * p.table_stride + max64(0, min64(lb, p.max_blocks - 1))) << p.table_i64;
@@ -261,7 +262,8 @@ __device__ __forceinline__ float column_sum(float v) {
 }
 
 // x / G, by a product with its reciprocal rounded up: with 2^s >= G the error of x ceil(2^(31 + s) / G) is below 2^(31 + s) / G.
-__device__ __forceinline__ uint32_t over_group(const Params& p, uint32_t x) { return p.G == 1 ? x : __umulhi(x, p.g_mul) >> p.g_shift; }
+template <typename P>  // Params, wherever they lie
+__device__ __forceinline__ uint32_t over_group(const P& p, uint32_t x) { return p.G == 1 ? x : __umulhi(x, p.g_mul) >> p.g_shift; }
 
 // o / l: zeros where a query saw nothing; a NaN stays one.
 __device__ __forceinline__ float normalised(float o, float l) {

@@ -19,9 +19,9 @@
 //
 // With few columns the keys are split over gridDim.z and a second launch joins the parts.
 //
-// Bound by the matrix and vector units together.  16 heads of 256 over 2: 2048 tokens behind 32000 875 us, 1270 TFLOP/s of
-// the two products (a large bf16 library product runs at 1210), eight chunks of 512 behind up to 8k 291 us, 1060; five
-// prompts of up to 700, 20 heads of 128 over 4, 32 us: a workgroup's start and end are 11 of them and its longest row 13.
+// Bound by the matrix and vector units together.  16 heads of 256 over 2: 2048 tokens behind 32000 867 us, 1280 TFLOP/s of
+// the two products (a large bf16 library product runs at 1210), eight chunks of 512 behind up to 8k 283 us, 1090; five
+// prompts of up to 700, 20 heads of 128 over 4, 31 us: a workgroup's start and end are 10 of them and its longest row 13.
 #include "attention_kv4.h"
 
 #include <algorithm>
@@ -63,6 +63,15 @@ struct Smem {
 
 // The products stay where they are written: the compiler would move them to where their sums are used.
 __device__ __forceinline__ void keep(floatx4_v (&s)[kRuns]) { asm volatile("" : "+v"(s[0]), "+v"(s[1]), "+v"(s[2]), "+v"(s[3])); }
+
+// The launch's parameters, read again: what only the start, the end or every sixteenth tile needs does not stay in scalar
+// registers over the loop, which else spilled 46 of them to vector lanes and read them back each tile.
+typedef const __attribute__((address_space(4))) PrefillParams* ParamsAgain;
+__device__ __forceinline__ ParamsAgain params_again() {
+  ParamsAgain p = (ParamsAgain)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return p;
+}
 
 template <int D>
 __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams pp) {
@@ -149,13 +158,14 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams p
   int64_t cur, nxt;
   uint64_t cur_mask, nxt_mask;
   auto chunk = [&](int64_t c) -> int64_t {
+    const ParamsAgain q = params_again();
     const int64_t run = 64 * c + lane;
-    const int64_t lb = run >> (p.bs_shift - 4);
-    const int64_t at = (b * p.table_stride + min64(lb, p.max_blocks - 1)) << p.table_i64;
-    const int32_t lo = reinterpret_cast<const int32_t*>(p.tables)[at];
-    const int32_t hi = reinterpret_cast<const int32_t*>(p.tables)[at + p.table_i64];  // the entry itself where it has one word
-    const bool ok = (run < runs) & (static_cast<uint32_t>(lo) < static_cast<uint32_t>(p.num_blocks)) & ((hi == 0) | (p.table_i64 == 0));
-    const int64_t o = static_cast<int64_t>(ok ? lo : 0) * p.sP + (run & ((1 << (p.bs_shift - 4)) - 1)) * kv4::Run<D>::kBytes;
+    const int64_t lb = run >> (q->c.bs_shift - 4);
+    const int64_t at = (b * q->c.table_stride + min64(lb, q->c.max_blocks - 1)) << q->c.table_i64;
+    const int32_t lo = reinterpret_cast<const int32_t*>(q->c.tables)[at];
+    const int32_t hi = reinterpret_cast<const int32_t*>(q->c.tables)[at + q->c.table_i64];  // the entry itself where it has one word
+    const bool ok = (run < runs) & (static_cast<uint32_t>(lo) < static_cast<uint32_t>(q->c.num_blocks)) & ((hi == 0) | (q->c.table_i64 == 0));
+    const int64_t o = static_cast<int64_t>(ok ? lo : 0) * q->c.sP + (run & ((1 << (q->c.bs_shift - 4)) - 1)) * kv4::Run<D>::kBytes;
     return ok ? o : -1;
   };
   // A wave loads only run `wave % 4` of a tile: waves 0 to 3 its values and half of its keys' codes, waves 4 to 7 the
@@ -244,6 +254,30 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams p
     for (int i = 0; i < MH; ++i) o[c][i] = floatx4_v{0.f, 0.f, 0.f, 0.f};
   uint32_t nan_rows = 0;  // bit 4 c + r: column c saw a NaN group at the dims of accumulator row r
 
+  // The output leaves through LDS as whole rows (31 us against 33 for five prompts of up to 700: as pieces of 8 bytes its
+  // stores kept the address unit busy), a lane eight dims: rows of column tiles 0 2 4 6 first, then of 1 3 5 7
+  constexpr int kLanes = D / 8;  // of a row
+  constexpr int kRowsAtOnce = 64 * kWaves / kLanes;
+  constexpr int kSweeps = kCols / 2 / kRowsAtOnce;
+  const int in_row = tid % kLanes;
+  auto column_of = [&](int pass, int i) {
+    const int at = tid / kLanes + i * kRowsAtOnce;
+    return (2 * (at >> 4) + pass) * 16 + (at & 15);
+  };
+  uint4 gate[2][kSweeps];
+  auto ask_gate = [&](ParamsAgain late) {
+    if (late->c.gate == nullptr || late->splits > 1) return;
+#pragma unroll
+    for (int pass = 0; pass < 2; ++pass)
+#pragma unroll
+      for (int i = 0; i < kSweeps; ++i) {
+        const int x = min(column_of(pass, i), n_cols - 1);
+        const int64_t t = over_group(late->c, static_cast<uint32_t>(x0 + x));
+        const uint2* src = reinterpret_cast<const uint2*>(late->c.gate + (tok0 + t) * late->c.gate_st + (x0 + x - t * late->c.G + g * late->c.G) * late->c.gate_sh + 8 * in_row);
+        const uint2 lo = src[0], hi = src[1];
+        gate[pass][i] = make_uint4(lo.x, lo.y, hi.x, hi.y);
+      }
+  };
   if (kt0 < kt1) {
     if (tid < 2) s_flag[tid] = 0;
     // what the first tiles need is asked for before any of it is waited for: the query, the table, then two tiles' keys
@@ -387,6 +421,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams p
     // us against 895, 2048 tokens behind 32000.)
     auto iterate = [&](int64_t kt, auto more) {
       const int buf = static_cast<int>((kt - kt0) & 1);
+      // a wave in its value products goes ahead of its neighbour on the SIMD that is still unpacking: 867 us against 901
+      // without priorities, 878 the other way round
+      __builtin_amdgcn_s_setprio(0);
       const int flag = s_flag[buf];
       const float c0 = s_corr[(buf * kWaves + wave) * 16 + col], c1 = s_corr[(buf * kWaves + (wave ^ 1)) * 16 + col];
       if constexpr (more) {
@@ -417,6 +454,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams p
         }
       }
       if constexpr (more) reference(kt + 1, there_next, buf ^ 1);
+      __builtin_amdgcn_s_setprio(1);
       const uint2* vt = reinterpret_cast<const uint2*>(smem + buf * S::kTileBytes) + half * MH * 128 + lane;
       constexpr int kAhead = 4;
       auto vread = [&](int f) {
@@ -440,11 +478,12 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams p
       if constexpr (more) publish(buf ^ 1);
       // ---- NaN groups among keys that not every column sees
       if (flag == static_cast<int>(kt - kt0) + 1) {
+        const ParamsAgain q = params_again();
         for (int t = 0; t < kTile; ++t) {
           const int64_t key = kt * kTile + t;
           if (!(there_cur >> (t >> 4) & 1) || key >= kv_end) continue;
-          const int32_t ph = block_of_run(p, b, key >> 4, runs);
-          const uint8_t* run = vb + static_cast<int64_t>(ph) * p.sP + ((key >> 4) & ((1 << (p.bs_shift - 4)) - 1)) * kv4::Run<D>::kBytes;
+          const int32_t ph = block_of_run(q->c, b, key >> 4, runs);
+          const uint8_t* run = q->c.vpool + g * q->c.sG + static_cast<int64_t>(ph) * q->c.sP + ((key >> 4) & ((1 << (q->c.bs_shift - 4)) - 1)) * kv4::Run<D>::kBytes;
 #pragma unroll
           for (int r = 0; r < 4; ++r)
             if (run[kv4::Run<D>::value_scale(t & 15, (4 * quad + r) / (512 / D))] == 255)
@@ -459,75 +498,78 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams p
     using yes = std::integral_constant<bool, true>;
     using no = std::integral_constant<bool, false>;
     for (int64_t kt = kt0; kt + 1 < kt1; ++kt) {
-      asm volatile(".p2align 6");  // the loop on a cache line: 875 us, unaligned 883
       iterate(kt, yes{});
     }
     iterate(kt1 - 1, no{});
   }
 
-  // ---- out: this wave's dims of both column tiles
+  // ---- out, through LDS
+  const ParamsAgain late = params_again();
+  auto token_late = [&](int64_t x) { return over_group(late->c, static_cast<uint32_t>(x)); };
+  ask_gate(late);
   __syncthreads();
-  float* s_l = s_corr;  // [wave][16]; then the reference points
+  float* s_l = s_corr;  // [column]; then the reference points
   const float l_own = column_sum(l_run);
   if (quad == 0) {
     s_l[wave * 16 + col] = l_own;
     s_l[(kWaves + wave) * 16 + col] = m_run;
   }
-  __syncthreads();
+  constexpr int kRowFloats = D + 4;
+  static_assert(kCols / 2 * kRowFloats * 4 <= S::kCorr, "half of the columns fit below the sums");
+  float* s_o = reinterpret_cast<float*>(smem);
 #pragma unroll
-  for (int c = 0; c < 2; ++c) {
-    const int x = (wave ^ c) * 16 + col;
-    if (x >= n_cols) continue;
-    const float l = s_l[(wave ^ c) * 16 + col];
-    const float over = l == 0.f ? 0.f : 1.f / l;
-    const int64_t tok = tok0 + token_of(x0 + x);
-    const int64_t head = x0 + x - (tok - tok0) * p.G + g * p.G;
-    const int64_t row = tok * p.H + head;
-    const int d0 = half * MH;  // dims (4 quad + r) MT + d0 + i
+  for (int c = 0; c < 2; ++c)
 #pragma unroll
     for (int r = 0; r < 4; ++r)
       if (nan_rows >> (4 * c + r) & 1) {
 #pragma unroll
         for (int i = 0; i < MH; ++i) o[c][i][r] = __uint_as_float(0x7fc00000u);
       }
-    if (pp.splits > 1) {
-      const int64_t at = blockIdx.z * p.total * p.H + row;
-      if (quad == 0 && half == 0) *reinterpret_cast<float2*>(pp.part_ml + at * 2) = make_float2(s_l[(kWaves + (wave ^ c)) * 16 + col], l);
-      if (kt0 < kt1) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-          for (int i = 0; i < MH; i += 4)
-            *reinterpret_cast<floatx4_v*>(pp.part_o + at * D + (4 * quad + r) * MT + d0 + i) = floatx4_v{o[c][i][r], o[c][i + 1][r], o[c][i + 2][r], o[c][i + 3][r]};
-      }
-      continue;
-    }
-    const bf16_t* gate = p.gate != nullptr ? p.gate + tok * p.gate_st + head * p.gate_sh : nullptr;
-    uint2 graw[4][MH / 4];
-    if (gate != nullptr) {
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-#pragma unroll
-        for (int i = 0; i < MH / 4; ++i) graw[r][i] = *reinterpret_cast<const uint2*>(gate + (4 * quad + r) * MT + d0 + 4 * i);
-    }
+  for (int pass = 0; pass < 2; ++pass) {
+    if (pass == 1) lds_barrier();  // the first tiles have been read
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
       for (int i = 0; i < MH; i += 4) {
-        float v[4];
+        floatx4_v v;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          v[e] = o[c][i + e][r] * over;
-          if (gate != nullptr) {
-            const uint32_t w = e < 2 ? graw[r][i / 4].x : graw[r][i / 4].y;
-            v[e] *= sigmoid(__uint_as_float(e & 1 ? w & 0xffff0000u : w << 16));
-          }
-        }
-        uint2 packed;
-        packed.x = static_cast<uint32_t>(f32_to_bf16(v[0])) | static_cast<uint32_t>(f32_to_bf16(v[1])) << 16;
-        packed.y = static_cast<uint32_t>(f32_to_bf16(v[2])) | static_cast<uint32_t>(f32_to_bf16(v[3])) << 16;
-        *reinterpret_cast<uint2*>(p.out + row * D + (4 * quad + r) * MT + d0 + i) = packed;
+        for (int e = 0; e < 4; ++e) v[e] = half == pass ? o[0][i + e][r] : o[1][i + e][r];
+        *reinterpret_cast<floatx4_v*>(s_o + (16 * (wave >> 1) + col) * kRowFloats + (4 * quad + r) * MT + half * MH + i) = v;
       }
+    lds_barrier();
+#pragma unroll
+    for (int i = 0; i < kSweeps; ++i) {
+      const int x = column_of(pass, i);
+      if (x >= n_cols) continue;
+      const float* at = s_o + (tid / kLanes + i * kRowsAtOnce) * kRowFloats;
+      const int64_t row = tok0 * late->c.H + g * late->c.G + x0 + x + static_cast<int64_t>(token_late(x0 + x)) * (late->c.H - late->c.G);
+      const float l = s_l[x];
+      if (late->splits > 1) {
+        const int64_t part = blockIdx.z * late->c.total * late->c.H + row;
+        if (in_row == 0) *reinterpret_cast<float2*>(late->part_ml + part * 2) = make_float2(s_l[kWaves * 16 + x], l);
+        if (kt0 < kt1) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+            *reinterpret_cast<floatx4_v*>(late->part_o + part * D + 4 * in_row + k * D / 2) = *reinterpret_cast<const floatx4_v*>(at + 4 * in_row + k * D / 2);
+        }
+        continue;
+      }
+      const float over = l == 0.f ? 0.f : 1.f / l;  // a query that saw nothing has sums of 0
+      const floatx4_v lo = *reinterpret_cast<const floatx4_v*>(at + 8 * in_row), hi = *reinterpret_cast<const floatx4_v*>(at + 8 * in_row + 4);
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = (e < 4 ? lo[e & 3] : hi[e & 3]) * over;
+      if (late->c.gate != nullptr) {
+        const uint32_t w[4] = {gate[pass][i].x, gate[pass][i].y, gate[pass][i].z, gate[pass][i].w};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] *= sigmoid(__uint_as_float(e & 1 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16));
+      }
+      uint32_t out[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) out[e] = static_cast<uint32_t>(f32_to_bf16(v[2 * e])) | static_cast<uint32_t>(f32_to_bf16(v[2 * e + 1])) << 16;
+      *reinterpret_cast<uint4*>(late->c.out + row * D + 8 * in_row) = make_uint4(out[0], out[1], out[2], out[3]);
+    }
   }
 }
 
