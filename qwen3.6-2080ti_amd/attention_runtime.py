@@ -408,6 +408,11 @@ def _check_step(by_slots: bool, plan: Any | None, no_alloc: bool, tables: Device
         raise ValueError("no_alloc is for bf16 pools: the 4-bit decode takes its workspace per call")
 
 
+def _check_positions(by_slots: bool, positions: Any | None) -> None:
+    if positions is not None and not by_slots:
+        raise ValueError("positions are for a 4-bit pool or mrope_section: elsewhere a token's position is its place in its row")
+
+
 def _qk_norm_rope(q_proj: Any, k_proj: Any, v_proj: Any, q_norm_weight: Any, k_norm_weight: Any, key_blocks: Any, value_blocks: Any,
                   block_tables: Any, cu_seqlens: Any, starts: Any, block_size: int, max_new: int, rope: "RopeConfig") -> tuple[Any, Any]:
     import hip_ops
@@ -487,6 +492,7 @@ def full_attention_decode_step_device(
         reason = "shape"
     by_slots = kv4 or rope.mrope_section is not None
     if reason == "no_kernel":
+        _check_positions(by_slots, positions)
         _check_step(by_slots, plan, no_alloc and kv4, tables)
     if reason != "no_kernel":
         record_native_paged_dispatch(runtime, reason, native=False)
@@ -596,6 +602,7 @@ def full_attention_prefill_device(
         return None
     import hip_ops
 
+    _check_positions(by_slots, positions)
     if by_slots and step.plan is None:
         raise ValueError("a 4-bit pool or mrope_section needs a step of plan_prefill")
     with runtime.profile_scope("full_attention.native_paged_prefill"):

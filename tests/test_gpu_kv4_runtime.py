@@ -251,7 +251,12 @@ def test_steps_without_a_plan_are_refused_before_anything_is_written() -> None:
     for blocks, rope, kw in ((pool, ar.RopeConfig(), {}), (bf16, mrope, {}), (pool, mrope, dict(plan=tables.plan_step(), no_alloc=True))):
         with pytest.raises(ValueError, match="plan|no_alloc"):
             ar.full_attention_decode_step_device(*x(2), *w, blocks.key_blocks, blocks.value_blocks, tables, config, runtime, rope, **kw)
+    at = torch.zeros(1, 2, dtype=torch.int32, device=DEV)
+    with pytest.raises(ValueError, match="positions"):
+        ar.full_attention_decode_step_device(*x(2), *w, bf16.key_blocks, bf16.value_blocks, tables, config, runtime, plan=tables.plan_step(), positions=at)
     step = tables.reserve_prefill([0], [4])
+    with pytest.raises(ValueError, match="positions"):
+        ar.full_attention_prefill_device(*x(4), *w, bf16.key_blocks, bf16.value_blocks, step, config, runtime, positions=at)
     for blocks, rope in ((pool, ar.RopeConfig()), (bf16, mrope)):
         with pytest.raises(ValueError, match="plan_prefill"):
             ar.full_attention_prefill_device(*x(4), *w, blocks.key_blocks, blocks.value_blocks, step, config, runtime, rope)
@@ -266,3 +271,61 @@ def test_steps_without_a_plan_are_refused_before_anything_is_written() -> None:
     with pytest.raises(RuntimeError, match="paged_kv_plan failed: more new tokens"):
         tables.check()
     assert (plan.slots == -1).all()
+
+
+@pytest.mark.parametrize("dim,kv_heads", [(256, 2), (128, 4)])
+def test_blocks_past_four_gigabytes(dim, kv_heads) -> None:
+    """The same step in the first blocks of a pool and in blocks whose bytes lie past 2^32."""
+    heads, block, rows = 8, 16, 2
+    tile = hip_ops.kv4_tile_bytes(dim, block)
+    blocks = (2**32 + 2**28) // (kv_heads * tile)
+    pools = [torch.empty(blocks, kv_heads, tile, dtype=torch.uint8, device=DEV) for _ in range(2)]
+    gen = torch.Generator().manual_seed(6)
+    lens = [1500, 37]
+    need = [-(-n // block) for n in lens]
+    tokens = sum(lens)
+    q, k, v = (torch.randn(tokens, h, dim, generator=gen).to(torch.bfloat16).to(DEV) for h in (2 * heads, kv_heads, kv_heads))
+    q = q.view(tokens, heads, 2 * dim)
+    w = torch.zeros(dim, dtype=torch.bfloat16, device=DEV)
+    at = torch.cat([torch.arange(n) for n in lens]).to(DEV)
+    cu = torch.tensor([0, *torch.tensor(lens).cumsum(0).tolist()], dtype=torch.int32, device=DEV)
+    results = []
+    for first in (0, blocks - sum(need)):
+        ids = first + torch.arange(sum(need), dtype=torch.int32, device=DEV)
+        tables = torch.full((rows, max(need)), -1, dtype=torch.int32, device=DEV)
+        tables[0, : need[0]], tables[1, : need[1]] = ids[: need[0]], ids[need[0] :]
+        row = torch.repeat_interleave(torch.arange(rows, device=DEV), torch.tensor(lens, device=DEV))
+        slots = tables[row, at // block].long() * block + at % block
+        query, gate = hip_ops.qk_norm_mrope_kv_append(q, k, v, w, w, at, (dim // 4,), *pools, slots, block, eps=1e-6, rope_theta=1e6)
+        prefill = hip_ops.paged_attention_prefill_kv4(query, cu, torch.zeros(rows, dtype=torch.int32, device=DEV), *pools, tables, block, max_new=max(lens), gate=gate)
+        decode = hip_ops.paged_attention_decode_kv4(query[:rows].unsqueeze(2), tables, *pools, torch.tensor(lens, dtype=torch.int32, device=DEV), block)
+        hip_ops.paged_kv4_append(k, v, *pools, slots, block)
+        results.append((prefill, decode, *hip_ops.paged_kv4_gather(*pools, tables[:1], lens[0], block)))
+    for low, high in zip(*results):
+        assert torch.isfinite(low.float()).all() and torch.equal(low, high)
+
+
+def test_two_streams_at_once() -> None:
+    heads, kv_heads, dim, block = 16, 2, 256, 16
+    pool = SharedKV4BlockPool(600, kv_heads, dim, block_size=block, device=DEV)
+    gen = torch.Generator().manual_seed(7)
+    k, v = (torch.randn(9600, kv_heads, dim, generator=gen).to(torch.bfloat16).to(DEV) for _ in range(2))
+    hip_ops.paged_kv4_append(k, v, pool.key_blocks, pool.value_blocks, torch.randperm(9600, generator=gen).to(DEV), block)
+    tables = torch.randperm(600, generator=gen)[:600].view(2, 300).to(DEV)
+    q = torch.randn(2, heads, 1, dim, generator=gen).to(torch.bfloat16).to(DEV)
+    new = torch.randn(40, heads, dim, generator=gen).to(torch.bfloat16).to(DEV)
+    cu, prefix = torch.tensor([0, 15, 40], device=DEV), torch.tensor([4700, 3000], device=DEV)
+    lens = [torch.tensor(n, device=DEV) for n in ([4800, 4000], [17, 4799])]
+    runs = [lambda n=n: hip_ops.paged_attention_decode_kv4(q, tables, pool.key_blocks, pool.value_blocks, n, block) for n in lens]
+    runs.append(lambda: hip_ops.paged_attention_prefill_kv4(new, cu, prefix, pool.key_blocks, pool.value_blocks, tables, block, max_new=25))
+    want = [run() for run in runs]
+    streams = [torch.cuda.Stream() for _ in runs]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = []
+        for stream, run in zip(streams, runs):
+            with torch.cuda.stream(stream):
+                got.append(run())
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)

@@ -64,7 +64,7 @@ def test_prologue_into_a_bf16_pool(heads, kv_heads, dim, sections, interleaved, 
     assert (keys[rest] == 9).all() and (values[rest] == 9).all()
 
 
-@pytest.mark.parametrize("heads,kv_heads,dim,sections,block", [(16, 2, 256, (11, 11, 10), 16), (8, 4, 128, (16, 24, 24), 32), (5, 5, 128, (8,), 64)])
+@pytest.mark.parametrize("heads,kv_heads,dim,sections,block", [(16, 2, 256, (11, 11, 10), 16), (8, 4, 128, (16, 24, 24), 32), (5, 5, 128, (8,), 64), (4, 2, 256, (4,), 32), (6, 3, 128, (2, 4), 16)])
 @pytest.mark.parametrize("tokens", [1, 50])
 def test_a_4_bit_pool_holds_the_4_bit_form_of_the_bf16_one(heads, kv_heads, dim, sections, block, tokens) -> None:
     q, k, v, qw, kw, positions = (x.to(DEV) for x in _inputs(7, tokens, heads, kv_heads, dim, len(sections), 5000))
