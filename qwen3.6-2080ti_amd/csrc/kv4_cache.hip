@@ -1,15 +1,19 @@
 // Writes and dense reads of the 4-bit paged KV cache (layout and number format: kv4.h), gfx950.
 //
 // Both are bound by memory: per token and KV head the append reads 2 x 2 D bytes of bf16 and writes 2 x 17 D / 32, the
-// gather the other way round.  A wave takes the group (head, 32 dims) of 16 consecutive tokens, four lanes a token and
-// eight dims a lane: loads are 64-byte pieces of rows, the group's maximum needs two quad swaps, and the 16 tokens of
+// gather the other way round.  A wave takes groups (head, 32 dims) of 16 consecutive tokens, four lanes a token and eight
+// dims a lane: loads are 64-byte pieces of rows, the group's maximum needs two quad swaps, and the 16 tokens of
 // a run land in 256 consecutive bytes of keys.  Rows that are adjacent in the source but not in the pool stay right:
-// every lane takes its own token's slot.  Three prompts of 4001 tokens, two heads of 256, 31 MB each way: append 10.1 us,
-// gather 8.8 (a launch that does nothing takes 2.5 of it, a copy of as much 6.4); five rows of one and of 334: 2.7, 3.4 us.
+// every lane takes its own token's slot.  Three prompts of 4001 tokens, two heads of 256, 31 MB each way: append 7.8 us,
+// gather 7.5 (a launch that does nothing takes 2.5 of it, a copy of as much 6.4); five rows of one and of 334: 2.8, 3.4 us.
 #include "kv4.h"
 
 namespace qa {
 namespace kv4 {
+
+// Groups of 32 dims a wave takes, its loads on their way together.  us at 1, 2 and 4 groups, heads of 256: append of 3 x 4001
+// tokens 10.1 7.8 8.4, of 8 x 8000 42.2 32.8 32.1, of 5 2.5 2.8 3.1; the gathers of as many 8.9 8.1 7.5, 38.8 30.9 28.9.
+constexpr int kAppendGroups = 2, kGatherGroups = 4;
 
 struct AppendParams {
   const void* key;
@@ -51,29 +55,37 @@ template <int D, bool F32, bool S64>
 __global__ __launch_bounds__(256) void append_kernel(AppendParams p) {
   using R = Run<D>;
   const int lane = threadIdx.x & 63;
-  const int group = blockIdx.y % R::kGroups;
-  const int h = blockIdx.y / R::kGroups;
+  constexpr int kSteps = R::kGroups / kAppendGroups;
+  const int group0 = blockIdx.y % kSteps * kAppendGroups;
+  const int h = blockIdx.y / kSteps;
   const int64_t n = (static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6)) * kRun + (lane >> 2);
   const int sub = lane & 3;
   const int64_t nn = min64(n, p.tokens - 1);  // no branch round the loads: a lane past the end reads the last token
   const int64_t slot = S64 ? reinterpret_cast<const int64_t*>(p.slots)[nn] : reinterpret_cast<const int32_t*>(p.slots)[nn];
-  float k[8], v[8];
-  const int d0 = group * 32 + 8 * sub;
-  load8<F32>(p.key, nn * p.k_st + h * p.k_sh + d0, k);
-  load8<F32>(p.value, nn * p.v_st + h * p.v_sh + d0, v);
-  const uint32_t kb = group_byte(k), vb = group_byte(v);
-  const uint32_t kc = pack_codes(k, kb), vc = pack_codes(v, vb);
-  if (n >= p.tokens || slot < 0 || slot >= p.num_slots) return;
-  const int at = static_cast<int>(slot & ((1 << p.bs_shift) - 1));
+  float k[kAppendGroups][8], v[kAppendGroups][8];
+#pragma unroll
+  for (int u = 0; u < kAppendGroups; ++u) {
+    load8<F32>(p.key, nn * p.k_st + h * p.k_sh + (group0 + u) * 32 + 8 * sub, k[u]);
+    load8<F32>(p.value, nn * p.v_st + h * p.v_sh + (group0 + u) * 32 + 8 * sub, v[u]);
+  }
+  const bool there = n < p.tokens && slot >= 0 && slot < p.num_slots;
+  const int at = there ? static_cast<int>(slot & ((1 << p.bs_shift) - 1)) : 0;
   const int t = at & 15;
-  const int64_t run = (slot >> p.bs_shift) * p.sP + h * p.sG + static_cast<int64_t>(at >> 4) * R::kBytes;
-  *reinterpret_cast<uint32_t*>(p.kpool + run + R::key_code(t, group) + 4 * sub) = kc;
-  // eight dims are half a chunk of values at D = 256 and a whole one at D = 128
-  const int chunk = d0 / (D / 16);
-  *reinterpret_cast<uint32_t*>(p.vpool + run + R::value_code(t, chunk) + d0 % (D / 16) / 2) = vc;
-  if (sub == 0) {
-    p.kpool[run + R::key_scale(t, group)] = static_cast<uint8_t>(kb);
-    p.vpool[run + R::value_scale(t, group)] = static_cast<uint8_t>(vb);
+  const int64_t run = there ? (slot >> p.bs_shift) * p.sP + h * p.sG + static_cast<int64_t>(at >> 4) * R::kBytes : 0;
+#pragma unroll
+  for (int u = 0; u < kAppendGroups; ++u) {
+    const uint32_t kb = group_byte(k[u]), vb = group_byte(v[u]);
+    const uint32_t kc = pack_codes(k[u], kb), vc = pack_codes(v[u], vb);
+    if (!there) continue;
+    const int group = group0 + u;
+    const int d0 = group * 32 + 8 * sub;
+    *reinterpret_cast<uint32_t*>(p.kpool + run + R::key_code(t, group) + 4 * sub) = kc;
+    // eight dims are half a chunk of values at D = 256 and a whole one at D = 128
+    *reinterpret_cast<uint32_t*>(p.vpool + run + R::value_code(t, d0 / (D / 16)) + d0 % (D / 16) / 2) = vc;
+    if (sub == 0) {
+      p.kpool[run + R::key_scale(t, group)] = static_cast<uint8_t>(kb);
+      p.vpool[run + R::value_scale(t, group)] = static_cast<uint8_t>(vb);
+    }
   }
 }
 
@@ -103,8 +115,9 @@ template <int D, bool T64>
 __global__ __launch_bounds__(256) void gather_kernel(GatherParams p) {
   using R = Run<D>;
   const int lane = threadIdx.x & 63;
-  const int group = blockIdx.y % R::kGroups;
-  const int h = blockIdx.y / R::kGroups;
+  constexpr int kSteps = R::kGroups / kGatherGroups;
+  const int group0 = blockIdx.y % kSteps * kGatherGroups;
+  const int h = blockIdx.y / kSteps;
   const int64_t b = blockIdx.z;
   const int64_t run16 = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);  // the wave's run of 16 tokens
   const int t = lane >> 2, sub = lane & 3;
@@ -115,22 +128,35 @@ __global__ __launch_bounds__(256) void gather_kernel(GatherParams p) {
     const int64_t off = b * p.table_stride + logical;
     phys = T64 ? reinterpret_cast<const int64_t*>(p.tables)[off] : reinterpret_cast<const int32_t*>(p.tables)[off];
   }
-  uint4 k = make_uint4(0, 0, 0, 0), v = k;
-  const int d0 = group * 32 + 8 * sub;
+  uint4 k[kGatherGroups], v[kGatherGroups];
+#pragma unroll
+  for (int u = 0; u < kGatherGroups; ++u) k[u] = v[u] = make_uint4(0, 0, 0, 0);
   if (phys >= 0 && phys < p.num_blocks) {
     const int64_t run = phys * p.sP + h * p.sG + (run16 & ((1 << (p.bs_shift - 4)) - 1)) * R::kBytes;
-    const uint32_t kc = *reinterpret_cast<const uint32_t*>(p.kpool + run + R::key_code(t, group) + 4 * sub);
-    const uint32_t vc = *reinterpret_cast<const uint32_t*>(p.vpool + run + R::value_code(t, d0 / (D / 16)) + d0 % (D / 16) / 2);
-    const uint32_t kb = p.kpool[run + R::key_scale(t, group)];
-    const uint32_t vb = p.vpool[run + R::value_scale(t, group)];
-    k = unpack_codes(kc, kb);
-    v = unpack_codes(vc, vb);
+    uint32_t kc[kGatherGroups], vc[kGatherGroups], kb[kGatherGroups], vb[kGatherGroups];
+#pragma unroll
+    for (int u = 0; u < kGatherGroups; ++u) {
+      const int group = group0 + u;
+      const int d0 = group * 32 + 8 * sub;
+      kc[u] = *reinterpret_cast<const uint32_t*>(p.kpool + run + R::key_code(t, group) + 4 * sub);
+      vc[u] = *reinterpret_cast<const uint32_t*>(p.vpool + run + R::value_code(t, d0 / (D / 16)) + d0 % (D / 16) / 2);
+      kb[u] = p.kpool[run + R::key_scale(t, group)];
+      vb[u] = p.vpool[run + R::value_scale(t, group)];
+    }
+#pragma unroll
+    for (int u = 0; u < kGatherGroups; ++u) {
+      k[u] = unpack_codes(kc[u], kb[u]);
+      v[u] = unpack_codes(vc[u], vb[u]);
+    }
   }
   const int64_t n = run16 * kRun + t;
   if (n >= p.valid) return;
-  const int64_t out = ((b * p.Hkv + h) * p.valid + n) * D + d0;
-  *reinterpret_cast<uint4*>(p.key_out + out) = k;
-  *reinterpret_cast<uint4*>(p.value_out + out) = v;
+  const int64_t out = ((b * p.Hkv + h) * p.valid + n) * D + group0 * 32 + 8 * sub;
+#pragma unroll
+  for (int u = 0; u < kGatherGroups; ++u) {
+    *reinterpret_cast<uint4*>(p.key_out + out + 32 * u) = k[u];
+    *reinterpret_cast<uint4*>(p.value_out + out + 32 * u) = v[u];
+  }
 }
 
 template <int D, bool F32>
@@ -161,7 +187,7 @@ extern "C" int qa_paged_kv4_append(const void* key_new, const void* value_new, i
   QA_REQUIRE(k_stride_t % al == 0 && k_stride_h % al == 0 && v_stride_t % al == 0 && v_stride_h % al == 0 &&
                  ((reinterpret_cast<uintptr_t>(key_new) | reinterpret_cast<uintptr_t>(value_new)) & 15u) == 0,
              "paged_kv4_append: rows must be 16-byte aligned");
-  const int64_t gy = static_cast<int64_t>(kv->kv_heads) * (head_dim / 32);
+  const int64_t gy = static_cast<int64_t>(kv->kv_heads) * (head_dim / 32 / kAppendGroups);
   QA_REQUIRE(gy <= 65535, "paged_kv4_append: too many KV heads");
   AppendParams p{};
   p.key = key_new;
@@ -203,7 +229,7 @@ extern "C" int qa_paged_kv4_gather(const qa_paged_kv* kv, int32_t head_dim, int6
   if (valid == 0 || batch == 0) return 0;
   QA_REQUIRE(key_out && value_out && ((reinterpret_cast<uintptr_t>(key_out) | reinterpret_cast<uintptr_t>(value_out)) & 15u) == 0,
              "paged_kv4_gather: outputs must be non-null and 16-byte aligned");
-  const int64_t gy = static_cast<int64_t>(kv->kv_heads) * (head_dim / 32);
+  const int64_t gy = static_cast<int64_t>(kv->kv_heads) * (head_dim / 32 / kGatherGroups);
   QA_REQUIRE(gy <= 65535, "paged_kv4_gather: too many KV heads");
   GatherParams p{};
   p.kpool = reinterpret_cast<const uint8_t*>(kv->key);

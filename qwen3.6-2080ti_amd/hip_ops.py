@@ -1335,10 +1335,10 @@ def paged_attention_decode_kv4(
     max_blocks = tables.shape[1]
     result = _kv4_out(out, query)
     nbytes = lib.qa_paged_attention_decode_kv4_workspace(batch, heads, desc.kv_heads, head_dim, max_blocks * block_size)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
     code = _launch(
         device, lib.qa_paged_attention_decode_kv4, q.data_ptr(), L.QA_BF16, q_sb, q_sh, batch, heads, head_dim, ctypes.byref(desc), tables.data_ptr(), _code(tables),
-        max_blocks, max_blocks, lens.data_ptr(), _code(lens), int(block_size), float(scale or 0.0), g_ptr, g_sb, g_sh, result.data_ptr(), ws.data_ptr(), nbytes,
+        max_blocks, max_blocks, lens.data_ptr(), _code(lens), int(block_size), float(scale or 0.0), g_ptr, g_sb, g_sh, result.data_ptr(), _ptr(ws), nbytes,
     )
     L.check(lib, code, "paged_attention_decode_kv4")
     return result
