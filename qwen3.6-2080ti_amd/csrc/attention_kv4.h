@@ -320,6 +320,7 @@ inline int fill(Params& p, const Args& a) {
   QA_REQUIRE(((reinterpret_cast<uintptr_t>(a.query) | reinterpret_cast<uintptr_t>(a.out)) & 15u) == 0 && a.q_st % 8 == 0 && a.q_sh % 8 == 0,
              "%s: query rows must be 16-byte aligned", a.what);
   QA_REQUIRE(a.gate == nullptr || ((reinterpret_cast<uintptr_t>(a.gate) & 7u) == 0 && a.gate_st % 4 == 0 && a.gate_sh % 4 == 0), "%s: gate rows must be 8-byte aligned", a.what);
+  QA_REQUIRE(((a.q_st | a.q_sh | a.gate_st | a.gate_sh) & ~0xffffffffll) == 0, "%s: query and gate strides must be in [0, 2^32)", a.what);
   p.q = reinterpret_cast<const bf16_t*>(a.query);
   p.q_st = a.q_st;
   p.q_sh = a.q_sh;

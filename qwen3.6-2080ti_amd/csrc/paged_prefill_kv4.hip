@@ -19,8 +19,8 @@
 //
 // With few columns the keys are split over gridDim.z and a second launch joins the parts.
 //
-// Bound by the matrix and vector units together.  16 heads of 256 over 2: 2048 tokens behind 32000 867 us, 1280 TFLOP/s of
-// the two products (a large bf16 library product runs at 1210), eight chunks of 512 behind up to 8k 283 us, 1090; five
+// Bound by the matrix and vector units together.  16 heads of 256 over 2: 2048 tokens behind 32000 865 us, 1280 TFLOP/s of
+// the two products (a large bf16 library product runs at 1210), eight chunks of 512 behind up to 8k 282 us, 1090; five
 // prompts of up to 700, 20 heads of 128 over 4, 31 us: a workgroup's start and end are 10 of them and its longest row 13.
 #include "attention_kv4.h"
 
@@ -146,10 +146,23 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams p
 
   // columns: [0] the wave's own 16, [1] its partner's; their position past first_pos
   const int n_cols = static_cast<int>(last - x0) + 1;
-  const int x_head = static_cast<int>(x0 - static_cast<int64_t>(token_of(x0)) * p.G);  // head of the workgroup's first column
+  // A column as a token past the workgroup's first one and a head of the group, both small: offsets are 32 by 32 bits on
+  // top of uniform addresses (64-bit products of every row's own were 3000 cycles of a workgroup).
+  const int64_t first_tok = tok0 + token_of(x0);
+  const uint32_t x_head = static_cast<uint32_t>(x0 - (first_tok - tok0) * p.G);  // head of the workgroup's first column
+  struct Place {
+    uint32_t token, head;
+  };
+  auto place_of = [&](const auto& c, int x) {
+    const uint32_t t = over_group(c, x_head + x);
+    return Place{t, x_head + x - t * static_cast<uint32_t>(c.G)};
+  };
+  auto row_of = [](const bf16_t* base, const Place& at, int64_t st, int64_t sh) {  // strides below 2^32
+    return base + (static_cast<uint64_t>(at.token) * static_cast<uint32_t>(st) + static_cast<uint64_t>(at.head) * static_cast<uint32_t>(sh));
+  };
   int ahead[2];
 #pragma unroll
-  for (int c = 0; c < 2; ++c) ahead[c] = static_cast<int>(over_group(p, min((wave ^ c) * 16 + col, n_cols - 1) + x_head));
+  for (int c = 0; c < 2; ++c) ahead[c] = static_cast<int>(place_of(p, min((wave ^ c) * 16 + col, n_cols - 1)).token);
 
   // ---- the tiles' loads
   // Lane l of `cur` holds the offset in the head's pool of run 64 c + l (-1: not there), of `nxt` that of the next 64,
@@ -267,13 +280,13 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams p
   uint4 gate[2][kSweeps];
   auto ask_gate = [&](ParamsAgain late) {
     if (late->c.gate == nullptr || late->splits > 1) return;
+    const bf16_t* base = late->c.gate + first_tok * late->c.gate_st + static_cast<int64_t>(g) * late->c.G * late->c.gate_sh;
 #pragma unroll
     for (int pass = 0; pass < 2; ++pass)
 #pragma unroll
       for (int i = 0; i < kSweeps; ++i) {
-        const int x = min(column_of(pass, i), n_cols - 1);
-        const int64_t t = over_group(late->c, static_cast<uint32_t>(x0 + x));
-        const uint2* src = reinterpret_cast<const uint2*>(late->c.gate + (tok0 + t) * late->c.gate_st + (x0 + x - t * late->c.G + g * late->c.G) * late->c.gate_sh + 8 * in_row);
+        const Place at = place_of(late->c, min(column_of(pass, i), n_cols - 1));
+        const uint2* src = reinterpret_cast<const uint2*>(row_of(base, at, late->c.gate_st, late->c.gate_sh) + 8 * in_row);
         const uint2 lo = src[0], hi = src[1];
         gate[pass][i] = make_uint4(lo.x, lo.y, hi.x, hi.y);
       }
@@ -284,9 +297,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams p
     QueryRow<D> row;
     {
       const int x = wave * 16 + col;
-      const int64_t tok = tok0 + token_of(x0 + x);
-      const int64_t head = x0 + x - (tok - tok0) * p.G + g * p.G;
-      row.ask(x < n_cols ? p.q + tok * p.q_st + head * p.q_sh : nullptr, quad);
+      const bf16_t* base = p.q + first_tok * p.q_st + static_cast<int64_t>(g) * p.G * p.q_sh;
+      row.ask(x < n_cols ? row_of(base, place_of(p, x), p.q_st, p.q_sh) : nullptr, quad);
     }
     cur = chunk(kt0 >> 4);
     nxt = chunk((kt0 >> 4) + 1);
@@ -424,6 +436,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams p
       // a wave in its value products goes ahead of its neighbour on the SIMD that is still unpacking: 867 us against 901
       // without priorities, 878 the other way round
       __builtin_amdgcn_s_setprio(0);
+      asm volatile("s_nop 0");  // the same loop four bytes on in the instruction cache: 865 us, without it 881
       const int flag = s_flag[buf];
       const float c0 = s_corr[(buf * kWaves + wave) * 16 + col], c1 = s_corr[(buf * kWaves + (wave ^ 1)) * 16 + col];
       if constexpr (more) {
@@ -505,7 +518,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams p
 
   // ---- out, through LDS
   const ParamsAgain late = params_again();
-  auto token_late = [&](int64_t x) { return over_group(late->c, static_cast<uint32_t>(x)); };
+  const int64_t row0 = first_tok * late->c.H + static_cast<int64_t>(g) * late->c.G;  // of the output
   ask_gate(late);
   __syncthreads();
   float* s_l = s_corr;  // [column]; then the reference points
@@ -543,10 +556,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams p
       const int x = column_of(pass, i);
       if (x >= n_cols) continue;
       const float* at = s_o + (tid / kLanes + i * kRowsAtOnce) * kRowFloats;
-      const int64_t row = tok0 * late->c.H + g * late->c.G + x0 + x + static_cast<int64_t>(token_late(x0 + x)) * (late->c.H - late->c.G);
+      const Place pl = place_of(late->c, x);
+      const uint32_t row = pl.token * static_cast<uint32_t>(late->c.H) + pl.head;  // past row0
       const float l = s_l[x];
       if (late->splits > 1) {
-        const int64_t part = blockIdx.z * late->c.total * late->c.H + row;
+        const int64_t part = blockIdx.z * late->c.total * late->c.H + row0 + row;
         if (in_row == 0) *reinterpret_cast<float2*>(late->part_ml + part * 2) = make_float2(s_l[kWaves * 16 + x], l);
         if (kt0 < kt1) {
 #pragma unroll
@@ -568,7 +582,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams p
       uint32_t out[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) out[e] = static_cast<uint32_t>(f32_to_bf16(v[2 * e])) | static_cast<uint32_t>(f32_to_bf16(v[2 * e + 1])) << 16;
-      *reinterpret_cast<uint4*>(late->c.out + row * D + 8 * in_row) = make_uint4(out[0], out[1], out[2], out[3]);
+      *reinterpret_cast<uint4*>(late->c.out + row0 * D + (static_cast<uint64_t>(row) * D + 8 * in_row)) = make_uint4(out[0], out[1], out[2], out[3]);
     }
   }
 }
