@@ -86,7 +86,7 @@ def _decode(lib, **changes) -> int:
 
 BAD_ATTENTION = [
     (dict(dtype=L.QA_F32), "must be bfloat16"), (dict(tdtype=L.QA_F32), "int32/int64"), (dict(heads=15), "multiple of KV heads"), (dict(heads=34), "larger than 16"),
-    (dict(heads=0), "multiple of KV heads"), (dict(width=0), "at least one entry"), (dict(qb=1 << 32), "strides"), (dict(gate=SOME, gh=1 << 33), "strides"), (dict(qh=-256), "strides"), (dict(qb=4100), "16-byte aligned"), (dict(q=P((1 << 20) + 8)), "16-byte aligned"),
+    (dict(heads=0), "multiple of KV heads"), (dict(width=0), "at least one entry"), (dict(qb=1 << 32), "strides"), (dict(gate=SOME, gb=1 << 33), "strides"), (dict(qh=-256), "strides"), (dict(qb=4100), "16-byte aligned"), (dict(q=P((1 << 20) + 8)), "16-byte aligned"),
     (dict(gate=P((1 << 20) + 2)), "8-byte aligned"), (dict(gate=SOME, gb=2), "8-byte aligned"), (dict(q=P(0)), "non-null"), (dict(out=P(0)), "non-null"), (dict(tables=P(0)), "non-null"),
     (dict(batch=-1), "out of range"),
 ]
