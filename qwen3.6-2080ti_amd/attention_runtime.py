@@ -26,8 +26,8 @@ engine and scheduler above it keep their calls:
 Host-side tensor preparation (L2 norm, transposes) is PyTorch on the same
 device; every hot loop is a HIP kernel.  Pools may hold bf16 or 4 bits
 (``decode_state.SharedKV4BlockPool``): the entry points choose by the pool's
-type, and ``RopeConfig.mrope_section`` adds rotary positions of several axes.  There is no CPU or dense fallback in
-this module.
+type, and ``RopeConfig.mrope_section`` adds rotary positions of several axes.
+There is no CPU or dense fallback in this module.
 """
 
 from __future__ import annotations

@@ -35,7 +35,8 @@ using namespace attn4;
 
 struct PrefillParams {
   Params c;
-  int splits;
+  int splits;      // parts of the keys that the launch has workgroups for
+  float per_tile;  // kPerTile / workgroups
   float* part_o;   // (splits, total, H, D)
   float* part_ml;  // (splits, total, H, 2)
 };
@@ -44,9 +45,23 @@ constexpr int kTile = 64;      // keys
 constexpr int kRuns = kTile / kv4::kRun;
 constexpr int kWaves = 8;
 constexpr int kCols = kWaves * 16;
+constexpr int kMaxSplits = 64;
 // Batches up to this many rows start with the longest row, so that the launch ends on short ones: 60 rows of up to 300 new
 // tokens behind up to 4000 439 -> 403 us, 12 of up to 1500 behind up to 8000 738 -> 677; 64 equal rows of 16 64.5 -> 65.8.
 constexpr int kRankRows = 64;
+
+// Keys that the columns up to the last, of a row with `prefix` cached tokens, see: not past the table.
+template <typename P>
+__device__ __forceinline__ int64_t keys_of(const P& p, int64_t prefix, int64_t last) {
+  return max64(0, min64(prefix + over_group(p, static_cast<uint32_t>(last)) + 1, p.max_blocks << p.bs_shift));
+}
+
+// Parts that `tiles` tiles are split into, the same in both launches: the tables may be much wider than the row.
+template <typename P>
+__device__ __forceinline__ int parts_of(const P& pp, int64_t tiles) {
+  const float best = __builtin_sqrtf(pp.per_tile * static_cast<float>(tiles));
+  return max(1, min(min(pp.splits, static_cast<int>(best)), static_cast<int>(min64(tiles, kMaxSplits))));
+}
 
 template <int D>
 struct Smem {
@@ -129,17 +144,19 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams p
   const int64_t ct0 = static_cast<int64_t>(gridDim.x) - 1 - blockIdx.x;
   const int64_t x0 = ct0 * kCols;  // first column of the workgroup
   if (tok0 < 0 || x0 >= n_new * p.G) return;
-  auto token_of = [&](int64_t x) { return over_group(p, static_cast<uint32_t>(x)); };  // columns fit 31 bits
-  const int64_t last = min64(n_new * p.G, x0 + kCols) - 1;
-  // keys that any column sees: not past the table
-  const int64_t kv_end = max64(0, min64(prefix + token_of(last) + 1, p.max_blocks << p.bs_shift));
-  const int64_t first_pos = prefix + token_of(x0);  // every column sees the keys up to here
+  const int64_t last = min64(n_new * p.G, x0 + kCols) - 1;  // columns fit 31 bits
+  const int64_t kv_end = keys_of(p, prefix, last);          // keys that any column sees
+  const int64_t first_new = over_group(p, static_cast<uint32_t>(x0));
+  const int64_t first_pos = prefix + first_new;  // every column sees the keys up to here
   const int64_t runs = (kv_end + kv4::kRun - 1) / kv4::kRun;
   const int64_t all_tiles = (kv_end + kTile - 1) / kTile;
   int64_t kt0 = 0, kt1 = all_tiles;
+  int parts = 1;
   if (pp.splits > 1) {
-    kt0 = all_tiles * blockIdx.z / pp.splits;
-    kt1 = all_tiles * (blockIdx.z + 1) / pp.splits;
+    parts = parts_of(pp, all_tiles);
+    if (static_cast<int>(blockIdx.z) >= parts) return;
+    kt0 = all_tiles * blockIdx.z / parts;
+    kt1 = all_tiles * (blockIdx.z + 1) / parts;
   }
   const uint8_t* kb = p.kpool + g * p.sG;
   const uint8_t* vb = p.vpool + g * p.sG;
@@ -148,7 +165,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams p
   const int n_cols = static_cast<int>(last - x0) + 1;
   // A column as a token past the workgroup's first one and a head of the group, both small: offsets are 32 by 32 bits on
   // top of uniform addresses (64-bit products of every row's own were 3000 cycles of a workgroup).
-  const int64_t first_tok = tok0 + token_of(x0);
+  const int64_t first_tok = tok0 + first_new;
   const uint32_t x_head = static_cast<uint32_t>(x0 - (first_tok - tok0) * p.G);  // head of the workgroup's first column
   struct Place {
     uint32_t token, head;
@@ -279,7 +296,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams p
   };
   uint4 gate[2][kSweeps];
   auto ask_gate = [&](ParamsAgain late) {
-    if (late->c.gate == nullptr || late->splits > 1) return;
+    if (late->c.gate == nullptr || parts > 1) return;
     const bf16_t* base = late->c.gate + first_tok * late->c.gate_st + static_cast<int64_t>(g) * late->c.G * late->c.gate_sh;
 #pragma unroll
     for (int pass = 0; pass < 2; ++pass)
@@ -559,14 +576,12 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams p
       const Place pl = place_of(late->c, x);
       const uint32_t row = pl.token * static_cast<uint32_t>(late->c.H) + pl.head;  // past row0
       const float l = s_l[x];
-      if (late->splits > 1) {
+      if (parts > 1) {
         const int64_t part = blockIdx.z * late->c.total * late->c.H + row0 + row;
         if (in_row == 0) *reinterpret_cast<float2*>(late->part_ml + part * 2) = make_float2(s_l[kWaves * 16 + x], l);
-        if (kt0 < kt1) {
 #pragma unroll
-          for (int k = 0; k < 2; ++k)
-            *reinterpret_cast<floatx4_v*>(late->part_o + part * D + 4 * in_row + k * D / 2) = *reinterpret_cast<const floatx4_v*>(at + 4 * in_row + k * D / 2);
-        }
+        for (int k = 0; k < 2; ++k)
+          *reinterpret_cast<floatx4_v*>(late->part_o + part * D + 4 * in_row + k * D / 2) = *reinterpret_cast<const floatx4_v*>(at + 4 * in_row + k * D / 2);
         continue;
       }
       const float over = l == 0.f ? 0.f : 1.f / l;  // a query that saw nothing has sums of 0
@@ -601,27 +616,30 @@ __global__ __launch_bounds__(256) void join_kernel(PrefillParams pp, int64_t max
   const int64_t tok0 = read_index(p.cu, p.idx_i64, b);
   const int64_t n_new = min64(max_new, min64(read_index(p.cu, p.idx_i64, b + 1), p.total) - tok0);
   if (tok0 < 0 || x >= n_new * p.H) return;
+  const uint32_t n = static_cast<uint32_t>(x) / static_cast<uint32_t>(p.H), h = static_cast<uint32_t>(x) - n * static_cast<uint32_t>(p.H);
+  // the workgroups that had this column
+  const int64_t column = static_cast<int64_t>(n) * p.G + (h - over_group(p, h) * static_cast<uint32_t>(p.G));
+  const int64_t last = min64((min64(read_index(p.cu, p.idx_i64, b + 1), p.total) - tok0) * p.G, column / kCols * kCols + kCols) - 1;
+  const int parts = parts_of(pp, (keys_of(p, read_index(p.prefix, p.idx_i64, b), last) + kTile - 1) / kTile);
+  if (parts == 1) return;  // written by the workgroup itself
   const int64_t row = tok0 * p.H + x;
   const int64_t stride = p.total * p.H;
-  const float2 ml = lane < pp.splits ? *reinterpret_cast<const float2*>(pp.part_ml + (lane * stride + row) * 2) : make_float2(-INFINITY, 0.f);
+  const float2 ml = lane < parts ? *reinterpret_cast<const float2*>(pp.part_ml + (lane * stride + row) * 2) : make_float2(-INFINITY, 0.f);
   const float m = wave_max(ml.x);
   const float f = __builtin_amdgcn_exp2f(ml.x - (m == -INFINITY ? 0.f : m));
   const float l = wave_sum(f * ml.y);
   vec_t acc = vec_t(0.f);
-  for (int s0 = 0; s0 < pp.splits; s0 += kJoinAhead) {
+  for (int s0 = 0; s0 < parts; s0 += kJoinAhead) {
     vec_t part[kJoinAhead];
 #pragma unroll
     for (int i = 0; i < kJoinAhead; ++i)  // past the end: the last part again
-      part[i] = *reinterpret_cast<const vec_t*>(pp.part_o + (min(s0 + i, pp.splits - 1) * stride + row) * D + E * lane);
+      part[i] = *reinterpret_cast<const vec_t*>(pp.part_o + (min(s0 + i, parts - 1) * stride + row) * D + E * lane);
 #pragma unroll
     for (int i = 0; i < kJoinAhead; ++i) {
-      const int s = min(s0 + i, pp.splits - 1);
-      const float fs = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f), s));
-      const float ls = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(ml.y), s));
-      if (s0 + i < pp.splits && ls != 0.f) acc += fs * part[i];  // a part that saw nothing wrote nothing
+      const float fs = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f), min(s0 + i, parts - 1)));
+      if (s0 + i < parts) acc += fs * part[i];
     }
   }
-  const uint32_t n = static_cast<uint32_t>(x) / static_cast<uint32_t>(p.H), h = static_cast<uint32_t>(x) - n * static_cast<uint32_t>(p.H);
   typedef uint32_t packed_t __attribute__((ext_vector_type(E / 2)));
   packed_t gate = packed_t(0u), out;
   if (p.gate != nullptr) gate = *reinterpret_cast<const packed_t*>(p.gate + (tok0 + n) * p.gate_st + h * p.gate_sh + E * lane);
@@ -637,18 +655,21 @@ __global__ __launch_bounds__(256) void join_kernel(PrefillParams pp, int64_t max
   *reinterpret_cast<packed_t*>(p.out + row * D + E * lane) = out;
 }
 
-constexpr int kMaxSplits = 64;
-
 // Parts the keys are split into where the workgroups leave CUs free.  A part saves a share of 1.5 us a tile and costs its
 // piece of the partial results, in time like parts times workgroups, which puts the best number at a root; the 30 is from
 // us with 1, 2, 4, 8, 16 parts, D = 256, one row: 16 tokens (2 workgroups) over 32 tiles 65.6 41.9 29.2 23.3 22.1, 128 tokens
 // (16) over 17 tiles 42.3 31.9 27.7 30.8 35.4, 512 tokens (64) over 8 tiles 28.6 33.6 35.4 51.4 64.5, over 32 tiles 67.2
 // 52.8 45.3 64.9 105.
+constexpr double kPerTile = 30.0;
+
+static int64_t workgroups_of(int64_t batch, int kv_heads, int group, int64_t max_new) { return batch * kv_heads * ceil_div(max_new * group, kCols); }
+
+// What the launch has room for, from the longest row that the tables hold; each row's own number is parts_of its tiles.
 static int splits_of(int64_t batch, int kv_heads, int group, int64_t max_new, int64_t max_tokens) {
-  const int64_t wgs = batch * kv_heads * ceil_div(max_new * group, kCols);
+  const int64_t wgs = workgroups_of(batch, kv_heads, group, max_new);
   const int64_t tiles = ceil_div(std::max<int64_t>(max_tokens, 1), kTile);
   if (wgs >= 256) return 1;
-  const int64_t best = static_cast<int64_t>(std::sqrt(30.0 * static_cast<double>(tiles) / static_cast<double>(wgs)));
+  const int64_t best = static_cast<int64_t>(std::sqrt(kPerTile * static_cast<double>(tiles) / static_cast<double>(wgs)));
   return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({kMaxSplits, 256 / wgs, tiles, best})));
 }
 
@@ -702,6 +723,7 @@ extern "C" int qa_paged_attention_prefill_kv4(const void* query, int32_t q_dtype
   p.c.prefix = prefix_lens;
   p.c.total = total_new;
   p.splits = splits_of(batch, kv->kv_heads, p.c.G, max_new, max_blocks * block_size);
+  p.per_tile = static_cast<float>(kPerTile / static_cast<double>(workgroups_of(batch, kv->kv_heads, p.c.G, max_new)));
   const int64_t need = workspace_of(p.splits, total_new, heads, head_dim);
   QA_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 15u) == 0),
              "paged prefill workspace too small or not 16-byte aligned: need %lld bytes, have %lld", static_cast<long long>(need), static_cast<long long>(workspace_bytes));

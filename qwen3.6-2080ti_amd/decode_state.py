@@ -408,9 +408,7 @@ class DeviceBatchPageTables:
 
     def plan_prefill(self, rows: Sequence[int], counts: Sequence[int]) -> "PrefillStep":
         """:meth:`reserve_prefill` with the slot map, for the layers that write by slot.  The step's tokens are packed in
-        row order, so ``rows`` must be ascending.  ``cu_seqlens``, ``starts`` and ``block_tables`` of the record have an
-        entry for every row of the tables, the ones not in the step without tokens; ``block_tables`` is the running
-        batch's own, so the step's layers run before the next reservation."""
+        row order, so ``rows`` must be ascending."""
         import torch
 
         rows, counts = self._step_rows(rows, counts, "plan_prefill")
@@ -420,11 +418,14 @@ class DeviceBatchPageTables:
         for r, c in zip(rows, counts):
             full[r] = c
         device = self.block_tables.device
+        index = torch.tensor(rows, dtype=torch.int64, device=device)
         plan = self.allocator.plan(self.block_tables, self.sequence_lengths, self.block_size, counts=torch.tensor(full, dtype=torch.int32, device=device), max_tokens=sum(counts))
         self.allocator.check()
         return PrefillStep(
-            rows=tuple(rows), counts=tuple(counts), index=torch.tensor(rows, dtype=torch.int64, device=device),
-            cu_seqlens=plan.cu_seqlens, starts=plan.starts, block_tables=self.block_tables,
+            rows=tuple(rows), counts=tuple(counts), index=index,
+            # rows without tokens take no part, so the last row's end is the total
+            cu_seqlens=torch.cat([plan.cu_seqlens.index_select(0, index), plan.cu_seqlens[-1:]]),
+            starts=plan.starts.index_select(0, index), block_tables=self.block_tables.index_select(0, index),
             max_new=max(counts), total_tokens=sum(counts), block_size=self.block_size, plan=plan,
         )
 

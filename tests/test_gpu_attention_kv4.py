@@ -202,9 +202,9 @@ def test_empty_batch() -> None:
 # --------------------------------------------------------------------------- prefill
 
 
-def _check_prefill(seed, new, prefix, heads, kv_heads, dim, block, index=torch.int32, gated=True, holes=False, pad=0, scale=None):
+def _check_prefill(seed, new, prefix, heads, kv_heads, dim, block, index=torch.int32, gated=True, holes=False, pad=0, scale=None, width=None):
     gen = torch.Generator().manual_seed(seed)
-    tables, pools = _cache(gen, [n + p for n, p in zip(new, prefix)], kv_heads, dim, block, index)
+    tables, pools = _cache(gen, [n + p for n, p in zip(new, prefix)], kv_heads, dim, block, index, width)
     if holes:
         tables[:, 0] = -1
         if tables.shape[1] > 3:
@@ -375,3 +375,10 @@ def test_decode_of_more_row_groups_than_take_a_workgroup_each() -> None:
     lens = [rng.choice((0, 1, 16, 40)) for _ in range(2100)]
     for width in (None, 70):
         _check_decode(24, lens, 4, 2, 128, 16, width=width)
+
+
+@pytest.mark.parametrize("new,prefix", [([200], [0]), ([3, 16, 40, 0, 1], [0, 5000, 700, 9, 300]), ([130, 2], [400, 0]), ([1], [0])])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 1, 256), (6, 1, 128), (16, 2, 256)])
+def test_prefill_with_tables_much_wider_than_the_rows(new, prefix, heads, kv_heads, dim) -> None:
+    """The launch has room for many parts; the columns of a row are split by what they see."""
+    _check_prefill(26, new, prefix, heads, kv_heads, dim, 16, width=3000, pad=3, holes=kv_heads == 2)
