@@ -38,8 +38,9 @@ constexpr int kUnit = 32;  // tokens
 // longer one, the second launch is left out.  us split / by row, 2 KV heads of 256: 4 rows of 512 12.1 / 9.1, of 1024 12.4 /
 // 13.3, of 2048 12.2 / 19.4; 64 rows of up to 1024 25.5 / 14.1, of up to 4096 34.5 / 36.3; 200 rows of 500 37.7 / 22.0.
 constexpr int kByRowTokens = 1024;
-// Row groups up to which a call of long tables has the workgroups for that; each of them reads all the lengths first.
-constexpr int kByRowGroups = 4096;
+// Row groups up to which a call of long tables has the workgroups for that; each of them reads all the lengths first.  us
+// split / by row, rows of 300, 2 KV heads: 200 rows 36 / 23, 500 68 / 51, 1000 122 / 116, 2000 229 / 291.
+constexpr int kByRowGroups = 2048;
 constexpr int kMaxWgs = 256;  // one per CU: eight waves of up to 256 registers fill it
 
 // Tokens and units of row b (0 for rows of length <= 0); lengths past the table stop at it.
