@@ -1131,7 +1131,8 @@ def _rows(tensor: torch.Tensor, multiple: int) -> tuple[torch.Tensor, int, int]:
     strides = tensor.stride()
     if strides[-1] == 1 and strides[0] % multiple == 0 and strides[1] % multiple == 0 and tensor.data_ptr() % (multiple * tensor.element_size()) == 0:
         return tensor, strides[0], strides[1]
-    tensor = tensor.contiguous()
+    # not .contiguous(): it gives back a contiguous tensor at an odd address, or a single row of an odd stride, as it is
+    tensor = tensor.clone(memory_format=torch.contiguous_format)
     strides = tensor.stride()
     return tensor, strides[0], strides[1]
 
