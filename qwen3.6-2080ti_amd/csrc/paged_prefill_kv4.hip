@@ -35,10 +35,11 @@ using namespace attn4;
 
 struct PrefillParams {
   Params c;
-  int splits;      // parts of the keys that the launch has workgroups for
-  float per_tile;  // kPerTile / workgroups
-  float* part_o;   // (splits, total, H, D)
-  float* part_ml;  // (splits, total, H, 2)
+  int64_t max_new;  // tokens of a row that are computed
+  int splits;       // parts of the keys that the launch has workgroups for
+  float per_tile;   // kPerTile / workgroups
+  float* part_o;    // (splits, total, H, D)
+  float* part_ml;   // (splits, total, H, 2)
 };
 
 constexpr int kTile = 64;      // keys
@@ -140,7 +141,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams p
     tok1 = read_index(p.cu, p.idx_i64, b + 1);
     prefix = read_index(p.prefix, p.idx_i64, b);
   }
-  const int64_t n_new = min64(tok1, p.total) - tok0;
+  const int64_t n_new = min64(pp.max_new, min64(tok1, p.total) - tok0);
   const int64_t ct0 = static_cast<int64_t>(gridDim.x) - 1 - blockIdx.x;
   const int64_t x0 = ct0 * kCols;  // first column of the workgroup
   if (tok0 < 0 || x0 >= n_new * p.G) return;
@@ -606,7 +607,7 @@ constexpr int kJoinAhead = 8;  // parts asked for at a time
 
 // Joins the parts of one (token, head): a wave each, lane l dims l D/64 ..
 template <int D>
-__global__ __launch_bounds__(256) void join_kernel(PrefillParams pp, int64_t max_new) {
+__global__ __launch_bounds__(256) void join_kernel(PrefillParams pp) {
   const Params& p = pp.c;
   constexpr int E = D / 64;
   typedef float vec_t __attribute__((ext_vector_type(E)));
@@ -614,12 +615,12 @@ __global__ __launch_bounds__(256) void join_kernel(PrefillParams pp, int64_t max
   const int64_t x = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int b = blockIdx.y;
   const int64_t tok0 = read_index(p.cu, p.idx_i64, b);
-  const int64_t n_new = min64(max_new, min64(read_index(p.cu, p.idx_i64, b + 1), p.total) - tok0);
+  const int64_t n_new = min64(pp.max_new, min64(read_index(p.cu, p.idx_i64, b + 1), p.total) - tok0);
   if (tok0 < 0 || x >= n_new * p.H) return;
   const uint32_t n = static_cast<uint32_t>(x) / static_cast<uint32_t>(p.H), h = static_cast<uint32_t>(x) - n * static_cast<uint32_t>(p.H);
   // the workgroups that had this column
   const int64_t column = static_cast<int64_t>(n) * p.G + (h - over_group(p, h) * static_cast<uint32_t>(p.G));
-  const int64_t last = min64((min64(read_index(p.cu, p.idx_i64, b + 1), p.total) - tok0) * p.G, column / kCols * kCols + kCols) - 1;
+  const int64_t last = min64(n_new * p.G, column / kCols * kCols + kCols) - 1;
   const int parts = parts_of(pp, (keys_of(p, read_index(p.prefix, p.idx_i64, b), last) + kTile - 1) / kTile);
   if (parts == 1) return;  // written by the workgroup itself
   const int64_t row = tok0 * p.H + x;
@@ -678,7 +679,7 @@ static int64_t workspace_of(int splits, int64_t total, int heads, int head_dim) 
 }
 
 template <int D>
-static int launch(const PrefillParams& p, dim3 grid, int64_t max_new, hipStream_t stream) {
+static int launch(const PrefillParams& p, dim3 grid, hipStream_t stream) {
   if (int rc = reserve_lds<&prefill_kernel<D>>("paged_attention_prefill_kv4", Smem<D>::kBytes)) return rc;
   {
     KernelTimer timer_("prefill_kv4", stream);
@@ -687,8 +688,8 @@ static int launch(const PrefillParams& p, dim3 grid, int64_t max_new, hipStream_
   if (int rc = check_launch("paged_attention_prefill_kv4")) return rc;
   if (p.splits > 1) {
     KernelTimer timer_("prefill_kv4_join", stream);
-    const dim3 jgrid(static_cast<unsigned>(ceil_div(max_new * p.c.H, 4)), static_cast<unsigned>(p.c.B));
-    hipLaunchKernelGGL(join_kernel<D>, jgrid, dim3(256), 0, stream, p, max_new);
+    const dim3 jgrid(static_cast<unsigned>(ceil_div(p.max_new * p.c.H, 4)), static_cast<unsigned>(p.c.B));
+    hipLaunchKernelGGL(join_kernel<D>, jgrid, dim3(256), 0, stream, p);
   }
   return check_launch("paged_attention_prefill_kv4");
 }
@@ -722,6 +723,7 @@ extern "C" int qa_paged_attention_prefill_kv4(const void* query, int32_t q_dtype
   p.c.cu = cu_seqlens;
   p.c.prefix = prefix_lens;
   p.c.total = total_new;
+  p.max_new = max_new;
   p.splits = splits_of(batch, kv->kv_heads, p.c.G, max_new, max_blocks * block_size);
   p.per_tile = static_cast<float>(kPerTile / static_cast<double>(workgroups_of(batch, kv->kv_heads, p.c.G, max_new)));
   const int64_t need = workspace_of(p.splits, total_new, heads, head_dim);
@@ -730,5 +732,5 @@ extern "C" int qa_paged_attention_prefill_kv4(const void* query, int32_t q_dtype
   p.part_o = reinterpret_cast<float*>(workspace);
   p.part_ml = p.part_o + static_cast<int64_t>(p.splits) * total_new * heads * head_dim;
   const dim3 grid(static_cast<unsigned>(ceil_div(max_new * p.c.G, kCols)), static_cast<unsigned>(batch * kv->kv_heads), static_cast<unsigned>(p.splits));
-  return head_dim == 256 ? launch<256>(p, grid, max_new, stream) : launch<128>(p, grid, max_new, stream);
+  return head_dim == 256 ? launch<256>(p, grid, stream) : launch<128>(p, grid, stream);
 }
