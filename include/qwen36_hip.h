@@ -330,7 +330,8 @@ int qa_paged_attention_decode_kv4(const void* query, int32_t q_dtype, int64_t q_
  * computed, and output rows past the last sequence are left as they were.
  * workspace: 16-byte aligned, qa_paged_attention_prefill_kv4_workspace(..,
  * max_blocks * block_size) bytes (0 for steps that fill the GPU by themselves;
- * then it may be NULL): the parts of a split of the keys.                      */
+ * then it may be NULL): the parts of a split of the keys, of at most
+ * min(total_new, batch * max_new) tokens and below 35 MB.                     */
 int64_t qa_paged_attention_prefill_kv4_workspace(int64_t total_new, int64_t batch, int64_t max_new, int32_t heads, int32_t kv_heads,
                                                  int32_t head_dim, int64_t max_tokens);
 int qa_paged_attention_prefill_kv4(const void* query, int32_t q_dtype, int64_t q_stride_t, int64_t q_stride_h, int64_t total_new,

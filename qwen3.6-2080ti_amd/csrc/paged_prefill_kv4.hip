@@ -38,8 +38,10 @@ struct PrefillParams {
   int64_t max_new;  // tokens of a row that are computed
   int splits;       // parts of the keys that the launch has workgroups for
   float per_tile;   // kPerTile / workgroups
-  float* part_o;    // (splits, total, H, D)
-  float* part_ml;   // (splits, total, H, 2)
+  int64_t part_tokens;  // tokens that the partial results have room for
+  int64_t per_row;      // 0: a token's are where its query is; else row b's begin at b per_row (a padded query)
+  float* part_o;        // (splits, part_tokens, H, D)
+  float* part_ml;       // (splits, part_tokens, H, 2)
 };
 
 constexpr int kTile = 64;      // keys
@@ -56,6 +58,10 @@ template <typename P>
 __device__ __forceinline__ int64_t keys_of(const P& p, int64_t prefix, int64_t last) {
   return max64(0, min64(prefix + over_group(p, static_cast<uint32_t>(last)) + 1, p.max_blocks << p.bs_shift));
 }
+
+// Where the partial results of row b begin, its first token being tok0.
+template <typename P>
+__device__ __forceinline__ int64_t part_base(const P& pp, int64_t b, int64_t tok0) { return pp.per_row != 0 ? b * pp.per_row : tok0; }
 
 // Parts that `tiles` tiles are split into, the same in both launches: the tables may be much wider than the row.
 template <typename P>
@@ -578,7 +584,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams p
       const uint32_t row = pl.token * static_cast<uint32_t>(late->c.H) + pl.head;  // past row0
       const float l = s_l[x];
       if (parts > 1) {
-        const int64_t part = blockIdx.z * late->c.total * late->c.H + row0 + row;
+        const int64_t part = (blockIdx.z * late->part_tokens + part_base(*late, b, tok0) - tok0) * late->c.H + row0 + row;
         if (in_row == 0) *reinterpret_cast<float2*>(late->part_ml + part * 2) = make_float2(s_l[kWaves * 16 + x], l);
 #pragma unroll
         for (int k = 0; k < 2; ++k)
@@ -623,8 +629,8 @@ __global__ __launch_bounds__(256) void join_kernel(PrefillParams pp) {
   const int64_t last = min64(n_new * p.G, column / kCols * kCols + kCols) - 1;
   const int parts = parts_of(pp, (keys_of(p, read_index(p.prefix, p.idx_i64, b), last) + kTile - 1) / kTile);
   if (parts == 1) return;  // written by the workgroup itself
-  const int64_t row = tok0 * p.H + x;
-  const int64_t stride = p.total * p.H;
+  const int64_t row = part_base(pp, b, tok0) * p.H + x;
+  const int64_t stride = pp.part_tokens * p.H;
   const float2 ml = lane < parts ? *reinterpret_cast<const float2*>(pp.part_ml + (lane * stride + row) * 2) : make_float2(-INFINITY, 0.f);
   const float m = wave_max(ml.x);
   const float f = __builtin_amdgcn_exp2f(ml.x - (m == -INFINITY ? 0.f : m));
@@ -653,7 +659,7 @@ __global__ __launch_bounds__(256) void join_kernel(PrefillParams pp) {
     }
     out[e / 2] = static_cast<uint32_t>(f32_to_bf16(lo)) | static_cast<uint32_t>(f32_to_bf16(hi)) << 16;
   }
-  *reinterpret_cast<packed_t*>(p.out + row * D + E * lane) = out;
+  *reinterpret_cast<packed_t*>(p.out + (tok0 * p.H + x) * D + E * lane) = out;
 }
 
 // Parts the keys are split into where the workgroups leave CUs free.  A part saves a share of 1.5 us a tile and costs its
@@ -674,8 +680,12 @@ static int splits_of(int64_t batch, int kv_heads, int group, int64_t max_new, in
   return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({kMaxSplits, 256 / wgs, tiles, best})));
 }
 
-static int64_t workspace_of(int splits, int64_t total, int heads, int head_dim) {
-  return splits > 1 ? splits * total * heads * (static_cast<int64_t>(head_dim) + 2) * 4 : 0;
+// Tokens that partial results are kept of: a query padded past its rows' bound is no reason for more.  With splits of at most
+// 256 / workgroups and a workgroup per 128 columns they are below 35 MB at any padding and any width of the tables.
+static int64_t part_tokens_of(int64_t total, int64_t batch, int64_t max_new) { return std::min(total, batch * max_new); }
+
+static int64_t workspace_of(int splits, int64_t part_tokens, int heads, int head_dim) {
+  return splits > 1 ? splits * part_tokens * heads * (static_cast<int64_t>(head_dim) + 2) * 4 : 0;
 }
 
 template <int D>
@@ -700,7 +710,9 @@ static int launch(const PrefillParams& p, dim3 grid, hipStream_t stream) {
 extern "C" int64_t qa_paged_attention_prefill_kv4_workspace(int64_t total_new, int64_t batch, int64_t max_new, int32_t heads, int32_t kv_heads, int32_t head_dim,
                                                             int64_t max_tokens) {
   if (total_new <= 0 || batch <= 0 || max_new <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 || head_dim <= 0 || max_tokens < 0) return 0;
-  return qa::prefill4::workspace_of(qa::prefill4::splits_of(batch, kv_heads, heads / kv_heads, std::min(max_new, total_new), max_tokens), total_new, heads, head_dim);
+  max_new = std::min(max_new, total_new);
+  return qa::prefill4::workspace_of(qa::prefill4::splits_of(batch, kv_heads, heads / kv_heads, max_new, max_tokens),
+                                    qa::prefill4::part_tokens_of(total_new, batch, max_new), heads, head_dim);
 }
 
 extern "C" int qa_paged_attention_prefill_kv4(const void* query, int32_t q_dtype, int64_t q_stride_t, int64_t q_stride_h, int64_t total_new, const void* cu_seqlens,
@@ -726,11 +738,13 @@ extern "C" int qa_paged_attention_prefill_kv4(const void* query, int32_t q_dtype
   p.max_new = max_new;
   p.splits = splits_of(batch, kv->kv_heads, p.c.G, max_new, max_blocks * block_size);
   p.per_tile = static_cast<float>(kPerTile / static_cast<double>(workgroups_of(batch, kv->kv_heads, p.c.G, max_new)));
-  const int64_t need = workspace_of(p.splits, total_new, heads, head_dim);
+  p.part_tokens = part_tokens_of(total_new, batch, max_new);
+  p.per_row = p.part_tokens < total_new ? max_new : 0;
+  const int64_t need = workspace_of(p.splits, p.part_tokens, heads, head_dim);
   QA_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 15u) == 0),
              "paged prefill workspace too small or not 16-byte aligned: need %lld bytes, have %lld", static_cast<long long>(need), static_cast<long long>(workspace_bytes));
   p.part_o = reinterpret_cast<float*>(workspace);
-  p.part_ml = p.part_o + static_cast<int64_t>(p.splits) * total_new * heads * head_dim;
+  p.part_ml = p.part_o + static_cast<int64_t>(p.splits) * p.part_tokens * heads * head_dim;
   const dim3 grid(static_cast<unsigned>(ceil_div(max_new * p.c.G, kCols)), static_cast<unsigned>(batch * kv->kv_heads), static_cast<unsigned>(p.splits));
   return head_dim == 256 ? launch<256>(p, grid, stream) : launch<128>(p, grid, stream);
 }

@@ -40,3 +40,10 @@ def _check(seed, new, prefix, max_new, heads, kv_heads, dim, block, width, padde
 @pytest.mark.parametrize("max_new", [1, 5, 33])
 def test_tokens_past_max_new_are_not_written(heads, kv_heads, dim, width, max_new) -> None:
     _check(heads + max_new, [40, 3, 0, 20, 90], [5, 700, 9, 0, 130], max_new, heads, kv_heads, dim, 16, width)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(16, 2, 256), (9, 1, 128)])
+@pytest.mark.parametrize("new,prefix,max_new", [([16], [3000], 16), ([3, 17, 0, 9], [900, 0, 5, 2500], 17), ([3, 17, 0, 9], [900, 0, 5, 2500], 6)])
+def test_a_step_in_a_padded_query(heads, kv_heads, dim, new, prefix, max_new) -> None:
+    """The keys are split; the partial results lie by row and not by the query's row."""
+    _check(heads + max_new, new, prefix, max_new, heads, kv_heads, dim, 16, 2000, padded=4096, index=torch.int64)
