@@ -354,7 +354,8 @@ def full_attention_decode_device(
     workspace.  Nothing here reads back to the host or copies host to device.
 
     On a 4-bit pool the step is reserved by ``plan = tables.plan_step()`` in place of
-    ``reserve_step``, and its K/V are written to the plan's slots; ``no_alloc`` is for bf16 pools.
+    ``reserve_step``, its K/V are written to the plan's slots and its lengths are the plan's: a
+    refused step writes nothing and gives zeros.  ``no_alloc`` is for bf16 pools.
     """
     reason = _device_pool_reason(config, query, key_blocks, value_blocks, tables)
     kv4 = is_kv4(key_blocks)
@@ -371,11 +372,12 @@ def full_attention_decode_device(
     with runtime.profile_scope("batch.full_attention.native_paged_device"):
         if kv4:
             hip_ops.paged_kv4_append(key[:, :, 0], value[:, :, 0], key_blocks, value_blocks, plan.slots, tables.block_size)
-            decode = hip_ops.paged_attention_decode_kv4
+            decode, lengths = hip_ops.paged_attention_decode_kv4, _step_lengths(plan)
         else:
             tables.append(key, value, key_blocks, value_blocks)
             decode = hip_ops.paged_attention_decode_batched_noalloc if no_alloc else hip_ops.paged_attention_decode_batched
-        heads = decode(query, tables.block_tables, key_blocks, value_blocks, tables.sequence_lengths, tables.block_size)
+            lengths = tables.sequence_lengths
+        heads = decode(query, tables.block_tables, key_blocks, value_blocks, lengths, tables.block_size)
     record_native_paged_dispatch(runtime, reason, native=True)
     return heads if gate is None else _gate_heads(heads, gate)
 
@@ -406,6 +408,12 @@ def _check_step(by_slots: bool, plan: Any | None, no_alloc: bool, tables: Device
         raise ValueError("a 4-bit pool or mrope_section needs the step's plan (tables.plan_step())")
     if no_alloc:
         raise ValueError("no_alloc is for bf16 pools: the 4-bit decode takes its workspace per call")
+
+
+def _step_lengths(plan: Any) -> Any:
+    """The lengths that the attention of a planned step reads (``hip_ops.PagedStepPlan``, or a plain plan of one entry a row)."""
+    lengths = getattr(plan, "lengths", None)
+    return plan.positions + 1 if lengths is None else lengths
 
 
 def _check_positions(by_slots: bool, positions: Any | None) -> None:
@@ -478,6 +486,7 @@ def full_attention_decode_step_device(
     With a 4-bit pool (``SharedKV4BlockPool``) or ``rope.mrope_section`` the step is reserved by
     ``plan = tables.plan_step()`` in place of ``reserve_step``; ``positions`` ``(axes, rows)`` then
     gives each row's rotary positions (its place in the row on every axis where omitted: text).
+    A refused step writes nothing and gives zeros; ``tables.check()`` tells.
     On a 4-bit pool the gate is applied inside the decode and ``no_alloc`` is refused.
     """
     rows = int(q_proj.shape[0])
@@ -506,14 +515,14 @@ def full_attention_decode_step_device(
             cu = _row_offsets(rows, q_proj.device)
             query, gate = _qk_norm_rope(q_proj, k_proj, v_proj, q_norm_weight, k_norm_weight, key_blocks, value_blocks, tables.block_tables,
                                         cu, tables.positions, tables.block_size, 1, rope)
+        lengths = _step_lengths(plan) if by_slots else tables.sequence_lengths
         if kv4:
-            out = hip_ops.paged_attention_decode_kv4(query.view(rows, heads, 1, head_dim), tables.block_tables, key_blocks, value_blocks, tables.sequence_lengths,
+            out = hip_ops.paged_attention_decode_kv4(query.view(rows, heads, 1, head_dim), tables.block_tables, key_blocks, value_blocks, lengths,
                                                      tables.block_size, gate=gate if full.output_gate else None)
             record_native_paged_dispatch(runtime, reason, native=True)
             return out.view(rows, 1, heads * head_dim)
         decode = hip_ops.paged_attention_decode_batched_noalloc if no_alloc else hip_ops.paged_attention_decode_batched
-        heads_out = decode(query.view(rows, heads, 1, head_dim), tables.block_tables, key_blocks, value_blocks, tables.sequence_lengths,
-                           tables.block_size)
+        heads_out = decode(query.view(rows, heads, 1, head_dim), tables.block_tables, key_blocks, value_blocks, lengths, tables.block_size)
     record_native_paged_dispatch(runtime, reason, native=True)
     if not full.output_gate:
         return heads_out.view(rows, 1, heads * head_dim)

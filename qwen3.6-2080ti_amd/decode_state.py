@@ -399,10 +399,14 @@ class DeviceBatchPageTables:
 
     def plan_step(self) -> Any:
         """:meth:`reserve_step` with the slot map of the step's tokens, for the layers that write by slot (4-bit pools,
-        rotary positions of several axes): a ``hip_ops.PagedPlan`` whose ``positions`` and ``slots`` have one entry for
+        rotary positions of several axes): a ``hip_ops.PagedStepPlan`` whose ``positions`` and ``slots`` have one entry for
         every row (-1 where it holds no request).  Leaves the append positions in ``positions`` and is device only, like
-        ``reserve_step``."""
-        plan = self.allocator.plan(self.block_tables, self.sequence_lengths, self.block_size, counts=self.step_counts, max_tokens=self.rows, per_row=1)
+        ``reserve_step``.  A step that does not fit takes nothing: its layers write nothing and give zeros, and ``check``
+        raises until the next plan overwrites the status, so it belongs after every step."""
+        import hip_ops
+
+        plan = hip_ops.PagedStepPlan.of(self.allocator.plan(
+            self.block_tables, self.sequence_lengths, self.block_size, counts=self.step_counts, max_tokens=self.rows, per_row=1))
         self.positions.copy_(plan.starts)
         return plan
 

@@ -1170,6 +1170,20 @@ class PagedPlan(NamedTuple):
     slots: torch.Tensor
 
 
+class PagedStepPlan(PagedPlan):
+    """The plan of a decode step, one entry a row (``DeviceBatchPageTables.plan_step``).  ``lengths`` ``(B,)`` int32 are
+    what the step's attention reads: a row's tokens with its new one, 0 where it takes none, so that a row without a
+    request, and every row of a step that was refused, gives zeros."""
+
+    lengths: torch.Tensor
+
+    @classmethod
+    def of(cls, plan: PagedPlan) -> "PagedStepPlan":
+        step = cls(*plan)
+        step.lengths = plan.positions + 1  # -1 where there is no new token
+        return step
+
+
 def paged_kv_plan(
     block_tables: torch.Tensor,
     lengths: torch.Tensor,
@@ -1191,8 +1205,10 @@ def paged_kv_plan(
     :func:`paged_attention_prefill_kv4`.  ``max_tokens`` bounds the step (the host need not know its size), and the
     token arrays are that long.  ``status`` (int32 ``[1]``) becomes 0, or 1 (pool exhausted), 2 (a table row too
     short), 3 (corrupt free state), 4 (negative or overflowing length or count), 5 (more than ``max_tokens``
-    tokens): then nothing is taken and the plan is empty, so that the operators fed by it do nothing.  Nothing is
-    read back, so the call can be captured in a HIP graph.
+    tokens): then nothing is taken and the plan is empty.  Operators fed by its slots and ``cu_seqlens`` write nothing
+    to the pool and compute no token; a decode takes ``positions + 1`` as its lengths (``lengths`` are the rows' old
+    ones) and gives zeros.  The next plan overwrites ``status``, so it has to be read before that.  Nothing is read
+    back here, so the call can be captured in a HIP graph.
 
     With ``per_row`` the token arrays are not packed but hold ``per_row`` entries for each row (``max_tokens`` is
     ``B * per_row``), a row's tokens first and -1 behind them: the form of a decode step, whose operators take one
