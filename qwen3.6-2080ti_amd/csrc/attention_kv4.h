@@ -296,6 +296,7 @@ struct Args {
   const void* query;
   int32_t q_dtype;
   int64_t q_st, q_sh;
+  int64_t q_rows;
   int64_t batch;
   int32_t heads, head_dim;
   const qa_paged_kv* kv;
@@ -317,7 +318,7 @@ inline int fill(Params& p, const Args& a) {
   QA_REQUIRE(a.heads > 0 && a.heads % a.kv->kv_heads == 0, "%s: query heads (%d) must be a multiple of KV heads (%d)", a.what, a.heads, a.kv->kv_heads);
   QA_REQUIRE(a.heads / a.kv->kv_heads <= 16, "%s: GQA group size %d is larger than 16", a.what, a.heads / a.kv->kv_heads);
   QA_REQUIRE(a.max_blocks > 0 && a.max_blocks <= 0x7fffffff && a.table_stride >= 0, "%s: block table must have at least one entry", a.what);
-  if (a.batch > 0) QA_REQUIRE(a.query && a.out && a.tables, "%s: pointers must be non-null", a.what);
+  if (a.batch > 0 && a.q_rows > 0) QA_REQUIRE(a.query && a.out && a.tables, "%s: pointers must be non-null", a.what);
   QA_REQUIRE(((reinterpret_cast<uintptr_t>(a.query) | reinterpret_cast<uintptr_t>(a.out)) & 15u) == 0 && a.q_st % 8 == 0 && a.q_sh % 8 == 0,
              "%s: query rows must be 16-byte aligned", a.what);
   QA_REQUIRE(a.gate == nullptr || ((reinterpret_cast<uintptr_t>(a.gate) & 7u) == 0 && a.gate_st % 4 == 0 && a.gate_sh % 4 == 0), "%s: gate rows must be 8-byte aligned", a.what);

@@ -222,7 +222,7 @@ extern "C" int qa_paged_kv4_gather(const qa_paged_kv* kv, int32_t head_dim, int6
   using namespace qa;
   using namespace qa::kv4;
   if (int rc = check_pool("paged_kv4_gather", kv, head_dim, block_size)) return rc;
-  QA_REQUIRE(block_tables != nullptr && is_index_dtype(table_dtype), "block table must be an int32/int64 device array");
+  QA_REQUIRE((block_tables != nullptr || batch == 0) && is_index_dtype(table_dtype), "block table must be an int32/int64 device array");
   QA_REQUIRE(batch >= 0 && batch <= 65535, "paged_kv4_gather: batch must be in [0, 65535]");
   QA_REQUIRE(max_blocks > 0 && table_stride >= 0, "paged_kv4_gather: max_blocks must be positive");
   QA_REQUIRE(valid >= 0 && valid <= 0x7fffffff, "paged_kv4_gather: valid out of range");

@@ -606,7 +606,7 @@ extern "C" int qa_paged_attention_decode_kv4(const void* query, int32_t q_dtype,
   using namespace qa;
   using namespace qa::attn4;
   DecodeParams p{};
-  const Args a{"paged_attention_decode_kv4", query, q_dtype, q_stride_b, q_stride_h, batch, heads, head_dim, kv, block_tables, table_dtype, table_stride, max_blocks,
+  const Args a{"paged_attention_decode_kv4", query, q_dtype, q_stride_b, q_stride_h, batch, batch, heads, head_dim, kv, block_tables, table_dtype, table_stride, max_blocks,
                lengths_dtype, block_size, scale, gate, gate_stride_b, gate_stride_h, output};
   if (int rc = fill(p.c, a)) return rc;
   if (batch == 0) return 0;

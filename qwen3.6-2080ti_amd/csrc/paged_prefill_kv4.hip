@@ -726,7 +726,7 @@ extern "C" int qa_paged_attention_prefill_kv4(const void* query, int32_t q_dtype
   using namespace qa;
   using namespace qa::prefill4;
   PrefillParams p{};
-  const Args a{"paged_attention_prefill_kv4", query, q_dtype, q_stride_t, q_stride_h, batch, heads, head_dim, kv, block_tables, table_dtype, table_stride, max_blocks,
+  const Args a{"paged_attention_prefill_kv4", query, q_dtype, q_stride_t, q_stride_h, total_new, batch, heads, head_dim, kv, block_tables, table_dtype, table_stride, max_blocks,
                idx_dtype, block_size, scale, gate, gate_stride_t, gate_stride_h, output};
   if (int rc = fill(p.c, a)) return rc;
   QA_REQUIRE(total_new >= 0 && total_new <= 0x7fffffff && max_new >= 0 && max_new <= 0x7fffffff, "%s: token counts out of range", a.what);

@@ -1477,9 +1477,10 @@ def qk_norm_mrope_kv_append(
     to bf16 once; angles are exact at any position.  ``sum(sections)`` is a multiple of ``D / 64``.
 
     ``q_proj`` ``(tokens, H, 2D)`` (query and gate halves) or ``(tokens, H, D)``, ``k_proj``/``v_proj`` ``(tokens,
-    H_kv, D)``, or flat in their last two dims, bf16.  k and v go to ``slots`` (:func:`paged_kv_plan`; those outside the
-    pool are skipped, the others have to be distinct) of a bf16 pool ``(P, H_kv, bs, D)`` or a 4-bit one ``(P, H_kv,
-    kv4_tile_bytes(D, bs))``; the latter then holds what :func:`paged_kv4_append` makes of the bf16 k and v.  Returns
+    H_kv, D)``, bf16, rows aligned to ``D / 64`` elements.  Flat in the last two dims, ``q_proj`` is the form with the
+    gate, ``(tokens, H*2D)``.  k and v go to ``slots`` (:func:`paged_kv_plan`; those outside the pool are skipped, the
+    others have to be distinct) of a bf16 pool ``(P, H_kv, bs, D)`` or a 4-bit one ``(P, H_kv, kv4_tile_bytes(D, bs))``;
+    the latter then holds what :func:`paged_kv4_append` makes of the bf16 k and v.  Returns
     ``(query (tokens, H, D) bf16, gate (tokens, H, D) view of q_proj or None)``.
     """
     lib = L.load_library()
@@ -1501,7 +1502,7 @@ def qk_norm_mrope_kv_append(
     v3 = v_proj.view(tokens, kv_heads, head_dim) if v_proj.dim() == 2 else v_proj
     q3 = q_proj
     if len(q_shape) == 2 and q_shape[1] % (2 * head_dim) == 0:
-        q3 = q_proj.view(tokens, -1, 2 * head_dim)
+        q3 = q_proj.view(tokens, q_shape[1] // (2 * head_dim), 2 * head_dim)
         q_shape = q3.shape
     _require(len(q_shape) == 3 and q_shape[2] in (head_dim, 2 * head_dim), "q_proj must be (tokens, heads, head_dim or 2*head_dim) or (tokens, heads*2*head_dim)")
     heads = q_shape[1]
