@@ -170,6 +170,29 @@ def norm_mrope(x: np.ndarray, weight: np.ndarray, positions: np.ndarray, section
     return y
 
 
+def _round_to(x: np.ndarray, bits: int, least: float) -> np.ndarray:
+    """x to the nearest number of ``bits`` significant bits and no place below ``least``, ties to even."""
+    place = np.maximum(2.0 ** (np.floor(np.log2(np.maximum(np.abs(x), 1e-300))) - (bits - 1)), least)
+    return np.rint(x / place) * place
+
+
+def query_pieces(row: np.ndarray) -> tuple[np.ndarray, np.ndarray, float]:
+    """A bf16 query row (D,) as the scores take it: hi, lo and a power of two ``scale``, the row being about ``scale (hi +
+    lo / 16)``.  The largest element lies in [128, 256) over the scale; hi is E4M3 (4 bits, places down to 2^-9) of the
+    element on a grid of 2^-10 of the power of two at the largest of its eight dims as E4M3 rounds it; lo is E4M3 of 16
+    times what is left."""
+    row = np.asarray(row, dtype=np.float64)
+    top = np.abs(row).max()
+    if top == 0.0:
+        return row, row, 1.0
+    scale = 2.0 ** (math.floor(math.log2(top)) - 7)
+    y = row / scale
+    eight = np.repeat(np.abs(y).reshape(-1, 8).max(1), 8)
+    grid = 2.0 ** (np.floor(np.log2(np.maximum(_round_to(eight, 4, 2.0**-140), 1e-300))) - 10)
+    hi = _round_to(np.rint(y / grid) * grid, 4, 2.0**-9)
+    return hi, _round_to((y - hi) * 16, 4, 2.0**-9), scale
+
+
 def attention(q: np.ndarray, keys: np.ndarray, values: np.ndarray, seen: np.ndarray, scale: float) -> np.ndarray:
     """One query head (D,) over keys/values (T, D) where seen (T,) holds; zeros where it sees nothing."""
     if not seen.any():

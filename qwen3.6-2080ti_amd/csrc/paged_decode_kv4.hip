@@ -280,11 +280,14 @@ __global__ __launch_bounds__(64 * kWaves, 2) void decode_kernel(DecodeParams dp)
       }
       const uint32_t byte = query_scale(wave_max_bits(top));
       const float inv = __uint_as_float((254u - byte) << 23);
+      uint32_t near = max(top, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(top), 0xB1, 0xF, 0xF, false)));  // of the eight dims: quad_perm [1,0,3,2]
+      if constexpr (E == 2) near = max(near, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(near), 0x4E, 0xF, 0xF, false)));  // quad_perm [2,3,0,1]
+      const float grid = piece_grid(near, inv);
       uint32_t hi8 = 0, lo8 = 0;
 #pragma unroll
       for (int e = 0; e < E; e += 2) {
         const float y0 = x[e] * inv, y1 = x[e + 1] * inv;
-        const uint32_t h2 = __builtin_amdgcn_cvt_pk_fp8_f32(y0, y1, 0, false);
+        const uint32_t h2 = __builtin_amdgcn_cvt_pk_fp8_f32(y0 + grid - grid, y1 + grid - grid, 0, false);
         const floatx2_v a = __builtin_amdgcn_cvt_pk_f32_fp8(h2, false);
         const uint32_t l2 = __builtin_amdgcn_cvt_pk_fp8_f32((y0 - a[0]) * 16.f, (y1 - a[1]) * 16.f, 0, false);
         hi8 |= (h2 & 0xffffu) << (8 * e);
