@@ -349,7 +349,9 @@ int qa_paged_attention_prefill_kv4(const void* query, int32_t q_dtype, int64_t q
  * fp32 throughout, rounded to bf16 once (k, then its 4-bit form where the pool
  * is one).  Tokens whose slot is outside the pool write no k and v; slots must
  * be distinct.  head_dim 64, 128, 256 (4-bit pool: 128, 256).  For equal
- * positions the rotation of src/reference_ops.py:203-224.                     */
+ * positions the rotation of src/reference_ops.py:203-224, but for its roundings:
+ * there, and in qa_qk_norm_rope_append, cos, sin, the norm and both products are
+ * rounded to bf16, and q and k differ from these by up to five half steps.     */
 int qa_qk_norm_mrope_append(const void* q_proj, int64_t q_stride_t, int64_t q_stride_h, const void* k_proj, int64_t k_stride_t,
                             int64_t k_stride_h, const void* v_proj, int64_t v_stride_t, int64_t v_stride_h,
                             const void* q_norm_weight, const void* k_norm_weight, int32_t weight_dtype, float eps,

@@ -440,7 +440,9 @@ class RopeConfig:
     rope_theta: float = 10_000_000.0
     partial_rotary_factor: float = 0.25
     # rotary positions of several axes (time, row, column of a picture's tokens): how many of the frequencies each axis
-    # turns, and whether the axes take turns (hip_ops.mrope_axes).  None: one position a token.
+    # turns, and whether the axes take turns (hip_ops.mrope_axes).  None: one position a token.  With sections, and on every
+    # 4-bit pool, the prologue rounds q and k to bf16 once; without, on a bf16 pool, it rounds cos, sin, the norm and both
+    # products as the reference does, so that the same tokens' q and k differ by up to five half steps between the two.
     mrope_section: tuple[int, ...] | None = None
     mrope_interleaved: bool = False
 

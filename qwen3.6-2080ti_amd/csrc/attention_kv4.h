@@ -19,7 +19,11 @@
 // one element 300 times the others 1e-2 and 9e-4.
 // Values.  v_cvt_scalef32_pk_bf16_fp4 turns a byte into two bf16 with the token's scale applied, exactly (their scales
 // differ from token to token, so the reduction over tokens cannot take them as the product's block scales); v_perm pairs
-// the tokens; the layout of kv4.h has a lane load the operand's own dims, so nothing goes through LDS.
+// the tokens; the layout of kv4.h has a lane load the operand's own dims, so nothing goes through LDS.  The probabilities
+// are rounded to bf16 for that product (2^-8 of each at most), as in the attention over bf16 pools: the bf16 instruction
+// is the fastest that takes values of 4 bits and a scale a token exactly, and the rounding of many tokens averages out.
+// The denominators sum the probabilities before it.  A result's error against 64 bits is then 2.0e-3 to 2.3e-3 of it (root
+// mean square), 1.7e-3 being its own rounding to bf16.
 #pragma once
 
 #include "kv4.h"

@@ -4,8 +4,9 @@
 // gather the other way round.  A wave takes groups (head, 32 dims) of 16 consecutive tokens, four lanes a token and eight
 // dims a lane: loads are 64-byte pieces of rows, the group's maximum needs two quad swaps, and the 16 tokens of
 // a run land in 256 consecutive bytes of keys.  Rows that are adjacent in the source but not in the pool stay right:
-// every lane takes its own token's slot.  Three prompts of 4001 tokens, two heads of 256, 31 MB each way: append 7.8 us,
-// gather 7.5 (a launch that does nothing takes 2.5 of it, a copy of as much 6.4); five rows of one and of 334: 2.8, 3.4 us.
+// every lane takes its own token's slot.  Three prompts of 4001 tokens, two heads of 256, 31 MB each way: append 7.3 us,
+// gather 7.3 (a launch that does nothing takes 2.5 of it, a copy of as much 6.4), append of fp32 rows, 56 MB, 9.3; five rows
+// of one and of 334: 2.9, 3.6 us.
 #include "kv4.h"
 
 namespace qa {

@@ -11,7 +11,7 @@
 // A few KB move, so latency bounds it: a launch of one workgroup reads lengths, counts and state at once (with a thread a
 // row the scan that plans is also the sum that is checked), looks the tokens' rows up in LDS and writes them.  128 rows of
 // one token: 5.5 us.  From kInlineTokens on a second launch of one workgroup per kSpanTokens tokens writes them, because
-// one CU stores only a few tens of GB/s; 61 rows of up to 8192 tokens: 4.4 + 5.5 us.
+// one CU stores only a few tens of GB/s; 61 rows of up to 8192 tokens: 4.4 + 5.0 us.
 #include "qa_common.h"
 
 namespace qa {

@@ -6,8 +6,8 @@
 // that neighbouring waves read neighbouring tiles, each with an online softmax of its own and no barrier; where the
 // range leaves a row group they merge in LDS and write one partial (m, l, o) of the G heads.  A workgroup that had the
 // whole row group writes the result; the other groups' partials are merged by combine_kernel.  Where all rows are short a
-// workgroup takes a row group as it is.  64 rows of 1k to 32k tokens, two KV heads of 256: 92.7 us for 529 MB, 5.7 TB/s (a
-// pure reader reaches 6.2), and 4.7 to merge; one row of 200k, a head of 128: 11.8 + 3.9; four of 512: 9.1, all latency.
+// workgroup takes a row group as it is.  64 rows of 1k to 32k tokens, two KV heads of 256: 91.6 us for 529 MB, 5.8 TB/s (a
+// pure reader reaches 6.2), and 4.7 to merge; one row of 200k, a head of 128: 12.1 + 4.0; four of 512: 9.0, all latency.
 //
 // A wave keeps two units of keys and values in flight in registers (buffer loads of zero records for what is skipped, so
 // every step issues the same loads and the wait counts are fixed), across row groups: the merge of one and the query of
@@ -393,7 +393,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void decode_kernel(DecodeParams dp)
       for (int k = 0; k < 8; ++k) {
         const float pr = __builtin_amdgcn_exp2f(sc[k] - use);
         l_run += pr;
-        pb[k] = static_cast<__bf16>(pr);
+        pb[k] = static_cast<__bf16>(pr);  // for the bf16 product; l_run has it unrounded
       }
       // ---- values
       accumulate<D>(vr[s], pb, o);

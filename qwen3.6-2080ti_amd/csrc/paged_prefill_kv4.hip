@@ -19,9 +19,9 @@
 //
 // With few columns the keys are split over gridDim.z and a second launch joins the parts.
 //
-// Bound by the matrix and vector units together.  16 heads of 256 over 2: 2048 tokens behind 32000 865 us, 1280 TFLOP/s of
-// the two products (a large bf16 library product runs at 1210), eight chunks of 512 behind up to 8k 282 us, 1090; five
-// prompts of up to 700, 20 heads of 128 over 4, 31 us: a workgroup's start and end are 10 of them and its longest row 13.
+// Bound by the matrix and vector units together.  16 heads of 256 over 2: 2048 tokens behind 32000 856 us, 1300 TFLOP/s of
+// the two products (a large bf16 library product runs at 1210), eight chunks of 512 behind up to 8k 283 us, 1090; five
+// prompts of up to 700, 20 heads of 128 over 4, 29 us: a workgroup's start and end are 10 of them and its longest row 13.
 #include "attention_kv4.h"
 
 #include <algorithm>
@@ -426,7 +426,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams p
     auto prob = [&](int k) {
       const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[k >> 2][k & 3], qk_scale, -use));
       l_run += pr;
-      pb[k >> 3][k & 7] = static_cast<__bf16>(pr);
+      pb[k >> 3][k & 7] = static_cast<__bf16>(pr);  // for the bf16 product; l_run has it unrounded
     };
     auto publish = [&](int buf) {
       uint4* dst = reinterpret_cast<uint4*>(smem + S::kP) + (buf * kWaves + wave) * 128 + lane;

@@ -17,7 +17,8 @@
 // time, the norm is a sum over one or two rows of lanes, the partner comes by DPP on packed values, and weight times
 // cosine is formed once a token.  It needs rd / 2 a multiple of 8 and rows on 16 bytes.  heads_kernel gives a lane D / 64
 // dims and a head the whole wave, and takes what is left (head_dim 64 among it).  5003 tokens of 16 + 2 x 4 heads of 128:
-// 26.5 us there, 17.0 us here (3.6 TB/s; a copy runs at 4.8); 128 tokens of 16 + 2 x 2 heads of 256: 7.3 and 5.5 us.
+// 26.5 us there, 16.5 us here (3.7 TB/s; a copy runs at 4.8); 128 tokens of 16 + 2 x 2 heads of 256: 7.3 and 5.8 us; into
+// a 4-bit pool 15.6 and 5.5 us here.  Heads of 64, half the bytes: 20.8 us there.
 #include <algorithm>
 
 #include "kv4.h"
