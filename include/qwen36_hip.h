@@ -290,7 +290,9 @@ int qa_qk_norm_rope_append(const void* q_proj, int64_t q_stride_t, int64_t q_str
  * lengths and free_state are left as they were.  tables, lengths int32.
  * per_row: 0, or the entries that positions and slots hold for each row (then
  * max_tokens is batch * per_row, a row's tokens are the first of its entries,
- * and a row with more is status 5).
+ * and a row with more is status 5).  Of a decode step (per_row 1), positions + 1
+ * are the lengths to attend over: 0 for rows without a token and for all rows
+ * of a step that was refused.  status is written by every call.
  * workspace: 4 bytes a row.  Replaces the host-side growth and slot arithmetic
  * of src/decode_state.py:72-78,271-293,365-374.                              */
 int qa_paged_kv_plan(int32_t* block_tables, int64_t table_stride, int64_t max_blocks, int32_t* lengths,
