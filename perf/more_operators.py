@@ -6,12 +6,12 @@
 * ``pages``    ``fork``: conversations forked, their last pages copied, the parents' pages freed; ``compact``: the pages of a
   scattered cache moved to its lowest places
 
-The 8-bit cache.  A run is 16 consecutive tokens of a block and one KV head.  It is held as a scale 2^e, one byte e + 127,
-and 16 D E4M3 codes.  Of the finite values written to a run in one call, e is the least integer with max |x| <= 448 2^e,
+The 8-bit cache.  A run is 16 consecutive tokens of a block and one KV head.  It is held as 16 D E4M3 codes and a scale 2^e,
+one byte e + 127.  Of the finite values written to a run in one call, e is the least integer with max |x| <= 448 2^e,
 within [-117, 120]; x / 2^e goes to the nearest code, ties to the even one, and what is not finite becomes NaN.  Where the call
 does not write the run's first token, e is not below what the run has, and if it is above, the codes of the tokens before the
-first new one are rounded to it.  The pools are float8_e4m3fn ``(blocks, kv_heads, block_size * D + max(16, block_size /
-16))``: per block and head, the runs' codes, then their scale bytes:
+first new one are rounded to it.  The pools are float8_e4m3fn ``(blocks, kv_heads, block_size * (D + 1))``: per block and
+head, runs of 16 tokens, each first the codes, then 16 bytes, the scale's and zeros:
 
 * keys    codes  [D/64][dim / 16 % 4][token][16 dims]
 * values  codes  [D/64][token / 4][dim / 4 % 16][dim % 4][token % 4]
@@ -189,14 +189,6 @@ def _channels(gen, kv_heads, dim):
     return torch.exp(0.5 * _randn(gen, kv_heads, 1, dim, dtype=torch.float32))
 
 
-def _tail(block):
-    return max(16, block // 16)
-
-
-def _tile(case):
-    return case["block"] * case["dim"] + _tail(case["block"])
-
-
 def _least(top):
     """The byte of the least scale for a largest magnitude, fp32."""
     mant, expo = torch.frexp(top)  # top = mant 2^expo, mant in [0.5, 1); 448 2^(expo-9) = 0.875 2^expo
@@ -214,15 +206,15 @@ def _pack(x, is_key):
         codes = codes.view(n, h, bs // 16, 16, d // 64, 4, 16).permute(0, 1, 2, 4, 5, 3, 6)
     else:
         codes = codes.view(n, h, bs // 16, 4, 4, d // 64, 16, 4).permute(0, 1, 2, 5, 3, 6, 7, 4)
-    tail = torch.zeros((n, h, _tail(bs)), dtype=torch.uint8, device=x.device)
-    tail[..., : bs // 16] = byte.to(torch.uint8)
-    return torch.cat((codes.reshape(n, h, -1), tail), dim=-1)
+    tail = torch.zeros((n, h, bs // 16, 16), dtype=torch.uint8, device=x.device)
+    tail[..., 0] = byte.to(torch.uint8)
+    return torch.cat((codes.reshape(n, h, bs // 16, -1), tail), dim=-1).view(n, h, -1)
 
 
 def _pools(case, gen, blocks):
     pools = []
     for is_key in (True, False):
-        pool = torch.empty((blocks, case["kv_heads"], _tile(case)), dtype=torch.uint8, device=DEVICE)
+        pool = torch.empty((blocks, case["kv_heads"], case["block"] * (case["dim"] + 1)), dtype=torch.uint8, device=DEVICE)
         scale = _channels(gen, case["kv_heads"], case["dim"]) if is_key else 1.0
         for lo in range(0, blocks, 8192):
             n = min(blocks - lo, 8192)
@@ -355,14 +347,14 @@ def _places(case, slots, is_key):
     """Places in the flat pool of the bytes of tokens in slots (tokens,): codes (tokens, kv_heads, D), scales (tokens, kv_heads)."""
     bs, dim, heads = case["block"], case["dim"], case["kv_heads"]
     t = (slots % 16)[:, None]
-    tile = ((slots // bs)[:, None] * heads + torch.arange(heads, device=slots.device)) * _tile(case)  # (tokens, heads)
-    run = (slots % bs // 16)[:, None]
+    tile = (slots // bs)[:, None] * heads + torch.arange(heads, device=slots.device)  # (tokens, heads)
+    run = (tile * (bs // 16) + (slots % bs // 16)[:, None]) * 16 * (dim + 1)
     d = torch.arange(dim, device=slots.device)
     if is_key:
         code = ((d // 16) * 16 + t) * 16 + d % 16
     else:
         code = (((d // 64 * 4 + t // 4) * 16 + d // 4 % 16) * 4 + d % 4) * 4 + t % 4
-    return (tile + run * 16 * dim)[..., None] + code[:, None], tile + bs * dim + run
+    return run[..., None] + code[:, None], run + 16 * dim
 
 
 def _read(case, pool, slots, is_key):
@@ -597,12 +589,13 @@ def _e4m3(byte):
 def _unpack(case, blocks, is_key):
     """The values (n, kv_heads, block_size, D) in 64 bits of pool blocks (n, kv_heads, bytes), and the exponents (n, kv_heads, runs)."""
     n, heads, dim, bs = blocks.shape[0], blocks.shape[1], case["dim"], case["block"]
-    codes = blocks[..., : bs * dim].reshape(n, heads, bs // 16, -1)
+    runs = blocks.view(n, heads, bs // 16, -1)
+    codes = runs[..., : 16 * dim].contiguous()
     if is_key:
         codes = codes.view(n, heads, -1, dim // 64, 4, 16, 16).permute(0, 1, 2, 5, 3, 4, 6)
     else:
         codes = codes.view(n, heads, -1, dim // 64, 4, 16, 4, 4).permute(0, 1, 2, 4, 7, 3, 5, 6)
-    exponent = blocks[..., bs * dim : bs * dim + bs // 16].double() - 127
+    exponent = runs[..., 16 * dim].double() - 127
     values = _e4m3(codes.reshape(n, heads, bs // 16, 16 * dim)) * torch.exp2(exponent)[..., None]
     return values.view(n, heads, bs, dim), exponent
 
