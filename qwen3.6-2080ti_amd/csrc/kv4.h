@@ -62,14 +62,6 @@ __device__ __forceinline__ uint32_t pack_codes(const float (&x)[8], uint32_t byt
   return byte == 255u ? 0u : r;
 }
 
-// max over the four lanes of a quad; a NaN anywhere gives NaN (fmaxf would drop it).  Magnitudes only: as integers the
-// bits of non-negative floats compare like the floats, infinity and NaN above all others.
-__device__ __forceinline__ uint32_t quad_max(uint32_t v) {
-  v = max(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0xB1, 0xF, 0xF, false)));  // quad_perm [1,0,3,2]
-  v = max(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x4E, 0xF, 0xF, false)));  // quad_perm [2,3,0,1]
-  return v;
-}
-
 // Host: what every entry point asks of a 4-bit pool.
 inline int check_pool(const char* what, const qa_paged_kv* kv, int32_t head_dim, int32_t block_size) {
   QA_REQUIRE(kv != nullptr && kv->key != nullptr && kv->value != nullptr && kv->row_key_ptrs == nullptr, "%s: needs one shared pool", what);

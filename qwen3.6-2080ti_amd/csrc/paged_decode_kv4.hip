@@ -17,23 +17,11 @@
 // row rotation adds the two; with more the pieces take two products.  The query is split once a workgroup, a head a wave,
 // through LDS.
 #include "attention_kv4.h"
-
-#include <algorithm>
+#include "decode_split.h"
 
 namespace qa {
 namespace attn4 {
 
-struct DecodeParams {
-  Params c;
-  int n_wgs;
-  int short_rows;     // the tables hold no row that is split: no partials, no workspace
-  float* part_o;      // (n_wgs + B Hkv, G, D)
-  float* part_ml;     // (n_wgs + B Hkv, G, 2)
-  int32_t* rg_wgs;    // (B Hkv, 2): first and last workgroup of a row group; -1: the result is written
-};
-
-constexpr int kWaves = 8;
-constexpr int kUnit = 32;  // tokens
 // Where no row is longer than this, a workgroup takes a row group and nothing is merged; where the tables cannot hold a
 // longer one, the second launch is left out.  us split / by row, 2 KV heads of 256: 4 rows of 512 12.1 / 9.1, of 1024 12.4 /
 // 13.3, of 2048 12.2 / 19.4; 64 rows of up to 1024 25.5 / 14.1, of up to 4096 34.5 / 36.3; 200 rows of 500 37.7 / 22.0.
@@ -41,51 +29,6 @@ constexpr int kByRowTokens = 1024;
 // Row groups up to which a call of long tables has the workgroups for that; each of them reads all the lengths first.  us
 // split / by row, rows of 300, 2 KV heads: 200 rows 36 / 23, 500 68 / 51, 1000 122 / 116, 2000 229 / 291.
 constexpr int kByRowGroups = 2048;
-constexpr int kMaxWgs = 256;  // one per CU: eight waves of up to 256 registers fill it
-
-// Tokens and units of row b (0 for rows of length <= 0); lengths past the table stop at it.
-__device__ __forceinline__ int64_t row_tokens(const Params& p, int b) {
-  const int64_t len = p.idx_i64 ? reinterpret_cast<const int64_t*>(p.lens)[b] : reinterpret_cast<const int32_t*>(p.lens)[b];
-  return max64(0, min64(len, p.max_blocks << p.bs_shift));
-}
-__device__ __forceinline__ int units_of(int64_t tokens) { return static_cast<int>((tokens + kUnit - 1) / kUnit); }
-
-// A row group: row b, KV head g, the units before it, its units.
-struct Cursor {
-  int b, g, cum, nu;
-};
-
-__device__ __forceinline__ void next_row_group(const Params& p, Cursor& c) {
-  c.cum += c.nu;
-  if (++c.g < p.Hkv) return;
-  c.g = 0;
-  do {
-    ++c.b;
-    c.nu = c.b < p.B ? __builtin_amdgcn_readfirstlane(units_of(row_tokens(p, c.b))) : 0;
-  } while (c.nu == 0 && c.b < p.B);
-}
-
-// Inclusive sum over the lanes: shifts within rows of 16, then the rows' last sums passed on (DPP, no LDS).
-__device__ __forceinline__ int lane_scan(int v) {
-  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // row_shr:1
-  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);  // row_shr:2
-  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);  // row_shr:4
-  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);  // row_shr:8
-  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row_bcast:15 into rows 1 and 3
-  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // row_bcast:31 into rows 2 and 3
-  return v;
-}
-
-// Max over the wave of non-negative floats' bits.
-__device__ __forceinline__ uint32_t wave_max_bits(uint32_t v) {
-  v = kv4::quad_max(v);
-  v = max(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x124, 0xF, 0xF, false)));  // row_ror:4
-  v = max(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x128, 0xF, 0xF, false)));  // row_ror:8
-  const uint32_t a = max(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16));
-  const uint32_t b = max(__builtin_amdgcn_readlane(v, 32), __builtin_amdgcn_readlane(v, 48));
-  return max(a, b);
-}
-
 template <int D, bool WIDE>
 struct Smem {
   static constexpr int kHeads = WIDE ? 16 : 8;
@@ -481,92 +424,6 @@ __global__ __launch_bounds__(64 * kWaves, 2) void decode_kernel(DecodeParams dp)
   }
 }
 
-// Merges the partials of one (row, head): slots first + rg .. last + rg.  A thread has four of a workgroup's CHUNK dims of
-// every SHARE-th partial, kPartsInFlight of them on their way at once.
-constexpr int kPartsInFlight = 8;
-constexpr int kCombineThreads = kMaxWgs;  // a thread for each partial's m and l
-
-template <int D, int CHUNK>
-__global__ __launch_bounds__(kCombineThreads) void combine_kernel(DecodeParams dp) {
-  const Params& p = dp.c;
-  constexpr int ACROSS = CHUNK / 4;
-  constexpr int SHARE = kCombineThreads / ACROSS;
-  __shared__ float s_f[kMaxWgs];
-  __shared__ float s_red[2][kCombineThreads / 64];
-  __shared__ __align__(16) float s_o[SHARE][CHUNK];
-  const int tid = threadIdx.x;
-  const int64_t bh = blockIdx.x;
-  const int b = static_cast<int>(static_cast<uint32_t>(bh) / static_cast<uint32_t>(p.H));
-  const int h = static_cast<int>(bh) - b * p.H;
-  const int g = static_cast<int>(over_group(p, h));
-  const int hh = h - g * p.G;
-  const int64_t rg = static_cast<int64_t>(b) * p.Hkv + g;
-  const int first = dp.rg_wgs[2 * rg], last = dp.rg_wgs[2 * rg + 1];
-  const int d0 = static_cast<int>(blockIdx.y) * CHUNK;
-  bf16_t* out = p.out + bh * D + d0;
-  if (row_tokens(p, b) == 0) {  // its record was never written
-    if (tid < CHUNK) out[tid] = 0;
-    return;
-  }
-  if (first < 0) return;
-  const int n = last - first + 1;
-  const int64_t row0 = (first + rg) * p.G + hh;
-  const int share = tid / ACROSS, d = 4 * (tid % ACROSS);
-  const float* po = dp.part_o + row0 * D + d0 + d;
-  const int64_t so = static_cast<int64_t>(p.G) * D;
-  floatx4_v part[kPartsInFlight];
-  auto ask = [&](int s0) {
-#pragma unroll
-    for (int i = 0; i < kPartsInFlight; ++i) part[i] = *reinterpret_cast<const floatx4_v*>(po + min(s0 + i * SHARE, n - 1) * so);  // past the end: the last one again
-  };
-  ask(share);
-  float2 ml = make_float2(-INFINITY, 0.f);
-  if (tid < n) ml = *reinterpret_cast<const float2*>(dp.part_ml + (row0 + static_cast<int64_t>(tid) * p.G) * 2);
-  float gate = 0.f;
-  if (p.gate != nullptr && tid < CHUNK) gate = bf16_to_f32(p.gate[b * p.gate_st + h * p.gate_sh + d0 + tid]);
-  const float wm = wave_max(ml.x);
-  if ((tid & 63) == 0) s_red[0][tid >> 6] = wm;
-  __syncthreads();
-  float m = s_red[0][0];
-#pragma unroll
-  for (int w = 1; w < kCombineThreads / 64; ++w) m = fmaxf(m, s_red[0][w]);
-  const float use = m == -INFINITY ? 0.f : m;
-  const float f = tid < n ? __builtin_amdgcn_exp2f(ml.x - use) : 0.f;
-  s_f[tid] = f;
-  const float wl = wave_sum(tid < n ? f * ml.y : 0.f);
-  if ((tid & 63) == 0) s_red[1][tid >> 6] = wl;
-  __syncthreads();
-  floatx4_v acc = {0.f, 0.f, 0.f, 0.f};
-  for (int s0 = share; s0 < n; s0 += kPartsInFlight * SHARE) {
-    if (s0 != share) ask(s0);
-#pragma unroll
-    for (int i = 0; i < kPartsInFlight; ++i)
-      if (s0 + i * SHARE < n) acc += s_f[s0 + i * SHARE] * part[i];
-  }
-  *reinterpret_cast<floatx4_v*>(&s_o[share][d]) = acc;
-  __syncthreads();
-  if (tid >= CHUNK) return;
-  float sum = 0.f;
-#pragma unroll
-  for (int i = 0; i < SHARE; ++i) sum += s_o[i][tid];
-  float l = 0.f;
-#pragma unroll
-  for (int w = 0; w < kCombineThreads / 64; ++w) l += s_red[1][w];
-  float r = normalised(sum, l);
-  if (p.gate != nullptr) r *= sigmoid(gate);
-  out[tid] = f32_to_bf16(r);
-}
-
-static int64_t decode_wgs(int64_t row_groups, int64_t max_tokens) {
-  return std::min<int64_t>(kMaxWgs, std::max<int64_t>(1, ceil_div(row_groups * ceil_div(std::max<int64_t>(max_tokens, 1), kUnit), kWaves)));
-}
-
-static int64_t workspace_bytes_of(int64_t batch, int heads, int kv_heads, int head_dim, int64_t max_tokens) {
-  const int64_t groups = batch * kv_heads;
-  if (max_tokens <= kByRowTokens) return 0;
-  return (decode_wgs(groups, max_tokens) + groups) * (heads / kv_heads) * (head_dim + 2) * 4 + groups * 8;
-}
-
 template <int D, bool WIDE>
 static int launch(const DecodeParams& p, hipStream_t stream) {
   using S = Smem<D, WIDE>;
@@ -579,18 +436,7 @@ static int launch(const DecodeParams& p, hipStream_t stream) {
   }
   if (int rc = check_launch("paged_attention_decode_kv4")) return rc;
   if (p.short_rows) return 0;
-  const unsigned rows = static_cast<unsigned>(static_cast<int64_t>(p.c.B) * p.c.H);
-  // many partials a row group: more workgroups share its dims.  us of the whole call, not shared / shared: 1 row of 20000 16.9 /
-  // 14.9, of 200000 30.8 / 28.0; 8 rows of 30000 31.4 / 32.0, 64 of up to 1024 25.5 / 34.3
-  const bool many = p.n_wgs > 16 * static_cast<int64_t>(p.c.B) * p.c.Hkv;
-  {
-    KernelTimer timer_("decode_kv4_combine", stream);
-    if (many)
-      hipLaunchKernelGGL((combine_kernel<D, 32>), dim3(rows, D / 32), dim3(kCombineThreads), 0, stream, p);
-    else
-      hipLaunchKernelGGL((combine_kernel<D, D>), dim3(rows), dim3(kCombineThreads), 0, stream, p);
-  }
-  return check_launch("paged_attention_decode_kv4");
+  return merge<D>(p, "paged_attention_decode_kv4", "decode_kv4_combine", stream);
 }
 
 }  // namespace attn4
@@ -598,7 +444,7 @@ static int launch(const DecodeParams& p, hipStream_t stream) {
 
 extern "C" int64_t qa_paged_attention_decode_kv4_workspace(int64_t batch, int32_t heads, int32_t kv_heads, int32_t head_dim, int64_t max_tokens) {
   if (batch <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0 || max_tokens < 0) return 0;
-  return qa::attn4::workspace_bytes_of(batch, heads, kv_heads, head_dim, max_tokens);
+  return qa::attn4::workspace_bytes_of(batch, heads, kv_heads, head_dim, max_tokens, qa::attn4::kByRowTokens);
 }
 
 extern "C" int qa_paged_attention_decode_kv4(const void* query, int32_t q_dtype, int64_t q_stride_b, int64_t q_stride_h, int64_t batch, int32_t heads,
@@ -613,22 +459,7 @@ extern "C" int qa_paged_attention_decode_kv4(const void* query, int32_t q_dtype,
                lengths_dtype, block_size, scale, gate, gate_stride_b, gate_stride_h, output};
   if (int rc = fill(p.c, a)) return rc;
   if (batch == 0) return 0;
-  QA_REQUIRE(sequence_lengths != nullptr, "sequence_lengths must be a device array");
-  QA_REQUIRE(batch * heads <= 0x7fffffff, "%s: batch * heads out of range", a.what);
-  p.c.lens = sequence_lengths;
-  const int64_t groups = batch * kv->kv_heads;
-  const int64_t max_tokens = max_blocks * block_size;
-  QA_REQUIRE(groups * ceil_div(max_tokens, kUnit) <= 0x7fffffff, "%s: the tables cover too many tokens: %lld row groups of up to %lld", a.what, static_cast<long long>(groups),
-             static_cast<long long>(max_tokens));
-  const int64_t need = workspace_bytes_of(batch, heads, kv->kv_heads, head_dim, max_tokens);
-  QA_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 15u) == 0),
-             "paged decode workspace too small or not 16-byte aligned: need %lld bytes, have %lld", static_cast<long long>(need), static_cast<long long>(workspace_bytes));
-  p.short_rows = max_tokens <= kByRowTokens;
-  p.n_wgs = static_cast<int>(decode_wgs(groups, max_tokens));
-  const int64_t rows = (p.n_wgs + groups) * p.c.G;
-  p.part_o = reinterpret_cast<float*>(workspace);
-  p.part_ml = p.part_o + rows * head_dim;
-  p.rg_wgs = reinterpret_cast<int32_t*>(p.part_ml + rows * 2);
+  if (int rc = share_out(p, a, sequence_lengths, workspace, workspace_bytes, kByRowTokens)) return rc;
   if (head_dim == 256) return p.c.G > 8 ? launch<256, true>(p, stream) : launch<256, false>(p, stream);
   return p.c.G > 8 ? launch<128, true>(p, stream) : launch<128, false>(p, stream);
 }

@@ -144,6 +144,14 @@ __device__ __forceinline__ float wave_max(float v) {
   return v;
 }
 
+// max over the four lanes of a quad; a NaN anywhere gives NaN (fmaxf would drop it).  Magnitudes only: as integers the
+// bits of non-negative floats compare like the floats, infinity and NaN above all others.
+__device__ __forceinline__ uint32_t quad_max(uint32_t v) {
+  v = max(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0xB1, 0xF, 0xF, false)));  // quad_perm [1,0,3,2]
+  v = max(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x4E, 0xF, 0xF, false)));  // quad_perm [2,3,0,1]
+  return v;
+}
+
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 inline bool is_float_dtype(int32_t d) { return d == QA_F32 || d == QA_BF16; }

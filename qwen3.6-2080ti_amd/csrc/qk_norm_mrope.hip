@@ -106,7 +106,7 @@ __device__ __forceinline__ Raw<E> narrow(const float (&x)[E]) {
 // Max of non-negative floats' bits over the 32 / E lanes of a group of 32 dims.
 template <int E>
 __device__ __forceinline__ uint32_t group_max(uint32_t v) {
-  v = kv4::quad_max(v);
+  v = quad_max(v);
   v = max(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x141, 0xF, 0xF, false)));  // row_half_mirror
   if constexpr (E == 2) v = max(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x140, 0xF, 0xF, false)));  // row_mirror
   return v;
@@ -367,7 +367,7 @@ __global__ __launch_bounds__(256) void rows_kernel(Params p, int waves_per_token
       uint32_t top = 0;
 #pragma unroll
       for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(z[e]) & 0x7fffffffu);
-      const uint32_t byte = kv4::scale_byte(__uint_as_float(kv4::quad_max(top)));
+      const uint32_t byte = kv4::scale_byte(__uint_as_float(quad_max(top)));
       const uint32_t codes = kv4::pack_codes(z, byte);
       const int t = at & 15, group = in_head / 4;
       const int to = value ? R::value_code(t, j0 / (D / 16)) + j0 % (D / 16) / 2 : R::key_code(t, group) + 4 * (in_head & 3);
