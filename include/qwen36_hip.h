@@ -32,7 +32,8 @@ enum {
   QA_F16 = 2,
   QA_I32 = 3,
   QA_I64 = 4,
-  QA_KV4 = 5 /* a pool of the 4-bit KV cache; its strides are in bytes */
+  QA_KV4 = 5, /* a pool of the 4-bit KV cache; its strides are in bytes */
+  QA_KV8 = 6  /* a pool of the 8-bit KV cache; its strides are in bytes */
 };
 
 /* Paged KV pool descriptor.
@@ -49,7 +50,8 @@ enum {
  * (1, heads, P_b, bs, D) of different P_b.
  * Physical ids outside [0, num_blocks) (or row_blocks[b]) are skipped.
  * dtype QA_KV4: a shared pool (P, H_kv, tile) of bytes for the entries named
- * kv4 and qa_qk_norm_mrope_append; strides in bytes, stride_token unused.    */
+ * kv4 and qa_qk_norm_mrope_append, QA_KV8: one for the entries named kv8;
+ * strides in bytes, stride_token unused.                                     */
 typedef struct qa_paged_kv {
   void* key;
   void* value;
@@ -62,7 +64,7 @@ typedef struct qa_paged_kv {
   int64_t stride_head;
   int64_t stride_token;
   int32_t kv_heads;
-  int32_t dtype;                 /* QA_F32, QA_BF16 or QA_KV4 */
+  int32_t dtype;                 /* QA_F32, QA_BF16, QA_KV4 or QA_KV8 */
 } qa_paged_kv;
 
 /* ---- library ---------------------------------------------------------- */
@@ -343,6 +345,103 @@ int qa_paged_attention_prefill_kv4(const void* query, int32_t q_dtype, int64_t q
                                    int32_t block_size, float scale, const void* gate, int64_t gate_stride_t,
                                    int64_t gate_stride_h, void* output, void* workspace, int64_t workspace_bytes,
                                    hipStream_t stream);
+
+/* ---- full attention: an 8-bit KV cache ------------------------------------- */
+/* A pool is (P, H_kv, tile) bytes, a tile block_size / 16 runs of 16 tokens,
+ * block_size a power of two from 16 to 1024, head_dim D 128 or 256.  A run is
+ * 16 D E4M3 codes (bias 7, no infinities, largest 448) and the byte e + 127 of
+ * its scale 2^e with 15 zeros: 16 D + 16 bytes.  Of the finite values that a
+ * call writes to a run, e is the least integer with max|x| <= 448 2^e, within
+ * [-117, 120]; x / 2^e goes to the nearest code, ties to even, and what is not
+ * finite is NaN.  Where the call does not write the run's first token, e is
+ * not below the run's, and if it is above, the codes of the tokens before the
+ * first new one are rounded to it.
+ *   keys    codes  [slice of 64 dims][dim / 16 % 4][token][16 bytes]
+ *   values  codes  [slice of 64 dims][token / 4][dim / 4 % 16][dim % 4][token % 4]
+ * Every value held is exact in bfloat16.  A new pool's bytes may be anything.
+ * No counterpart in the reference, whose cache holds the activations' dtype
+ * (src/decode_state.py:37-44).                                               */
+
+/* qa_paged_kv4_append into an 8-bit pool.  Slots must be distinct, and the
+ * tokens of a run stand together in slots, as a plan's do: of a run that
+ * appears twice apart, the codes and the scale may not belong together.      */
+int qa_paged_kv8_append(const void* key_new, const void* value_new, int32_t dtype, int64_t k_stride_t, int64_t k_stride_h,
+                        int64_t v_stride_t, int64_t v_stride_h, int64_t tokens, int32_t head_dim, const qa_paged_kv* kv,
+                        const void* slots, int32_t slots_dtype, int32_t block_size, hipStream_t stream);
+
+/* qa_paged_kv_gather of an 8-bit pool: the values as bfloat16 (exact).        */
+int qa_paged_kv8_gather(const qa_paged_kv* kv, int32_t head_dim, int64_t batch, const void* block_tables, int32_t table_dtype,
+                        int64_t table_stride, int64_t max_blocks, int64_t valid, int32_t block_size, void* key_out,
+                        void* value_out, hipStream_t stream);
+
+/* qa_paged_attention_decode_kv4 and qa_paged_attention_prefill_kv4 over an
+ * 8-bit pool, with the same arguments and limits.                             */
+int64_t qa_paged_attention_decode_kv8_workspace(int64_t batch, int32_t heads, int32_t kv_heads, int32_t head_dim, int64_t max_tokens);
+int qa_paged_attention_decode_kv8(const void* query, int32_t q_dtype, int64_t q_stride_b, int64_t q_stride_h, int64_t batch,
+                                  int32_t heads, int32_t head_dim, const qa_paged_kv* kv, const void* block_tables,
+                                  int32_t table_dtype, int64_t table_stride, int64_t max_blocks,
+                                  const void* sequence_lengths, int32_t lengths_dtype, int32_t block_size, float scale,
+                                  const void* gate, int64_t gate_stride_b, int64_t gate_stride_h, void* output,
+                                  void* workspace, int64_t workspace_bytes, hipStream_t stream);
+int64_t qa_paged_attention_prefill_kv8_workspace(int64_t total_new, int64_t batch, int64_t max_new, int32_t heads, int32_t kv_heads,
+                                                 int32_t head_dim, int64_t max_tokens);
+int qa_paged_attention_prefill_kv8(const void* query, int32_t q_dtype, int64_t q_stride_t, int64_t q_stride_h, int64_t total_new,
+                                   const void* cu_seqlens, const void* prefix_lens, int32_t idx_dtype, int64_t batch,
+                                   int64_t max_new, int32_t heads, int32_t head_dim, const qa_paged_kv* kv,
+                                   const void* block_tables, int32_t table_dtype, int64_t table_stride, int64_t max_blocks,
+                                   int32_t block_size, float scale, const void* gate, int64_t gate_stride_t,
+                                   int64_t gate_stride_h, void* output, void* workspace, int64_t workspace_bytes,
+                                   hipStream_t stream);
+
+/* ---- full attention: pages shared, copied, freed and moved ------------------ */
+/* Books of a pool of free_capacity blocks: int32 block tables (rows,
+ * max_blocks), lengths (rows), the ascending free list and its cursor
+ * free_state {head, count}, as qa_paged_kv_reserve and qa_paged_kv_plan advance
+ * them, and references (free_capacity): the holders of a block beyond its first
+ * (0 for a block that one row has).  status: 0, or 1 (no block left), 3 (a
+ * cursor out of range), 4 (a length out of range), 6 (a row out of range, a
+ * target that is not empty, named twice, or a source too); with a status other
+ * than 0 nothing has changed and no page is to be copied.  The reference has no
+ * shared blocks; its frees are host lists (src/decode_state.py:80-84).        */
+
+/* Row target_rows[i] becomes a copy of row source_rows[i] (n of them, at most
+ * 1024; a source of -1: no fork).  It shares the full blocks and gets a block of
+ * its own, the list's first ones in order of i, for a partly filled last one:
+ * then sources[i] and targets[i] are the page to be copied, else -1.  Between the
+ * steps of the rows: the source's K/V must be written up to its length.        */
+int qa_paged_kv_fork(int32_t* block_tables, int64_t table_stride, int64_t max_blocks, int32_t* lengths, int64_t rows,
+                     const void* source_rows, const void* target_rows, int32_t rows_dtype, int64_t n, int32_t block_size,
+                     const int32_t* free_list, int64_t free_capacity, int32_t* free_state, int32_t* references,
+                     int32_t* status, int32_t* sources, int32_t* targets, hipStream_t stream);
+
+/* Frees the blocks of rows release_rows[0 .. n - 1] (out of range: skipped): each
+ * loses a holder and with its last one goes back to the list.  The rows become
+ * empty (-1, length 0), the list ascending from 0 with -1 behind its end.
+ * workspace: zeros.                                                           */
+int64_t qa_paged_kv_release_workspace(int64_t free_capacity);
+int qa_paged_kv_release(int32_t* block_tables, int64_t table_stride, int64_t max_blocks, int32_t* lengths, int64_t rows,
+                        const void* release_rows, int32_t rows_dtype, int64_t n, int32_t* free_list, int64_t free_capacity,
+                        int32_t* free_state, int32_t* references, int32_t* status, void* workspace, int64_t workspace_bytes,
+                        hipStream_t stream);
+
+/* Moves the largest ids that the tables hold to the lowest free ones, the k-th
+ * largest to the k-th lowest, as long as that is a lower id and k < max_moves:
+ * tables, references and the list as after the moves, sources and targets
+ * (max_moves) the pages to be copied, then -1.  Blocks that are neither free nor
+ * in these tables stay where they are.  workspace: zeros.                      */
+int64_t qa_paged_kv_compact_workspace(int64_t free_capacity);
+int qa_paged_kv_compact(int32_t* block_tables, int64_t table_stride, int64_t max_blocks, int64_t rows, int32_t* free_list,
+                        int64_t free_capacity, int32_t* free_state, int32_t* references, int32_t* status, int64_t max_moves,
+                        int32_t* sources, int32_t* targets, void* workspace, int64_t workspace_bytes, hipStream_t stream);
+
+/* Copies page sources[i] to page targets[i], i < n, of each pool: page j lies at
+ * pools[k] + j * page_strides[k] and has page_bytes[k] bytes, multiples of 4 (of
+ * 16 for the fast form).  Pairs with an id outside [0, page_counts[k]) are
+ * skipped.  No target may be another pair's target or any pair's source.  The
+ * four arrays of num_pools are in host memory.                                */
+int qa_paged_kv_copy(void* const* pools, const int64_t* page_strides, const int64_t* page_bytes, const int64_t* page_counts,
+                     int64_t num_pools, const void* sources, const void* targets, int32_t ids_dtype, int64_t n,
+                     hipStream_t stream);
 
 /* qa_qk_norm_rope_append with several position axes, through a slot map, into a
  * bf16 or a 4-bit pool.  positions (axes, tokens), axis a at a*positions_stride;

@@ -57,16 +57,6 @@ __device__ __forceinline__ int lane_scan(int v) {
   return v;
 }
 
-// Max over the wave of non-negative floats' bits.
-__device__ __forceinline__ uint32_t wave_max_bits(uint32_t v) {
-  v = quad_max(v);
-  v = max(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x124, 0xF, 0xF, false)));  // row_ror:4
-  v = max(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x128, 0xF, 0xF, false)));  // row_ror:8
-  const uint32_t a = max(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16));
-  const uint32_t b = max(__builtin_amdgcn_readlane(v, 32), __builtin_amdgcn_readlane(v, 48));
-  return max(a, b);
-}
-
 // Merges the partials of one (row, head): slots first + rg .. last + rg.  A thread has four of a workgroup's CHUNK dims of
 // every SHARE-th partial, kPartsInFlight of them on their way at once.
 constexpr int kPartsInFlight = 8;

@@ -1,0 +1,548 @@
+// Pages of a paged KV cache on the device: forked, copied, freed and compacted, gfx950.
+//
+// A block id is one page of every layer's key and value pools.  references[id] counts its holders beyond the first, so that
+// blocks that were never shared need no entry and the reserving kernels (kv_cache.hip, kv_plan.hip) know nothing of it.
+//   fork     a new row shares the full blocks of its source and gets a fresh block for a partly filled last one, whose page is
+//            then copied: no row ever writes to a block that another holds.
+//   release  a row's blocks lose a holder, and go back to the free list with the last one.
+//   compact  the largest ids that the tables hold move to the lowest free ones as long as that is lower: then the pools' ends are
+//            free.
+// The free list stays ascending: release and compact mark the free blocks in a bitmap, 32 blocks a word, and write the list anew
+// from it; a workgroup counts all words before its own (a few tens of KB out of L2) rather than wait for its neighbours.  So the
+// result does not depend on the order of the atomics that set the bits.
+//
+// Books are small and latency bounds them; copies are bound by memory, each page read once and written once for each
+// copy of it.
+#include "qa_common.h"
+
+#include <algorithm>
+
+namespace qa {
+namespace pages {
+
+struct Books {
+  int32_t* tables;
+  int64_t table_stride, max_blocks;
+  int32_t* lengths;
+  int32_t* free_list;
+  int32_t* free_state;  // head, count
+  int32_t* references;
+  int32_t* status;
+  int64_t capacity, rows;
+};
+
+__device__ __forceinline__ int64_t index_of(const void* base, int is64, int64_t i) {
+  return is64 ? reinterpret_cast<const int64_t*>(base)[i] : reinterpret_cast<const int32_t*>(base)[i];
+}
+
+__device__ __forceinline__ bool corrupt(const Books& k) {
+  const int64_t head = k.free_state[0], count = k.free_state[1];
+  return head < 0 || count < 0 || head + count > k.capacity;
+}
+
+// Inclusive sum over the workgroup of 64 kThreads / 64 waves; total: of all.
+template <int THREADS>
+__device__ __forceinline__ int32_t block_scan(int32_t v, int32_t* s_wave, int32_t& total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int32_t incl = v;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int32_t u = __shfl_up(incl, off, 64);
+    if (lane >= off) incl += u;
+  }
+  __syncthreads();  // s_wave may still be read
+  if (lane == 63) s_wave[wave] = incl;
+  __syncthreads();
+  int32_t before = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 64; ++w) {
+    if (w < wave) before += s_wave[w];
+    total += s_wave[w];
+  }
+  return before + incl;
+}
+
+// ---- fork -------------------------------------------------------------------
+
+struct ForkParams {
+  Books k;
+  const void* source_rows;
+  const void* target_rows;
+  int n, rows_i64, bs;
+  int32_t* sources;  // (n): the page to be copied, -1: none
+  int32_t* targets;
+};
+
+constexpr int kForks = 1024;  // of a call: a thread each
+
+__global__ __launch_bounds__(kForks) void fork_kernel(ForkParams p) {
+  __shared__ int64_t s_source[kForks], s_target[kForks];
+  __shared__ int32_t s_wave[kForks / 64];
+  __shared__ int s_code;
+  const Books& k = p.k;
+  const int i = threadIdx.x;
+  int64_t source = -1, target = -1;
+  if (i < p.n) {
+    source = index_of(p.source_rows, p.rows_i64, i);
+    target = index_of(p.target_rows, p.rows_i64, i);
+  }
+  const bool live = source >= 0;  // -1: no fork
+  s_source[i] = live ? source : -1;
+  s_target[i] = live ? target : -1;
+  const int64_t head = k.free_state[0], count = k.free_state[1];
+  if (i == 0) s_code = head < 0 || count < 0 || head + count > k.capacity ? 3 : 0;
+  __syncthreads();
+  int64_t length = 0;
+  int32_t last = -1;
+  int bad = 0;
+  if (live) {
+    if (source >= k.rows || target < 0 || target >= k.rows || k.lengths[target] != 0) {
+      bad = 6;
+    } else {
+      for (int j = 0; j < p.n; ++j)
+        if ((j != i && s_target[j] == target) || s_source[j] == target) bad = 6;
+      length = k.lengths[source];
+      if (length < 0 || length > k.max_blocks * p.bs) bad = 4;
+    }
+    if (bad == 0 && length % p.bs != 0) last = k.tables[source * k.table_stride + length / p.bs];
+  }
+  if (bad != 0) atomicMax(&s_code, bad);
+  const bool need = last >= 0 && last < k.capacity;
+  int32_t total;
+  const int32_t upto = block_scan<kForks>(need ? 1 : 0, s_wave, total);
+  const int code = s_code != 0 ? s_code : total > count ? 1 : 0;  // the scan's barriers stand between the atomics and this
+  if (i < p.n) {
+    p.sources[i] = need && code == 0 ? last : -1;
+    p.targets[i] = need && code == 0 ? k.free_list[head + upto - 1] : -1;
+    if (live && code == 0) k.lengths[target] = static_cast<int32_t>(length);
+  }
+  if (i == 0) {
+    k.status[0] = code;
+    if (code == 0) {
+      k.free_state[0] = static_cast<int32_t>(head + total);
+      k.free_state[1] = static_cast<int32_t>(count - total);
+    }
+  }
+}
+
+// Table entries of fork blockIdx.y, a holder more for each block that it shares.
+__global__ __launch_bounds__(256) void fork_tables_kernel(ForkParams p) {
+  const Books& k = p.k;
+  const int i = blockIdx.y;
+  const int64_t source = index_of(p.source_rows, p.rows_i64, i);
+  if (source < 0 || k.status[0] != 0) return;
+  const int64_t target = index_of(p.target_rows, p.rows_i64, i);
+  const int64_t length = k.lengths[source];
+  const int64_t entries = (length + p.bs - 1) / p.bs;
+  const int32_t own = p.targets[i];
+  for (int64_t e = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; e < entries; e += static_cast<int64_t>(gridDim.x) * 256) {
+    int32_t id = k.tables[source * k.table_stride + e];
+    if (own >= 0 && e == entries - 1)
+      id = own;
+    else if (id >= 0 && id < k.capacity)
+      atomicAdd(&k.references[id], 1);
+    k.tables[target * k.table_stride + e] = id;
+  }
+}
+
+// ---- the free list from a bitmap ----------------------------------------------
+
+constexpr int kListThreads = 256;  // a word each
+
+__device__ __forceinline__ void set_bit(uint32_t* bits, int32_t id) { atomicOr(&bits[id >> 5], 1u << (id & 31)); }
+
+// Marks the free list's blocks.
+__device__ __forceinline__ void mark_free(const Books& k, uint32_t* bits, int64_t first, int64_t step) {
+  const int64_t head = k.free_state[0], count = k.free_state[1];
+  for (int64_t i = first; i < count; i += step) {
+    const int32_t id = k.free_list[head + i];
+    if (id >= 0 && id < k.capacity) set_bit(bits, id);
+  }
+}
+
+// Bits below word `mine` of the words that `word` gives, and of all of them.
+template <typename F>
+__device__ __forceinline__ void count_before(int64_t words, F word, int32_t* s_wave, int32_t& incl, int32_t& total) {
+  const int64_t base = static_cast<int64_t>(blockIdx.x) * kListThreads;
+  int32_t before = 0, all = 0;
+  for (int64_t w = threadIdx.x; w < words; w += kListThreads) {
+    const int32_t c = __popc(word(w));
+    if (w < base) before += c;
+    all += c;
+  }
+  int32_t sum;
+  block_scan<kListThreads>(before, s_wave, sum);
+  block_scan<kListThreads>(all, s_wave, total);
+  int32_t own;
+  incl = sum + block_scan<kListThreads>(base + threadIdx.x < words ? __popc(word(base + threadIdx.x)) : 0, s_wave, own);
+}
+
+// Writes the list and its cursor: this workgroup's words, and -1 at its share of the places behind the list's end.
+template <typename F>
+__device__ __forceinline__ void write_list(const Books& k, int64_t words, F word, int32_t* s_wave) {
+  int32_t incl, total;
+  count_before(words, word, s_wave, incl, total);
+  const int64_t w = static_cast<int64_t>(blockIdx.x) * kListThreads + threadIdx.x;
+  if (w < words) {
+    uint32_t bits = word(w);
+    int32_t at = incl - __popc(bits);
+    while (bits != 0) {
+      const int b = __ffs(bits) - 1;
+      bits &= bits - 1;
+      k.free_list[at++] = static_cast<int32_t>(32 * w + b);
+    }
+  }
+  const int64_t lo = max64(total, static_cast<int64_t>(blockIdx.x) * kListThreads * 32);
+  const int64_t hi = min64(k.capacity, (static_cast<int64_t>(blockIdx.x) + 1) * kListThreads * 32);
+  for (int64_t i = lo + threadIdx.x; i < hi; i += kListThreads) k.free_list[i] = -1;
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    k.free_state[0] = 0;
+    k.free_state[1] = total;
+    k.status[0] = 0;
+  }
+}
+
+// ---- release ------------------------------------------------------------------
+
+struct ReleaseParams {
+  Books k;
+  const void* release_rows;
+  int n, rows_i64;
+  uint32_t* bits;    // (words + 1), zeros: free blocks; the last word is 1 where the free list's cursor is out of range
+  int64_t words;
+};
+
+// blockIdx.y < n: the blocks of a row; n: the free list.
+__global__ __launch_bounds__(256) void release_kernel(ReleaseParams p) {
+  const Books& k = p.k;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, step = static_cast<int64_t>(gridDim.x) * 256;
+  if (corrupt(k)) {
+    if (first == 0) p.bits[p.words] = 1;
+    return;
+  }
+  if (static_cast<int>(blockIdx.y) == p.n) {
+    mark_free(k, p.bits, first, step);
+    return;
+  }
+  const int64_t row = index_of(p.release_rows, p.rows_i64, blockIdx.y);
+  if (row < 0 || row >= k.rows) return;
+  for (int64_t e = first; e < k.max_blocks; e += step) {
+    int32_t* entry = &k.tables[row * k.table_stride + e];
+    if (*entry == -1) continue;
+    const int32_t id = atomicExch(entry, -1);  // a row named twice is freed once
+    if (id < 0 || id >= k.capacity) continue;
+    if (atomicSub(&k.references[id], 1) > 0) continue;
+    atomicAdd(&k.references[id], 1);
+    set_bit(p.bits, id);
+  }
+  if (first == 0) k.lengths[row] = 0;
+}
+
+__global__ __launch_bounds__(kListThreads) void release_list_kernel(ReleaseParams p) {
+  __shared__ int32_t s_wave[kListThreads / 64];
+  if (p.bits[p.words] != 0) {
+    if (blockIdx.x == 0 && threadIdx.x == 0) p.k.status[0] = 3;
+    return;
+  }
+  write_list(p.k, p.words, [&](int64_t w) { return p.bits[w]; }, s_wave);
+}
+
+// ---- compact --------------------------------------------------------------------
+
+struct CompactParams {
+  Books k;
+  int64_t words, max_moves;
+  uint32_t* free_bits;  // (words), zeros
+  uint32_t* held;       // (words), zeros: blocks that the tables hold
+  uint32_t* flip;       // (words), zeros: blocks that are taken or left
+  uint32_t* refused;    // (1), zero
+  int32_t* place;       // (capacity): where a block that is left has gone
+  int32_t* sources;     // (max_moves)
+  int32_t* targets;
+  int list_groups;
+};
+
+// blockIdx.y < rows: the blocks of a row; then the free list; then the pairs, set to none.
+__global__ __launch_bounds__(256) void compact_mark_kernel(CompactParams p) {
+  const Books& k = p.k;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, step = static_cast<int64_t>(gridDim.x) * 256;
+  const int64_t y = blockIdx.y;
+  if (y == k.rows + 1) {
+    for (int64_t i = first; i < p.max_moves; i += step) p.sources[i] = p.targets[i] = -1;
+    return;
+  }
+  if (corrupt(k)) {
+    if (first == 0) p.refused[0] = 1;
+    return;
+  }
+  if (y == k.rows) {
+    mark_free(k, p.free_bits, first, step);
+    return;
+  }
+  for (int64_t e = first; e < k.max_blocks; e += step) {
+    const int32_t id = k.tables[y * k.table_stride + e];
+    if (id >= 0 && id < k.capacity) set_bit(p.held, id);
+  }
+}
+
+// The block with k held ones above it moves to the k-th free one where that is lower.
+__global__ __launch_bounds__(kListThreads) void compact_moves_kernel(CompactParams p) {
+  __shared__ int32_t s_wave[kListThreads / 64];
+  const Books& k = p.k;
+  if (p.refused[0] != 0) return;
+  auto word = [&](int64_t w) { return p.held[w] & ~p.free_bits[w]; };
+  int32_t incl, total;
+  count_before(p.words, word, s_wave, incl, total);
+  const int64_t w = static_cast<int64_t>(blockIdx.x) * kListThreads + threadIdx.x;
+  if (w >= p.words) return;
+  const int64_t head = k.free_state[0], most = min64(p.max_moves, k.free_state[1]);
+  uint32_t bits = word(w);
+  int32_t nth = total - incl + __popc(bits);  // held blocks from this word on
+  while (bits != 0) {
+    const int b = __ffs(bits) - 1;
+    bits &= bits - 1;
+    const int32_t source = static_cast<int32_t>(32 * w + b);
+    if (--nth >= most) continue;
+    const int32_t target = k.free_list[head + nth];
+    if (target < 0 || target >= source) continue;
+    p.sources[nth] = source;
+    p.targets[nth] = target;
+    p.place[source] = target;
+    k.references[target] = k.references[source];
+    k.references[source] = 0;
+    set_bit(p.flip, source);
+    set_bit(p.flip, target);
+  }
+}
+
+// blockIdx.y 0: the free list; then the tables' rows.
+__global__ __launch_bounds__(kListThreads) void compact_list_kernel(CompactParams p) {
+  __shared__ int32_t s_wave[kListThreads / 64];
+  const Books& k = p.k;
+  if (p.refused[0] != 0) {
+    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) k.status[0] = 3;
+    return;
+  }
+  if (blockIdx.y == 0) {
+    if (static_cast<int>(blockIdx.x) < p.list_groups) write_list(k, p.words, [&](int64_t w) { return p.free_bits[w] ^ p.flip[w]; }, s_wave);
+    return;
+  }
+  for (int64_t e = static_cast<int64_t>(blockIdx.x) * kListThreads + threadIdx.x; e < k.max_blocks; e += static_cast<int64_t>(gridDim.x) * kListThreads) {
+    int32_t* entry = &k.tables[(blockIdx.y - 1) * k.table_stride + e];
+    const int32_t id = *entry;
+    if (id < 0 || id >= k.capacity) continue;
+    const uint32_t bit = 1u << (id & 31);
+    if (p.flip[id >> 5] & p.held[id >> 5] & ~p.free_bits[id >> 5] & bit) *entry = p.place[id];
+  }
+}
+
+// ---- copy -----------------------------------------------------------------------
+
+constexpr int kPools = 32;  // of a launch
+
+struct CopyParams {
+  uint8_t* base[kPools];
+  int64_t stride[kPools];  // bytes from page to page
+  int64_t bytes[kPools];   // of a page
+  int64_t count[kPools];   // pages
+  const void* sources;
+  const void* targets;
+  int64_t n;
+  int ids_i64;
+};
+
+constexpr int kCopyThreads = 256;
+constexpr int kInFlight = 4;  // units a thread has on their way
+constexpr int64_t kCopyGroups = 4096;
+
+// UNIT: 16 or 4 bytes.  Workgroups take pieces of kCopyThreads * kInFlight units of the pages of pool blockIdx.y in turn.
+template <typename UNIT>
+__global__ __launch_bounds__(kCopyThreads) void copy_kernel(CopyParams p) {
+  const int pool = blockIdx.y;
+  const int64_t units = p.bytes[pool] / static_cast<int64_t>(sizeof(UNIT));
+  const int64_t pieces = (units + kCopyThreads * kInFlight - 1) / (kCopyThreads * kInFlight);
+  for (int64_t x = blockIdx.x; x < p.n * pieces; x += gridDim.x) {
+    const int64_t pair = x / pieces, piece = x - pair * pieces;
+    const int64_t source = index_of(p.sources, p.ids_i64, pair), target = index_of(p.targets, p.ids_i64, pair);
+    if (source < 0 || target < 0 || source >= p.count[pool] || target >= p.count[pool]) continue;
+    const UNIT* from = reinterpret_cast<const UNIT*>(p.base[pool] + source * p.stride[pool]);
+    UNIT* to = reinterpret_cast<UNIT*>(p.base[pool] + target * p.stride[pool]);
+    const int64_t u0 = piece * (kCopyThreads * kInFlight) + threadIdx.x;
+    UNIT u[kInFlight];
+#pragma unroll
+    for (int i = 0; i < kInFlight; ++i) u[i] = from[min64(u0 + i * kCopyThreads, units - 1)];
+#pragma unroll
+    for (int i = 0; i < kInFlight; ++i)
+      if (u0 + i * kCopyThreads < units) to[u0 + i * kCopyThreads] = u[i];
+  }
+}
+
+// ---- host -----------------------------------------------------------------------
+
+static int64_t words_of(int64_t capacity) { return ceil_div(capacity, 32); }
+
+static int check_books(const char* what, const Books& k) {
+  QA_REQUIRE(k.tables && k.free_list && k.free_state && k.references && k.status, "%s: pointers must be non-null", what);
+  QA_REQUIRE(k.rows >= 1 && k.rows <= 65533, "%s: the tables must have 1 to 65533 rows", what);
+  QA_REQUIRE(k.max_blocks >= 1 && k.max_blocks <= 0x7fffffff, "%s: block table must have at least one entry", what);
+  QA_REQUIRE(k.table_stride >= k.max_blocks || k.rows == 1, "table rows overlap: stride %lld < max_blocks %lld", static_cast<long long>(k.table_stride), static_cast<long long>(k.max_blocks));
+  QA_REQUIRE(k.capacity >= 1 && k.capacity <= 0x7fffffff, "free list capacity must be in [1, 2^31)");
+  return 0;
+}
+
+// Workgroups along an axis of `n` entries: enough for a few entries a thread.
+static unsigned groups_of(int64_t n) { return static_cast<unsigned>(std::min<int64_t>(std::max<int64_t>(ceil_div(n, 256), 1), 64)); }
+
+}  // namespace pages
+}  // namespace qa
+
+extern "C" int qa_paged_kv_fork(int32_t* block_tables, int64_t table_stride, int64_t max_blocks, int32_t* lengths, int64_t rows, const void* source_rows,
+                                const void* target_rows, int32_t rows_dtype, int64_t n, int32_t block_size, const int32_t* free_list, int64_t free_capacity,
+                                int32_t* free_state, int32_t* references, int32_t* status, int32_t* sources, int32_t* targets, hipStream_t stream) {
+  using namespace qa;
+  using namespace qa::pages;
+  ForkParams p{};
+  p.k = {block_tables, table_stride, max_blocks, lengths, const_cast<int32_t*>(free_list), free_state, references, status, free_capacity, rows};
+  if (int rc = check_books("paged_kv_fork", p.k)) return rc;
+  QA_REQUIRE(is_index_dtype(rows_dtype), "paged_kv_fork: rows must be int32 or int64");
+  QA_REQUIRE(n >= 0 && n <= kForks, "paged_kv_fork: at most %d forks a call", kForks);
+  QA_REQUIRE(block_size > 0 && block_size <= 65536, "paged_kv_fork: block_size must be in [1, 65536]");
+  QA_REQUIRE(lengths != nullptr && (n == 0 || (source_rows && target_rows && sources && targets)), "paged_kv_fork: pointers must be non-null");
+  p.source_rows = source_rows;
+  p.target_rows = target_rows;
+  p.n = static_cast<int>(n);
+  p.rows_i64 = rows_dtype == QA_I64;
+  p.bs = block_size;
+  p.sources = sources;
+  p.targets = targets;
+  {
+    KernelTimer timer_("kv_fork", stream);
+    hipLaunchKernelGGL(fork_kernel, dim3(1), dim3(kForks), 0, stream, p);
+  }
+  if (int rc = check_launch("paged_kv_fork")) return rc;
+  if (n == 0) return 0;
+  {
+    KernelTimer timer_("kv_fork_tables", stream);
+    hipLaunchKernelGGL(fork_tables_kernel, dim3(groups_of(max_blocks), static_cast<unsigned>(n)), dim3(256), 0, stream, p);
+  }
+  return check_launch("paged_kv_fork");
+}
+
+extern "C" int64_t qa_paged_kv_release_workspace(int64_t free_capacity) { return free_capacity <= 0 ? 0 : 4 * (qa::pages::words_of(free_capacity) + 1); }
+
+extern "C" int qa_paged_kv_release(int32_t* block_tables, int64_t table_stride, int64_t max_blocks, int32_t* lengths, int64_t rows, const void* release_rows,
+                                   int32_t rows_dtype, int64_t n, int32_t* free_list, int64_t free_capacity, int32_t* free_state, int32_t* references, int32_t* status,
+                                   void* workspace, int64_t workspace_bytes, hipStream_t stream) {
+  using namespace qa;
+  using namespace qa::pages;
+  ReleaseParams p{};
+  p.k = {block_tables, table_stride, max_blocks, lengths, free_list, free_state, references, status, free_capacity, rows};
+  if (int rc = check_books("paged_kv_release", p.k)) return rc;
+  QA_REQUIRE(is_index_dtype(rows_dtype), "paged_kv_release: rows must be int32 or int64");
+  QA_REQUIRE(n >= 0 && n <= 65533, "paged_kv_release: at most 65533 rows a call");
+  QA_REQUIRE(lengths != nullptr && (n == 0 || release_rows != nullptr), "paged_kv_release: pointers must be non-null");
+  QA_REQUIRE(workspace != nullptr && workspace_bytes >= qa_paged_kv_release_workspace(free_capacity) && (reinterpret_cast<uintptr_t>(workspace) & 3u) == 0,
+             "paged_kv_release: workspace too small or not 4-byte aligned: need %lld bytes", static_cast<long long>(qa_paged_kv_release_workspace(free_capacity)));
+  p.release_rows = release_rows;
+  p.n = static_cast<int>(n);
+  p.rows_i64 = rows_dtype == QA_I64;
+  p.bits = reinterpret_cast<uint32_t*>(workspace);
+  p.words = words_of(free_capacity);
+  {
+    KernelTimer timer_("kv_release", stream);
+    hipLaunchKernelGGL(release_kernel, dim3(groups_of(std::max(max_blocks, free_capacity)), static_cast<unsigned>(n + 1)), dim3(256), 0, stream, p);
+  }
+  if (int rc = check_launch("paged_kv_release")) return rc;
+  {
+    KernelTimer timer_("kv_release_list", stream);
+    hipLaunchKernelGGL(release_list_kernel, dim3(static_cast<unsigned>(ceil_div(p.words, kListThreads))), dim3(kListThreads), 0, stream, p);
+  }
+  return check_launch("paged_kv_release");
+}
+
+extern "C" int64_t qa_paged_kv_compact_workspace(int64_t free_capacity) {
+  return free_capacity <= 0 ? 0 : 4 * (3 * qa::pages::words_of(free_capacity) + 1 + free_capacity);
+}
+
+extern "C" int qa_paged_kv_compact(int32_t* block_tables, int64_t table_stride, int64_t max_blocks, int64_t rows, int32_t* free_list, int64_t free_capacity,
+                                   int32_t* free_state, int32_t* references, int32_t* status, int64_t max_moves, int32_t* sources, int32_t* targets, void* workspace,
+                                   int64_t workspace_bytes, hipStream_t stream) {
+  using namespace qa;
+  using namespace qa::pages;
+  CompactParams p{};
+  p.k = {block_tables, table_stride, max_blocks, nullptr, free_list, free_state, references, status, free_capacity, rows};
+  if (int rc = check_books("paged_kv_compact", p.k)) return rc;
+  QA_REQUIRE(max_moves >= 0 && max_moves <= 0x7fffffff, "paged_kv_compact: max_moves out of range");
+  QA_REQUIRE(max_moves == 0 || (sources && targets), "paged_kv_compact: pointers must be non-null");
+  QA_REQUIRE(workspace != nullptr && workspace_bytes >= qa_paged_kv_compact_workspace(free_capacity) && (reinterpret_cast<uintptr_t>(workspace) & 3u) == 0,
+             "paged_kv_compact: workspace too small or not 4-byte aligned: need %lld bytes", static_cast<long long>(qa_paged_kv_compact_workspace(free_capacity)));
+  p.words = words_of(free_capacity);
+  p.max_moves = max_moves;
+  p.free_bits = reinterpret_cast<uint32_t*>(workspace);
+  p.held = p.free_bits + p.words;
+  p.flip = p.held + p.words;
+  p.refused = p.flip + p.words;
+  p.place = reinterpret_cast<int32_t*>(p.refused + 1);
+  p.sources = sources;
+  p.targets = targets;
+  const unsigned lists = static_cast<unsigned>(ceil_div(p.words, kListThreads));
+  p.list_groups = static_cast<int>(lists);
+  {
+    KernelTimer timer_("kv_compact_mark", stream);
+    hipLaunchKernelGGL(compact_mark_kernel, dim3(groups_of(std::max(max_blocks, free_capacity)), static_cast<unsigned>(rows + 2)), dim3(256), 0, stream, p);
+  }
+  if (int rc = check_launch("paged_kv_compact")) return rc;
+  {
+    KernelTimer timer_("kv_compact_moves", stream);
+    hipLaunchKernelGGL(compact_moves_kernel, dim3(lists), dim3(kListThreads), 0, stream, p);
+  }
+  if (int rc = check_launch("paged_kv_compact")) return rc;
+  {
+    KernelTimer timer_("kv_compact_list", stream);
+    hipLaunchKernelGGL(compact_list_kernel, dim3(std::max(lists, groups_of(max_blocks)), static_cast<unsigned>(rows + 1)), dim3(kListThreads), 0, stream, p);
+  }
+  return check_launch("paged_kv_compact");
+}
+
+extern "C" int qa_paged_kv_copy(void* const* pools, const int64_t* page_strides, const int64_t* page_bytes, const int64_t* page_counts, int64_t num_pools,
+                                const void* sources, const void* targets, int32_t ids_dtype, int64_t n, hipStream_t stream) {
+  using namespace qa;
+  using namespace qa::pages;
+  QA_REQUIRE(num_pools >= 0 && n >= 0 && n <= 0x7fffffff, "paged_kv_copy: counts out of range");
+  QA_REQUIRE(is_index_dtype(ids_dtype), "paged_kv_copy: page ids must be int32 or int64");
+  if (num_pools == 0 || n == 0) return 0;
+  QA_REQUIRE(pools && page_strides && page_bytes && page_counts && sources && targets, "paged_kv_copy: pointers must be non-null");
+  bool wide = true;
+  for (int64_t i = 0; i < num_pools; ++i) {
+    QA_REQUIRE(pools[i] != nullptr || page_counts[i] == 0, "paged_kv_copy: pool %lld is null", static_cast<long long>(i));
+    QA_REQUIRE(page_counts[i] >= 0 && page_bytes[i] >= 0 && (page_strides[i] >= page_bytes[i] || page_counts[i] <= 1), "paged_kv_copy: pages of pool %lld overlap", static_cast<long long>(i));
+    const uint64_t all = reinterpret_cast<uintptr_t>(pools[i]) | static_cast<uint64_t>(page_strides[i]) | static_cast<uint64_t>(page_bytes[i]);
+    QA_REQUIRE((all & 3u) == 0, "paged_kv_copy: pages of pool %lld are not of 4-byte units", static_cast<long long>(i));
+    if (all & 15u) wide = false;
+  }
+  for (int64_t i0 = 0; i0 < num_pools; i0 += kPools) {
+    const int64_t here = std::min<int64_t>(kPools, num_pools - i0);
+    CopyParams p{};
+    int64_t units = 0;
+    for (int64_t i = 0; i < here; ++i) {
+      p.base[i] = reinterpret_cast<uint8_t*>(pools[i0 + i]);
+      p.stride[i] = page_strides[i0 + i];
+      p.bytes[i] = page_bytes[i0 + i];
+      p.count[i] = page_counts[i0 + i];
+      units = std::max(units, p.bytes[i] / (wide ? 16 : 4));
+    }
+    if (units == 0) continue;
+    p.sources = sources;
+    p.targets = targets;
+    p.n = n;
+    p.ids_i64 = ids_dtype == QA_I64;
+    const dim3 grid(static_cast<unsigned>(std::min<int64_t>(n * ceil_div(units, kCopyThreads * kInFlight), kCopyGroups)), static_cast<unsigned>(here));
+    KernelTimer timer_("kv_copy", stream);
+    if (wide)
+      hipLaunchKernelGGL(copy_kernel<uint4>, grid, dim3(kCopyThreads), 0, stream, p);
+    else
+      hipLaunchKernelGGL(copy_kernel<uint32_t>, grid, dim3(kCopyThreads), 0, stream, p);
+  }
+  return check_launch("paged_kv_copy");
+}

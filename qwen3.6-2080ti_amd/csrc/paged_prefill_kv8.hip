@@ -1,0 +1,503 @@
+// Chunked causal prefill attention over the 8-bit paged KV cache (attention_kv8.h, kv8.h), gfx950.
+//
+// Columns of the products are (new position, query head of the KV head's group), position-major, so any group size
+// fills them.  A workgroup owns 128 of one row and KV head and walks the keys in tiles of 64.  Its eight waves are four
+// pairs of 32 columns: a wave takes the scores and the softmax of half of the tile's keys, then the products with the values of
+// all of them for half of the dims, its partner's probabilities through LDS.  So a key read from LDS feeds 32 columns and is
+// converted by four waves, and the accumulators of a wave stay at 64 registers, two waves to a SIMD.
+//
+// Codes go from memory to LDS as they are, a run a wave, and to bf16 next to the products.
+//
+// Iteration i, one barrier: the scores of tile i + 1 and the largest of each column, the probabilities of tile i, for which the
+// pair shares its columns' reference points, and the products of tile i - 1's values.
+//
+// With few columns the keys are split over gridDim.z and a second launch joins the parts.
+#include "attention_kv8.h"
+#include "prefill_split.h"
+
+#include <type_traits>
+
+namespace qa {
+namespace prefill8 {
+
+using namespace attn8;
+
+typedef float floatx16_v __attribute__((ext_vector_type(16)));
+
+constexpr int kKeyBufs = 2, kValueBufs = 4;
+
+template <int D>
+struct Smem {
+  static constexpr int kRunBytes = kv8::Run<D>::kCodes;
+  static constexpr int kTileBytes = kRuns * kRunBytes;
+  static constexpr int kValues = kKeyBufs * kTileBytes;               // after the keys: [buffer][run]
+  static constexpr int kP = kValues + kValueBufs * kTileBytes;        // probabilities: [buffer][wave][run][lane][16 bytes]
+  static constexpr int kMax = kP + 2 * kWaves * 2 * 1024;             // [buffer][wave][32] floats
+  static constexpr int kScale = kMax + 2 * kWaves * 32 * 4;           // of keys [buffer][run], of values [buffer][run]
+  static constexpr int kFlag = kScale + (kKeyBufs + kValueBufs) * kRuns * 4;  // [buffer of values]: 1 + the last tile that had a NaN
+  static constexpr int kBytes = kFlag + kValueBufs * 4;
+};
+
+template <int D>
+__global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams pp) {
+  const Params& p = pp.c;
+  constexpr int N = kv8::Run<D>::kSlices;
+  constexpr int MT = D / 64;        // tiles of 32 dims of a wave
+  using S = Smem<D>;
+  extern __shared__ __align__(16) unsigned char smem[];
+  float* s_max = reinterpret_cast<float*>(smem + S::kMax);
+  float* s_kscale = reinterpret_cast<float*>(smem + S::kScale);
+  float* s_vscale = s_kscale + 2 * kRuns;
+  int* s_flag = reinterpret_cast<int*>(smem + S::kFlag);
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int pair = wave >> 1;
+  const int col = lane & 31;  // of the pair's
+  const int hi = lane >> 5;
+
+  // rows from the longest down, the last columns of a row first: a short tail of the launch
+  const int rr = blockIdx.y / p.Hkv;
+  const int g = blockIdx.y - rr * p.Hkv;
+  int b = rr;
+  int64_t tok0, tok1, prefix;
+  if (p.B <= kRankRows && p.B > 1) {
+    int64_t* s_len = reinterpret_cast<int64_t*>(smem);
+    int64_t* s_row = s_len + kRankRows;  // of the row of each rank: itself, its first token, the next row's, its prefix
+    int64_t c0 = 0, c1 = 0, before = 0;
+    if (tid < p.B) {
+      c0 = read_index(p.cu, p.idx_i64, tid);
+      c1 = read_index(p.cu, p.idx_i64, tid + 1);
+      before = read_index(p.prefix, p.idx_i64, tid);
+      s_len[tid] = c1 - c0 + before;
+    }
+    __syncthreads();
+    if (tid < p.B) {
+      const int64_t mine = c1 - c0 + before;
+      int rank = 0;
+      for (int u = 0; u < p.B; ++u) rank += s_len[u] > mine || (s_len[u] == mine && u < tid);
+      s_row[4 * rank] = tid;
+      s_row[4 * rank + 1] = c0;
+      s_row[4 * rank + 2] = c1;
+      s_row[4 * rank + 3] = before;
+    }
+    __syncthreads();
+    b = __builtin_amdgcn_readfirstlane(static_cast<int>(s_row[4 * rr]));
+    tok0 = uniform64(s_row[4 * rr + 1]);
+    tok1 = uniform64(s_row[4 * rr + 2]);
+    prefix = uniform64(s_row[4 * rr + 3]);
+    __syncthreads();
+  } else {
+    tok0 = read_index(p.cu, p.idx_i64, b);
+    tok1 = read_index(p.cu, p.idx_i64, b + 1);
+    prefix = read_index(p.prefix, p.idx_i64, b);
+  }
+  const int64_t n_new = min64(pp.max_new, min64(tok1, p.total) - tok0);
+  const int64_t ct0 = static_cast<int64_t>(gridDim.x) - 1 - blockIdx.x;
+  const int64_t x0 = ct0 * kCols;  // first column of the workgroup
+  if (tok0 < 0 || x0 >= n_new * p.G) return;
+  const int64_t last = min64(n_new * p.G, x0 + kCols) - 1;  // columns fit 31 bits
+  const int64_t kv_end = keys_of(p, prefix, last);          // keys that any column sees
+  const int64_t first_new = over_group(p, static_cast<uint32_t>(x0));
+  const int64_t first_pos = prefix + first_new;  // every column sees the keys up to here
+  const int64_t runs = (kv_end + kv8::kRun - 1) / kv8::kRun;
+  const int64_t all_tiles = (kv_end + kTile - 1) / kTile;
+  int64_t kt0 = 0, kt1 = all_tiles;
+  int parts = 1;
+  if (pp.splits > 1) {
+    parts = parts_of(pp, all_tiles);
+    if (static_cast<int>(blockIdx.z) >= parts) return;
+    kt0 = all_tiles * blockIdx.z / parts;
+    kt1 = all_tiles * (blockIdx.z + 1) / parts;
+  }
+  const uint8_t* kb = p.kpool + g * p.sG;
+  const uint8_t* vb = p.vpool + g * p.sG;
+
+  // columns and their positions past first_pos
+  const int n_cols = static_cast<int>(last - x0) + 1;
+  // A column as a token past the workgroup's first one and a head of the group, both small: offsets are 32 by 32 bits on
+  // top of uniform addresses (64-bit products of every row's own were 3000 cycles of a workgroup).
+  const int64_t first_tok = tok0 + first_new;
+  const uint32_t x_head = static_cast<uint32_t>(x0 - (first_tok - tok0) * p.G);  // head of the workgroup's first column
+  struct Place {
+    uint32_t token, head;
+  };
+  auto place_of = [&](const auto& c, int x) {
+    const uint32_t t = over_group(c, x_head + x);
+    return Place{t, x_head + x - t * static_cast<uint32_t>(c.G)};
+  };
+  auto row_of = [](const bf16_t* base, const Place& at, int64_t st, int64_t sh) {  // strides below 2^32
+    return base + (static_cast<uint64_t>(at.token) * static_cast<uint32_t>(st) + static_cast<uint64_t>(at.head) * static_cast<uint32_t>(sh));
+  };
+  // this lane's column as a position past first_pos
+  const int ahead = static_cast<int>(place_of(p, min(pair * 32 + col, n_cols - 1)).token);
+
+  // ---- the tiles' loads
+  // Lane l of `cur` holds the offset in the head's pool of run 64 c + l (-1: not there), of `nxt` that of the next 64,
+  // one vector load each 16 tiles (scalar loads of the table share their wait counter with LDS, and every tile stalled
+  // about 1000 cycles for them); the masks say which runs are there.
+  int64_t cur, nxt;
+  uint64_t cur_mask, nxt_mask;
+  auto chunk = [&](int64_t c) -> int64_t {
+    const ParamsAgain q = params_again();
+    const int64_t run = 64 * c + lane;
+    const int64_t lb = run >> (q->c.bs_shift - 4);
+    const int64_t at = (b * q->c.table_stride + min64(lb, q->c.max_blocks - 1)) << q->c.table_i64;
+    const int32_t lo = reinterpret_cast<const int32_t*>(q->c.tables)[at];
+    const int32_t hi = reinterpret_cast<const int32_t*>(q->c.tables)[at + q->c.table_i64];  // the entry itself where it has one word
+    const bool ok = (run < runs) & (static_cast<uint32_t>(lo) < static_cast<uint32_t>(q->c.num_blocks)) & ((hi == 0) | (q->c.table_i64 == 0));
+    const int64_t o = static_cast<int64_t>(ok ? lo : 0) * q->c.sP + (run & ((1 << (q->c.bs_shift - 4)) - 1)) * kv8::Run<D>::kBytes;
+    return ok ? o : -1;
+  };
+  // A wave loads run wave % 4 of a tile, waves 0 to 3 of its keys, 4 to 7 of its values.  One that is not there has no records
+  // and reads zeros.
+  const bool of_values = wave >= 4;
+  const uint8_t* own_pool = of_values ? vb : kb;
+  int64_t own;  // offset of that run of the tile last asked for, -1: not there
+  int there;    // which runs of that tile are there
+  auto offsets = [&](int64_t kt) {
+    const int at = static_cast<int>(kt & 15) * kRuns;
+    if (at == 0 && kt != kt0) {
+      cur = nxt;
+      cur_mask = nxt_mask;
+      nxt = chunk((kt >> 4) + 1);
+      nxt_mask = __ballot(nxt >= 0);
+    }
+    const uint32_t lo = __builtin_amdgcn_readlane(static_cast<uint32_t>(cur), at + (wave & 3));
+    const uint32_t hi = __builtin_amdgcn_readlane(static_cast<uint32_t>(cur >> 32), at + (wave & 3));
+    own = static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
+    there = static_cast<int>(cur_mask >> at) & 15;
+  };
+  uint4 stage[N];
+  uint32_t stage_scale;
+  auto ask = [&](int64_t kt) {
+    offsets(kt);
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(own_pool + (own < 0 ? 0 : own)), 0, own < 0 ? 0 : kv8::Run<D>::kBytes, 0x00020000);
+#pragma unroll
+    for (int s = 0; s < N; ++s) stage[s] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, 16 * lane + 1024 * s, 0, kShared));
+    stage_scale = __builtin_amdgcn_raw_buffer_load_b8(r, kv8::Run<D>::kCodes, 0, kShared);
+  };
+  // what of the stage no column sees, or not every column where it is NaN, leaves the product
+  auto trim = [&](int64_t kt, int buf) {
+    if (kt * kTile + kTile <= first_pos + 1) return;  // every column sees all of the tile
+    // keys that no column sees may hold anything, and 0 times a NaN is one
+    const uint32_t mask = tokens_mask(kv_end - kt * kTile - kv8::kRun * (wave & 3) - 4 * (lane >> 4));
+    uint32_t any = 0;
+    auto clean = [&](uint32_t& w) {
+      w &= mask;
+      const uint32_t bad = ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;  // bytes 0x7f and 0xff
+      any |= bad;
+      w &= ~((bad >> 7) * 255u);  // a NaN reaches only the columns that see its token: marked for them below
+    };
+#pragma unroll
+    for (int s = 0; s < N; ++s) {
+      clean(stage[s].x);
+      clean(stage[s].y);
+      clean(stage[s].z);
+      clean(stage[s].w);
+    }
+    if (any != 0) s_flag[buf] = static_cast<int>(kt - kt0) + 1;
+  };
+  auto put = [&](int64_t kt) {
+    const int i = static_cast<int>(kt - kt0);
+    const int buf = of_values ? i & (kValueBufs - 1) : i & (kKeyBufs - 1);
+    if (of_values) trim(kt, buf);
+    uint4* dst = reinterpret_cast<uint4*>(smem + (of_values ? S::kValues : 0) + (buf * kRuns + (wave & 3)) * S::kRunBytes) + lane;
+#pragma unroll
+    for (int s = 0; s < N; ++s) dst[64 * s] = stage[s];
+    if (lane == 0) (of_values ? s_vscale : s_kscale)[buf * kRuns + (wave & 3)] = kv8::scale_of(stage_scale);
+  };
+
+  float m_run = -INFINITY, l_run = 0.f, corr = 1.f;  // of the lane's column; corr: what the sums are still to be multiplied with
+  floatx16_v o[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) o[m] = floatx16_v(0.f);
+
+  // The output leaves through LDS as whole rows, a lane eight dims: the first two pairs' columns, then the
+  // others'
+  constexpr int kLanes = D / 8;  // of a row
+  constexpr int kRowsAtOnce = 64 * kWaves / kLanes;
+  constexpr int kSweeps = kCols / 2 / kRowsAtOnce;
+  const int in_row = tid % kLanes;
+  auto column_of = [&](int pass, int i) {
+    return kCols / 2 * pass + tid / kLanes + i * kRowsAtOnce;
+  };
+  uint4 gate[2][kSweeps];
+  auto ask_gate = [&](ParamsAgain late) {
+    if (late->c.gate == nullptr || parts > 1) return;
+    const bf16_t* base = late->c.gate + first_tok * late->c.gate_st + static_cast<int64_t>(g) * late->c.G * late->c.gate_sh;
+#pragma unroll
+    for (int pass = 0; pass < 2; ++pass)
+#pragma unroll
+      for (int i = 0; i < kSweeps; ++i) {
+        const Place at = place_of(late->c, min(column_of(pass, i), n_cols - 1));
+        const uint2* src = reinterpret_cast<const uint2*>(row_of(base, at, late->c.gate_st, late->c.gate_sh) + 8 * in_row);
+        const uint2 lo = src[0], hi = src[1];
+        gate[pass][i] = make_uint4(lo.x, lo.y, hi.x, hi.y);
+      }
+  };
+  if (kt0 < kt1) {
+    if (tid < kValueBufs) s_flag[tid] = 0;
+    // the query: lane 32 h + n has dims 64 s + 16 (h + 2 e) .. + 15 of column n, as the keys' lanes have them
+    bf16x8_v q[4 * N];
+    {
+      const int x = pair * 32 + col;
+      const bf16_t* base = p.q + first_tok * p.q_st + static_cast<int64_t>(g) * p.G * p.q_sh;
+      const uint4* row = reinterpret_cast<const uint4*>(row_of(base, place_of(p, min(x, n_cols - 1)), p.q_st, p.q_sh) + 16 * hi);
+#pragma unroll
+      for (int f = 0; f < 2 * N; ++f)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          uint4 u = row[4 * f + e];
+          if (x >= n_cols) u = make_uint4(0, 0, 0, 0);
+          q[2 * f + e] = __builtin_bit_cast(bf16x8_v, u);
+        }
+    }
+    cur = chunk(kt0 >> 4);
+    nxt = chunk((kt0 >> 4) + 1);
+    cur_mask = __ballot(cur >= 0);
+    nxt_mask = __ballot(nxt >= 0);
+    const float qk_scale = p.scale * kLog2e;
+    const int n = static_cast<int>(kt1 - kt0);
+    ask(kt0);
+    int there_next = there;
+    lds_barrier();  // the flags
+    put(kt0);
+    ask(kt0 + 1);
+    int there_after = there;
+    lds_barrier();  // the first tile
+
+    floatx16_v sc;       // scores of the tile whose probabilities come next
+    float top = 0.f;     // of its column, in this wave's half
+    bf16x8_v pb[2];      // the own probabilities of the tile whose products come next
+    const unsigned char* key_lane = smem + 2 * (wave & 1) * S::kRunBytes + (col >> 4) * S::kRunBytes + hi * 256 + (col & 15) * 16;
+    // scores of tile i against the wave's 32 keys, masked, and their largest
+    auto scores = [&](int i, int have, floatx16_v& x) {
+      const int buf = i & (kKeyBufs - 1);
+      const unsigned char* at = key_lane + buf * S::kTileBytes;
+      const float scale = s_kscale[buf * kRuns + 2 * (wave & 1) + (col >> 4)];
+      x = floatx16_v(0.f);
+#pragma unroll
+      for (int f = 0; f < 2 * N; ++f) {
+        const uint4 u = *reinterpret_cast<const uint4*>(at + 512 * f);
+        x = __builtin_amdgcn_mfma_f32_32x32x16_bf16(operand(u.x, u.y, scale, scale), q[2 * f], x, 0, 0, 0);
+        x = __builtin_amdgcn_mfma_f32_32x32x16_bf16(operand(u.z, u.w, scale, scale), q[2 * f + 1], x, 0, 0, 0);
+      }
+      const int64_t key0 = (kt0 + i) * kTile;
+      if (!(key0 + kTile <= first_pos + 1 && have == 15)) {
+        const int lim = static_cast<int>(max64(-1, min64(kTile - 1, min64(first_pos + ahead, kv_end - 1) - key0))) - 32 * (wave & 1);  // the last key the column sees
+        const int runs2 = have >> (2 * (wave & 1));
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (8 * (r >> 2) + 4 * hi + (r & 3) > lim || !(runs2 >> (r >> 3) & 1)) x[r] = -INFINITY;
+      }
+      float mx = fmaxf(x[0], x[1]);
+#pragma unroll
+      for (int r = 2; r < 16; ++r) mx = fmaxf(mx, x[r]);
+      const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+      top = fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
+      if (hi == 0) s_max[((i & 1) * kWaves + wave) * 32 + col] = top;
+    };
+    // probabilities of tile i: both waves of a pair move their columns' reference points alike
+    auto probabilities = [&](int i) {
+      const float mx = fmaxf(top, s_max[((i & 1) * kWaves + (wave ^ 1)) * 32 + col]) * qk_scale;
+      corr = 1.f;
+      if (__ballot(mx > m_run + kLazy) != 0) {
+        const float m_new = fmaxf(m_run, mx);
+        corr = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run - m_new);
+        m_run = m_new;
+        l_run *= corr;
+      }
+      const float use = m_run == -INFINITY ? 0.f : m_run;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r], qk_scale, -use));
+        l_run += pr;
+        pb[r >> 3][r & 7] = static_cast<__bf16>(pr);  // for the bf16 product; l_run has it unrounded
+      }
+      uint4* dst = reinterpret_cast<uint4*>(smem + S::kP) + ((i & 1) * kWaves + wave) * 128 + lane;
+      dst[0] = __builtin_bit_cast(uint4, pb[0]);
+      dst[64] = __builtin_bit_cast(uint4, pb[1]);
+    };
+    // products of tile i's values: o[m] has row 8 (r >> 2) + 4 h + (r & 3) = chunk c of 16 slice + c, dim 64 slice + 4 c + m of the
+    // wave's half (D = 256: slices 2 and 3 are the second half; D = 128: m 2 and 3 are)
+    constexpr int kHalf = D == 256 ? 2 * 1024 : 8;
+    const unsigned char* value_lane = smem + S::kValues + (wave & 1) * kHalf + (col >> 4) * 1024 + hi * 256 + (col & 15) * 16;
+    auto products = [&](int i, const bf16x8_v (&own_p)[2]) {
+      const uint4* src = reinterpret_cast<const uint4*>(smem + S::kP) + ((i & 1) * kWaves + (wave ^ 1)) * 128 + lane;
+      const bf16x8_v other[2] = {__builtin_bit_cast(bf16x8_v, src[0]), __builtin_bit_cast(bf16x8_v, src[64])};
+      const int buf = i & (kValueBufs - 1);
+      const unsigned char* at = value_lane + buf * S::kTileBytes;
+      const bool first = (wave & 1) == 0;
+#pragma unroll
+      for (int r = 0; r < kRuns; ++r) {
+        const float scale = s_vscale[buf * kRuns + r];
+        const bf16x8_v pr = (r < 2) == first ? own_p[r & 1] : other[r & 1];
+        uint32_t lo[MT], up[MT];
+        if constexpr (D == 256) {
+          const uint4 a = *reinterpret_cast<const uint4*>(at + r * S::kRunBytes), c = *reinterpret_cast<const uint4*>(at + r * S::kRunBytes + 512);
+          lo[0] = a.x, lo[1] = a.y, lo[2] = a.z, lo[3] = a.w;
+          up[0] = c.x, up[1] = c.y, up[2] = c.z, up[3] = c.w;
+        } else {
+          const uint2 a = *reinterpret_cast<const uint2*>(at + r * S::kRunBytes), c = *reinterpret_cast<const uint2*>(at + r * S::kRunBytes + 512);
+          lo[0] = a.x, lo[1] = a.y;
+          up[0] = c.x, up[1] = c.y;
+        }
+#pragma unroll
+        for (int m = 0; m < MT; ++m) o[m] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(operand(lo[m], up[m], scale, scale), pr, o[m], 0, 0, 0);
+      }
+      // ---- NaNs among keys that not every column sees
+      if (s_flag[buf] == i + 1) {
+        const ParamsAgain again = params_again();
+        for (int t = 0; t < kTile; ++t) {
+          const int64_t key = (kt0 + i) * kTile + t;
+          const int32_t ph = block_of_run(again->c, b, key >> 4, runs);
+          if (ph < 0 || key >= kv_end) continue;
+          const uint8_t* run = again->c.vpool + g * again->c.sG + static_cast<int64_t>(ph) * again->c.sP + ((key >> 4) & ((1 << (again->c.bs_shift - 4)) - 1)) * kv8::Run<D>::kBytes;
+          const uint8_t* mine = run + (wave & 1) * kHalf + ((t & 15) >> 2) * 256 + (t & 3);
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+              if ((mine[(r >> 3) * 1024 + (8 * (r >> 2 & 1) + 4 * hi + (r & 3)) * 16 + 4 * m] & 0x7f) == 0x7f && key <= first_pos + ahead) o[m][r] = __uint_as_float(0x7fc00000u);
+        }
+      }
+    };
+    scores(0, there_next, sc);
+    put(kt0 + 1);
+    there_next = there_after;
+    lds_barrier();
+
+    auto iterate = [&](int i, auto has_scores, auto has_values) {
+      if constexpr (has_scores) ask(kt0 + i + 2);
+      if constexpr (has_values) {
+        if (__ballot(corr != 1.f) != 0) {  // columns whose reference point moved at the tile whose products come now
+#pragma unroll
+          for (int m = 0; m < MT; ++m) o[m] *= corr;
+        }
+      }
+      bf16x8_v before[2] = {pb[0], pb[1]};
+      floatx16_v sc_next;
+      if constexpr (has_values) products(i - 1, before);
+      probabilities(i);
+      if constexpr (has_scores) {
+        scores(i + 1, there_next, sc_next);
+        sc = sc_next;
+        there_next = there;
+        put(kt0 + i + 2);
+      }
+      lds_barrier();
+    };
+    using yes = std::integral_constant<bool, true>;
+    using no = std::integral_constant<bool, false>;
+    if (n > 1) {
+      iterate(0, yes{}, no{});
+      for (int i = 1; i + 1 < n; ++i) iterate(i, yes{}, yes{});
+      iterate(n - 1, no{}, yes{});
+    } else {
+      iterate(0, no{}, no{});
+    }
+    if (__ballot(corr != 1.f) != 0) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m) o[m] *= corr;
+    }
+    products(n - 1, pb);
+  }
+
+  // ---- out, through LDS
+  const ParamsAgain late = params_again();
+  const int64_t row0 = first_tok * late->c.H + static_cast<int64_t>(g) * late->c.G;  // of the output
+  ask_gate(late);
+  __syncthreads();
+  float* s_l = s_max;  // [half][column]; then the reference points
+  const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(l_run), __float_as_uint(l_run), false, false);
+  if (hi == 0) {
+    s_l[(wave & 1) * kCols + 32 * pair + col] = __uint_as_float(both[0]) + __uint_as_float(both[1]);
+    s_l[2 * kCols + 32 * pair + col] = m_run;  // of either wave, the same
+  }
+  constexpr int kRowFloats = D + 4;
+  static_assert(kCols / 2 * kRowFloats * 4 <= S::kP && 3 * kCols <= 2 * kWaves * 32, "half of the columns fit below the sums");
+  float* s_o = reinterpret_cast<float*>(smem);
+#pragma unroll
+  for (int pass = 0; pass < 2; ++pass) {
+    if (pass == 1) lds_barrier();  // the first columns have been read
+    if (pair >> 1 == pass) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        float* row = s_o + (32 * (pair & 1) + col) * kRowFloats + 64 * (r >> 3) + 4 * (8 * (r >> 2 & 1) + 4 * hi + (r & 3));
+        if constexpr (D == 256)
+          *reinterpret_cast<floatx4_v*>(row + 128 * (wave & 1)) = floatx4_v{o[0][r], o[1][r], o[2][r], o[3][r]};
+        else
+          *reinterpret_cast<floatx2_v*>(row + 2 * (wave & 1)) = floatx2_v{o[0][r], o[1][r]};
+      }
+    }
+    lds_barrier();
+#pragma unroll
+    for (int i = 0; i < kSweeps; ++i) {
+      const int x = column_of(pass, i);
+      if (x >= n_cols) continue;
+      const float* at = s_o + (tid / kLanes + i * kRowsAtOnce) * kRowFloats;
+      const Place pl = place_of(late->c, x);
+      const uint32_t row = pl.token * static_cast<uint32_t>(late->c.H) + pl.head;  // past row0
+      const float l = s_l[x] + s_l[kCols + x];
+      if (parts > 1) {
+        const int64_t part = (blockIdx.z * late->part_tokens + part_base(*late, b, tok0) - tok0) * late->c.H + row0 + row;
+        if (in_row == 0) *reinterpret_cast<float2*>(late->part_ml + part * 2) = make_float2(s_l[2 * kCols + x], l);
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+          *reinterpret_cast<floatx4_v*>(late->part_o + part * D + 4 * in_row + k * D / 2) = *reinterpret_cast<const floatx4_v*>(at + 4 * in_row + k * D / 2);
+        continue;
+      }
+      const float over = l == 0.f ? 0.f : 1.f / l;  // a query that saw nothing has sums of 0
+      const floatx4_v lo = *reinterpret_cast<const floatx4_v*>(at + 8 * in_row), hi = *reinterpret_cast<const floatx4_v*>(at + 8 * in_row + 4);
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = (e < 4 ? lo[e & 3] : hi[e & 3]) * over;
+      if (late->c.gate != nullptr) {
+        const uint32_t w[4] = {gate[pass][i].x, gate[pass][i].y, gate[pass][i].z, gate[pass][i].w};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] *= sigmoid(__uint_as_float(e & 1 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16));
+      }
+      uint32_t out[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) out[e] = static_cast<uint32_t>(f32_to_bf16(v[2 * e])) | static_cast<uint32_t>(f32_to_bf16(v[2 * e + 1])) << 16;
+      *reinterpret_cast<uint4*>(late->c.out + row0 * D + (static_cast<uint64_t>(row) * D + 8 * in_row)) = make_uint4(out[0], out[1], out[2], out[3]);
+    }
+  }
+}
+
+template <int D>
+static int launch(const PrefillParams& p, dim3 grid, hipStream_t stream) {
+  if (int rc = reserve_lds<&prefill_kernel<D>>("paged_attention_prefill_kv8", Smem<D>::kBytes)) return rc;
+  {
+    KernelTimer timer_("prefill_kv8", stream);
+    hipLaunchKernelGGL(prefill_kernel<D>, grid, dim3(64 * kWaves), Smem<D>::kBytes, stream, p);
+  }
+  if (int rc = check_launch("paged_attention_prefill_kv8")) return rc;
+  return join<D>(p, "paged_attention_prefill_kv8", "prefill_kv8_join", stream);
+}
+
+}  // namespace prefill8
+}  // namespace qa
+
+extern "C" int64_t qa_paged_attention_prefill_kv8_workspace(int64_t total_new, int64_t batch, int64_t max_new, int32_t heads, int32_t kv_heads, int32_t head_dim,
+                                                            int64_t max_tokens) {
+  return qa::attn::workspace_bytes_of(total_new, batch, max_new, heads, kv_heads, head_dim, max_tokens);
+}
+
+extern "C" int qa_paged_attention_prefill_kv8(const void* query, int32_t q_dtype, int64_t q_stride_t, int64_t q_stride_h, int64_t total_new, const void* cu_seqlens,
+                                              const void* prefix_lens, int32_t idx_dtype, int64_t batch, int64_t max_new, int32_t heads, int32_t head_dim,
+                                              const qa_paged_kv* kv, const void* block_tables, int32_t table_dtype, int64_t table_stride, int64_t max_blocks,
+                                              int32_t block_size, float scale, const void* gate, int64_t gate_stride_t, int64_t gate_stride_h, void* output,
+                                              void* workspace, int64_t workspace_bytes, hipStream_t stream) {
+  using namespace qa;
+  using namespace qa::prefill8;
+  PrefillParams p{};
+  const Args a{"paged_attention_prefill_kv8", query, q_dtype, q_stride_t, q_stride_h, total_new, batch, heads, head_dim, kv, block_tables, table_dtype, table_stride, max_blocks,
+               idx_dtype, block_size, scale, gate, gate_stride_t, gate_stride_h, output};
+  if (int rc = fill(p.c, a)) return rc;
+  if (int rc = share_out(p, a, cu_seqlens, prefix_lens, max_new, workspace, workspace_bytes)) return rc;
+  if (p.max_new == 0) return 0;
+  const dim3 grid(static_cast<unsigned>(ceil_div(p.max_new * p.c.G, kCols)), static_cast<unsigned>(batch * kv->kv_heads), static_cast<unsigned>(p.splits));
+  return head_dim == 256 ? launch<256>(p, grid, stream) : launch<128>(p, grid, stream);
+}

@@ -23,7 +23,7 @@ LIBRARY_PATH = PACKAGE_DIR / "build" / "libqwen36_hip.so"
 
 _LIB: Any | None = None
 
-QA_F32, QA_BF16, QA_F16, QA_I32, QA_I64, QA_KV4 = 0, 1, 2, 3, 4, 5
+QA_F32, QA_BF16, QA_F16, QA_I32, QA_I64, QA_KV4, QA_KV8 = 0, 1, 2, 3, 4, 5, 6
 
 c_void_p = ctypes.c_void_p
 c_int32 = ctypes.c_int32
@@ -176,6 +176,42 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
          c_int64, c_int64, c_int32, c_float, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_void_p],
     ),
     "qa_paged_attention_prefill_kv4_workspace": (c_int64, [c_int64, c_int64, c_int64, c_int32, c_int32, c_int32, c_int64]),
+    "qa_paged_kv8_append": (
+        c_int32,
+        [c_void_p, c_void_p, c_int32, c_int64, c_int64, c_int64, c_int64, c_int64, c_int32, ctypes.POINTER(PagedKV), c_void_p, c_int32, c_int32, c_void_p],
+    ),
+    "qa_paged_kv8_gather": (
+        c_int32,
+        [ctypes.POINTER(PagedKV), c_int32, c_int64, c_void_p, c_int32, c_int64, c_int64, c_int64, c_int32, c_void_p, c_void_p, c_void_p],
+    ),
+    "qa_paged_attention_decode_kv8_workspace": (c_int64, [c_int64, c_int32, c_int32, c_int32, c_int64]),
+    "qa_paged_attention_decode_kv8": (
+        c_int32,
+        [c_void_p, c_int32, c_int64, c_int64, c_int64, c_int32, c_int32, ctypes.POINTER(PagedKV), c_void_p, c_int32, c_int64, c_int64, c_void_p, c_int32, c_int32,
+         c_float, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_void_p],
+    ),
+    "qa_paged_attention_prefill_kv8": (
+        c_int32,
+        [c_void_p, c_int32, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int32, c_int64, c_int64, c_int32, c_int32, ctypes.POINTER(PagedKV), c_void_p, c_int32,
+         c_int64, c_int64, c_int32, c_float, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_void_p],
+    ),
+    "qa_paged_attention_prefill_kv8_workspace": (c_int64, [c_int64, c_int64, c_int64, c_int32, c_int32, c_int32, c_int64]),
+    "qa_paged_kv_fork": (
+        c_int32,
+        [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int32, c_int64, c_int32, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+         c_void_p],
+    ),
+    "qa_paged_kv_release_workspace": (c_int64, [c_int64]),
+    "qa_paged_kv_release": (
+        c_int32,
+        [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int32, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p],
+    ),
+    "qa_paged_kv_compact_workspace": (c_int64, [c_int64]),
+    "qa_paged_kv_compact": (
+        c_int32,
+        [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_void_p],
+    ),
+    "qa_paged_kv_copy": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int32, c_int64, c_void_p]),
     "qa_qk_norm_mrope_append": (
         c_int32,
         [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int32, c_float, c_void_p, c_void_p, c_int32,

@@ -1254,20 +1254,14 @@ def paged_kv_plan(
     return PagedPlan(cu_seqlens, starts, positions, slots)
 
 
-def paged_kv4_append(key: torch.Tensor, value: torch.Tensor, key_pool: torch.Tensor, value_pool: torch.Tensor, slots: torch.Tensor, block_size: int) -> None:
-    """Quantise packed K/V rows ``(tokens, H_kv, D)`` (bf16 or fp32) into ``slots`` of a 4-bit pool, in place.
-
-    The pools are uint8 ``(P, H_kv, kv4_tile_bytes(D, block_size))``; per 32 dims of a token a power-of-two scale and
-    E2M1 codes (the format and layout stand in ``qwen36_hip.h``).  ``slots`` ``(tokens,)`` hold ``block id *
-    block_size + position % block_size`` (:func:`paged_kv_plan`); those outside the pool, such as -1, are skipped.
-    They have to be distinct.
-    """
+def _tiles_append(what: str, descriptor: Any, key: torch.Tensor, value: torch.Tensor, key_pool: torch.Tensor, value_pool: torch.Tensor, slots: torch.Tensor, block_size: int) -> None:
+    """``paged_kv4_append`` and ``paged_kv8_append``: the operator of a pool of tiles in 4 or 8 bits; ``descriptor`` checks the pool."""
     lib = L.load_library()
     device = key.device
     if device.type != "cuda" or not (value.device == slots.device == device):
         _same_device(device, key=key, value=value, slots=slots)
     _index_dtype(slots, "slots")
-    desc, head_dim = _kv4_descriptor(key_pool, value_pool, block_size, device)
+    desc, head_dim = descriptor(key_pool, value_pool, block_size, device)
     shape = key.shape
     _require(len(shape) == 3 and shape[1] == desc.kv_heads and shape[2] == head_dim and value.shape == shape, "key/value must be (tokens, kv_heads, head_dim) of the pool's heads")
     _float_dtype(key, "key")
@@ -1278,24 +1272,20 @@ def paged_kv4_append(key: torch.Tensor, value: torch.Tensor, key_pool: torch.Ten
     v, v_st, v_sh = _rows(value, multiple)
     s = slots.contiguous()
     code = _launch(
-        device, lib.qa_paged_kv4_append, k.data_ptr(), v.data_ptr(), _code(k), k_st, k_sh, v_st, v_sh, shape[0], head_dim, ctypes.byref(desc), s.data_ptr(), _code(s),
+        device, getattr(lib, f"qa_{what}"), k.data_ptr(), v.data_ptr(), _code(k), k_st, k_sh, v_st, v_sh, shape[0], head_dim, ctypes.byref(desc), s.data_ptr(), _code(s),
         int(block_size),
     )
-    L.check(lib, code, "paged_kv4_append")
+    L.check(lib, code, what)
 
 
-def paged_kv4_gather(key_pool: torch.Tensor, value_pool: torch.Tensor, block_tables: torch.Tensor, valid: int, block_size: int) -> tuple[torch.Tensor, torch.Tensor]:
-    """Dense ``(B, H_kv, valid, D)`` bf16 K/V of a 4-bit pool in logical order (:func:`paged_kv_gather`'s counterpart).
-
-    Every value the cache holds is exact in bf16.  Tokens whose block id is outside the pool, or past the table, are
-    zeros; a group stored from an infinity or a NaN reads as NaN.
-    """
+def _tiles_gather(what: str, descriptor: Any, key_pool: torch.Tensor, value_pool: torch.Tensor, block_tables: torch.Tensor, valid: int, block_size: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """``paged_kv4_gather`` and ``paged_kv8_gather``: the operator of a pool of tiles in 4 or 8 bits; ``descriptor`` checks the pool."""
     lib = L.load_library()
     device = key_pool.device
     if device.type != "cuda" or block_tables.device != device:
         _same_device(device, key_pool=key_pool, block_tables=block_tables)
     _index_dtype(block_tables, "block_tables")
-    desc, head_dim = _kv4_descriptor(key_pool, value_pool, block_size, device)
+    desc, head_dim = descriptor(key_pool, value_pool, block_size, device)
     tables = block_tables.contiguous()
     if tables.dim() == 1:
         tables = tables.unsqueeze(0)
@@ -1306,11 +1296,103 @@ def paged_kv4_gather(key_pool: torch.Tensor, value_pool: torch.Tensor, block_tab
     key_out = torch.empty((batch, desc.kv_heads, valid, head_dim), dtype=torch.bfloat16, device=device)
     value_out = torch.empty_like(key_out)
     code = _launch(
-        device, lib.qa_paged_kv4_gather, ctypes.byref(desc), head_dim, batch, tables.data_ptr(), _code(tables), max_blocks, max_blocks, valid, int(block_size),
+        device, getattr(lib, f"qa_{what}"), ctypes.byref(desc), head_dim, batch, tables.data_ptr(), _code(tables), max_blocks, max_blocks, valid, int(block_size),
         key_out.data_ptr(), value_out.data_ptr(),
     )
-    L.check(lib, code, "paged_kv4_gather")
+    L.check(lib, code, what)
     return key_out, value_out
+
+
+def _tiles_decode(
+    what: str, descriptor: Any, query: torch.Tensor, block_tables: torch.Tensor, key_pool: torch.Tensor, value_pool: torch.Tensor, sequence_lengths: torch.Tensor, block_size: int,
+    gate: torch.Tensor | None, scale: float | None, out: torch.Tensor | None,
+) -> torch.Tensor:
+    """``paged_attention_decode_kv4`` and ``paged_attention_decode_kv8``: the operator of a pool of tiles in 4 or 8 bits; ``descriptor`` checks the pool."""
+    lib = L.load_library()
+    device = query.device
+    if device.type != "cuda" or not (block_tables.device == sequence_lengths.device == device):
+        _same_device(device, query=query, block_tables=block_tables, sequence_lengths=sequence_lengths)
+    _require(query.dtype is torch.bfloat16, "query must be bfloat16")
+    _index_dtype(block_tables, "block_tables")
+    _index_dtype(sequence_lengths, "sequence_lengths")
+    shape = query.shape
+    _require(len(shape) == 4 and shape[2] == 1, "query must have shape [batch, heads, 1, head_dim]")
+    desc, head_dim = descriptor(key_pool, value_pool, block_size, device)
+    batch, heads = shape[0], shape[1]
+    _require(shape[3] == head_dim, "KV head_dim must match query")
+    _require(block_tables.dim() == 2 and block_tables.shape[0] == batch and block_tables.shape[1] > 0, "block_tables must have shape [batch, max_blocks]")
+    _require(sequence_lengths.shape == shape[:1], "sequence_lengths batch must match query")
+    _require(heads % desc.kv_heads == 0, "KV heads must divide query heads")
+    q, q_sb, q_sh = _rows(query, 8)
+    g, g_ptr, g_sb, g_sh = _kv4_gate(gate, batch, heads, head_dim, device)
+    tables, lens = block_tables.contiguous(), sequence_lengths.contiguous()
+    max_blocks = tables.shape[1]
+    result = _kv4_out(out, query)
+    nbytes = getattr(lib, f"qa_{what}_workspace")(batch, heads, desc.kv_heads, head_dim, max_blocks * block_size)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    code = _launch(
+        device, getattr(lib, f"qa_{what}"), q.data_ptr(), L.QA_BF16, q_sb, q_sh, batch, heads, head_dim, ctypes.byref(desc), tables.data_ptr(), _code(tables),
+        max_blocks, max_blocks, lens.data_ptr(), _code(lens), int(block_size), float(scale or 0.0), g_ptr, g_sb, g_sh, result.data_ptr(), _ptr(ws), nbytes,
+    )
+    L.check(lib, code, what)
+    return result
+
+
+def _tiles_prefill(
+    what: str, descriptor: Any, query: torch.Tensor, cu_seqlens: torch.Tensor, prefix_lens: torch.Tensor, key_pool: torch.Tensor, value_pool: torch.Tensor, block_tables: torch.Tensor,
+    block_size: int, max_new: int, gate: torch.Tensor | None, scale: float | None, out: torch.Tensor | None,
+) -> torch.Tensor:
+    """``paged_attention_prefill_kv4`` and ``paged_attention_prefill_kv8``: the operator of a pool of tiles in 4 or 8 bits; ``descriptor`` checks the pool."""
+    lib = L.load_library()
+    device = query.device
+    if device.type != "cuda" or not (cu_seqlens.device == prefix_lens.device == block_tables.device == device):
+        _same_device(device, query=query, cu_seqlens=cu_seqlens, prefix_lens=prefix_lens, block_tables=block_tables)
+    shape = query.shape
+    _require(query.dtype is torch.bfloat16 and len(shape) == 3, "query must be (tokens, heads, head_dim) bfloat16")
+    _index_dtype(cu_seqlens, "cu_seqlens")
+    _index_dtype(block_tables, "block_tables")
+    _require(cu_seqlens.dtype is prefix_lens.dtype, "cu_seqlens and prefix_lens must share a dtype")
+    desc, head_dim = descriptor(key_pool, value_pool, block_size, device)
+    tokens, heads = shape[0], shape[1]
+    _require(shape[2] == head_dim, "KV head_dim must match query")
+    _require(heads % desc.kv_heads == 0, "KV heads must divide query heads")
+    _require(prefix_lens.dim() == 1 and cu_seqlens.shape == (prefix_lens.shape[0] + 1,), "cu_seqlens must have batch + 1 entries")
+    batch = prefix_lens.shape[0]
+    _require(block_tables.dim() == 2 and block_tables.shape[0] == batch and block_tables.shape[1] > 0, "block_tables must have shape [batch, max_blocks]")
+    q, q_st, q_sh = _rows(query, 8)
+    g, g_ptr, g_st, g_sh = _kv4_gate(gate, tokens, heads, head_dim, device)
+    cu, prefix, tables = cu_seqlens.contiguous(), prefix_lens.contiguous(), block_tables.contiguous()
+    max_blocks = tables.shape[1]
+    result = _kv4_out(out, query)
+    nbytes = getattr(lib, f"qa_{what}_workspace")(tokens, batch, int(max_new), heads, desc.kv_heads, head_dim, max_blocks * block_size)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    code = _launch(
+        device, getattr(lib, f"qa_{what}"), q.data_ptr(), L.QA_BF16, q_st, q_sh, tokens, cu.data_ptr(), prefix.data_ptr(), _code(cu), batch, int(max_new),
+        heads, head_dim, ctypes.byref(desc), tables.data_ptr(), _code(tables), max_blocks, max_blocks, int(block_size), float(scale or 0.0), g_ptr, g_st, g_sh,
+        result.data_ptr(), _ptr(ws), nbytes,
+    )
+    L.check(lib, code, what)
+    return result
+
+
+def paged_kv4_append(key: torch.Tensor, value: torch.Tensor, key_pool: torch.Tensor, value_pool: torch.Tensor, slots: torch.Tensor, block_size: int) -> None:
+    """Quantise packed K/V rows ``(tokens, H_kv, D)`` (bf16 or fp32) into ``slots`` of a 4-bit pool, in place.
+
+    The pools are uint8 ``(P, H_kv, kv4_tile_bytes(D, block_size))``; per 32 dims of a token a power-of-two scale and
+    E2M1 codes (the format and layout stand in ``qwen36_hip.h``).  ``slots`` ``(tokens,)`` hold ``block id *
+    block_size + position % block_size`` (:func:`paged_kv_plan`); those outside the pool, such as -1, are skipped.
+    They have to be distinct.
+    """
+    _tiles_append("paged_kv4_append", _kv4_descriptor, key, value, key_pool, value_pool, slots, block_size)
+
+
+def paged_kv4_gather(key_pool: torch.Tensor, value_pool: torch.Tensor, block_tables: torch.Tensor, valid: int, block_size: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """Dense ``(B, H_kv, valid, D)`` bf16 K/V of a 4-bit pool in logical order (:func:`paged_kv_gather`'s counterpart).
+
+    Every value the cache holds is exact in bf16.  Tokens whose block id is outside the pool, or past the table, are
+    zeros; a group stored from an infinity or a NaN reads as NaN.
+    """
+    return _tiles_gather("paged_kv4_gather", _kv4_descriptor, key_pool, value_pool, block_tables, valid, block_size)
 
 
 def paged_attention_decode_kv4(
@@ -1331,34 +1413,7 @@ def paged_attention_decode_kv4(
     sigmoid(gate)``.  Rows of length <= 0, and rows that see only blocks outside the pool, give zeros.  Returns
     ``(B, H, 1, D)`` bf16, in ``out`` where it is given.
     """
-    lib = L.load_library()
-    device = query.device
-    if device.type != "cuda" or not (block_tables.device == sequence_lengths.device == device):
-        _same_device(device, query=query, block_tables=block_tables, sequence_lengths=sequence_lengths)
-    _require(query.dtype is torch.bfloat16, "query must be bfloat16")
-    _index_dtype(block_tables, "block_tables")
-    _index_dtype(sequence_lengths, "sequence_lengths")
-    shape = query.shape
-    _require(len(shape) == 4 and shape[2] == 1, "query must have shape [batch, heads, 1, head_dim]")
-    desc, head_dim = _kv4_descriptor(key_pool, value_pool, block_size, device)
-    batch, heads = shape[0], shape[1]
-    _require(shape[3] == head_dim, "KV head_dim must match query")
-    _require(block_tables.dim() == 2 and block_tables.shape[0] == batch and block_tables.shape[1] > 0, "block_tables must have shape [batch, max_blocks]")
-    _require(sequence_lengths.shape == shape[:1], "sequence_lengths batch must match query")
-    _require(heads % desc.kv_heads == 0, "KV heads must divide query heads")
-    q, q_sb, q_sh = _rows(query, 8)
-    g, g_ptr, g_sb, g_sh = _kv4_gate(gate, batch, heads, head_dim, device)
-    tables, lens = block_tables.contiguous(), sequence_lengths.contiguous()
-    max_blocks = tables.shape[1]
-    result = _kv4_out(out, query)
-    nbytes = lib.qa_paged_attention_decode_kv4_workspace(batch, heads, desc.kv_heads, head_dim, max_blocks * block_size)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-    code = _launch(
-        device, lib.qa_paged_attention_decode_kv4, q.data_ptr(), L.QA_BF16, q_sb, q_sh, batch, heads, head_dim, ctypes.byref(desc), tables.data_ptr(), _code(tables),
-        max_blocks, max_blocks, lens.data_ptr(), _code(lens), int(block_size), float(scale or 0.0), g_ptr, g_sb, g_sh, result.data_ptr(), _ptr(ws), nbytes,
-    )
-    L.check(lib, code, "paged_attention_decode_kv4")
-    return result
+    return _tiles_decode("paged_attention_decode_kv4", _kv4_descriptor, query, block_tables, key_pool, value_pool, sequence_lengths, block_size, gate, scale, out)
 
 
 def paged_attention_prefill_kv4(
@@ -1382,36 +1437,240 @@ def paged_attention_prefill_kv4(
     (tokens past it are not computed).  Returns ``(tokens, H, D)`` bf16, in ``out`` where it is given; rows past the
     last sequence are not written.
     """
+    return _tiles_prefill("paged_attention_prefill_kv4", _kv4_descriptor, query, cu_seqlens, prefix_lens, key_pool, value_pool, block_tables, block_size, max_new, gate, scale, out)
+
+
+def kv8_tile_bytes(head_dim: int, block_size: int) -> int:
+    """Bytes of one block of one KV head in an 8-bit pool: 8 bits a value, and 16 bytes per 16 tokens for their scale."""
+    _require(head_dim in (128, 256), "8-bit pools need head_dim 128 or 256")
+    _require(16 <= block_size <= 1024 and block_size & (block_size - 1) == 0, "8-bit pools need a block_size that is a power of two from 16 to 1024")
+    return block_size * (head_dim + 1)
+
+
+def _kv8_descriptor(key_pool: torch.Tensor, value_pool: torch.Tensor, block_size: int, device: torch.device) -> tuple[L.PagedKV, int]:
+    """Descriptor and head_dim of an 8-bit pool ``(P, H_kv, kv8_tile_bytes(D, block_size))``."""
+    if key_pool.device != device or value_pool.device != device:
+        _same_device(device, key_pool=key_pool, value_pool=value_pool)
+    shape, strides = key_pool.shape, key_pool.stride()
+    if key_pool.dtype is not torch.float8_e4m3fn or value_pool.dtype is not torch.float8_e4m3fn or len(shape) != 3 or value_pool.shape != shape:
+        raise RuntimeError("8-bit pools must be float8_e4m3fn (blocks, kv_heads, tile bytes) and alike")
+    if strides[2] != 1 or value_pool.stride() != strides:
+        raise RuntimeError("key/value pools must share strides with contiguous tiles")
+    blocks, kv_heads, tile = shape
+    for head_dim in (256, 128):
+        if tile == block_size * (head_dim + 1):
+            return L.PagedKV(key_pool.data_ptr(), value_pool.data_ptr(), None, None, None, blocks, 0, strides[0], strides[1], 0, kv_heads, L.QA_KV8), head_dim
+    raise RuntimeError(f"a tile of {tile} bytes is no block of {block_size} tokens of 128 or 256 dims in 8 bits")
+
+
+def paged_kv8_append(key: torch.Tensor, value: torch.Tensor, key_pool: torch.Tensor, value_pool: torch.Tensor, slots: torch.Tensor, block_size: int) -> None:
+    """Quantise packed K/V rows ``(tokens, H_kv, D)`` (bf16 or fp32) into ``slots`` of an 8-bit pool, in place.
+
+    The pools are float8_e4m3fn ``(P, H_kv, kv8_tile_bytes(D, block_size))``: E4M3 codes, and a power-of-two scale for each run of
+    16 tokens of a block and head (the format and layout stand in ``qwen36_hip.h``).  A run's scale fits the values that the call
+    writes to it; a call that goes on with a run never makes its scale smaller, and where it grows, rounds the codes of the
+    tokens before to it.  ``slots`` ``(tokens,)`` hold ``block id * block_size + position % block_size``
+    (:func:`paged_kv_plan`); those outside the pool, such as -1, are skipped.  They have to be distinct, with the tokens of
+    a run next to each other, as a plan's are.
+    """
+    _tiles_append("paged_kv8_append", _kv8_descriptor, key, value, key_pool, value_pool, slots, block_size)
+
+
+def paged_kv8_gather(key_pool: torch.Tensor, value_pool: torch.Tensor, block_tables: torch.Tensor, valid: int, block_size: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """Dense ``(B, H_kv, valid, D)`` bf16 K/V of an 8-bit pool in logical order (:func:`paged_kv_gather`'s counterpart).
+
+    Every value the cache holds is exact in bf16.  Tokens whose block id is outside the pool, or past the table, are
+    zeros; a value stored from an infinity or a NaN reads as NaN.
+    """
+    return _tiles_gather("paged_kv8_gather", _kv8_descriptor, key_pool, value_pool, block_tables, valid, block_size)
+
+
+def paged_attention_decode_kv8(
+    query: torch.Tensor,
+    block_tables: torch.Tensor,
+    key_pool: torch.Tensor,
+    value_pool: torch.Tensor,
+    sequence_lengths: torch.Tensor,
+    block_size: int,
+    *,
+    gate: torch.Tensor | None = None,
+    scale: float | None = None,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """``paged_attention_decode_batched`` over an 8-bit pool: one token per row, ``query`` ``(B, H, 1, D)`` bf16.
+
+    ``gate`` ``(B, H*D)`` or ``(B, H, D)`` bf16 logits (a view of ``q_proj`` is read in place) give ``out *
+    sigmoid(gate)``.  Rows of length <= 0, and rows that see only blocks outside the pool, give zeros.  Returns
+    ``(B, H, 1, D)`` bf16, in ``out`` where it is given.
+    """
+    return _tiles_decode("paged_attention_decode_kv8", _kv8_descriptor, query, block_tables, key_pool, value_pool, sequence_lengths, block_size, gate, scale, out)
+
+
+def paged_attention_prefill_kv8(
+    query: torch.Tensor,
+    cu_seqlens: torch.Tensor,
+    prefix_lens: torch.Tensor,
+    key_pool: torch.Tensor,
+    value_pool: torch.Tensor,
+    block_tables: torch.Tensor,
+    block_size: int,
+    *,
+    max_new: int,
+    gate: torch.Tensor | None = None,
+    scale: float | None = None,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """:func:`paged_attention_prefill` over an 8-bit pool: causal attention of packed new tokens.
+
+    ``query`` ``(tokens, H, D)`` bf16; the new tokens' K/V are in the pool already, so a new token sees itself and
+    its neighbours in 8 bits, as every later step will.  ``max_new`` is at least the longest row of ``cu_seqlens``
+    (tokens past it are not computed).  Returns ``(tokens, H, D)`` bf16, in ``out`` where it is given; rows past the
+    last sequence are not written.
+    """
+    return _tiles_prefill("paged_attention_prefill_kv8", _kv8_descriptor, query, cu_seqlens, prefix_lens, key_pool, value_pool, block_tables, block_size, max_new, gate, scale, out)
+
+
+class PagedCopy(NamedTuple):
+    """Pages to be copied (:func:`paged_kv_copy`): int32 ``sources`` and ``targets``, -1 where there is none."""
+
+    sources: torch.Tensor
+    targets: torch.Tensor
+
+
+def _books(
+    device: torch.device, block_tables: torch.Tensor, lengths: torch.Tensor | None, free_list: torch.Tensor, free_state: torch.Tensor, references: torch.Tensor, status: torch.Tensor,
+) -> tuple[int, int]:
+    """Checks the books of a pool; their rows and the table's width."""
+    if device.type != "cuda" or not (free_list.device == free_state.device == references.device == status.device == device) or (lengths is not None and lengths.device != device):
+        _same_device(device, block_tables=block_tables, lengths=block_tables if lengths is None else lengths, free_list=free_list, free_state=free_state, references=references,
+                     status=status)
+    i32 = torch.int32
+    _require(block_tables.dtype is i32 and block_tables.dim() == 2 and block_tables.stride(1) == 1, "block_tables must be int32 [rows, max_blocks] with contiguous rows")
+    rows, max_blocks = block_tables.shape
+    _require(rows > 0 and max_blocks > 0, "block_tables must have shape [rows, max_blocks]")
+    if lengths is not None:
+        _require(lengths.dtype is i32 and lengths.shape == (rows,) and lengths.is_contiguous(), "lengths must be a contiguous int32 [rows] tensor")
+    _require(free_list.dtype is i32 and free_list.dim() == 1 and free_list.is_contiguous(), "free_list must be a contiguous int32 vector")
+    _require(free_state.dtype is i32 and free_state.numel() == 2 and free_state.is_contiguous(), "free_state must be int32 [head, count]")
+    _require(references.dtype is i32 and references.shape == free_list.shape and references.is_contiguous(), "references must be a contiguous int32 tensor with an entry for each block")
+    _require(status.dtype is i32 and status.numel() >= 1, "status must be an int32 tensor")
+    return rows, max_blocks
+
+
+def _row_list(rows: torch.Tensor, name: str, device: torch.device) -> torch.Tensor:
+    if rows.device != device:
+        _require_cuda(rows, name, device)
+    _index_dtype(rows, name)
+    _require(rows.dim() == 1, f"{name} must be a vector of table rows")
+    return rows.contiguous()
+
+
+def paged_kv_fork(
+    block_tables: torch.Tensor, lengths: torch.Tensor, source_rows: torch.Tensor, target_rows: torch.Tensor, free_list: torch.Tensor, free_state: torch.Tensor,
+    references: torch.Tensor, status: torch.Tensor, block_size: int,
+) -> PagedCopy:
+    """Makes each row ``target_rows[i]`` a copy of row ``source_rows[i]`` on the device, without copying what is full.
+
+    The new row shares the source's full blocks (``references`` ``(blocks,)`` int32 counts a block's holders beyond its first)
+    and takes the next block of the ascending ``free_list`` for a partly filled last one: the returned pages are to be copied in
+    every layer's pools (:func:`paged_kv_copy`) before either row grows.  Target rows have to be empty (length 0), distinct
+    and no sources; a source of -1 is no fork; at most 1024 a call.  Tables, lengths and ``free_state`` are those of
+    :func:`paged_kv_plan`.  ``status`` becomes 0, or 1 (pool exhausted), 3 (corrupt free state), 4 (a length that the table does
+    not hold), 6 (rows out of range, targets that are not empty or not distinct): then nothing is changed and no page is to be
+    copied.  Nothing is read back, so the call can be captured in a HIP graph.
+    """
     lib = L.load_library()
-    device = query.device
-    if device.type != "cuda" or not (cu_seqlens.device == prefix_lens.device == block_tables.device == device):
-        _same_device(device, query=query, cu_seqlens=cu_seqlens, prefix_lens=prefix_lens, block_tables=block_tables)
-    shape = query.shape
-    _require(query.dtype is torch.bfloat16 and len(shape) == 3, "query must be (tokens, heads, head_dim) bfloat16")
-    _index_dtype(cu_seqlens, "cu_seqlens")
-    _index_dtype(block_tables, "block_tables")
-    _require(cu_seqlens.dtype is prefix_lens.dtype, "cu_seqlens and prefix_lens must share a dtype")
-    desc, head_dim = _kv4_descriptor(key_pool, value_pool, block_size, device)
-    tokens, heads = shape[0], shape[1]
-    _require(shape[2] == head_dim, "KV head_dim must match query")
-    _require(heads % desc.kv_heads == 0, "KV heads must divide query heads")
-    _require(prefix_lens.dim() == 1 and cu_seqlens.shape == (prefix_lens.shape[0] + 1,), "cu_seqlens must have batch + 1 entries")
-    batch = prefix_lens.shape[0]
-    _require(block_tables.dim() == 2 and block_tables.shape[0] == batch and block_tables.shape[1] > 0, "block_tables must have shape [batch, max_blocks]")
-    q, q_st, q_sh = _rows(query, 8)
-    g, g_ptr, g_st, g_sh = _kv4_gate(gate, tokens, heads, head_dim, device)
-    cu, prefix, tables = cu_seqlens.contiguous(), prefix_lens.contiguous(), block_tables.contiguous()
-    max_blocks = tables.shape[1]
-    result = _kv4_out(out, query)
-    nbytes = lib.qa_paged_attention_prefill_kv4_workspace(tokens, batch, int(max_new), heads, desc.kv_heads, head_dim, max_blocks * block_size)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    device = block_tables.device
+    rows, max_blocks = _books(device, block_tables, lengths, free_list, free_state, references, status)
+    source, target = _row_list(source_rows, "source_rows", device), _row_list(target_rows, "target_rows", device)
+    _require(source.shape == target.shape and source.dtype is target.dtype, "source_rows and target_rows must be alike")
+    n = source.numel()
+    pages = lengths.new_empty((2, n))
     code = _launch(
-        device, lib.qa_paged_attention_prefill_kv4, q.data_ptr(), L.QA_BF16, q_st, q_sh, tokens, cu.data_ptr(), prefix.data_ptr(), _code(cu), batch, int(max_new),
-        heads, head_dim, ctypes.byref(desc), tables.data_ptr(), _code(tables), max_blocks, max_blocks, int(block_size), float(scale or 0.0), g_ptr, g_st, g_sh,
-        result.data_ptr(), _ptr(ws), nbytes,
+        device, lib.qa_paged_kv_fork, block_tables.data_ptr(), block_tables.stride(0), max_blocks, lengths.data_ptr(), rows, source.data_ptr(), target.data_ptr(), _code(source), n,
+        int(block_size), free_list.data_ptr(), free_list.numel(), free_state.data_ptr(), references.data_ptr(), status.data_ptr(), pages.data_ptr(), pages.data_ptr() + 4 * n,
     )
-    L.check(lib, code, "paged_attention_prefill_kv4")
-    return result
+    L.check(lib, code, "paged_kv_fork")
+    return PagedCopy(pages[0], pages[1])
+
+
+def paged_kv_release(
+    block_tables: torch.Tensor, lengths: torch.Tensor, release_rows: torch.Tensor, free_list: torch.Tensor, free_state: torch.Tensor, references: torch.Tensor,
+    status: torch.Tensor,
+) -> None:
+    """Frees the blocks of ``release_rows`` on the device and empties the rows.
+
+    A block that other rows hold too (:func:`paged_kv_fork`) loses a holder, the others go back to ``free_list``, which is then
+    ascending from its front.  Rows out of range are skipped, a row named twice is freed once.  ``status`` becomes 0, or 3
+    (corrupt free state: nothing is changed).  The device form of ``DeviceBlockAllocator.release``: nothing is read back.
+    """
+    lib = L.load_library()
+    device = block_tables.device
+    rows, max_blocks = _books(device, block_tables, lengths, free_list, free_state, references, status)
+    which = _row_list(release_rows, "release_rows", device)
+    nbytes = lib.qa_paged_kv_release_workspace(free_list.numel())
+    ws = torch.zeros(nbytes // 4, dtype=torch.int32, device=device)
+    code = _launch(
+        device, lib.qa_paged_kv_release, block_tables.data_ptr(), block_tables.stride(0), max_blocks, lengths.data_ptr(), rows, which.data_ptr(), _code(which), which.numel(),
+        free_list.data_ptr(), free_list.numel(), free_state.data_ptr(), references.data_ptr(), status.data_ptr(), ws.data_ptr(), nbytes,
+    )
+    L.check(lib, code, "paged_kv_release")
+
+
+def paged_kv_compact(
+    block_tables: torch.Tensor, free_list: torch.Tensor, free_state: torch.Tensor, references: torch.Tensor, status: torch.Tensor, *, max_moves: int,
+) -> PagedCopy:
+    """Moves the blocks of the tables to the pool's lowest ids, at most ``max_moves`` of them, on the device.
+
+    The largest id that the tables hold takes the lowest free one, and so on as long as that is lower: tables, ``references``
+    and ``free_list`` are as after the moves, and the returned pages ``(max_moves,)`` are to be copied in every layer's pools
+    (:func:`paged_kv_copy`).  Blocks that are neither free nor in these tables (another batch's, a host cache's) stay.
+    ``status`` becomes 0, or 3 (corrupt free state: nothing is changed).  Nothing is read back.
+    """
+    lib = L.load_library()
+    device = block_tables.device
+    rows, max_blocks = _books(device, block_tables, None, free_list, free_state, references, status)
+    max_moves = int(max_moves)
+    _require(max_moves >= 0, "max_moves must be non-negative")
+    pages = block_tables.new_empty((2, max_moves))
+    nbytes = lib.qa_paged_kv_compact_workspace(free_list.numel())
+    ws = torch.zeros(nbytes // 4, dtype=torch.int32, device=device)
+    code = _launch(
+        device, lib.qa_paged_kv_compact, block_tables.data_ptr(), block_tables.stride(0), max_blocks, rows, free_list.data_ptr(), free_list.numel(), free_state.data_ptr(),
+        references.data_ptr(), status.data_ptr(), max_moves, pages.data_ptr(), pages.data_ptr() + 4 * max_moves, ws.data_ptr(), nbytes,
+    )
+    L.check(lib, code, "paged_kv_compact")
+    return PagedCopy(pages[0], pages[1])
+
+
+def paged_kv_copy(pools: Sequence[torch.Tensor], sources: torch.Tensor, targets: torch.Tensor) -> None:
+    """Copies page ``sources[i]`` to page ``targets[i]`` of every pool, in place.
+
+    A pool is any tensor whose first axis counts pages of contiguous elements: ``(P, H_kv, bs, D)``, 4- or 8-bit tiles, states of
+    a ``LinearStatePool``; a page's size and stride are multiples of 4 bytes.  Pairs with an id outside a pool, such as -1,
+    are skipped there.  Targets have to be distinct, and none may be a source, as the pages of :func:`paged_kv_fork` and
+    :func:`paged_kv_compact` are.
+    """
+    lib = L.load_library()
+    pools = list(pools)
+    _require(len(pools) > 0, "pools must name at least one tensor")
+    device = pools[0].device
+    if device.type != "cuda" or not (sources.device == targets.device == device):
+        _same_device(device, pools=pools[0], sources=sources, targets=targets)
+    _index_dtype(sources, "sources")
+    _require(sources.dtype is targets.dtype and sources.dim() == 1 and sources.shape == targets.shape, "sources and targets must be vectors of page ids, alike")
+    n = len(pools)
+    longs = ctypes.c_int64 * n
+    bases, strides, sizes, counts = (ctypes.c_void_p * n)(), longs(), longs(), longs()
+    for i, pool in enumerate(pools):
+        if pool.device != device:
+            _require_cuda(pool, "pools", device)
+        _require(pool.dim() >= 2 and (pool.numel() == 0 or pool[0].is_contiguous()), "a pool's pages must be contiguous along its first axis")
+        each = pool.element_size()
+        bases[i], strides[i], sizes[i], counts[i] = pool.data_ptr(), pool.stride(0) * each, math.prod(pool.shape[1:]) * each, pool.shape[0]
+    s, t = sources.contiguous(), targets.contiguous()
+    code = _launch(device, lib.qa_paged_kv_copy, bases, strides, sizes, counts, n, s.data_ptr(), t.data_ptr(), _code(s), s.numel())
+    L.check(lib, code, "paged_kv_copy")
 
 
 def mrope_axes(sections: Sequence[int], interleaved: bool) -> list[int]:
