@@ -363,8 +363,9 @@ int qa_paged_attention_prefill_kv4(const void* query, int32_t q_dtype, int64_t q
  * (src/decode_state.py:37-44).                                               */
 
 /* qa_paged_kv4_append into an 8-bit pool.  Slots must be distinct, and the
- * tokens of a run stand together in slots, as a plan's do: of a run that
- * appears twice apart, the codes and the scale may not belong together.      */
+ * tokens of a run follow one another in slots, with none but skipped ones
+ * between them, as a plan's do: of a run that appears twice apart, the codes and
+ * the scale may not belong together.                                         */
 int qa_paged_kv8_append(const void* key_new, const void* value_new, int32_t dtype, int64_t k_stride_t, int64_t k_stride_h,
                         int64_t v_stride_t, int64_t v_stride_h, int64_t tokens, int32_t head_dim, const qa_paged_kv* kv,
                         const void* slots, int32_t slots_dtype, int32_t block_size, hipStream_t stream);

@@ -3,8 +3,8 @@
 // Both are bound by memory: per token and KV head the append reads 2 x 2 D bytes of bf16 and writes 2 x D, the gather the
 // other way round.  A wave takes the keys, or the values, of one run: its scale needs the largest magnitude of all tokens of the
 // run that the call brings, so one wave holds them all in registers and reads them once, and no two waves write to one run.
-// Tokens of a run stand together in the slot map; the first of them leads, and the waves look for leaders among `window` tokens
-// each.
+// Tokens of a run follow one another in the slot map, with none but skipped ones between them; the first of them leads, and the waves
+// look for leaders among `window` tokens each.
 #include "kv8.h"
 
 namespace qa {
@@ -73,9 +73,9 @@ __device__ __forceinline__ uint32_t rescaled(uint32_t codes, float down) {
 // Of a run: where its codes lie, and what the call brings.
 struct Bring {
   uint8_t* at;
-  int64_t n;       // its first token in the call
+  int64_t n;       // the first of the call's tokens of the run
   int64_t head;    // of the source: h * head stride
-  int nth;         // lane t < 16: 1 + which of the call's tokens of the run is token t, 0: none
+  int nth;         // lane t < 16: 1 + how far behind that one token t stands, 0: none
   int first;       // the first token that the call brings
   int count;
   uint32_t old;    // scale byte before; 0 where the run starts anew
@@ -190,30 +190,62 @@ __global__ __launch_bounds__(256) void append_kernel(AppendParams p) {
   const bool values = blockIdx.y & 1;
   const int64_t n0 = (static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * p.window;
   if (n0 >= p.tokens) return;
-  // lane i has the slot of token n0 - 1 + i: the token before the window, the window, and what may follow its last leader
-  const int64_t n = n0 - 1 + lane;
-  const int64_t nn = max64(0, min64(n, p.tokens - 1));
-  const int64_t slot = S64 ? reinterpret_cast<const int64_t*>(p.slots)[nn] : reinterpret_cast<const int32_t*>(p.slots)[nn];
-  const int64_t run = n == nn && slot >= 0 && slot < p.num_slots ? slot >> 4 : -1;
-  const int64_t before = (static_cast<int64_t>(__shfl_up(static_cast<int>(run >> 32), 1, 64)) << 32) | static_cast<uint32_t>(__shfl_up(static_cast<int>(run), 1, 64));
+  int at;  // place of the token in its run
+  auto run_of = [&](int64_t n) -> int64_t {  // -1: skipped
+    const int64_t nn = max64(0, min64(n, p.tokens - 1));
+    const int64_t slot = S64 ? reinterpret_cast<const int64_t*>(p.slots)[nn] : reinterpret_cast<const int32_t*>(p.slots)[nn];
+    at = static_cast<int>(slot & 15);
+    return n == nn && slot >= 0 && slot < p.num_slots ? slot >> 4 : -1;
+  };
+  auto of_lane = [&](int64_t v, int from) {
+    return (static_cast<int64_t>(__shfl(static_cast<int>(v >> 32), from, 64)) << 32) | static_cast<uint32_t>(__shfl(static_cast<int>(v), from, 64));
+  };
+  // Lane i has token n0 - 1 + i: the one before the window, the window, and those that may follow its last leader.  A token leads
+  // its run where the last one before it that is not skipped belongs to another.
+  const int64_t run = run_of(n0 - 1 + lane);
+  const int place = at;
+  const uint64_t there = __ballot(run >= 0);
+  const uint64_t below = there & ((1ull << lane) - 1ull);
+  int64_t before = of_lane(run, below != 0 ? 63 - __clzll(static_cast<long long>(below)) : 0);
+  if ((there & 1) == 0 && (there >> 1 & ((1ull << p.window) - 1)) != 0) {
+    int64_t last = -1;  // of the tokens before those: the last that is not skipped
+    for (int64_t n = n0 - 1; n > 0 && last < 0; n -= 64) {
+      const int64_t earlier = run_of(n - 64 + lane);
+      const uint64_t some = __ballot(earlier >= 0);
+      if (some != 0) last = of_lane(earlier, 63 - __clzll(static_cast<long long>(some)));
+    }
+    if (below == 0) before = last;
+  }
   uint64_t leaders = __ballot(run >= 0 && run != before && lane >= 1 && lane <= p.window);
   while (leaders != 0) {
     const int lead = __ffsll(static_cast<unsigned long long>(leaders)) - 1;
     leaders &= leaders - 1;
     const uint32_t lo = __builtin_amdgcn_readlane(static_cast<uint32_t>(run), lead), hi = __builtin_amdgcn_readlane(static_cast<uint32_t>(run >> 32), lead);
     const int64_t own = static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
-    const uint64_t same = __ballot(run == own) >> lead;
     Bring r;
-    r.count = min(static_cast<int>(__ffsll(static_cast<unsigned long long>(~same))) - 1, kRun);
-    const bool member = lane >= lead && lane < lead + r.count;
-    // each token of the run tells the lane of its place; the others talk past lane 31
-    r.nth = __builtin_amdgcn_ds_permute(4 * (member ? static_cast<int>(slot & 15) : 32 + (lane & 31)), lane - lead + 1);
-    if (lane >= kRun) r.nth = 0;
+    r.n = n0 - 1 + lead;
+    r.nth = 0;
+    r.count = 0;
+    int64_t mine = run;  // of this lane's token, lane `from` being the first that counts
+    int its = place, from = lead;
+    for (int64_t n = n0 - 1;;) {
+      const uint64_t others = __ballot(mine >= 0 && mine != own) >> from;
+      const int end = others != 0 ? from + __ffsll(static_cast<unsigned long long>(others)) - 1 : 64;
+      const bool member = mine == own && lane >= from && lane < end;
+      // each token of the run tells the lane of its place; the others talk past lane 31
+      const int nth = __builtin_amdgcn_ds_permute(4 * (member ? its : 32 + (lane & 31)), static_cast<int>(n + lane - r.n) + 1);
+      if (lane < kRun) r.nth = max(r.nth, nth);
+      r.count = __popcll(__ballot(r.nth > 0));
+      n += 64;
+      if (end < 64 || r.count == kRun || n >= p.tokens) break;
+      mine = run_of(n + lane);
+      its = at;
+      from = 0;
+    }
     r.first = __ffsll(static_cast<unsigned long long>(__ballot(r.nth > 0))) - 1;
     const int bs_runs = p.bs_shift - 4;
     const int64_t o = (own >> bs_runs) * p.sP + h * p.sG + (own & ((1 << bs_runs) - 1)) * Run<D>::kBytes;
     r.at = (values ? p.vpool : p.kpool) + o;
-    r.n = n0 - 1 + lead;
     r.head = h * (values ? p.v_sh : p.k_sh);
     r.old = 0;
     if (r.first > 0) r.old = min(max(static_cast<uint32_t>(r.at[Run<D>::kCodes]), kLeast), kMost);

@@ -1470,8 +1470,8 @@ def paged_kv8_append(key: torch.Tensor, value: torch.Tensor, key_pool: torch.Ten
     16 tokens of a block and head (the format and layout stand in ``qwen36_hip.h``).  A run's scale fits the values that the call
     writes to it; a call that goes on with a run never makes its scale smaller, and where it grows, rounds the codes of the
     tokens before to it.  ``slots`` ``(tokens,)`` hold ``block id * block_size + position % block_size``
-    (:func:`paged_kv_plan`); those outside the pool, such as -1, are skipped.  They have to be distinct, with the tokens of
-    a run next to each other, as a plan's are.
+    (:func:`paged_kv_plan`); those outside the pool, such as -1, are skipped.  They have to be distinct, and the tokens of a
+    run have to follow one another, with none but skipped ones between them, as a plan's do.
     """
     _tiles_append("paged_kv8_append", _kv8_descriptor, key, value, key_pool, value_pool, slots, block_size)
 
