@@ -24,9 +24,9 @@ engine and scheduler above it keep their calls:
   kernel.
 
 Host-side tensor preparation (L2 norm, transposes) is PyTorch on the same
-device; every hot loop is a HIP kernel.  Pools may hold bf16 or 4 bits
-(``decode_state.SharedKV4BlockPool``): the entry points choose by the pool's
-type, and ``RopeConfig.mrope_section`` adds rotary positions of several axes.
+device; every hot loop is a HIP kernel.  Pools may hold bf16, 8 or 4 bits
+(``decode_state.SharedKV8BlockPool``, ``SharedKV4BlockPool``): the entry points
+choose by the pool's type, and ``RopeConfig.mrope_section`` adds rotary positions of several axes.
 There is no CPU or dense fallback in this module.
 """
 
@@ -36,7 +36,7 @@ import contextlib
 from dataclasses import dataclass, field
 from typing import Any, Iterator, Sequence
 
-from decode_state import DeviceBatchPageTables, FullAttentionCache, LinearStatePool, PrefillStep, batch_page_tables, is_kv4, kv4_head_dim
+from decode_state import DeviceBatchPageTables, FullAttentionCache, LinearStatePool, PrefillStep, batch_page_tables, tile_bits, tile_head_dim, tile_op
 
 # --------------------------------------------------------------------------- config
 
@@ -168,8 +168,8 @@ def paged_attention_fallback_reason(config: AttentionConfig, query: Any, key: An
     q_shape = tuple(getattr(query, "shape", ()))
     k_shape = tuple(getattr(key, "shape", ()))
     v_shape = tuple(getattr(value, "shape", ()))
-    if is_kv4(key):
-        return _kv4_reason(query, key, value)
+    if tile_bits(key):
+        return _tile_reason(query, key, value)
     if len(q_shape) != 4 or len(k_shape) not in (4, 5) or len(v_shape) != len(k_shape):
         return "shape"
     if len(k_shape) == 5:
@@ -191,17 +191,18 @@ def paged_attention_fallback_reason(config: AttentionConfig, query: Any, key: An
     return "no_kernel"
 
 
-def _kv4_reason(query: Any, key: Any, value: Any, block_size: int | None = None) -> str:
-    """The ladder's last rung for a 4-bit pool ``(P, H_kv, tile)``, which the reference does not have: a bf16 query
+def _tile_reason(query: Any, key: Any, value: Any, block_size: int | None = None) -> str:
+    """The ladder's last rung for a 4- or 8-bit pool ``(P, H_kv, tile)``, which the reference does not have: a bf16 query
     ``(B, H, 1, D)`` of a group of up to 16 heads, over tiles of its head_dim (and of ``block_size`` tokens)."""
     q_shape = tuple(query.shape)
-    if len(q_shape) != 4 or str(query.dtype) != "torch.bfloat16" or not is_kv4(value) or key.dim() != 3 or tuple(value.shape) != tuple(key.shape):
+    if len(q_shape) != 4 or str(query.dtype) != "torch.bfloat16" or tile_bits(value) != tile_bits(key) or key.dim() != 3 or tuple(value.shape) != tuple(key.shape):
         return "shape"
     if q_shape[1] % int(key.shape[1]) or q_shape[1] // int(key.shape[1]) > 16 or q_shape[3] not in (128, 256):
         return "shape"
     if block_size is None:
-        return "no_kernel" if int(key.shape[2]) * 32 % (17 * q_shape[3]) == 0 else "shape"
-    return "no_kernel" if kv4_head_dim(key, value, block_size) == q_shape[3] else "shape"
+        unit = 17 * q_shape[3] // 2 if tile_bits(key) == 4 else 16 * (q_shape[3] + 1)  # of 16 tokens
+        return "no_kernel" if int(key.shape[2]) % unit == 0 else "shape"
+    return "no_kernel" if tile_head_dim(key, value, block_size) == q_shape[3] else "shape"
 
 
 def batched_paged_attention_fallback_reason(config: AttentionConfig, query: Any, caches: Sequence[FullAttentionCache], page_tables: Any, *, seq_len: int) -> str:
@@ -275,10 +276,11 @@ def full_attention_paged(query: Any, gate: Any | None, cache: FullAttentionCache
 
     try:
         with runtime.profile_scope("full_attention.native_paged"):
-            if is_kv4(page_table.key_blocks):
+            bits = tile_bits(page_table.key_blocks)
+            if bits:
                 table = page_table.block_table.unsqueeze(0)
                 lengths = table.new_full((1,), page_table.sequence_length)
-                heads = hip_ops.paged_attention_decode_kv4(query, table, page_table.key_blocks, page_table.value_blocks, lengths, page_table.block_size)
+                heads = tile_op("paged_attention_decode_{}", bits)(query, table, page_table.key_blocks, page_table.value_blocks, lengths, page_table.block_size)
             else:
                 heads = hip_ops.paged_attention_decode(
                     query, page_table.block_table, page_table.key_blocks, page_table.value_blocks, page_table.sequence_length, page_table.block_size
@@ -299,12 +301,12 @@ def full_attention_paged_batch(query: Any, gate: Any | None, caches: Sequence[Fu
 
     Caches may each own a reference-layout pool or share one
     ``SharedKVBlockPool``; either way one kernel launch serves the batch.  Caches
-    on 4-bit pools must share one.
+    on 4- or 8-bit pools must share one.
     """
     page_tables = batch_page_tables(caches) if config.full_attention.paged_kv_metadata else None
     reason = batched_paged_attention_fallback_reason(config, query, caches, page_tables, seq_len=int(query.shape[2]))
-    kv4 = any(is_kv4(cache.key_blocks) for cache in caches)
-    if reason == "no_kernel" and kv4 and any(cache.key_blocks is not caches[0].key_blocks for cache in caches):
+    bits = max((tile_bits(cache.key_blocks) for cache in caches), default=0)
+    if reason == "no_kernel" and bits and any(cache.key_blocks is not caches[0].key_blocks for cache in caches):
         reason = "per_request_pools"
     if reason != "no_kernel" or page_tables is None:
         record_native_paged_dispatch(runtime, reason, native=False)
@@ -314,8 +316,8 @@ def full_attention_paged_batch(query: Any, gate: Any | None, caches: Sequence[Fu
 
     try:
         with runtime.profile_scope("batch.full_attention.native_paged"):
-            if kv4:
-                heads = hip_ops.paged_attention_decode_kv4(
+            if bits:
+                heads = tile_op("paged_attention_decode_{}", bits)(
                     query, page_tables.block_tables, page_tables.key_blocks[0], page_tables.value_blocks[0], page_tables.sequence_lengths, page_tables.block_size
                 )
             else:
@@ -353,14 +355,14 @@ def full_attention_decode_device(
     library's static scratch (``qa_paged_attention_decode_batched_noalloc``) instead of a
     workspace.  Nothing here reads back to the host or copies host to device.
 
-    On a 4-bit pool the step is reserved by ``plan = tables.plan_step()`` in place of
+    On a 4- or 8-bit pool the step is reserved by ``plan = tables.plan_step()`` in place of
     ``reserve_step``, its K/V are written to the plan's slots and its lengths are the plan's: a
     refused step writes nothing and gives zeros.  ``no_alloc`` is for bf16 pools.
     """
     reason = _device_pool_reason(config, query, key_blocks, value_blocks, tables)
-    kv4 = is_kv4(key_blocks)
+    bits = tile_bits(key_blocks)
     if reason == "no_kernel":
-        _check_step(kv4, plan, no_alloc, tables)
+        _check_step(bits > 0, plan, no_alloc, tables)
     if reason != "no_kernel":
         record_native_paged_dispatch(runtime, reason, native=False)
         return None
@@ -370,9 +372,9 @@ def full_attention_decode_device(
     # later kernel error propagates: a dense fallback would attend over a cache that already
     # holds the step (and under graph capture would record a step without attention).
     with runtime.profile_scope("batch.full_attention.native_paged_device"):
-        if kv4:
-            hip_ops.paged_kv4_append(key[:, :, 0], value[:, :, 0], key_blocks, value_blocks, plan.slots, tables.block_size)
-            decode, lengths = hip_ops.paged_attention_decode_kv4, _step_lengths(plan)
+        if bits:
+            tile_op("paged_{}_append", bits)(key[:, :, 0], value[:, :, 0], key_blocks, value_blocks, plan.slots, tables.block_size)
+            decode, lengths = tile_op("paged_attention_decode_{}", bits), _step_lengths(plan)
         else:
             tables.append(key, value, key_blocks, value_blocks)
             decode = hip_ops.paged_attention_decode_batched_noalloc if no_alloc else hip_ops.paged_attention_decode_batched
@@ -386,13 +388,13 @@ def _device_pool_reason(config: AttentionConfig, query: Any, key_blocks: Any, va
     """The dispatch ladder for a step on device page tables, checked before anything is written:
     the reference's reasons (one token per row), then what the native kernels need of the pool
     (a shared ``(P, H_kv, bs, D)`` bf16 pool with the tables' block size and block count, or such
-    a pool of 4-bit tiles)."""
+    a pool of 4- or 8-bit tiles)."""
     seq_len = int(query.shape[2]) if len(tuple(getattr(query, "shape", ()))) == 4 else 1
     reason = paged_attention_fallback_reason(config, query, key_blocks, value_blocks, seq_len=seq_len, batched=False)
     if reason != "no_kernel":
         return reason
-    if is_kv4(key_blocks):
-        return _kv4_reason(query, key_blocks, value_blocks, tables.block_size) if int(key_blocks.shape[0]) == tables.num_blocks else "shape"
+    if tile_bits(key_blocks):
+        return _tile_reason(query, key_blocks, value_blocks, tables.block_size) if int(key_blocks.shape[0]) == tables.num_blocks else "shape"
     if key_blocks.dim() != 4 or tuple(value_blocks.shape) != tuple(key_blocks.shape):
         return "shape"
     if int(key_blocks.shape[2]) != tables.block_size or int(key_blocks.shape[0]) != tables.num_blocks:
@@ -405,9 +407,9 @@ def _check_step(by_slots: bool, plan: Any | None, no_alloc: bool, tables: Device
     if not by_slots:
         return
     if plan is None or tuple(plan.slots.shape) != (tables.rows,):
-        raise ValueError("a 4-bit pool or mrope_section needs the step's plan (tables.plan_step())")
+        raise ValueError("a 4-bit pool or mrope_section needs the step's plan (tables.plan_step()), as an 8-bit pool does")
     if no_alloc:
-        raise ValueError("no_alloc is for bf16 pools: the 4-bit decode takes its workspace per call")
+        raise ValueError("no_alloc is for bf16 pools: the 4-bit decode takes its workspace per call, as the 8-bit one does")
 
 
 def _step_lengths(plan: Any) -> Any:
@@ -418,7 +420,7 @@ def _step_lengths(plan: Any) -> Any:
 
 def _check_positions(by_slots: bool, positions: Any | None) -> None:
     if positions is not None and not by_slots:
-        raise ValueError("positions are for a 4-bit pool or mrope_section: elsewhere a token's position is its place in its row")
+        raise ValueError("positions are for a 4-bit pool or mrope_section (or an 8-bit pool): elsewhere a token's position is its place in its row")
 
 
 def _qk_norm_rope(q_proj: Any, k_proj: Any, v_proj: Any, q_norm_weight: Any, k_norm_weight: Any, key_blocks: Any, value_blocks: Any,
@@ -441,7 +443,7 @@ class RopeConfig:
     partial_rotary_factor: float = 0.25
     # rotary positions of several axes (time, row, column of a picture's tokens): how many of the frequencies each axis
     # turns, and whether the axes take turns (hip_ops.mrope_axes).  None: one position a token.  With sections, and on every
-    # 4-bit pool, the prologue rounds q and k to bf16 once; without, on a bf16 pool, it rounds cos, sin, the norm and both
+    # 4- or 8-bit pool, the prologue rounds q and k to bf16 once; without, on a bf16 pool, it rounds cos, sin, the norm and both
     # products as the reference does, so that the same tokens' q and k differ by up to five half steps between the two.
     mrope_section: tuple[int, ...] | None = None
     mrope_interleaved: bool = False
@@ -458,10 +460,21 @@ def _qk_norm_mrope(q_proj: Any, k_proj: Any, v_proj: Any, q_norm_weight: Any, k_
     sections = rope.sections(head_dim)
     if positions is None:
         positions = plan.positions.expand(len(sections), -1)
-    return hip_ops.qk_norm_mrope_kv_append(
-        q_proj, k_proj, v_proj, q_norm_weight, k_norm_weight, positions, sections, key_blocks, value_blocks, plan.slots, block_size,
+    keys, values, slots, block = key_blocks, value_blocks, plan.slots, block_size
+    if tile_bits(key_blocks) == 8:
+        # a run's scale needs all of its new tokens: the prologue writes k and v of the step alone, blocks of one token, and
+        # the append takes them from there
+        tokens = int(q_proj.shape[0])
+        keys = q_proj.new_empty((tokens, int(key_blocks.shape[1]), 1, head_dim))
+        values = q_proj.new_empty(keys.shape)
+        slots, block = _count_up(tokens, q_proj.device), 1
+    out = hip_ops.qk_norm_mrope_kv_append(
+        q_proj, k_proj, v_proj, q_norm_weight, k_norm_weight, positions, sections, keys, values, slots, block,
         eps=rope.rms_norm_eps, rope_theta=rope.rope_theta, interleaved=rope.mrope_interleaved,
     )
+    if keys is not key_blocks:
+        hip_ops.paged_kv8_append(keys[:, :, 0], values[:, :, 0], key_blocks, value_blocks, plan.slots, block_size)
+    return out
 
 
 def full_attention_decode_step_device(
@@ -485,26 +498,26 @@ def full_attention_decode_step_device(
     exceed the library's 32 MiB scratch raises ``RuntimeError`` with the token already in the
     cache, so the caller must not append it again.
 
-    With a 4-bit pool (``SharedKV4BlockPool``) or ``rope.mrope_section`` the step is reserved by
+    With a 4- or 8-bit pool (``SharedKV4BlockPool``, ``SharedKV8BlockPool``) or ``rope.mrope_section`` the step is reserved by
     ``plan = tables.plan_step()`` in place of ``reserve_step``; ``positions`` ``(axes, rows)`` then
     gives each row's rotary positions (its place in the row on every axis where omitted: text).
     A refused step writes nothing and gives zeros; ``tables.check()`` tells.
-    On a 4-bit pool the gate is applied inside the decode and ``no_alloc`` is refused.
+    On a 4- or 8-bit pool the gate is applied inside the decode and ``no_alloc`` is refused.
     """
     rows = int(q_proj.shape[0])
     full = config.full_attention
     heads, head_dim, kv_heads = full.num_heads, full.head_dim, full.num_key_value_heads
     probe = _query_probe(q_proj, heads, head_dim)
     reason = _device_pool_reason(config, probe, key_blocks, value_blocks, tables)
-    kv4 = is_kv4(key_blocks)
+    bits = tile_bits(key_blocks)
     if reason == "no_kernel" and (rows != tables.rows or int(key_blocks.shape[1]) != kv_heads or str(q_proj.dtype) != "torch.bfloat16"):
         reason = "shape"
-    if reason == "no_kernel" and not kv4 and (int(key_blocks.shape[3]) != head_dim or str(key_blocks.dtype) != "torch.bfloat16"):
+    if reason == "no_kernel" and not bits and (int(key_blocks.shape[3]) != head_dim or str(key_blocks.dtype) != "torch.bfloat16"):
         reason = "shape"
-    by_slots = kv4 or rope.mrope_section is not None
+    by_slots = bits > 0 or rope.mrope_section is not None
     if reason == "no_kernel":
         _check_positions(by_slots, positions)
-        _check_step(by_slots, plan, no_alloc and kv4, tables)
+        _check_step(by_slots, plan, no_alloc and bits > 0, tables)
     if reason != "no_kernel":
         record_native_paged_dispatch(runtime, reason, native=False)
         return None
@@ -518,9 +531,9 @@ def full_attention_decode_step_device(
             query, gate = _qk_norm_rope(q_proj, k_proj, v_proj, q_norm_weight, k_norm_weight, key_blocks, value_blocks, tables.block_tables,
                                         cu, tables.positions, tables.block_size, 1, rope)
         lengths = _step_lengths(plan) if by_slots else tables.sequence_lengths
-        if kv4:
-            out = hip_ops.paged_attention_decode_kv4(query.view(rows, heads, 1, head_dim), tables.block_tables, key_blocks, value_blocks, lengths,
-                                                     tables.block_size, gate=gate if full.output_gate else None)
+        if bits:
+            out = tile_op("paged_attention_decode_{}", bits)(query.view(rows, heads, 1, head_dim), tables.block_tables, key_blocks, value_blocks, lengths,
+                                                             tables.block_size, gate=gate if full.output_gate else None)
             record_native_paged_dispatch(runtime, reason, native=True)
             return out.view(rows, 1, heads * head_dim)
         decode = hip_ops.paged_attention_decode_batched_noalloc if no_alloc else hip_ops.paged_attention_decode_batched
@@ -545,6 +558,21 @@ def _row_offsets(rows: int, device: Any) -> Any:
         cached = torch.arange(rows + 1, dtype=torch.int32, device=device)
         _ROW_OFFSETS[key] = cached
     return cached
+
+
+_COUNT_UP: dict[tuple[int, str], Any] = {}
+
+
+def _count_up(tokens: int, device: Any) -> Any:
+    """``[0, 1, .., tokens - 1]`` int64, a part of the next power of two, cached per (power, device) as ``_row_offsets`` is."""
+    import torch
+
+    key = (1 << max(tokens - 1, 0).bit_length(), str(device))
+    cached = _COUNT_UP.get(key)
+    if cached is None:
+        cached = torch.arange(key[0], dtype=torch.int64, device=device)
+        _COUNT_UP[key] = cached
+    return cached[:tokens]
 
 
 def _query_probe(q_proj: Any, heads: int, head_dim: int) -> Any:
@@ -582,7 +610,7 @@ def full_attention_prefill_device(
     reference's reason for every multi-token call) or ``"shape"``, so the caller's dense path
     runs; nothing has been written by then.  Native calls count in ``native_prefill_hits``.
 
-    A 4-bit pool or ``rope.mrope_section`` needs the ``step`` of ``DeviceBatchPageTables.plan_prefill``;
+    A 4- or 8-bit pool or ``rope.mrope_section`` needs the ``step`` of ``DeviceBatchPageTables.plan_prefill``;
     ``positions`` ``(axes, tokens)`` are the tokens' rotary positions, by default their places in
     their rows on every axis.
     """
@@ -591,16 +619,16 @@ def full_attention_prefill_device(
     tokens = int(q_proj.shape[0])
     full = config.full_attention
     heads, head_dim, kv_heads = full.num_heads, full.head_dim, full.num_key_value_heads
-    kv4 = is_kv4(key_blocks)
-    by_slots = kv4 or rope.mrope_section is not None
+    bits = tile_bits(key_blocks)
+    by_slots = bits > 0 or rope.mrope_section is not None
     probe = _query_probe(q_proj, heads, head_dim)
     if probe.dim() == 4:
         probe = probe[:1]  # one token stands for the step: the ladder reads heads and widths, not rows
     reason = paged_attention_fallback_reason(config, probe, key_blocks, value_blocks, seq_len=1, batched=False)
     if reason == "no_kernel":
-        if kv4:
+        if bits:
             if (int(key_blocks.shape[1]) != kv_heads or tokens != step.total_tokens or q_proj.dtype != torch.bfloat16
-                    or kv4_head_dim(key_blocks, value_blocks, step.block_size) != head_dim):
+                    or tile_head_dim(key_blocks, value_blocks, step.block_size) != head_dim):
                 reason = "shape"
         elif key_blocks.dim() != 4:
             reason = "prefill_or_multitoken"  # per-request (reference-layout) pools: the dense path
@@ -615,14 +643,14 @@ def full_attention_prefill_device(
 
     _check_positions(by_slots, positions)
     if by_slots and step.plan is None:
-        raise ValueError("a 4-bit pool or mrope_section needs a step of plan_prefill")
+        raise ValueError("a 4-bit pool or mrope_section needs a step of plan_prefill, as an 8-bit pool does")
     with runtime.profile_scope("full_attention.native_paged_prefill"):
         if by_slots:
             query, gate = _qk_norm_mrope(q_proj, k_proj, v_proj, q_norm_weight, k_norm_weight, key_blocks, value_blocks, step.plan, step.block_size, rope, head_dim, positions)
         else:
             query, gate = _qk_norm_rope(q_proj, k_proj, v_proj, q_norm_weight, k_norm_weight, key_blocks, value_blocks, step.block_tables,
                                         step.cu_seqlens, step.starts, step.block_size, step.max_new, rope)
-        prefill = hip_ops.paged_attention_prefill_kv4 if kv4 else hip_ops.paged_attention_prefill
+        prefill = tile_op("paged_attention_prefill_{}", bits) if bits else hip_ops.paged_attention_prefill
         out = prefill(query, step.cu_seqlens, step.starts, key_blocks, value_blocks, step.block_tables,
                       step.block_size, max_new=step.max_new, gate=gate if full.output_gate else None)
     stats = runtime.paged_attention_stats

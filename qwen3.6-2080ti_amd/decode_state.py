@@ -20,8 +20,12 @@ What changes underneath:
   every request; caches created with ``shared_pool=`` draw blocks from it, so
   growth never reallocates and ``batch_page_tables`` hands the decode kernel a
   single pool.
-* ``SharedKV4BlockPool`` is the same pool in 4 bits (17 bytes per 32 values in
-  place of 64): the reference has no quantised cache.
+* ``SharedKV4BlockPool`` and ``SharedKV8BlockPool`` are the same pool in 4 and in
+  8 bits (17 bytes per 32 values, and 257 per 256, in place of 2 each): the
+  reference has no quantised cache.
+* Rows of ``DeviceBatchPageTables`` may share blocks: ``fork_request`` gives a
+  request copies that share what is full, ``release_requests`` frees on the
+  device, ``compact`` moves a scattered cache to the pool's front.
 * ``LinearStatePool`` keeps recurrent and conv states of many requests in
   slot-indexed device tensors updated in place (the reference stacks and
   scatters per-request states each step, ``src/tp_runtime.py:2678-2707``).
@@ -231,24 +235,79 @@ class SharedKV4BlockPool(SharedKVBlockPool):
         return pool
 
 
-def is_kv4(blocks: Any) -> bool:
-    """Whether a pool tensor is one of 4-bit tiles."""
-    return str(getattr(blocks, "dtype", "")) == "torch.uint8"
+class SharedKV8BlockPool(SharedKVBlockPool):
+    """:class:`SharedKVBlockPool` in 8 bits: float8_e4m3fn tensors ``(num_blocks, kv_heads, kv8_tile_bytes(head_dim, block_size))``.
+
+    E4M3 codes with a power-of-two scale for each run of 16 tokens of a block and head (``qwen36_hip.h``), half the bytes of a
+    bf16 pool.  Sizes, operators and use are those of :class:`SharedKV4BlockPool`.
+    """
+
+    def __init__(self, num_blocks: int, kv_heads: int, head_dim: int, *, block_size: int = DEFAULT_KV_BLOCK_SIZE, device: Any = None) -> None:
+        import torch
+
+        import hip_ops
+
+        if num_blocks <= 0 or kv_heads <= 0:
+            raise ValueError("num_blocks and kv_heads must be positive")
+        self.block_size = block_size
+        self.kv_heads = kv_heads
+        self.head_dim = head_dim
+        self.key_blocks = torch.zeros((num_blocks, kv_heads, hip_ops.kv8_tile_bytes(head_dim, block_size)), dtype=torch.uint8, device=device).view(torch.float8_e4m3fn)
+        self.value_blocks = torch.zeros_like(self.key_blocks)
+        self.free_blocks = list(range(num_blocks))
+        self.allocator = None
+
+    @classmethod
+    def from_tensors(cls, key_blocks: Any, value_blocks: Any, *, block_size: int = DEFAULT_KV_BLOCK_SIZE, free_blocks: Sequence[int] | None = None) -> "SharedKV8BlockPool":
+        """A pool over existing tiles; ``block_size`` says how many tokens one holds."""
+        head_dim = tile_head_dim(key_blocks, value_blocks, block_size)
+        if head_dim is None or tile_bits(key_blocks) != 8:
+            raise ValueError("pool tensors must be float8_e4m3fn (num_blocks, kv_heads, tile bytes of the block size) and alike")
+        pool = cls.__new__(cls)
+        pool.block_size = block_size
+        pool.kv_heads = int(key_blocks.shape[1])
+        pool.head_dim = head_dim
+        pool.key_blocks = key_blocks
+        pool.value_blocks = value_blocks
+        pool.free_blocks = list(range(int(key_blocks.shape[0]))) if free_blocks is None else sorted(int(b) for b in free_blocks)
+        pool.allocator = None
+        return pool
 
 
-def kv4_head_dim(key_blocks: Any, value_blocks: Any, block_size: int) -> int | None:
-    """The head_dim of a 4-bit pool whose tiles hold ``block_size`` tokens, or ``None`` where they do not."""
+def tile_bits(blocks: Any) -> int:
+    """4 or 8 for a pool tensor of such tiles, 0 for one of plain values."""
+    return {"torch.uint8": 4, "torch.float8_e4m3fn": 8}.get(str(getattr(blocks, "dtype", "")), 0)
+
+
+def tile_op(name: str, bits: int) -> Any:
+    """The operator of ``hip_ops`` for pools of ``bits``: ``name`` with a place for ``kv4`` or ``kv8``."""
     import hip_ops
 
-    if not is_kv4(key_blocks) or not is_kv4(value_blocks) or key_blocks.dim() != 3 or tuple(value_blocks.shape) != tuple(key_blocks.shape):
+    return getattr(hip_ops, name.format(f"kv{bits}"))
+
+
+def tile_head_dim(key_blocks: Any, value_blocks: Any, block_size: int) -> int | None:
+    """The head_dim of a pool of tiles that hold ``block_size`` tokens, or ``None`` where they do not."""
+    bits = tile_bits(key_blocks)
+    if not bits or tile_bits(value_blocks) != bits or key_blocks.dim() != 3 or tuple(value_blocks.shape) != tuple(key_blocks.shape):
         return None
     for head_dim in (128, 256):
         try:
-            if hip_ops.kv4_tile_bytes(head_dim, block_size) == int(key_blocks.shape[2]):
+            if tile_op("{}_tile_bytes", bits)(head_dim, block_size) == int(key_blocks.shape[2]):
                 return head_dim
         except RuntimeError:
             return None
     return None
+
+
+def is_kv4(blocks: Any) -> bool:
+    """Whether a pool tensor is one of 4-bit tiles."""
+    return tile_bits(blocks) == 4
+
+
+def kv4_head_dim(key_blocks: Any, value_blocks: Any, block_size: int) -> int | None:
+    """:func:`tile_head_dim` of a 4-bit pool."""
+    return tile_head_dim(key_blocks, value_blocks, block_size) if is_kv4(key_blocks) else None
 
 
 class DeviceBlockAllocator:
@@ -280,6 +339,8 @@ class DeviceBlockAllocator:
             self.free_list[: len(ids)] = torch.tensor(ids, dtype=torch.int32, device=self.device)
         self.free_state = torch.tensor([0, len(ids)], dtype=torch.int32, device=self.device)
         self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
+        # holders of a block beyond its first (fork): 0 for all that one row has
+        self.references = torch.zeros(num_blocks, dtype=torch.int32, device=self.device)
         self._last = "paged_kv_reserve"
 
     _STATUS = {
@@ -288,6 +349,7 @@ class DeviceBlockAllocator:
         3: "device free list state is corrupt",
         4: "negative or overflowing length/count",
         5: "more new tokens than the step has room for",
+        6: "rows out of range, or target rows that are not empty or not distinct",
     }
 
     def reserve(self, block_tables: Any, lengths: Any, block_size: int, *, counts: Any = 1, positions: Any = None) -> None:
@@ -304,6 +366,27 @@ class DeviceBlockAllocator:
         self._last = "paged_kv_plan"
         return hip_ops.paged_kv_plan(block_tables, lengths, counts, self.free_list, self.free_state, self.status, block_size, max_tokens=max_tokens, per_row=per_row)
 
+    def fork(self, block_tables: Any, lengths: Any, source_rows: Any, target_rows: Any, block_size: int) -> Any:
+        """Rows that share their sources' full blocks (``hip_ops.paged_kv_fork``): the ``PagedCopy`` that every layer's pools need."""
+        import hip_ops
+
+        self._last = "paged_kv_fork"
+        return hip_ops.paged_kv_fork(block_tables, lengths, source_rows, target_rows, self.free_list, self.free_state, self.references, self.status, block_size)
+
+    def release_rows(self, block_tables: Any, lengths: Any, rows: Any) -> None:
+        """Free the blocks of table rows on the device, without reading anything back (``hip_ops.paged_kv_release``)."""
+        import hip_ops
+
+        self._last = "paged_kv_release"
+        hip_ops.paged_kv_release(block_tables, lengths, rows, self.free_list, self.free_state, self.references, self.status)
+
+    def compact(self, block_tables: Any, max_moves: int) -> Any:
+        """Move the tables' blocks to the lowest ids (``hip_ops.paged_kv_compact``): the ``PagedCopy`` that every layer's pools need."""
+        import hip_ops
+
+        self._last = "paged_kv_compact"
+        return hip_ops.paged_kv_compact(block_tables, self.free_list, self.free_state, self.references, self.status, max_moves=max_moves)
+
     def check(self) -> None:
         """Raise ``RuntimeError`` if the last reservation failed (reads the status: a sync)."""
         code = int(self.status.item())
@@ -318,17 +401,29 @@ class DeviceBlockAllocator:
     def free_count(self) -> int:
         return int(self.free_state[1].item())
 
-    def release(self, blocks: Sequence[int]) -> None:
+    def release(self, blocks: Sequence[int]) -> list[int]:
+        """Take a holder from each block and merge those that had no other into the list; returns these, in the order given."""
         import torch
 
         blocks = [int(b) for b in blocks]
         if not blocks:
-            return
-        merged = sorted(self.free_blocks() + blocks)
-        if merged[0] < 0 or merged[-1] >= self.capacity or len(set(merged)) != len(merged):
+            return []
+        free = self.free_blocks()
+        if min(blocks) < 0 or max(blocks) >= self.capacity or len(set(blocks)) != len(blocks) or set(blocks) & set(free):
             raise ValueError("released block ids must be in range and not already free")
+        index = torch.tensor(blocks, dtype=torch.int64, device=self.device)
+        held = self.references[index]
+        shared = held.tolist()
+        if any(shared):
+            self.references[index] = (held - 1).clamp(min=0)
+        gone = [b for b, n in zip(blocks, shared) if n == 0]
+        merged = sorted(free + gone)
         self.free_list[: len(merged)] = torch.tensor(merged, dtype=torch.int32, device=self.device)
         self.free_state.copy_(torch.tensor([0, len(merged)], dtype=torch.int32))
+        return gone
+
+
+_FORKS = 1024  # of a launch
 
 
 class DeviceBatchPageTables:
@@ -508,16 +603,86 @@ class DeviceBatchPageTables:
 
     def release_request(self, row: int) -> list[int]:
         """The request in ``row`` finished: its blocks return to the device free list (one read of
-        the row) and the row is emptied.  Returns the released block ids."""
+        the row) and the row is emptied.  Returns the released block ids: blocks that a fork of the
+        request still holds are not among them."""
         if not self.active[row]:
             raise ValueError(f"row {row} holds no request")
-        ids = [int(b) for b in self.block_tables[row].tolist() if b >= 0]
-        self.allocator.release(ids)
+        ids = self.allocator.release([int(b) for b in self.block_tables[row].tolist() if b >= 0])
         self.block_tables[row].fill_(-1)
         self.sequence_lengths[row] = 0
         self.step_counts[row] = 0
         self.active[row] = False
         return ids
+
+    def fork_request(self, row: int, count: int, pools: Sequence[Any]) -> list[int]:
+        """Take the lowest ``count`` free rows for copies of the request in ``row``: several answers to one prompt, the beams of a
+        search.  They share its full blocks; a partly filled last one is copied, in ``pools`` -- the key and value tensors of
+        every full-attention layer that shares these tables.  Between steps: the K/V of all layers are written up to the row's
+        length.  A hybrid model's recurrent states are forked beside it (``LinearStatePool.fork``).  One read of the status:
+        a fork for which the pool has no block raises and takes nothing."""
+        import torch
+
+        if not self.active[row]:
+            raise ValueError(f"row {row} holds no request")
+        if count <= 0:
+            raise ValueError("count must be positive")
+        self._check_pools(pools)
+        targets = [r for r, used in enumerate(self.active) if not used][:count]
+        if len(targets) < count:
+            raise RuntimeError(f"device page tables: {count} rows needed, {len(targets)} hold no request")
+        device = self.block_tables.device
+        import hip_ops
+
+        for lo in range(0, count, _FORKS):
+            part = torch.tensor(targets[lo : lo + _FORKS], dtype=torch.int32, device=device)
+            copies = self.allocator.fork(self.block_tables, self.sequence_lengths, torch.full_like(part, row), part, self.block_size)
+            try:
+                self.allocator.check()
+            except RuntimeError:
+                if lo:
+                    self.allocator.release_rows(self.block_tables, self.sequence_lengths, torch.tensor(targets[:lo], dtype=torch.int32, device=device))
+                raise
+            hip_ops.paged_kv_copy(pools, copies.sources, copies.targets)
+        for target in targets:
+            self.active[target] = True
+        self.step_counts[torch.tensor(targets, device=device)] = self.step_counts[row].clone()
+        return targets
+
+    def release_requests(self, rows: Sequence[int]) -> None:
+        """:meth:`release_request` of several rows on the device, without reading anything back."""
+        import torch
+
+        rows = [int(r) for r in rows]
+        for r in rows:
+            if not 0 <= r < self.rows or not self.active[r]:
+                raise ValueError(f"row {r} holds no request")
+        if len(set(rows)) != len(rows):
+            raise ValueError("release_requests rows must be distinct")
+        if not rows:
+            return
+        index = torch.tensor(rows, dtype=torch.int64, device=self.block_tables.device)
+        self.allocator.release_rows(self.block_tables, self.sequence_lengths, index)
+        self.step_counts[index] = 0
+        for r in rows:
+            self.active[r] = False
+
+    def compact(self, pools: Sequence[Any], *, max_moves: int | None = None) -> None:
+        """Move the requests' blocks to the pool's lowest ids, their pages in ``pools`` (as in :meth:`fork_request`) with them,
+        at most ``max_moves`` in a call: then the pools' ends are free, to be saved or given back.  Between steps; nothing is
+        read back.  Blocks in use that these tables do not hold stay where they are."""
+        import hip_ops
+
+        if max_moves is not None and max_moves < 0:
+            raise ValueError("max_moves must be non-negative")
+        self._check_pools(pools)
+        copies = self.allocator.compact(self.block_tables, self.num_blocks // 2 if max_moves is None else min(max_moves, self.num_blocks // 2))
+        hip_ops.paged_kv_copy(pools, copies.sources, copies.targets)
+
+    def _check_pools(self, pools: Sequence[Any]) -> None:
+        if not pools or any(int(pool.shape[0]) != self.num_blocks for pool in pools):
+            raise ValueError(f"pools must be the key and value tensors of the layers on these tables, {self.num_blocks} blocks each")
+        if not all(any(pool is own for pool in pools) for own in (self.pool.key_blocks, self.pool.value_blocks)):
+            raise ValueError("pools must have the key and value tensors of the tables' own pool among them")
 
 
 @dataclass(frozen=True)
@@ -636,8 +801,8 @@ class FullAttentionCache:
     seq, head_dim)``; ``block_table`` maps logical blocks to physical ones.
     With ``shared_pool`` set, ``heads`` is the KV head count of the shared
     GQA-native pool and the cache's batch dimension must be 1.  On a
-    ``SharedKV4BlockPool`` (GPU tensors only) ``append_blocks`` quantises and
-    ``as_tensors`` gives the values the cache holds, in bf16.
+    ``SharedKV4BlockPool`` or ``SharedKV8BlockPool`` (GPU tensors only) ``append_blocks``
+    quantises and ``as_tensors`` gives the values the cache holds, in bf16.
     """
 
     capacity_hint: int | None = None
@@ -693,8 +858,9 @@ class FullAttentionCache:
     def append_blocks(self, key: Any, value: Any) -> None:
         """Write new K/V into slots ``(table[pos // bs], pos % bs)`` (``src/decode_state.py:271-293``)."""
         seq = int(key.shape[2])
-        if is_kv4(self.pool.key_blocks) and not _on_gpu(key):
-            raise RuntimeError("a 4-bit pool is written from GPU tensors only")
+        bits = tile_bits(self.pool.key_blocks)
+        if bits and not _on_gpu(key):
+            raise RuntimeError(f"{'an 8' if bits == 8 else 'a 4'}-bit pool is written from GPU tensors only")
         self.append_calls += 1
         self.appended_tokens += seq
         target = self.valid + seq
@@ -734,10 +900,11 @@ class FullAttentionCache:
         if self.shared_pool is not None:
             if key.shape[0] != 1:
                 raise ValueError("caches on a shared pool hold one request (batch 1)")
-            if is_kv4(self.pool.key_blocks):
+            bits = tile_bits(self.pool.key_blocks)
+            if bits:
                 at = torch.arange(self.valid, self.valid + int(key.shape[2]), device=key.device)
                 slots = table.long()[at // self.block_size] * self.block_size + at % self.block_size
-                hip_ops.paged_kv4_append(key[0].transpose(0, 1), value[0].transpose(0, 1), self.pool.key_blocks, self.pool.value_blocks, slots, self.block_size)
+                tile_op("paged_{}_append", bits)(key[0].transpose(0, 1), value[0].transpose(0, 1), self.pool.key_blocks, self.pool.value_blocks, slots, self.block_size)
                 return
             hip_ops.paged_kv_append(key, value, self.pool.key_blocks, self.pool.value_blocks, table, self.valid, self.block_size)
             return
@@ -857,12 +1024,13 @@ class FullAttentionCache:
         import torch
 
         keys, values = self.pool.key_blocks, self.pool.value_blocks
-        if _on_gpu(keys) or is_kv4(keys):
+        bits = tile_bits(keys)
+        if _on_gpu(keys) or bits:
             import hip_ops
 
             table = torch.tensor(self.block_table, dtype=torch.int32, device=keys.device)
-            if is_kv4(keys):
-                return hip_ops.paged_kv4_gather(keys, values, table, self.valid, self.block_size)
+            if bits:
+                return tile_op("paged_{}_gather", bits)(keys, values, table, self.valid, self.block_size)
             if self.shared_pool is not None:
                 return hip_ops.paged_kv_gather(keys, values, table, self.valid, self.block_size)
             return hip_ops.paged_kv_gather(keys, values, table, self.valid, self.block_size)
@@ -912,6 +1080,19 @@ class LinearStatePool:
         self.state[slot].zero_()
         self.conv[slot].zero_()
         return slot
+
+    def fork(self, slot: int, count: int = 1) -> list[int]:
+        """Slots with copies of ``slot``'s states, for the requests that ``DeviceBatchPageTables.fork_request`` makes."""
+        import torch
+
+        import hip_ops
+
+        if count > len(self.free_slots):
+            raise RuntimeError("linear state pool exhausted")
+        taken, self.free_slots = self.free_slots[:count], self.free_slots[count:]
+        targets = torch.tensor(taken, dtype=torch.int32, device=self.state.device)
+        hip_ops.paged_kv_copy([self.state, self.conv], torch.full_like(targets, slot), targets)
+        return taken
 
     def release(self, slot: int) -> None:
         self.free_slots = sorted(self.free_slots + [slot])
