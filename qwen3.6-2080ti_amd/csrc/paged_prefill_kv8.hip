@@ -34,8 +34,8 @@ struct Smem {
   static constexpr int kP = kValues + kValueBufs * kTileBytes;        // probabilities: [buffer][wave][run][lane][16 bytes]
   static constexpr int kMax = kP + 2 * kWaves * 2 * 1024;             // [buffer][wave][32] floats
   static constexpr int kScale = kMax + 2 * kWaves * 32 * 4;           // of keys [buffer][run], of values [buffer][run]
-  static constexpr int kFlag = kScale + (kKeyBufs + kValueBufs) * kRuns * 4;  // [buffer of values]: 1 + the last tile that had a NaN
-  static constexpr int kBytes = kFlag + kValueBufs * 4;
+  static constexpr int kFlag = kScale + (kKeyBufs + kValueBufs) * kRuns * 4;  // whether a tile that not every column sees whole had a NaN
+  static constexpr int kBytes = kFlag + 16;
 };
 
 template <int D>
@@ -177,17 +177,19 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams p
     for (int s = 0; s < N; ++s) stage[s] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, 16 * lane + 1024 * s, 0, kShared));
     stage_scale = __builtin_amdgcn_raw_buffer_load_b8(r, kv8::Run<D>::kCodes, 0, kShared);
   };
-  // what of the stage no column sees, or not every column where it is NaN, leaves the product
-  auto trim = [&](int64_t kt, int buf) {
-    if (kt * kTile + kTile <= first_pos + 1) return;  // every column sees all of the tile
-    // keys that no column sees may hold anything, and 0 times a NaN is one
-    const uint32_t mask = tokens_mask(kv_end - kt * kTile - kv8::kRun * (wave & 3) - 4 * (lane >> 4));
+  // What of the stage no column sees leaves the product.  A NaN among what not every column sees leaves it too: 0 times it is
+  // one.  It is marked at the end for the columns that see it.
+  const int64_t first_mixed = (first_pos + 1) / kTile;  // the first tile that not every column sees whole
+  auto nans_of = [](uint32_t w) -> uint32_t { return ((w & 0x7f7f7f7fu) + 0x01010101u) >> 7 & 0x01010101u; };  // 1 in each byte 0x7f or 0xff
+  auto trim = [&](int64_t kt) {
+    if (kt < first_mixed) return;
+    const uint32_t mask = tokens_mask(kv_end - kt * kTile - kv8::kRun * (wave & 3) - 4 * (lane >> 4));  // past it the pool may hold anything
     uint32_t any = 0;
     auto clean = [&](uint32_t& w) {
       w &= mask;
-      const uint32_t bad = ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;  // bytes 0x7f and 0xff
+      const uint32_t bad = nans_of(w);
+      w &= ~(bad * 255u);
       any |= bad;
-      w &= ~((bad >> 7) * 255u);  // a NaN reaches only the columns that see its token: marked for them below
     };
 #pragma unroll
     for (int s = 0; s < N; ++s) {
@@ -196,12 +198,12 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams p
       clean(stage[s].z);
       clean(stage[s].w);
     }
-    if (any != 0) s_flag[buf] = static_cast<int>(kt - kt0) + 1;
+    if (any != 0) *s_flag = 1;
   };
   auto put = [&](int64_t kt) {
     const int i = static_cast<int>(kt - kt0);
     const int buf = of_values ? i & (kValueBufs - 1) : i & (kKeyBufs - 1);
-    if (of_values) trim(kt, buf);
+    if (of_values) trim(kt);
     uint4* dst = reinterpret_cast<uint4*>(smem + (of_values ? S::kValues : 0) + (buf * kRuns + (wave & 3)) * S::kRunBytes) + lane;
 #pragma unroll
     for (int s = 0; s < N; ++s) dst[64 * s] = stage[s];
@@ -237,7 +239,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams p
       }
   };
   if (kt0 < kt1) {
-    if (tid < kValueBufs) s_flag[tid] = 0;
+    if (tid == 0) *s_flag = 0;
     // the query: lane 32 h + n has dims 64 s + 16 (h + 2 e) .. + 15 of column n, as the keys' lanes have them
     bf16x8_v q[4 * N];
     {
@@ -261,28 +263,18 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams p
     const int n = static_cast<int>(kt1 - kt0);
     ask(kt0);
     int there_next = there;
-    lds_barrier();  // the flags
+    lds_barrier();  // the flag
     put(kt0);
-    ask(kt0 + 1);
-    int there_after = there;
     lds_barrier();  // the first tile
-
-    floatx16_v sc;       // scores of the tile whose probabilities come next
-    float top = 0.f;     // of its column, in this wave's half
-    bf16x8_v pb[2];      // the own probabilities of the tile whose products come next
+    float top = 0.f;  // the largest score of the lane's column in this wave's half of the tile whose probabilities come next
     const unsigned char* key_lane = smem + 2 * (wave & 1) * S::kRunBytes + (col >> 4) * S::kRunBytes + hi * 256 + (col & 15) * 16;
-    // scores of tile i against the wave's 32 keys, masked, and their largest
-    auto scores = [&](int i, int have, floatx16_v& x) {
-      const int buf = i & (kKeyBufs - 1);
-      const unsigned char* at = key_lane + buf * S::kTileBytes;
-      const float scale = s_kscale[buf * kRuns + 2 * (wave & 1) + (col >> 4)];
-      x = floatx16_v(0.f);
-#pragma unroll
-      for (int f = 0; f < 2 * N; ++f) {
-        const uint4 u = *reinterpret_cast<const uint4*>(at + 512 * f);
-        x = __builtin_amdgcn_mfma_f32_32x32x16_bf16(operand(u.x, u.y, scale, scale), q[2 * f], x, 0, 0, 0);
-        x = __builtin_amdgcn_mfma_f32_32x32x16_bf16(operand(u.z, u.w, scale, scale), q[2 * f + 1], x, 0, 0, 0);
-      }
+    // o[m] has row 8 (r >> 2) + 4 h + (r & 3) = chunk c of 16 slice + c, dim 64 slice + 4 c + m of the wave's half (D = 256: slices 2
+    // and 3 are the second half; D = 128: m 2 and 3 are)
+    constexpr int kHalf = D == 256 ? 2 * 1024 : 8;
+    const unsigned char* value_lane = smem + S::kValues + (wave & 1) * kHalf + (col >> 4) * 1024 + hi * 256 + (col & 15) * 16;
+    const uint4* p_own = reinterpret_cast<const uint4*>(smem + S::kP) + wave * 128 + lane;
+    // masks the scores of tile i and tells the pair their largest
+    auto largest = [&](int i, int have, floatx16_v& x) {
       const int64_t key0 = (kt0 + i) * kTile;
       if (!(key0 + kTile <= first_pos + 1 && have == 15)) {
         const int lim = static_cast<int>(max64(-1, min64(kTile - 1, min64(first_pos + ahead, kv_end - 1) - key0))) - 32 * (wave & 1);  // the last key the column sees
@@ -298,110 +290,146 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams p
       top = fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
       if (hi == 0) s_max[((i & 1) * kWaves + wave) * 32 + col] = top;
     };
-    // probabilities of tile i: both waves of a pair move their columns' reference points alike
-    auto probabilities = [&](int i) {
-      const float mx = fmaxf(top, s_max[((i & 1) * kWaves + (wave ^ 1)) * 32 + col]) * qk_scale;
-      corr = 1.f;
-      if (__ballot(mx > m_run + kLazy) != 0) {
-        const float m_new = fmaxf(m_run, mx);
-        corr = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run - m_new);
-        m_run = m_new;
-        l_run *= corr;
-      }
-      const float use = m_run == -INFINITY ? 0.f : m_run;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r], qk_scale, -use));
-        l_run += pr;
-        pb[r >> 3][r & 7] = static_cast<__bf16>(pr);  // for the bf16 product; l_run has it unrounded
-      }
-      uint4* dst = reinterpret_cast<uint4*>(smem + S::kP) + ((i & 1) * kWaves + wave) * 128 + lane;
-      dst[0] = __builtin_bit_cast(uint4, pb[0]);
-      dst[64] = __builtin_bit_cast(uint4, pb[1]);
-    };
-    // products of tile i's values: o[m] has row 8 (r >> 2) + 4 h + (r & 3) = chunk c of 16 slice + c, dim 64 slice + 4 c + m of the
-    // wave's half (D = 256: slices 2 and 3 are the second half; D = 128: m 2 and 3 are)
-    constexpr int kHalf = D == 256 ? 2 * 1024 : 8;
-    const unsigned char* value_lane = smem + S::kValues + (wave & 1) * kHalf + (col >> 4) * 1024 + hi * 256 + (col & 15) * 16;
-    auto products = [&](int i, const bf16x8_v (&own_p)[2]) {
-      const uint4* src = reinterpret_cast<const uint4*>(smem + S::kP) + ((i & 1) * kWaves + (wave ^ 1)) * 128 + lane;
-      const bf16x8_v other[2] = {__builtin_bit_cast(bf16x8_v, src[0]), __builtin_bit_cast(bf16x8_v, src[64])};
-      const int buf = i & (kValueBufs - 1);
-      const unsigned char* at = value_lane + buf * S::kTileBytes;
-      const bool first = (wave & 1) == 0;
-#pragma unroll
-      for (int r = 0; r < kRuns; ++r) {
-        const float scale = s_vscale[buf * kRuns + r];
-        const bf16x8_v pr = (r < 2) == first ? own_p[r & 1] : other[r & 1];
-        uint32_t lo[MT], up[MT];
-        if constexpr (D == 256) {
-          const uint4 a = *reinterpret_cast<const uint4*>(at + r * S::kRunBytes), c = *reinterpret_cast<const uint4*>(at + r * S::kRunBytes + 512);
-          lo[0] = a.x, lo[1] = a.y, lo[2] = a.z, lo[3] = a.w;
-          up[0] = c.x, up[1] = c.y, up[2] = c.z, up[3] = c.w;
-        } else {
-          const uint2 a = *reinterpret_cast<const uint2*>(at + r * S::kRunBytes), c = *reinterpret_cast<const uint2*>(at + r * S::kRunBytes + 512);
-          lo[0] = a.x, lo[1] = a.y;
-          up[0] = c.x, up[1] = c.y;
-        }
-#pragma unroll
-        for (int m = 0; m < MT; ++m) o[m] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(operand(lo[m], up[m], scale, scale), pr, o[m], 0, 0, 0);
-      }
-      // ---- NaNs among keys that not every column sees
-      if (s_flag[buf] == i + 1) {
-        const ParamsAgain again = params_again();
-        for (int t = 0; t < kTile; ++t) {
-          const int64_t key = (kt0 + i) * kTile + t;
-          const int32_t ph = block_of_run(again->c, b, key >> 4, runs);
-          if (ph < 0 || key >= kv_end) continue;
-          const uint8_t* run = again->c.vpool + g * again->c.sG + static_cast<int64_t>(ph) * again->c.sP + ((key >> 4) & ((1 << (again->c.bs_shift - 4)) - 1)) * kv8::Run<D>::kBytes;
-          const uint8_t* mine = run + (wave & 1) * kHalf + ((t & 15) >> 2) * 256 + (t & 3);
-#pragma unroll
-          for (int r = 0; r < 16; ++r)
-#pragma unroll
-            for (int m = 0; m < MT; ++m)
-              if ((mine[(r >> 3) * 1024 + (8 * (r >> 2 & 1) + 4 * hi + (r & 3)) * 16 + 4 * m] & 0x7f) == 0x7f && key <= first_pos + ahead) o[m][r] = __uint_as_float(0x7fc00000u);
-        }
-      }
-    };
-    scores(0, there_next, sc);
-    put(kt0 + 1);
-    there_next = there_after;
-    lds_barrier();
-
-    auto iterate = [&](int i, auto has_scores, auto has_values) {
+    // Iteration i: the probabilities of tile i between the products of tile i - 1's values, then the scores of tile i + 1.
+    constexpr int kValues = 4 * MT;  // products of a tile's values
+    floatx16_v sc;
+    auto iterate = [&](int i, auto has_scores, auto has_probs, auto has_values) {
       if constexpr (has_scores) ask(kt0 + i + 2);
+      const unsigned char* vat = value_lane + ((i - 1) & (kValueBufs - 1)) * S::kTileBytes;
+      const float* vsc = s_vscale + ((i - 1) & (kValueBufs - 1)) * kRuns;
+      const uint4* pat = p_own + ((i - 1) & 1) * kWaves * 128 - (wave & 1) * 128;  // runs 0 and 1 are the first wave's of the pair
+      uint32_t vlo[2][MT], vup[2][MT];
+      float vscale[2];
+      bf16x8_v pv[2];
+      auto ask_values = [&](int r) {
+        vscale[r & 1] = vsc[r];
+        pv[r & 1] = __builtin_bit_cast(bf16x8_v, pat[(r >> 1) * 128 + 64 * (r & 1)]);
+        if constexpr (D == 256) {
+          const uint4 a = *reinterpret_cast<const uint4*>(vat + r * S::kRunBytes), c = *reinterpret_cast<const uint4*>(vat + r * S::kRunBytes + 512);
+          vlo[r & 1][0] = a.x, vlo[r & 1][1] = a.y, vlo[r & 1][2] = a.z, vlo[r & 1][3] = a.w;
+          vup[r & 1][0] = c.x, vup[r & 1][1] = c.y, vup[r & 1][2] = c.z, vup[r & 1][3] = c.w;
+        } else {
+          const uint2 a = *reinterpret_cast<const uint2*>(vat + r * S::kRunBytes), c = *reinterpret_cast<const uint2*>(vat + r * S::kRunBytes + 512);
+          vlo[r & 1][0] = a.x, vlo[r & 1][1] = a.y;
+          vup[r & 1][0] = c.x, vup[r & 1][1] = c.y;
+        }
+      };
       if constexpr (has_values) {
+        ask_values(0);
         if (__ballot(corr != 1.f) != 0) {  // columns whose reference point moved at the tile whose products come now
 #pragma unroll
           for (int m = 0; m < MT; ++m) o[m] *= corr;
         }
       }
-      bf16x8_v before[2] = {pb[0], pb[1]};
-      floatx16_v sc_next;
-      if constexpr (has_values) products(i - 1, before);
-      probabilities(i);
+      // ---- the reference points of tile i: both waves of a pair move their columns' alike
+      float use = 0.f;
+      if constexpr (has_probs) {
+        const float mx = fmaxf(top, s_max[((i & 1) * kWaves + (wave ^ 1)) * 32 + col]) * qk_scale;
+        corr = 1.f;
+        if (__ballot(mx > m_run + kLazy) != 0) {
+          const float m_new = fmaxf(m_run, mx);
+          corr = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run - m_new);
+          m_run = m_new;
+          l_run *= corr;
+        }
+        use = m_run == -INFINITY ? 0.f : m_run;
+      }
+      bf16x8_v pb;
+#pragma unroll
+      for (int f = 0; f < kValues; ++f) {
+        if constexpr (has_values) {
+          const int r = f / MT, m = f % MT;
+          if (m == 0 && r + 1 < kRuns) ask_values(r + 1);
+          o[m] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(operand(vlo[r & 1][m], vup[r & 1][m], vscale[r & 1], vscale[r & 1]), pv[r & 1], o[m], 0, 0, 0);
+        }
+        if constexpr (has_probs) {
+#pragma unroll
+          for (int r = f * (16 / kValues); r < (f + 1) * (16 / kValues); ++r) {
+            const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r], qk_scale, -use));
+            l_run += pr;
+            pb[r & 7] = static_cast<__bf16>(pr);  // for the bf16 product; l_run has it unrounded
+            if ((r & 7) == 7) const_cast<uint4*>(p_own)[(i & 1) * kWaves * 128 + 64 * (r >> 3)] = __builtin_bit_cast(uint4, pb);
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
       if constexpr (has_scores) {
-        scores(i + 1, there_next, sc_next);
-        sc = sc_next;
+        const int kbuf = (i + 1) & (kKeyBufs - 1);
+        const unsigned char* kat = key_lane + kbuf * S::kTileBytes;
+        const float kscale = s_kscale[kbuf * kRuns + 2 * (wave & 1) + (col >> 4)];
+        uint4 kc[3];
+        kc[0] = *reinterpret_cast<const uint4*>(kat);
+        kc[1] = *reinterpret_cast<const uint4*>(kat + 512);
+        sc = floatx16_v(0.f);
+#pragma unroll
+        for (int f = 0; f < 2 * N; ++f) {
+          const uint4 u = kc[f % 3];
+          if (f + 2 < 2 * N) kc[(f + 2) % 3] = *reinterpret_cast<const uint4*>(kat + 512 * (f + 2));
+          sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(operand(u.x, u.y, kscale, kscale), q[2 * f], sc, 0, 0, 0);
+          sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(operand(u.z, u.w, kscale, kscale), q[2 * f + 1], sc, 0, 0, 0);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        largest(i + 1, there_next, sc);
         there_next = there;
         put(kt0 + i + 2);
       }
-      lds_barrier();
+      if constexpr (has_probs || has_scores) lds_barrier();
     };
     using yes = std::integral_constant<bool, true>;
     using no = std::integral_constant<bool, false>;
+    iterate(-1, yes{}, no{}, no{});  // the first scores
     if (n > 1) {
-      iterate(0, yes{}, no{});
-      for (int i = 1; i + 1 < n; ++i) iterate(i, yes{}, yes{});
-      iterate(n - 1, no{}, yes{});
+      iterate(0, yes{}, yes{}, no{});
+      for (int i = 1; i + 1 < n; ++i) iterate(i, yes{}, yes{}, yes{});
+      iterate(n - 1, no{}, yes{}, yes{});
     } else {
-      iterate(0, no{}, no{});
+      iterate(0, no{}, yes{}, no{});
     }
-    if (__ballot(corr != 1.f) != 0) {
+    iterate(n, no{}, no{}, yes{});
+
+    // ---- NaNs among keys that not every column sees: products of their places with what each column sees
+    if (*s_flag != 0) {
+      uint16_t* s_nans = reinterpret_cast<uint16_t*>(smem);  // [run][slice][lane]: a bit a code
+      for (int64_t kt = max64(kt0, first_mixed); kt < kt1; ++kt) {
+        __syncthreads();
+        if (wave < kRuns) {
+          const ParamsAgain again = params_again();
+          const int64_t run = kt * kRuns + wave;
+          const int32_t id = block_of_run(again->c, b, run, runs);
+          const uint4* at = reinterpret_cast<const uint4*>(vb + static_cast<int64_t>(max(id, 0)) * again->c.sP + (run & ((1 << (again->c.bs_shift - 4)) - 1)) * kv8::Run<D>::kBytes) + lane;
+          const uint32_t mask = id < 0 ? 0u : tokens_mask(kv_end - run * kv8::kRun - 4 * (lane >> 4));
 #pragma unroll
-      for (int m = 0; m < MT; ++m) o[m] *= corr;
+          for (int s = 0; s < N; ++s) {
+            const uint4 u = at[64 * s];
+            uint32_t bits = 0;
+#pragma unroll
+            for (int m = 0; m < 4; ++m) bits |= ((nans_of(dword(u, m) & mask) * 0x10204080u) >> 28) << (4 * m);  // a dword's four side by side, token t at bit t
+            s_nans[(wave * N + s) * 64 + lane] = static_cast<uint16_t>(bits);
+          }
+        }
+        __syncthreads();
+        const uint16_t* at = s_nans + ((D == 256 ? 2 * (wave & 1) : 0) + (col >> 4)) * 64 + hi * 16 + (col & 15);
+        const int seen = static_cast<int>(max64(-1, min64(kTile, first_pos + ahead - kt * kTile)));  // the last key of the tile that the column sees
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          const int shift = 4 * m + (D == 256 ? 0 : 8 * (wave & 1));
+          floatx16_v found = floatx16_v(0.f);
+          for (int r = 0; r < kRuns; ++r) {
+            const uint32_t lo = at[r * N * 64] >> shift, up = at[r * N * 64 + 32] >> shift;
+            bf16x8_v there, sees;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              there[e] = static_cast<__bf16>(static_cast<float>((e < 4 ? lo : up) >> (e & 3) & 1));
+              sees[e] = static_cast<__bf16>(16 * r + 8 * (e >> 2) + 4 * hi + (e & 3) <= seen ? 1.f : 0.f);
+            }
+            found = __builtin_amdgcn_mfma_f32_32x32x16_bf16(there, sees, found, 0, 0, 0);
+          }
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (found[r] > 0.f) o[m][r] = __uint_as_float(0x7fc00000u);
+        }
+      }
     }
-    products(n - 1, pb);
   }
 
   // ---- out, through LDS
