@@ -334,6 +334,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams p
         }
         use = m_run == -INFINITY ? 0.f : m_run;
       }
+      // a wave in its value products goes ahead of its neighbour on the SIMD that is at its scores: 1034 us against 1048 without
+      // priorities and 1052 the other way round, 2048 tokens behind 32000
+      __builtin_amdgcn_s_setprio(1);
       bf16x8_v pb;
 #pragma unroll
       for (int f = 0; f < kValues; ++f) {
@@ -360,6 +363,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams p
         uint4 kc[3];
         kc[0] = *reinterpret_cast<const uint4*>(kat);
         kc[1] = *reinterpret_cast<const uint4*>(kat + 512);
+        __builtin_amdgcn_s_setprio(0);
         sc = floatx16_v(0.f);
 #pragma unroll
         for (int f = 0; f < 2 * N; ++f) {
