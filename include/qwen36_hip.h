@@ -418,8 +418,9 @@ int qa_paged_kv_fork(int32_t* block_tables, int64_t table_stride, int64_t max_bl
 /* Frees the blocks of rows release_rows[0 .. n - 1] (out of range: skipped): each
  * loses a holder and with its last one goes back to the list.  The rows become
  * empty (-1, length 0), the list ascending from 0 with -1 behind its end.
- * workspace: zeros.                                                           */
-int64_t qa_paged_kv_release_workspace(int64_t free_capacity);
+ * workspace: zeros, qa_paged_kv_release_workspace bytes (0 for small books:
+ * then it may be NULL).                                                       */
+int64_t qa_paged_kv_release_workspace(int64_t free_capacity, int64_t n, int64_t max_blocks);
 int qa_paged_kv_release(int32_t* block_tables, int64_t table_stride, int64_t max_blocks, int32_t* lengths, int64_t rows,
                         const void* release_rows, int32_t rows_dtype, int64_t n, int32_t* free_list, int64_t free_capacity,
                         int32_t* free_state, int32_t* references, int32_t* status, void* workspace, int64_t workspace_bytes,
@@ -429,8 +430,8 @@ int qa_paged_kv_release(int32_t* block_tables, int64_t table_stride, int64_t max
  * largest to the k-th lowest, as long as that is a lower id and k < max_moves:
  * tables, references and the list as after the moves, sources and targets
  * (max_moves) the pages to be copied, then -1.  Blocks that are neither free nor
- * in these tables stay where they are.  workspace: zeros.                      */
-int64_t qa_paged_kv_compact_workspace(int64_t free_capacity);
+ * in these tables stay where they are.  workspace as above.                    */
+int64_t qa_paged_kv_compact_workspace(int64_t free_capacity, int64_t rows, int64_t max_blocks, int64_t max_moves);
 int qa_paged_kv_compact(int32_t* block_tables, int64_t table_stride, int64_t max_blocks, int64_t rows, int32_t* free_list,
                         int64_t free_capacity, int32_t* free_state, int32_t* references, int32_t* status, int64_t max_moves,
                         int32_t* sources, int32_t* targets, void* workspace, int64_t workspace_bytes, hipStream_t stream);

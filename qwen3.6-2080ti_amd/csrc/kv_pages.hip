@@ -8,8 +8,9 @@
 //   compact  the largest ids that the tables hold move to the lowest free ones as long as that is lower: then the pools' ends are
 //            free.
 // The free list stays ascending: release and compact mark the free blocks in a bitmap, 32 blocks a word, and write the list anew
-// from it; a workgroup counts all words before its own (a few tens of KB out of L2) rather than wait for its neighbours.  So the
-// result does not depend on the order of the atomics that set the bits.
+// from it, a block's place being the bits below its own.  So the result does not depend on the order of the atomics that set the
+// bits.  Where the books are small one workgroup does all of it in LDS, in one launch; else the bitmap lies in the workspace and a
+// workgroup counts all words before its own (a few tens of KB out of L2) rather than wait for its neighbours.
 //
 // Books are small and latency bounds them; copies are bound by memory, each page read once and written once for each
 // copy of it.
@@ -74,11 +75,25 @@ struct ForkParams {
   int32_t* targets;
 };
 
-constexpr int kForks = 1024;  // of a call: a thread each
+constexpr int kForks = 1024;        // of a call: a thread each
+constexpr int kMaxRows = 65533;
+// Table entries up to which the forking workgroup writes them itself.
+constexpr int64_t kInlineEntries = 8192;
 
-__global__ __launch_bounds__(kForks) void fork_kernel(ForkParams p) {
-  __shared__ int64_t s_source[kForks], s_target[kForks];
+// Entry e of fork i, and a holder more for a block that it shares.
+__device__ __forceinline__ void fork_entry(const Books& k, int64_t source, int64_t target, int64_t e, int64_t entries, int32_t own) {
+  int32_t id = k.tables[source * k.table_stride + e];
+  if (own >= 0 && e == entries - 1)
+    id = own;
+  else if (id >= 0 && id < k.capacity)
+    atomicAdd(&k.references[id], 1);
+  k.tables[target * k.table_stride + e] = id;
+}
+
+__global__ __launch_bounds__(kForks) void fork_kernel(ForkParams p, int inline_entries) {
+  __shared__ uint32_t s_targets[(kMaxRows + 31) / 32 + 1], s_sources[(kMaxRows + 31) / 32 + 1];
   __shared__ int32_t s_wave[kForks / 64];
+  __shared__ int32_t s_row[kForks][2], s_own[kForks], s_entries[kForks];
   __shared__ int s_code;
   const Books& k = p.k;
   const int i = threadIdx.x;
@@ -88,33 +103,38 @@ __global__ __launch_bounds__(kForks) void fork_kernel(ForkParams p) {
     target = index_of(p.target_rows, p.rows_i64, i);
   }
   const bool live = source >= 0;  // -1: no fork
-  s_source[i] = live ? source : -1;
-  s_target[i] = live ? target : -1;
   const int64_t head = k.free_state[0], count = k.free_state[1];
+  for (int w = i; w < (k.rows + 31) / 32; w += kForks) s_targets[w] = s_sources[w] = 0;
   if (i == 0) s_code = head < 0 || count < 0 || head + count > k.capacity ? 3 : 0;
   __syncthreads();
+  const bool rows_ok = live && source < k.rows && target >= 0 && target < k.rows;
+  int bad = live && !rows_ok ? 6 : 0;
+  if (rows_ok) {
+    const uint32_t bit = 1u << (target & 31);
+    if (atomicOr(&s_targets[target >> 5], bit) & bit) bad = 6;  // named twice
+    atomicOr(&s_sources[source >> 5], 1u << (source & 31));
+  }
   int64_t length = 0;
   int32_t last = -1;
-  int bad = 0;
-  if (live) {
-    if (source >= k.rows || target < 0 || target >= k.rows || k.lengths[target] != 0) {
-      bad = 6;
-    } else {
-      for (int j = 0; j < p.n; ++j)
-        if ((j != i && s_target[j] == target) || s_source[j] == target) bad = 6;
-      length = k.lengths[source];
-      if (length < 0 || length > k.max_blocks * p.bs) bad = 4;
-    }
-    if (bad == 0 && length % p.bs != 0) last = k.tables[source * k.table_stride + length / p.bs];
+  if (rows_ok) {
+    if (k.lengths[target] != 0) bad = 6;
+    length = k.lengths[source];
+    if (length < 0 || length > k.max_blocks * p.bs)
+      bad = max(bad, 4);
+    else if (length % p.bs != 0)
+      last = k.tables[source * k.table_stride + length / p.bs];
   }
+  __syncthreads();
+  if (rows_ok && (s_sources[target >> 5] >> (target & 31) & 1)) bad = 6;
   if (bad != 0) atomicMax(&s_code, bad);
   const bool need = last >= 0 && last < k.capacity;
   int32_t total;
   const int32_t upto = block_scan<kForks>(need ? 1 : 0, s_wave, total);
   const int code = s_code != 0 ? s_code : total > count ? 1 : 0;  // the scan's barriers stand between the atomics and this
+  const int32_t own = need && code == 0 ? k.free_list[head + upto - 1] : -1;
   if (i < p.n) {
     p.sources[i] = need && code == 0 ? last : -1;
-    p.targets[i] = need && code == 0 ? k.free_list[head + upto - 1] : -1;
+    p.targets[i] = own;
     if (live && code == 0) k.lengths[target] = static_cast<int32_t>(length);
   }
   if (i == 0) {
@@ -124,6 +144,14 @@ __global__ __launch_bounds__(kForks) void fork_kernel(ForkParams p) {
       k.free_state[1] = static_cast<int32_t>(count - total);
     }
   }
+  if (!inline_entries || code != 0) return;
+  s_row[i][0] = static_cast<int32_t>(source);
+  s_row[i][1] = static_cast<int32_t>(target);
+  s_own[i] = own;
+  s_entries[i] = live ? static_cast<int32_t>((length + p.bs - 1) / p.bs) : 0;
+  __syncthreads();
+  for (int f = i / 64; f < p.n; f += kForks / 64)  // a wave a fork
+    for (int e = i % 64; e < s_entries[f]; e += 64) fork_entry(k, s_row[f][0], s_row[f][1], e, s_entries[f], s_own[f]);
 }
 
 // Table entries of fork blockIdx.y, a holder more for each block that it shares.
@@ -136,21 +164,22 @@ __global__ __launch_bounds__(256) void fork_tables_kernel(ForkParams p) {
   const int64_t length = k.lengths[source];
   const int64_t entries = (length + p.bs - 1) / p.bs;
   const int32_t own = p.targets[i];
-  for (int64_t e = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; e < entries; e += static_cast<int64_t>(gridDim.x) * 256) {
-    int32_t id = k.tables[source * k.table_stride + e];
-    if (own >= 0 && e == entries - 1)
-      id = own;
-    else if (id >= 0 && id < k.capacity)
-      atomicAdd(&k.references[id], 1);
-    k.tables[target * k.table_stride + e] = id;
-  }
+  for (int64_t e = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; e < entries; e += static_cast<int64_t>(gridDim.x) * 256) fork_entry(k, source, target, e, entries, own);
 }
 
 // ---- the free list from a bitmap ----------------------------------------------
 
-constexpr int kListThreads = 256;  // a word each
+constexpr int kListThreads = 256;
+constexpr int kListWords = 64;  // of a workgroup where the bitmap lies in the workspace
+
+// One workgroup does a release or a compaction where the pool has up to so many blocks (a word of the bitmap a thread) ..
+constexpr int kSmallThreads = 1024;
+constexpr int64_t kSmallBlocks = 32 * kSmallThreads;
+// .. and the rows so many table entries, and a compaction so many pairs.
+constexpr int64_t kSmallEntries = 16384;
 
 __device__ __forceinline__ void set_bit(uint32_t* bits, int32_t id) { atomicOr(&bits[id >> 5], 1u << (id & 31)); }
+__device__ __forceinline__ uint32_t below(int32_t id) { return (1u << (id & 31)) - 1u; }
 
 // Marks the free list's blocks.
 __device__ __forceinline__ void mark_free(const Books& k, uint32_t* bits, int64_t first, int64_t step) {
@@ -161,46 +190,40 @@ __device__ __forceinline__ void mark_free(const Books& k, uint32_t* bits, int64_
   }
 }
 
-// Bits below word `mine` of the words that `word` gives, and of all of them.
+// Where the bitmap lies in the workspace: the bits below each of this workgroup's words go to s_before, `total` is all of them.
 template <typename F>
-__device__ __forceinline__ void count_before(int64_t words, F word, int32_t* s_wave, int32_t& incl, int32_t& total) {
-  const int64_t base = static_cast<int64_t>(blockIdx.x) * kListThreads;
+__device__ __forceinline__ void count_words(int64_t words, F word, int32_t* s_wave, int32_t* s_before, int32_t& total) {
+  const int64_t base = static_cast<int64_t>(blockIdx.x) * kListWords;
   int32_t before = 0, all = 0;
   for (int64_t w = threadIdx.x; w < words; w += kListThreads) {
     const int32_t c = __popc(word(w));
     if (w < base) before += c;
     all += c;
   }
-  int32_t sum;
+  int32_t sum, own;
   block_scan<kListThreads>(before, s_wave, sum);
   block_scan<kListThreads>(all, s_wave, total);
-  int32_t own;
-  incl = sum + block_scan<kListThreads>(base + threadIdx.x < words ? __popc(word(base + threadIdx.x)) : 0, s_wave, own);
+  const int32_t mine = threadIdx.x < kListWords && base + threadIdx.x < words ? __popc(word(base + threadIdx.x)) : 0;
+  const int32_t incl = block_scan<kListThreads>(mine, s_wave, own);
+  if (threadIdx.x < kListWords) s_before[threadIdx.x] = sum + incl - mine;
+  __syncthreads();
 }
 
-// Writes the list and its cursor: this workgroup's words, and -1 at its share of the places behind the list's end.
+// Blocks id0, id0 + step .. below id1 of the list: a free block at the place that the bits below it give, -1 behind the end.
 template <typename F>
-__device__ __forceinline__ void write_list(const Books& k, int64_t words, F word, int32_t* s_wave) {
-  int32_t incl, total;
-  count_before(words, word, s_wave, incl, total);
-  const int64_t w = static_cast<int64_t>(blockIdx.x) * kListThreads + threadIdx.x;
-  if (w < words) {
-    uint32_t bits = word(w);
-    int32_t at = incl - __popc(bits);
-    while (bits != 0) {
-      const int b = __ffs(bits) - 1;
-      bits &= bits - 1;
-      k.free_list[at++] = static_cast<int32_t>(32 * w + b);
-    }
+__device__ __forceinline__ void write_list(const Books& k, int64_t id0, int64_t id1, int64_t step, F word, const int32_t* before, int64_t first_word, int32_t total) {
+  for (int64_t i = id0; i < id1; i += step) {
+    const int32_t id = static_cast<int32_t>(i);
+    const uint32_t bits = word(id >> 5);
+    if (bits >> (id & 31) & 1) k.free_list[before[(id >> 5) - first_word] + __popc(bits & below(id))] = id;
+    if (i >= total) k.free_list[i] = -1;
   }
-  const int64_t lo = max64(total, static_cast<int64_t>(blockIdx.x) * kListThreads * 32);
-  const int64_t hi = min64(k.capacity, (static_cast<int64_t>(blockIdx.x) + 1) * kListThreads * 32);
-  for (int64_t i = lo + threadIdx.x; i < hi; i += kListThreads) k.free_list[i] = -1;
-  if (blockIdx.x == 0 && threadIdx.x == 0) {
-    k.free_state[0] = 0;
-    k.free_state[1] = total;
-    k.status[0] = 0;
-  }
+}
+
+__device__ __forceinline__ void close_books(const Books& k, int32_t total) {
+  k.free_state[0] = 0;
+  k.free_state[1] = total;
+  k.status[0] = 0;
 }
 
 // ---- release ------------------------------------------------------------------
@@ -212,6 +235,45 @@ struct ReleaseParams {
   uint32_t* bits;    // (words + 1), zeros: free blocks; the last word is 1 where the free list's cursor is out of range
   int64_t words;
 };
+
+// Table entry e of a row loses its block.
+__device__ __forceinline__ void release_entry(const Books& k, int64_t row, int64_t e, uint32_t* bits) {
+  int32_t* entry = &k.tables[row * k.table_stride + e];
+  if (*entry == -1) return;
+  const int32_t id = atomicExch(entry, -1);  // a row named twice is freed once
+  if (id < 0 || id >= k.capacity) return;
+  if (atomicSub(&k.references[id], 1) > 0) return;
+  atomicAdd(&k.references[id], 1);
+  set_bit(bits, id);
+}
+
+// All of it in one workgroup.
+__global__ __launch_bounds__(kSmallThreads) void release_small_kernel(ReleaseParams p) {
+  __shared__ uint32_t s_bits[kSmallThreads];
+  __shared__ int32_t s_before[kSmallThreads], s_wave[kSmallThreads / 64];
+  const Books& k = p.k;
+  const int tid = threadIdx.x;
+  s_bits[tid] = 0;
+  if (corrupt(k)) {
+    if (tid == 0) k.status[0] = 3;
+    return;
+  }
+  __syncthreads();
+  mark_free(k, s_bits, tid, kSmallThreads);
+  for (int i = tid / 64; i < p.n; i += kSmallThreads / 64) {  // a wave a row
+    const int64_t row = index_of(p.release_rows, p.rows_i64, i);
+    if (row < 0 || row >= k.rows) continue;
+    for (int64_t e = tid % 64; e < k.max_blocks; e += 64) release_entry(k, row, e, s_bits);
+    if (tid % 64 == 0) k.lengths[row] = 0;
+  }
+  __syncthreads();
+  int32_t total;
+  const int32_t mine = __popc(s_bits[tid]);
+  s_before[tid] = block_scan<kSmallThreads>(mine, s_wave, total) - mine;
+  __syncthreads();
+  write_list(k, tid, k.capacity, kSmallThreads, [&](int64_t w) { return s_bits[w]; }, s_before, 0, total);
+  if (tid == 0) close_books(k, total);
+}
 
 // blockIdx.y < n: the blocks of a row; n: the free list.
 __global__ __launch_bounds__(256) void release_kernel(ReleaseParams p) {
@@ -227,25 +289,23 @@ __global__ __launch_bounds__(256) void release_kernel(ReleaseParams p) {
   }
   const int64_t row = index_of(p.release_rows, p.rows_i64, blockIdx.y);
   if (row < 0 || row >= k.rows) return;
-  for (int64_t e = first; e < k.max_blocks; e += step) {
-    int32_t* entry = &k.tables[row * k.table_stride + e];
-    if (*entry == -1) continue;
-    const int32_t id = atomicExch(entry, -1);  // a row named twice is freed once
-    if (id < 0 || id >= k.capacity) continue;
-    if (atomicSub(&k.references[id], 1) > 0) continue;
-    atomicAdd(&k.references[id], 1);
-    set_bit(p.bits, id);
-  }
+  for (int64_t e = first; e < k.max_blocks; e += step) release_entry(k, row, e, p.bits);
   if (first == 0) k.lengths[row] = 0;
 }
 
 __global__ __launch_bounds__(kListThreads) void release_list_kernel(ReleaseParams p) {
-  __shared__ int32_t s_wave[kListThreads / 64];
+  __shared__ int32_t s_wave[kListThreads / 64], s_before[kListWords];
+  const Books& k = p.k;
   if (p.bits[p.words] != 0) {
-    if (blockIdx.x == 0 && threadIdx.x == 0) p.k.status[0] = 3;
+    if (blockIdx.x == 0 && threadIdx.x == 0) k.status[0] = 3;
     return;
   }
-  write_list(p.k, p.words, [&](int64_t w) { return p.bits[w]; }, s_wave);
+  auto word = [&](int64_t w) { return p.bits[w]; };
+  int32_t total;
+  count_words(p.words, word, s_wave, s_before, total);
+  const int64_t w0 = static_cast<int64_t>(blockIdx.x) * kListWords;
+  write_list(k, 32 * w0 + threadIdx.x, min64(k.capacity, 32 * (w0 + kListWords)), kListThreads, word, s_before, w0, total);
+  if (blockIdx.x == 0 && threadIdx.x == 0) close_books(k, total);
 }
 
 // ---- compact --------------------------------------------------------------------
@@ -262,6 +322,72 @@ struct CompactParams {
   int32_t* targets;
   int list_groups;
 };
+
+// Where a held block with `nth` held ones above it goes, -1: it stays.
+__device__ __forceinline__ int32_t place_of(const CompactParams& p, int32_t nth, int32_t source) {
+  if (nth >= min64(p.max_moves, p.k.free_state[1])) return -1;
+  const int32_t target = p.k.free_list[p.k.free_state[0] + static_cast<int64_t>(nth)];
+  return target < source ? target : -1;
+}
+
+__device__ __forceinline__ void move_block(const CompactParams& p, int32_t nth, int32_t source, int32_t target, uint32_t* flip) {
+  p.sources[nth] = source;
+  p.targets[nth] = target;
+  p.k.references[target] = p.k.references[source];
+  p.k.references[source] = 0;
+  set_bit(flip, source);
+  set_bit(flip, target);
+}
+
+// All of it in one workgroup.
+__global__ __launch_bounds__(kSmallThreads) void compact_small_kernel(CompactParams p) {
+  __shared__ uint32_t s_free[kSmallThreads], s_held[kSmallThreads], s_flip[kSmallThreads];
+  __shared__ int32_t s_before[kSmallThreads], s_wave[kSmallThreads / 64];
+  const Books& k = p.k;
+  const int tid = threadIdx.x;
+  s_free[tid] = s_held[tid] = s_flip[tid] = 0;
+  for (int64_t i = tid; i < p.max_moves; i += kSmallThreads) p.sources[i] = p.targets[i] = -1;
+  if (corrupt(k)) {
+    if (tid == 0) k.status[0] = 3;
+    return;
+  }
+  __syncthreads();
+  mark_free(k, s_free, tid, kSmallThreads);
+  for (int64_t row = tid / 64; row < k.rows; row += kSmallThreads / 64)
+    for (int64_t e = tid % 64; e < k.max_blocks; e += 64) {
+      const int32_t id = k.tables[row * k.table_stride + e];
+      if (id >= 0 && id < k.capacity) set_bit(s_held, id);
+    }
+  __syncthreads();
+  s_held[tid] &= ~s_free[tid];
+  int32_t total;
+  const int32_t mine = __popc(s_held[tid]);
+  s_before[tid] = block_scan<kSmallThreads>(mine, s_wave, total) - mine;
+  __syncthreads();
+  auto nth_of = [&](int32_t id) { return total - 1 - s_before[id >> 5] - __popc(s_held[id >> 5] & below(id)); };
+  for (int64_t i = tid; i < k.capacity; i += kSmallThreads) {
+    const int32_t id = static_cast<int32_t>(i);
+    if (!(s_held[id >> 5] >> (id & 31) & 1)) continue;
+    const int32_t nth = nth_of(id), target = place_of(p, nth, id);
+    if (target >= 0) move_block(p, nth, id, target, s_flip);
+  }
+  __syncthreads();
+  for (int64_t row = tid / 64; row < k.rows; row += kSmallThreads / 64)
+    for (int64_t e = tid % 64; e < k.max_blocks; e += 64) {
+      int32_t* entry = &k.tables[row * k.table_stride + e];
+      const int32_t id = *entry;
+      if (id >= 0 && id < k.capacity && (s_held[id >> 5] & s_flip[id >> 5]) >> (id & 31) & 1) *entry = place_of(p, nth_of(id), id);
+    }
+  __syncthreads();  // the old list has been read
+  const uint32_t bits = s_free[tid] ^ s_flip[tid];
+  const int32_t free_here = __popc(bits);
+  const int32_t incl = block_scan<kSmallThreads>(free_here, s_wave, total);
+  s_before[tid] = incl - free_here;
+  s_free[tid] = bits;
+  __syncthreads();
+  write_list(k, tid, k.capacity, kSmallThreads, [&](int64_t w) { return s_free[w]; }, s_before, 0, total);
+  if (tid == 0) close_books(k, total);
+}
 
 // blockIdx.y < rows: the blocks of a row; then the free list; then the pairs, set to none.
 __global__ __launch_bounds__(256) void compact_mark_kernel(CompactParams p) {
@@ -286,54 +412,48 @@ __global__ __launch_bounds__(256) void compact_mark_kernel(CompactParams p) {
   }
 }
 
-// The block with k held ones above it moves to the k-th free one where that is lower.
 __global__ __launch_bounds__(kListThreads) void compact_moves_kernel(CompactParams p) {
-  __shared__ int32_t s_wave[kListThreads / 64];
+  __shared__ int32_t s_wave[kListThreads / 64], s_before[kListWords];
   const Books& k = p.k;
   if (p.refused[0] != 0) return;
   auto word = [&](int64_t w) { return p.held[w] & ~p.free_bits[w]; };
-  int32_t incl, total;
-  count_before(p.words, word, s_wave, incl, total);
-  const int64_t w = static_cast<int64_t>(blockIdx.x) * kListThreads + threadIdx.x;
-  if (w >= p.words) return;
-  const int64_t head = k.free_state[0], most = min64(p.max_moves, k.free_state[1]);
-  uint32_t bits = word(w);
-  int32_t nth = total - incl + __popc(bits);  // held blocks from this word on
-  while (bits != 0) {
-    const int b = __ffs(bits) - 1;
-    bits &= bits - 1;
-    const int32_t source = static_cast<int32_t>(32 * w + b);
-    if (--nth >= most) continue;
-    const int32_t target = k.free_list[head + nth];
-    if (target < 0 || target >= source) continue;
-    p.sources[nth] = source;
-    p.targets[nth] = target;
-    p.place[source] = target;
-    k.references[target] = k.references[source];
-    k.references[source] = 0;
-    set_bit(p.flip, source);
-    set_bit(p.flip, target);
+  int32_t total;
+  count_words(p.words, word, s_wave, s_before, total);
+  const int64_t w0 = static_cast<int64_t>(blockIdx.x) * kListWords, end = min64(k.capacity, 32 * (w0 + kListWords));
+  for (int64_t i = 32 * w0 + threadIdx.x; i < end; i += kListThreads) {
+    const int32_t id = static_cast<int32_t>(i);
+    const uint32_t bits = word(id >> 5);
+    if (!(bits >> (id & 31) & 1)) continue;
+    const int32_t nth = total - 1 - s_before[(id >> 5) - w0] - __popc(bits & below(id)), target = place_of(p, nth, id);
+    if (target < 0) continue;
+    p.place[id] = target;
+    move_block(p, nth, id, target, p.flip);
   }
 }
 
 // blockIdx.y 0: the free list; then the tables' rows.
 __global__ __launch_bounds__(kListThreads) void compact_list_kernel(CompactParams p) {
-  __shared__ int32_t s_wave[kListThreads / 64];
+  __shared__ int32_t s_wave[kListThreads / 64], s_before[kListWords];
   const Books& k = p.k;
   if (p.refused[0] != 0) {
     if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) k.status[0] = 3;
     return;
   }
   if (blockIdx.y == 0) {
-    if (static_cast<int>(blockIdx.x) < p.list_groups) write_list(k, p.words, [&](int64_t w) { return p.free_bits[w] ^ p.flip[w]; }, s_wave);
+    if (static_cast<int>(blockIdx.x) >= p.list_groups) return;
+    auto word = [&](int64_t w) { return p.free_bits[w] ^ p.flip[w]; };
+    int32_t total;
+    count_words(p.words, word, s_wave, s_before, total);
+    const int64_t w0 = static_cast<int64_t>(blockIdx.x) * kListWords;
+    write_list(k, 32 * w0 + threadIdx.x, min64(k.capacity, 32 * (w0 + kListWords)), kListThreads, word, s_before, w0, total);
+    if (blockIdx.x == 0 && threadIdx.x == 0) close_books(k, total);
     return;
   }
   for (int64_t e = static_cast<int64_t>(blockIdx.x) * kListThreads + threadIdx.x; e < k.max_blocks; e += static_cast<int64_t>(gridDim.x) * kListThreads) {
     int32_t* entry = &k.tables[(blockIdx.y - 1) * k.table_stride + e];
     const int32_t id = *entry;
     if (id < 0 || id >= k.capacity) continue;
-    const uint32_t bit = 1u << (id & 31);
-    if (p.flip[id >> 5] & p.held[id >> 5] & ~p.free_bits[id >> 5] & bit) *entry = p.place[id];
+    if ((p.flip[id >> 5] & p.held[id >> 5] & ~p.free_bits[id >> 5]) >> (id & 31) & 1) *entry = p.place[id];
   }
 }
 
@@ -382,9 +502,12 @@ __global__ __launch_bounds__(kCopyThreads) void copy_kernel(CopyParams p) {
 
 static int64_t words_of(int64_t capacity) { return ceil_div(capacity, 32); }
 
+// Whether one workgroup does a release or a compaction.
+static bool small(int64_t capacity, int64_t entries, int64_t pairs) { return capacity <= kSmallBlocks && entries <= kSmallEntries && pairs <= kSmallBlocks; }
+
 static int check_books(const char* what, const Books& k) {
   QA_REQUIRE(k.tables && k.free_list && k.free_state && k.references && k.status, "%s: pointers must be non-null", what);
-  QA_REQUIRE(k.rows >= 1 && k.rows <= 65533, "%s: the tables must have 1 to 65533 rows", what);
+  QA_REQUIRE(k.rows >= 1 && k.rows <= kMaxRows, "%s: the tables must have 1 to 65533 rows", what);
   QA_REQUIRE(k.max_blocks >= 1 && k.max_blocks <= 0x7fffffff, "%s: block table must have at least one entry", what);
   QA_REQUIRE(k.table_stride >= k.max_blocks || k.rows == 1, "table rows overlap: stride %lld < max_blocks %lld", static_cast<long long>(k.table_stride), static_cast<long long>(k.max_blocks));
   QA_REQUIRE(k.capacity >= 1 && k.capacity <= 0x7fffffff, "free list capacity must be in [1, 2^31)");
@@ -418,10 +541,10 @@ extern "C" int qa_paged_kv_fork(int32_t* block_tables, int64_t table_stride, int
   p.targets = targets;
   {
     KernelTimer timer_("kv_fork", stream);
-    hipLaunchKernelGGL(fork_kernel, dim3(1), dim3(kForks), 0, stream, p);
+    hipLaunchKernelGGL(fork_kernel, dim3(1), dim3(kForks), 0, stream, p, n * max_blocks <= kInlineEntries ? 1 : 0);
   }
   if (int rc = check_launch("paged_kv_fork")) return rc;
-  if (n == 0) return 0;
+  if (n * max_blocks <= kInlineEntries) return 0;
   {
     KernelTimer timer_("kv_fork_tables", stream);
     hipLaunchKernelGGL(fork_tables_kernel, dim3(groups_of(max_blocks), static_cast<unsigned>(n)), dim3(256), 0, stream, p);
@@ -429,7 +552,10 @@ extern "C" int qa_paged_kv_fork(int32_t* block_tables, int64_t table_stride, int
   return check_launch("paged_kv_fork");
 }
 
-extern "C" int64_t qa_paged_kv_release_workspace(int64_t free_capacity) { return free_capacity <= 0 ? 0 : 4 * (qa::pages::words_of(free_capacity) + 1); }
+extern "C" int64_t qa_paged_kv_release_workspace(int64_t free_capacity, int64_t n, int64_t max_blocks) {
+  if (free_capacity <= 0 || n < 0 || max_blocks <= 0 || qa::pages::small(free_capacity, n * max_blocks, 0)) return 0;
+  return 4 * (qa::pages::words_of(free_capacity) + 1);
+}
 
 extern "C" int qa_paged_kv_release(int32_t* block_tables, int64_t table_stride, int64_t max_blocks, int32_t* lengths, int64_t rows, const void* release_rows,
                                    int32_t rows_dtype, int64_t n, int32_t* free_list, int64_t free_capacity, int32_t* free_state, int32_t* references, int32_t* status,
@@ -442,13 +568,21 @@ extern "C" int qa_paged_kv_release(int32_t* block_tables, int64_t table_stride, 
   QA_REQUIRE(is_index_dtype(rows_dtype), "paged_kv_release: rows must be int32 or int64");
   QA_REQUIRE(n >= 0 && n <= 65533, "paged_kv_release: at most 65533 rows a call");
   QA_REQUIRE(lengths != nullptr && (n == 0 || release_rows != nullptr), "paged_kv_release: pointers must be non-null");
-  QA_REQUIRE(workspace != nullptr && workspace_bytes >= qa_paged_kv_release_workspace(free_capacity) && (reinterpret_cast<uintptr_t>(workspace) & 3u) == 0,
-             "paged_kv_release: workspace too small or not 4-byte aligned: need %lld bytes", static_cast<long long>(qa_paged_kv_release_workspace(free_capacity)));
+  const int64_t need = qa_paged_kv_release_workspace(free_capacity, n, max_blocks);
+  QA_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 3u) == 0),
+             "paged_kv_release: workspace too small or not 4-byte aligned: need %lld bytes", static_cast<long long>(need));
   p.release_rows = release_rows;
   p.n = static_cast<int>(n);
   p.rows_i64 = rows_dtype == QA_I64;
   p.bits = reinterpret_cast<uint32_t*>(workspace);
   p.words = words_of(free_capacity);
+  if (need == 0) {
+    {
+      KernelTimer timer_("kv_release", stream);
+      hipLaunchKernelGGL(release_small_kernel, dim3(1), dim3(kSmallThreads), 0, stream, p);
+    }
+    return check_launch("paged_kv_release");
+  }
   {
     KernelTimer timer_("kv_release", stream);
     hipLaunchKernelGGL(release_kernel, dim3(groups_of(std::max(max_blocks, free_capacity)), static_cast<unsigned>(n + 1)), dim3(256), 0, stream, p);
@@ -456,13 +590,14 @@ extern "C" int qa_paged_kv_release(int32_t* block_tables, int64_t table_stride, 
   if (int rc = check_launch("paged_kv_release")) return rc;
   {
     KernelTimer timer_("kv_release_list", stream);
-    hipLaunchKernelGGL(release_list_kernel, dim3(static_cast<unsigned>(ceil_div(p.words, kListThreads))), dim3(kListThreads), 0, stream, p);
+    hipLaunchKernelGGL(release_list_kernel, dim3(static_cast<unsigned>(ceil_div(p.words, kListWords))), dim3(kListThreads), 0, stream, p);
   }
   return check_launch("paged_kv_release");
 }
 
-extern "C" int64_t qa_paged_kv_compact_workspace(int64_t free_capacity) {
-  return free_capacity <= 0 ? 0 : 4 * (3 * qa::pages::words_of(free_capacity) + 1 + free_capacity);
+extern "C" int64_t qa_paged_kv_compact_workspace(int64_t free_capacity, int64_t rows, int64_t max_blocks, int64_t max_moves) {
+  if (free_capacity <= 0 || rows <= 0 || max_blocks <= 0 || max_moves < 0 || qa::pages::small(free_capacity, rows * max_blocks, max_moves)) return 0;
+  return 4 * (3 * qa::pages::words_of(free_capacity) + 1 + free_capacity);
 }
 
 extern "C" int qa_paged_kv_compact(int32_t* block_tables, int64_t table_stride, int64_t max_blocks, int64_t rows, int32_t* free_list, int64_t free_capacity,
@@ -475,18 +610,26 @@ extern "C" int qa_paged_kv_compact(int32_t* block_tables, int64_t table_stride, 
   if (int rc = check_books("paged_kv_compact", p.k)) return rc;
   QA_REQUIRE(max_moves >= 0 && max_moves <= 0x7fffffff, "paged_kv_compact: max_moves out of range");
   QA_REQUIRE(max_moves == 0 || (sources && targets), "paged_kv_compact: pointers must be non-null");
-  QA_REQUIRE(workspace != nullptr && workspace_bytes >= qa_paged_kv_compact_workspace(free_capacity) && (reinterpret_cast<uintptr_t>(workspace) & 3u) == 0,
-             "paged_kv_compact: workspace too small or not 4-byte aligned: need %lld bytes", static_cast<long long>(qa_paged_kv_compact_workspace(free_capacity)));
+  const int64_t need = qa_paged_kv_compact_workspace(free_capacity, rows, max_blocks, max_moves);
+  QA_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 3u) == 0),
+             "paged_kv_compact: workspace too small or not 4-byte aligned: need %lld bytes", static_cast<long long>(need));
   p.words = words_of(free_capacity);
   p.max_moves = max_moves;
+  p.sources = sources;
+  p.targets = targets;
+  if (need == 0) {
+    {
+      KernelTimer timer_("kv_compact", stream);
+      hipLaunchKernelGGL(compact_small_kernel, dim3(1), dim3(kSmallThreads), 0, stream, p);
+    }
+    return check_launch("paged_kv_compact");
+  }
   p.free_bits = reinterpret_cast<uint32_t*>(workspace);
   p.held = p.free_bits + p.words;
   p.flip = p.held + p.words;
   p.refused = p.flip + p.words;
   p.place = reinterpret_cast<int32_t*>(p.refused + 1);
-  p.sources = sources;
-  p.targets = targets;
-  const unsigned lists = static_cast<unsigned>(ceil_div(p.words, kListThreads));
+  const unsigned lists = static_cast<unsigned>(ceil_div(p.words, kListWords));
   p.list_groups = static_cast<int>(lists);
   {
     KernelTimer timer_("kv_compact_mark", stream);

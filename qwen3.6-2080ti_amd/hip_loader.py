@@ -201,12 +201,12 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
         [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int32, c_int64, c_int32, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
          c_void_p],
     ),
-    "qa_paged_kv_release_workspace": (c_int64, [c_int64]),
+    "qa_paged_kv_release_workspace": (c_int64, [c_int64, c_int64, c_int64]),
     "qa_paged_kv_release": (
         c_int32,
         [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int32, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p],
     ),
-    "qa_paged_kv_compact_workspace": (c_int64, [c_int64]),
+    "qa_paged_kv_compact_workspace": (c_int64, [c_int64, c_int64, c_int64, c_int64]),
     "qa_paged_kv_compact": (
         c_int32,
         [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_void_p],

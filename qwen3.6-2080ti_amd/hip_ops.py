@@ -1541,20 +1541,24 @@ def _books(
     device: torch.device, block_tables: torch.Tensor, lengths: torch.Tensor | None, free_list: torch.Tensor, free_state: torch.Tensor, references: torch.Tensor, status: torch.Tensor,
 ) -> tuple[int, int]:
     """Checks the books of a pool; their rows and the table's width."""
-    if device.type != "cuda" or not (free_list.device == free_state.device == references.device == status.device == device) or (lengths is not None and lengths.device != device):
-        _same_device(device, block_tables=block_tables, lengths=block_tables if lengths is None else lengths, free_list=free_list, free_state=free_state, references=references,
-                     status=status)
     i32 = torch.int32
-    _require(block_tables.dtype is i32 and block_tables.dim() == 2 and block_tables.stride(1) == 1, "block_tables must be int32 [rows, max_blocks] with contiguous rows")
-    rows, max_blocks = block_tables.shape
-    _require(rows > 0 and max_blocks > 0, "block_tables must have shape [rows, max_blocks]")
-    if lengths is not None:
-        _require(lengths.dtype is i32 and lengths.shape == (rows,) and lengths.is_contiguous(), "lengths must be a contiguous int32 [rows] tensor")
+    shape = block_tables.shape
+    if (
+        device.type == "cuda" and free_list.device == free_state.device == references.device == status.device == device
+        and block_tables.dtype is i32 and len(shape) == 2 and block_tables.stride(1) == 1 and shape[0] > 0 and shape[1] > 0
+        and (lengths is None or (lengths.device == device and lengths.dtype is i32 and lengths.shape == shape[:1] and lengths.is_contiguous()))
+        and free_list.dtype is i32 and free_list.dim() == 1 and free_list.is_contiguous() and free_state.dtype is i32 and free_state.shape == (2,) and free_state.is_contiguous()
+        and references.dtype is i32 and references.shape == free_list.shape and references.is_contiguous() and status.dtype is i32 and status.numel() >= 1
+    ):
+        return shape
+    _same_device(device, block_tables=block_tables, lengths=block_tables if lengths is None else lengths, free_list=free_list, free_state=free_state, references=references, status=status)
+    _require(block_tables.dtype is i32 and len(shape) == 2 and block_tables.stride(1) == 1, "block_tables must be int32 [rows, max_blocks] with contiguous rows")
+    _require(shape[0] > 0 and shape[1] > 0, "block_tables must have shape [rows, max_blocks]")
+    _require(lengths is None or (lengths.dtype is i32 and lengths.shape == shape[:1] and lengths.is_contiguous()), "lengths must be a contiguous int32 [rows] tensor")
     _require(free_list.dtype is i32 and free_list.dim() == 1 and free_list.is_contiguous(), "free_list must be a contiguous int32 vector")
-    _require(free_state.dtype is i32 and free_state.numel() == 2 and free_state.is_contiguous(), "free_state must be int32 [head, count]")
+    _require(free_state.dtype is i32 and free_state.shape == (2,) and free_state.is_contiguous(), "free_state must be int32 [head, count]")
     _require(references.dtype is i32 and references.shape == free_list.shape and references.is_contiguous(), "references must be a contiguous int32 tensor with an entry for each block")
-    _require(status.dtype is i32 and status.numel() >= 1, "status must be an int32 tensor")
-    return rows, max_blocks
+    raise RuntimeError("status must be an int32 tensor")
 
 
 def _row_list(rows: torch.Tensor, name: str, device: torch.device) -> torch.Tensor:
@@ -1591,7 +1595,7 @@ def paged_kv_fork(
         int(block_size), free_list.data_ptr(), free_list.numel(), free_state.data_ptr(), references.data_ptr(), status.data_ptr(), pages.data_ptr(), pages.data_ptr() + 4 * n,
     )
     L.check(lib, code, "paged_kv_fork")
-    return PagedCopy(pages[0], pages[1])
+    return PagedCopy(*pages.unbind())
 
 
 def paged_kv_release(
@@ -1608,11 +1612,11 @@ def paged_kv_release(
     device = block_tables.device
     rows, max_blocks = _books(device, block_tables, lengths, free_list, free_state, references, status)
     which = _row_list(release_rows, "release_rows", device)
-    nbytes = lib.qa_paged_kv_release_workspace(free_list.numel())
-    ws = torch.zeros(nbytes // 4, dtype=torch.int32, device=device)
+    nbytes = lib.qa_paged_kv_release_workspace(free_list.numel(), which.numel(), max_blocks)
+    ws = torch.zeros(nbytes // 4, dtype=torch.int32, device=device) if nbytes else None
     code = _launch(
         device, lib.qa_paged_kv_release, block_tables.data_ptr(), block_tables.stride(0), max_blocks, lengths.data_ptr(), rows, which.data_ptr(), _code(which), which.numel(),
-        free_list.data_ptr(), free_list.numel(), free_state.data_ptr(), references.data_ptr(), status.data_ptr(), ws.data_ptr(), nbytes,
+        free_list.data_ptr(), free_list.numel(), free_state.data_ptr(), references.data_ptr(), status.data_ptr(), _ptr(ws), nbytes,
     )
     L.check(lib, code, "paged_kv_release")
 
@@ -1633,14 +1637,14 @@ def paged_kv_compact(
     max_moves = int(max_moves)
     _require(max_moves >= 0, "max_moves must be non-negative")
     pages = block_tables.new_empty((2, max_moves))
-    nbytes = lib.qa_paged_kv_compact_workspace(free_list.numel())
-    ws = torch.zeros(nbytes // 4, dtype=torch.int32, device=device)
+    nbytes = lib.qa_paged_kv_compact_workspace(free_list.numel(), rows, max_blocks, max_moves)
+    ws = torch.zeros(nbytes // 4, dtype=torch.int32, device=device) if nbytes else None
     code = _launch(
         device, lib.qa_paged_kv_compact, block_tables.data_ptr(), block_tables.stride(0), max_blocks, rows, free_list.data_ptr(), free_list.numel(), free_state.data_ptr(),
-        references.data_ptr(), status.data_ptr(), max_moves, pages.data_ptr(), pages.data_ptr() + 4 * max_moves, ws.data_ptr(), nbytes,
+        references.data_ptr(), status.data_ptr(), max_moves, pages.data_ptr(), pages.data_ptr() + 4 * max_moves, _ptr(ws), nbytes,
     )
     L.check(lib, code, "paged_kv_compact")
-    return PagedCopy(pages[0], pages[1])
+    return PagedCopy(*pages.unbind())
 
 
 def paged_kv_copy(pools: Sequence[torch.Tensor], sources: torch.Tensor, targets: torch.Tensor) -> None:
@@ -1660,14 +1664,22 @@ def paged_kv_copy(pools: Sequence[torch.Tensor], sources: torch.Tensor, targets:
     _index_dtype(sources, "sources")
     _require(sources.dtype is targets.dtype and sources.dim() == 1 and sources.shape == targets.shape, "sources and targets must be vectors of page ids, alike")
     n = len(pools)
-    longs = ctypes.c_int64 * n
-    bases, strides, sizes, counts = (ctypes.c_void_p * n)(), longs(), longs(), longs()
-    for i, pool in enumerate(pools):
+    bases, strides, sizes, counts = [], [], [], []
+    for pool in pools:
         if pool.device != device:
             _require_cuda(pool, "pools", device)
-        _require(pool.dim() >= 2 and (pool.numel() == 0 or pool[0].is_contiguous()), "a pool's pages must be contiguous along its first axis")
-        each = pool.element_size()
-        bases[i], strides[i], sizes[i], counts[i] = pool.data_ptr(), pool.stride(0) * each, math.prod(pool.shape[1:]) * each, pool.shape[0]
+        shape, each = pool.shape, pool.element_size()
+        if pool.is_contiguous() and len(shape) > 1 and shape[0]:
+            size = stride = pool.numel() // shape[0] * each
+        else:
+            _require(len(shape) > 1 and (pool.numel() == 0 or pool[0].is_contiguous()), "a pool's pages must be contiguous along its first axis")
+            size, stride = math.prod(shape[1:]) * each, pool.stride(0) * each
+        bases.append(pool.data_ptr())
+        strides.append(stride)
+        sizes.append(size)
+        counts.append(shape[0])
+    longs = ctypes.c_int64 * n
+    bases, strides, sizes, counts = (ctypes.c_void_p * n)(*bases), longs(*strides), longs(*sizes), longs(*counts)
     s, t = sources.contiguous(), targets.contiguous()
     code = _launch(device, lib.qa_paged_kv_copy, bases, strides, sizes, counts, n, s.data_ptr(), t.data_ptr(), _code(s), s.numel())
     L.check(lib, code, "paged_kv_copy")

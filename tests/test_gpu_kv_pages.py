@@ -71,10 +71,11 @@ class Device:
 
 
 @pytest.mark.parametrize("block", [16, 64, 5])
-@pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
-def test_forks_releases_and_compactions_in_any_order(block, dtype) -> None:
+@pytest.mark.parametrize("dtype,width", [(torch.int32, 70), (torch.int64, 70), (torch.int32, 4200)])
+def test_forks_releases_and_compactions_in_any_order(block, dtype, width) -> None:
+    """Small books, which one workgroup keeps, and tables too wide for that."""
     rng = random.Random(block)
-    d = Device(block, [rng.randint(0, 300) for _ in range(12)], 40, 70, 1200, block)
+    d = Device(block, [rng.randint(0, 300) for _ in range(12)], 40, width, 1200, block)
     for step in range(30):
         live = [r for r in range(40) if d.host.rows[r] or d.host.lengths[r]]
         empty = [r for r in range(40) if d.host.lengths[r] == 0 and not d.host.rows[r]]
@@ -160,7 +161,7 @@ def test_compaction_leaves_blocks_of_others_where_they_are() -> None:
     assert d.compact(0).sources.shape == (0,)
 
 
-@pytest.mark.parametrize("capacity", [1, 31, 32, 33, 8192, 8193, 100_003])
+@pytest.mark.parametrize("capacity", [1, 31, 32, 33, 2047, 8193, 32_768, 32_769, 34_817, 100_003])
 def test_lists_of_any_length(capacity) -> None:
     """Words and workgroups that the list's end does not fill."""
     n = min(capacity, 70)

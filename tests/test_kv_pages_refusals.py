@@ -60,7 +60,8 @@ def test_fork_refuses(changes, message) -> None:
 
 @pytest.mark.parametrize("changes,message", BAD_BOOKS + [
     (dict(dtype=L.QA_F32), "int32 or int64"), (dict(n=-1), "rows a call"), (dict(n=65534), "rows a call"), (dict(lengths=P(0)), "non-null"), (dict(which=P(0)), "non-null"),
-    (dict(ws=P(0)), "workspace"), (dict(wsb=7), "workspace"), (dict(ws=P((1 << 20) + 2)), "workspace"),
+    (dict(capacity=40_000, ws=P(0)), "workspace"), (dict(capacity=40_000, wsb=5003), "workspace"), (dict(capacity=40_000, ws=P((1 << 20) + 2)), "workspace"),
+    (dict(width=9000, stride=9000, ws=P(0)), "workspace"),
 ])
 def test_release_refuses(changes, message) -> None:
     lib = _lib()
@@ -69,8 +70,9 @@ def test_release_refuses(changes, message) -> None:
 
 
 @pytest.mark.parametrize("changes,message", BAD_BOOKS + [
-    (dict(moves=-1), "max_moves"), (dict(moves=1 << 31), "max_moves"), (dict(sources=P(0)), "non-null"), (dict(targets=P(0)), "non-null"), (dict(ws=P(0)), "workspace"),
-    (dict(wsb=47), "workspace"),
+    (dict(moves=-1), "max_moves"), (dict(moves=1 << 31), "max_moves"), (dict(sources=P(0)), "non-null"), (dict(targets=P(0)), "non-null"),
+    (dict(capacity=40_000, ws=P(0)), "workspace"), (dict(capacity=40_000, wsb=175_003), "workspace"), (dict(width=9000, stride=9000, ws=P(0)), "workspace"),
+    (dict(moves=40_000, ws=P(0)), "workspace"),
 ])
 def test_compact_refuses(changes, message) -> None:
     lib = _lib()
