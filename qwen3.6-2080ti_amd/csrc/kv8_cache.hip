@@ -5,6 +5,8 @@
 // run that the call brings, so one wave holds them all in registers and reads them once, and no two waves write to one run.
 // Tokens of a run follow one another in the slot map, with none but skipped ones between them; the first of them leads, and the waves
 // look for leaders among `window` tokens each.
+// Four prompts of 6003 tokens, two heads of 256, 74 MB each way: append 15.2 us, gather 13.5; a token for each of seven rows 5.2, and
+// their dense view of 428 tokens 4.1.
 #include "kv8.h"
 
 namespace qa {
@@ -180,9 +182,6 @@ __device__ __forceinline__ void write_values(const AppendParams& p, const Bring&
   if (lane == 0) *reinterpret_cast<uint4*>(r.at + Run<D>::kCodes) = make_uint4(byte, 0, 0, 0);
 }
 
-// Tokens among which a wave looks for leaders: one where there are few, so that every run has a wave at once.
-constexpr int kWindow = 16;
-
 template <int D, bool F32, bool S64>
 __global__ __launch_bounds__(256) void append_kernel(AppendParams p) {
   const int lane = threadIdx.x & 63;
@@ -344,8 +343,10 @@ static void launch_gather(const GatherParams& p, bool t64, dim3 grid, hipStream_
     hipLaunchKernelGGL((gather_kernel<D, false>), grid, dim3(256), 0, stream, p);
 }
 
-// Tokens up to which every token has a wave for each head's keys and values, which returns unless it leads a run.
-constexpr int64_t kOneEach = 1024;
+// Tokens among which a wave looks for leaders: one where there are few, so that every run has a wave at once; more where waves
+// that lead nothing would be too many.  us with windows of 1, 4, 16, two heads of 256: 128 rows of a token 5.1 13.3 41.9, 512 rows 6.6
+// 13.2 42.4, 2000 rows 16.5 18.9 44.7; prompts of 500 tokens 4.5 4.3 4.8, of 1000 4.8 4.4 4.8, 4000 13.5 5.8 5.3, 24000 61 19.8 16.2.
+static int window_of(int64_t tokens) { return tokens <= 1024 ? 1 : tokens <= 4096 ? 4 : 16; }
 
 static int shift_of(int32_t block_size) { return __builtin_ctz(static_cast<unsigned>(block_size)); }
 
@@ -384,7 +385,7 @@ extern "C" int qa_paged_kv8_append(const void* key_new, const void* value_new, i
   p.tokens = tokens;
   p.Hkv = kv->kv_heads;
   p.bs_shift = shift_of(block_size);
-  p.window = tokens <= kOneEach ? 1 : kWindow;
+  p.window = window_of(tokens);
   const dim3 grid(static_cast<unsigned>(ceil_div(tokens, 4 * p.window)), 2u * kv->kv_heads);
   const bool s64 = slots_dtype == QA_I64;
   {

@@ -170,21 +170,46 @@ __global__ __launch_bounds__(256) void fork_tables_kernel(ForkParams p) {
 // ---- the free list from a bitmap ----------------------------------------------
 
 constexpr int kListThreads = 256;
-constexpr int kListWords = 64;  // of a workgroup where the bitmap lies in the workspace
+constexpr int kListWords = 64;  // of a workgroup where the bitmap lies in the workspace, at most
 
-// One workgroup does a release or a compaction where the pool has up to so many blocks (a word of the bitmap a thread) ..
-constexpr int kSmallThreads = 1024;
-constexpr int64_t kSmallBlocks = 32 * kSmallThreads;
-// .. and the rows so many table entries, and a compaction so many pairs.
+// One workgroup does a release or a compaction where the pool has up to so many blocks, the rows so many table entries, and a
+// compaction so many pairs.  us of a release and a compaction in one workgroup / in several: 8000 blocks 13 / 9 and 18 / 17, but a
+// fill and a launch more each, 8 us of the host; 470 blocks, a compaction 6 / 13; 32000 blocks 27 / 9 and 50 / 22.
+constexpr int kSmallThreads = 1024;  // each a word of the bitmap at most
+constexpr int64_t kSmallBlocks = 8192;
 constexpr int64_t kSmallEntries = 16384;
+static_assert(kSmallBlocks <= 32 * kSmallThreads, "a word a thread");
 
 __device__ __forceinline__ void set_bit(uint32_t* bits, int32_t id) { atomicOr(&bits[id >> 5], 1u << (id & 31)); }
 __device__ __forceinline__ uint32_t below(int32_t id) { return (1u << (id & 31)) - 1u; }
 
-// Marks the free list's blocks.
+// Marks the free list's blocks in the workspace's bitmap.  Neighbours in the list share words, so a wave gathers the bits of a word first; what is left after
+// a few words goes by itself: a release in a pool of 322,000 blocks 105 -> 29 us.
 __device__ __forceinline__ void mark_free(const Books& k, uint32_t* bits, int64_t first, int64_t step) {
   const int64_t head = k.free_state[0], count = k.free_state[1];
-  for (int64_t i = first; i < count; i += step) {
+  const int lane = threadIdx.x & 63;
+  for (int64_t i = first; i - lane < count; i += step) {
+    const int32_t id = i < count ? k.free_list[head + i] : -1;
+    bool left = id >= 0 && id < k.capacity;
+    for (int turn = 0; turn < 4; ++turn) {
+      const uint64_t some = __ballot(left);
+      if (some == 0) break;
+      const int leader = __ffsll(static_cast<unsigned long long>(some)) - 1;
+      const int32_t word = __builtin_amdgcn_readlane(id >> 5, leader);
+      const bool mine = left && id >> 5 == word;
+      uint32_t all = mine ? 1u << (id & 31) : 0u;
+#pragma unroll
+      for (int off = 1; off < 64; off <<= 1) all |= __shfl_xor(all, off, 64);
+      if (lane == leader) atomicOr(&bits[word], all);
+      left = left && !mine;
+    }
+    if (left) set_bit(bits, id);
+  }
+}
+
+__device__ __forceinline__ void mark_free_lds(const Books& k, uint32_t* bits, int tid) {
+  const int64_t head = k.free_state[0], count = k.free_state[1];
+  for (int64_t i = tid; i < count; i += kSmallThreads) {
     const int32_t id = k.free_list[head + i];
     if (id >= 0 && id < k.capacity) set_bit(bits, id);
   }
@@ -192,8 +217,8 @@ __device__ __forceinline__ void mark_free(const Books& k, uint32_t* bits, int64_
 
 // Where the bitmap lies in the workspace: the bits below each of this workgroup's words go to s_before, `total` is all of them.
 template <typename F>
-__device__ __forceinline__ void count_words(int64_t words, F word, int32_t* s_wave, int32_t* s_before, int32_t& total) {
-  const int64_t base = static_cast<int64_t>(blockIdx.x) * kListWords;
+__device__ __forceinline__ void count_words(int64_t words, int list_words, F word, int32_t* s_wave, int32_t* s_before, int32_t& total) {
+  const int64_t base = static_cast<int64_t>(blockIdx.x) * list_words;
   int32_t before = 0, all = 0;
   for (int64_t w = threadIdx.x; w < words; w += kListThreads) {
     const int32_t c = __popc(word(w));
@@ -203,9 +228,9 @@ __device__ __forceinline__ void count_words(int64_t words, F word, int32_t* s_wa
   int32_t sum, own;
   block_scan<kListThreads>(before, s_wave, sum);
   block_scan<kListThreads>(all, s_wave, total);
-  const int32_t mine = threadIdx.x < kListWords && base + threadIdx.x < words ? __popc(word(base + threadIdx.x)) : 0;
+  const int32_t mine = threadIdx.x < list_words && base + threadIdx.x < words ? __popc(word(base + threadIdx.x)) : 0;
   const int32_t incl = block_scan<kListThreads>(mine, s_wave, own);
-  if (threadIdx.x < kListWords) s_before[threadIdx.x] = sum + incl - mine;
+  if (threadIdx.x < list_words) s_before[threadIdx.x] = sum + incl - mine;
   __syncthreads();
 }
 
@@ -234,6 +259,7 @@ struct ReleaseParams {
   int n, rows_i64;
   uint32_t* bits;    // (words + 1), zeros: free blocks; the last word is 1 where the free list's cursor is out of range
   int64_t words;
+  int list_words;    // of a workgroup of the second launch
 };
 
 // Table entry e of a row loses its block.
@@ -259,7 +285,7 @@ __global__ __launch_bounds__(kSmallThreads) void release_small_kernel(ReleasePar
     return;
   }
   __syncthreads();
-  mark_free(k, s_bits, tid, kSmallThreads);
+  mark_free_lds(k, s_bits, tid);
   for (int i = tid / 64; i < p.n; i += kSmallThreads / 64) {  // a wave a row
     const int64_t row = index_of(p.release_rows, p.rows_i64, i);
     if (row < 0 || row >= k.rows) continue;
@@ -302,9 +328,9 @@ __global__ __launch_bounds__(kListThreads) void release_list_kernel(ReleaseParam
   }
   auto word = [&](int64_t w) { return p.bits[w]; };
   int32_t total;
-  count_words(p.words, word, s_wave, s_before, total);
-  const int64_t w0 = static_cast<int64_t>(blockIdx.x) * kListWords;
-  write_list(k, 32 * w0 + threadIdx.x, min64(k.capacity, 32 * (w0 + kListWords)), kListThreads, word, s_before, w0, total);
+  count_words(p.words, p.list_words, word, s_wave, s_before, total);
+  const int64_t w0 = static_cast<int64_t>(blockIdx.x) * p.list_words;
+  write_list(k, 32 * w0 + threadIdx.x, min64(k.capacity, 32 * (w0 + p.list_words)), kListThreads, word, s_before, w0, total);
   if (blockIdx.x == 0 && threadIdx.x == 0) close_books(k, total);
 }
 
@@ -320,7 +346,7 @@ struct CompactParams {
   int32_t* place;       // (capacity): where a block that is left has gone
   int32_t* sources;     // (max_moves)
   int32_t* targets;
-  int list_groups;
+  int list_words, list_groups;  // words of a workgroup that counts them, and workgroups
 };
 
 // Where a held block with `nth` held ones above it goes, -1: it stays.
@@ -352,7 +378,7 @@ __global__ __launch_bounds__(kSmallThreads) void compact_small_kernel(CompactPar
     return;
   }
   __syncthreads();
-  mark_free(k, s_free, tid, kSmallThreads);
+  mark_free_lds(k, s_free, tid);
   for (int64_t row = tid / 64; row < k.rows; row += kSmallThreads / 64)
     for (int64_t e = tid % 64; e < k.max_blocks; e += 64) {
       const int32_t id = k.tables[row * k.table_stride + e];
@@ -418,8 +444,8 @@ __global__ __launch_bounds__(kListThreads) void compact_moves_kernel(CompactPara
   if (p.refused[0] != 0) return;
   auto word = [&](int64_t w) { return p.held[w] & ~p.free_bits[w]; };
   int32_t total;
-  count_words(p.words, word, s_wave, s_before, total);
-  const int64_t w0 = static_cast<int64_t>(blockIdx.x) * kListWords, end = min64(k.capacity, 32 * (w0 + kListWords));
+  count_words(p.words, p.list_words, word, s_wave, s_before, total);
+  const int64_t w0 = static_cast<int64_t>(blockIdx.x) * p.list_words, end = min64(k.capacity, 32 * (w0 + p.list_words));
   for (int64_t i = 32 * w0 + threadIdx.x; i < end; i += kListThreads) {
     const int32_t id = static_cast<int32_t>(i);
     const uint32_t bits = word(id >> 5);
@@ -443,9 +469,9 @@ __global__ __launch_bounds__(kListThreads) void compact_list_kernel(CompactParam
     if (static_cast<int>(blockIdx.x) >= p.list_groups) return;
     auto word = [&](int64_t w) { return p.free_bits[w] ^ p.flip[w]; };
     int32_t total;
-    count_words(p.words, word, s_wave, s_before, total);
-    const int64_t w0 = static_cast<int64_t>(blockIdx.x) * kListWords;
-    write_list(k, 32 * w0 + threadIdx.x, min64(k.capacity, 32 * (w0 + kListWords)), kListThreads, word, s_before, w0, total);
+    count_words(p.words, p.list_words, word, s_wave, s_before, total);
+    const int64_t w0 = static_cast<int64_t>(blockIdx.x) * p.list_words;
+    write_list(k, 32 * w0 + threadIdx.x, min64(k.capacity, 32 * (w0 + p.list_words)), kListThreads, word, s_before, w0, total);
     if (blockIdx.x == 0 && threadIdx.x == 0) close_books(k, total);
     return;
   }
@@ -514,8 +540,12 @@ static int check_books(const char* what, const Books& k) {
   return 0;
 }
 
+// Words of a workgroup that counts them: few, so that its threads have a block or two each, but no more workgroups than 256,
+// since each reads all words.
+static int list_words_of(int64_t words) { return static_cast<int>(std::min<int64_t>(kListWords, std::max<int64_t>(16, ceil_div(words, 256)))); }
+
 // Workgroups along an axis of `n` entries: enough for a few entries a thread.
-static unsigned groups_of(int64_t n) { return static_cast<unsigned>(std::min<int64_t>(std::max<int64_t>(ceil_div(n, 256), 1), 64)); }
+static unsigned groups_of(int64_t n) { return static_cast<unsigned>(std::min<int64_t>(std::max<int64_t>(ceil_div(n, 256), 1), 256)); }
 
 }  // namespace pages
 }  // namespace qa
@@ -576,6 +606,7 @@ extern "C" int qa_paged_kv_release(int32_t* block_tables, int64_t table_stride, 
   p.rows_i64 = rows_dtype == QA_I64;
   p.bits = reinterpret_cast<uint32_t*>(workspace);
   p.words = words_of(free_capacity);
+  p.list_words = list_words_of(p.words);
   if (need == 0) {
     {
       KernelTimer timer_("kv_release", stream);
@@ -590,7 +621,7 @@ extern "C" int qa_paged_kv_release(int32_t* block_tables, int64_t table_stride, 
   if (int rc = check_launch("paged_kv_release")) return rc;
   {
     KernelTimer timer_("kv_release_list", stream);
-    hipLaunchKernelGGL(release_list_kernel, dim3(static_cast<unsigned>(ceil_div(p.words, kListWords))), dim3(kListThreads), 0, stream, p);
+    hipLaunchKernelGGL(release_list_kernel, dim3(static_cast<unsigned>(ceil_div(p.words, p.list_words))), dim3(kListThreads), 0, stream, p);
   }
   return check_launch("paged_kv_release");
 }
@@ -629,7 +660,8 @@ extern "C" int qa_paged_kv_compact(int32_t* block_tables, int64_t table_stride, 
   p.flip = p.held + p.words;
   p.refused = p.flip + p.words;
   p.place = reinterpret_cast<int32_t*>(p.refused + 1);
-  const unsigned lists = static_cast<unsigned>(ceil_div(p.words, kListWords));
+  p.list_words = list_words_of(p.words);
+  const unsigned lists = static_cast<unsigned>(ceil_div(p.words, p.list_words));
   p.list_groups = static_cast<int>(lists);
   {
     KernelTimer timer_("kv_compact_mark", stream);
