@@ -32,6 +32,9 @@ namespace prefill4 {
 
 using namespace attn4;
 
+constexpr int kWaves = 8;
+constexpr int kCols = kWaves * 16;
+
 template <int D>
 struct Smem {
   static constexpr int kTileBytes = kTile * D * 2;
@@ -573,7 +576,7 @@ static int launch(const PrefillParams& p, dim3 grid, hipStream_t stream) {
     hipLaunchKernelGGL(prefill_kernel<D>, grid, dim3(64 * kWaves), Smem<D>::kBytes, stream, p);
   }
   if (int rc = check_launch("paged_attention_prefill_kv4")) return rc;
-  return join<D>(p, "paged_attention_prefill_kv4", "prefill_kv4_join", stream);
+  return join<D, kCols>(p, "paged_attention_prefill_kv4", "prefill_kv4_join", stream);
 }
 
 }  // namespace prefill4
@@ -581,7 +584,7 @@ static int launch(const PrefillParams& p, dim3 grid, hipStream_t stream) {
 
 extern "C" int64_t qa_paged_attention_prefill_kv4_workspace(int64_t total_new, int64_t batch, int64_t max_new, int32_t heads, int32_t kv_heads, int32_t head_dim,
                                                             int64_t max_tokens) {
-  return qa::attn::workspace_bytes_of(total_new, batch, max_new, heads, kv_heads, head_dim, max_tokens);
+  return qa::attn::workspace_bytes_of(total_new, batch, max_new, heads, kv_heads, head_dim, max_tokens, qa::prefill4::kCols);
 }
 
 extern "C" int qa_paged_attention_prefill_kv4(const void* query, int32_t q_dtype, int64_t q_stride_t, int64_t q_stride_h, int64_t total_new, const void* cu_seqlens,
@@ -595,7 +598,7 @@ extern "C" int qa_paged_attention_prefill_kv4(const void* query, int32_t q_dtype
   const Args a{"paged_attention_prefill_kv4", query, q_dtype, q_stride_t, q_stride_h, total_new, batch, heads, head_dim, kv, block_tables, table_dtype, table_stride, max_blocks,
                idx_dtype, block_size, scale, gate, gate_stride_t, gate_stride_h, output};
   if (int rc = fill(p.c, a)) return rc;
-  if (int rc = share_out(p, a, cu_seqlens, prefix_lens, max_new, workspace, workspace_bytes)) return rc;
+  if (int rc = share_out(p, a, cu_seqlens, prefix_lens, max_new, workspace, workspace_bytes, kCols)) return rc;
   if (p.max_new == 0) return 0;
   const dim3 grid(static_cast<unsigned>(ceil_div(p.max_new * p.c.G, kCols)), static_cast<unsigned>(batch * kv->kv_heads), static_cast<unsigned>(p.splits));
   return head_dim == 256 ? launch<256>(p, grid, stream) : launch<128>(p, grid, stream);

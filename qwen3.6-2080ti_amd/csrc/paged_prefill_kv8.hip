@@ -1,17 +1,30 @@
 // Chunked causal prefill attention over the 8-bit paged KV cache (attention_kv8.h, kv8.h), gfx950.
 //
 // Columns of the products are (new position, query head of the KV head's group), position-major, so any group size
-// fills them.  A workgroup owns 128 of one row and KV head and walks the keys in tiles of 64.  Its eight waves are four
+// fills them.  A workgroup owns 128 or 64 of one row and KV head (columns_of) and walks the keys in tiles of 64.  Its waves are
 // pairs of 32 columns: a wave takes the scores and the softmax of half of the tile's keys, then the products with the values of
 // all of them for half of the dims, its partner's probabilities through LDS.  So a key read from LDS feeds 32 columns and is
-// converted by four waves, and the accumulators of a wave stay at 64 registers, two waves to a SIMD.
+// converted once a pair, and the accumulators of a wave stay at 64 registers, two waves to a SIMD.
 //
-// Codes go from memory to LDS as they are, a run a wave, and to bf16 next to the products.
+// Codes go from memory to LDS as they are, a run a wave, and to bf16 next to the products: exact, where
+// products of 8 bits would round the query and the probabilities to 4.  Keys converted into LDS, once a workgroup, cost more
+// there than they save (1048 -> 1090 us at the longest size below).
 //
-// Iteration i, one barrier: the scores of tile i + 1 and the largest of each column, the probabilities of tile i, for which the
-// pair shares its columns' reference points, and the products of tile i - 1's values.
+// 128 columns, eight waves, one barrier an iteration: the probabilities of tile i, for which the pair shares its columns'
+// reference points, between the products of tile i - 1's values, then the scores of tile i + 1.  64 columns, four waves, keys
+// and values in one buffer each, so that two workgroups fill a CU and work while the other waits: a barrier after the
+// products with values and one after the scores.
 //
 // With few columns the keys are split over gridDim.z and a second launch joins the parts.
+//
+// What bounds it: issue.  A tile of 64 keys, D = 256, is 32 matrix instructions of 32 cycles a wave, two waves a SIMD, and
+// beside them 128 conversions, 16 exponentials and their shares of loads, masks and sums; a matrix instruction lets the other
+// wave's vector ones by half of its time, which would take 2984 cycles a tile, and it takes 4050 (matrix units busy 49 %).
+// Measured, 16 heads, 2 of keys, D = 256: 2048 new behind 32 000 1046 us (1108 Gflop, 1060 Tflop/s; a library's 8192 x 8192
+// x 8192 product 1268), 8 x 512 behind up to 8192 331 us (930 Tflop/s); 20 heads, 4 of keys, D = 128, five prompts of up to 700 25 us.
+// Values' products at a raised wave priority 1048 -> 1034, probabilities between them 1221 -> 1055.  Not kept: the two halves of
+// the workgroup half a tile apart 1040, two accumulators of scores 1049, three key buffers 1065, four waves of 64 columns with
+// 512 registers 1187, workgroups of 64 columns at that size 1130.
 #include "attention_kv8.h"
 #include "prefill_split.h"
 
@@ -24,30 +37,34 @@ using namespace attn8;
 
 typedef float floatx16_v __attribute__((ext_vector_type(16)));
 
-constexpr int kKeyBufs = 2, kValueBufs = 4;
-
-template <int D>
+template <int D, int COLS>
 struct Smem {
+  static constexpr int kWaves = COLS / 16;
+  static constexpr int kKeyBufs = COLS == 128 ? 2 : 1;
+  static constexpr int kValueBufs = COLS == 128 ? 4 : 1;
+  static constexpr int kPBufs = COLS == 128 ? 2 : 1;
   static constexpr int kRunBytes = kv8::Run<D>::kCodes;
   static constexpr int kTileBytes = kRuns * kRunBytes;
   static constexpr int kValues = kKeyBufs * kTileBytes;               // after the keys: [buffer][run]
   static constexpr int kP = kValues + kValueBufs * kTileBytes;        // probabilities: [buffer][wave][run][lane][16 bytes]
-  static constexpr int kMax = kP + 2 * kWaves * 2 * 1024;             // [buffer][wave][32] floats
-  static constexpr int kScale = kMax + 2 * kWaves * 32 * 4;           // of keys [buffer][run], of values [buffer][run]
+  static constexpr int kMax = kP + kPBufs * kWaves * 2 * 1024;        // [buffer][wave][32] floats; at the end sums and reference points
+  static constexpr int kScale = kMax + std::max(kPBufs * kWaves * 32, 3 * COLS) * 4;  // of keys [buffer][run], of values [buffer][run]
   static constexpr int kFlag = kScale + (kKeyBufs + kValueBufs) * kRuns * 4;  // whether a tile that not every column sees whole had a NaN
   static constexpr int kBytes = kFlag + 16;
 };
 
-template <int D>
-__global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams pp) {
+template <int D, int COLS>
+__global__ __launch_bounds__(4 * COLS, 2) void prefill_kernel(PrefillParams pp) {
   const Params& p = pp.c;
   constexpr int N = kv8::Run<D>::kSlices;
   constexpr int MT = D / 64;        // tiles of 32 dims of a wave
-  using S = Smem<D>;
+  constexpr bool kWide = COLS == 128;
+  using S = Smem<D, COLS>;
+  constexpr int kWaves = S::kWaves;
   extern __shared__ __align__(16) unsigned char smem[];
   float* s_max = reinterpret_cast<float*>(smem + S::kMax);
   float* s_kscale = reinterpret_cast<float*>(smem + S::kScale);
-  float* s_vscale = s_kscale + 2 * kRuns;
+  float* s_vscale = s_kscale + S::kKeyBufs * kRuns;
   int* s_flag = reinterpret_cast<int*>(smem + S::kFlag);
   const int tid = threadIdx.x;
   const int lane = tid & 63;
@@ -94,9 +111,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams p
   }
   const int64_t n_new = min64(pp.max_new, min64(tok1, p.total) - tok0);
   const int64_t ct0 = static_cast<int64_t>(gridDim.x) - 1 - blockIdx.x;
-  const int64_t x0 = ct0 * kCols;  // first column of the workgroup
+  const int64_t x0 = ct0 * COLS;  // first column of the workgroup
   if (tok0 < 0 || x0 >= n_new * p.G) return;
-  const int64_t last = min64(n_new * p.G, x0 + kCols) - 1;  // columns fit 31 bits
+  const int64_t last = min64(n_new * p.G, x0 + COLS) - 1;  // columns fit 31 bits
   const int64_t kv_end = keys_of(p, prefix, last);          // keys that any column sees
   const int64_t first_new = over_group(p, static_cast<uint32_t>(x0));
   const int64_t first_pos = prefix + first_new;  // every column sees the keys up to here
@@ -149,10 +166,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams p
     const int64_t o = static_cast<int64_t>(ok ? lo : 0) * q->c.sP + (run & ((1 << (q->c.bs_shift - 4)) - 1)) * kv8::Run<D>::kBytes;
     return ok ? o : -1;
   };
-  // A wave loads run wave % 4 of a tile, waves 0 to 3 of its keys, 4 to 7 of its values.  One that is not there has no records
-  // and reads zeros.
-  const bool of_values = wave >= 4;
-  const uint8_t* own_pool = of_values ? vb : kb;
+  // A wave loads run wave % 4 of a tile: of eight, 0 to 3 its keys and 4 to 7 its values; of four, its keys and then its values.
+  // One that is not there has no records and reads zeros.
+  const bool of_values = kWide && wave >= 4;
   int64_t own;  // offset of that run of the tile last asked for, -1: not there
   int there;    // which runs of that tile are there
   auto offsets = [&](int64_t kt) {
@@ -170,9 +186,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams p
   };
   uint4 stage[N];
   uint32_t stage_scale;
-  auto ask = [&](int64_t kt) {
-    offsets(kt);
-    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(own_pool + (own < 0 ? 0 : own)), 0, own < 0 ? 0 : kv8::Run<D>::kBytes, 0x00020000);
+  auto ask = [&](const uint8_t* pool, int64_t at) {
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(pool + (at < 0 ? 0 : at)), 0, at < 0 ? 0 : kv8::Run<D>::kBytes, 0x00020000);
 #pragma unroll
     for (int s = 0; s < N; ++s) stage[s] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, 16 * lane + 1024 * s, 0, kShared));
     stage_scale = __builtin_amdgcn_raw_buffer_load_b8(r, kv8::Run<D>::kCodes, 0, kShared);
@@ -200,14 +215,13 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams p
     }
     if (any != 0) *s_flag = 1;
   };
-  auto put = [&](int64_t kt) {
-    const int i = static_cast<int>(kt - kt0);
-    const int buf = of_values ? i & (kValueBufs - 1) : i & (kKeyBufs - 1);
-    if (of_values) trim(kt);
-    uint4* dst = reinterpret_cast<uint4*>(smem + (of_values ? S::kValues : 0) + (buf * kRuns + (wave & 3)) * S::kRunBytes) + lane;
+  auto put = [&](bool values, int i) {
+    const int buf = values ? i & (S::kValueBufs - 1) : i & (S::kKeyBufs - 1);
+    if (values) trim(kt0 + i);
+    uint4* dst = reinterpret_cast<uint4*>(smem + (values ? S::kValues : 0) + (buf * kRuns + (wave & 3)) * S::kRunBytes) + lane;
 #pragma unroll
     for (int s = 0; s < N; ++s) dst[64 * s] = stage[s];
-    if (lane == 0) (of_values ? s_vscale : s_kscale)[buf * kRuns + (wave & 3)] = kv8::scale_of(stage_scale);
+    if (lane == 0) (values ? s_vscale : s_kscale)[buf * kRuns + (wave & 3)] = kv8::scale_of(stage_scale);
   };
 
   float m_run = -INFINITY, l_run = 0.f, corr = 1.f;  // of the lane's column; corr: what the sums are still to be multiplied with
@@ -215,14 +229,13 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams p
 #pragma unroll
   for (int m = 0; m < MT; ++m) o[m] = floatx16_v(0.f);
 
-  // The output leaves through LDS as whole rows, a lane eight dims: the first two pairs' columns, then the
-  // others'
+  // The output leaves through LDS as whole rows, a lane eight dims: the first half of the columns, then the other
   constexpr int kLanes = D / 8;  // of a row
   constexpr int kRowsAtOnce = 64 * kWaves / kLanes;
-  constexpr int kSweeps = kCols / 2 / kRowsAtOnce;
+  constexpr int kSweeps = COLS / 2 / kRowsAtOnce;
   const int in_row = tid % kLanes;
   auto column_of = [&](int pass, int i) {
-    return kCols / 2 * pass + tid / kLanes + i * kRowsAtOnce;
+    return COLS / 2 * pass + tid / kLanes + i * kRowsAtOnce;
   };
   uint4 gate[2][kSweeps];
   auto ask_gate = [&](ParamsAgain late) {
@@ -261,10 +274,14 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams p
     nxt_mask = __ballot(nxt >= 0);
     const float qk_scale = p.scale * kLog2e;
     const int n = static_cast<int>(kt1 - kt0);
-    ask(kt0);
+    offsets(kt0);
+    const uint8_t* own_pool = of_values ? vb : kb;
+    ask(own_pool, own);
+    int64_t own_keys = own;    // of the tile asked for last, its keys'
+    int64_t own_values = own;  // of the tile before it, its values'
     int there_next = there;
     lds_barrier();  // the flag
-    put(kt0);
+    put(of_values, 0);
     lds_barrier();  // the first tile
     float top = 0.f;  // the largest score of the lane's column in this wave's half of the tile whose probabilities come next
     const unsigned char* key_lane = smem + 2 * (wave & 1) * S::kRunBytes + (col >> 4) * S::kRunBytes + hi * 256 + (col & 15) * 16;
@@ -272,7 +289,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams p
     // and 3 are the second half; D = 128: m 2 and 3 are)
     constexpr int kHalf = D == 256 ? 2 * 1024 : 8;
     const unsigned char* value_lane = smem + S::kValues + (wave & 1) * kHalf + (col >> 4) * 1024 + hi * 256 + (col & 15) * 16;
-    const uint4* p_own = reinterpret_cast<const uint4*>(smem + S::kP) + wave * 128 + lane;
+    uint4* p_own = reinterpret_cast<uint4*>(smem + S::kP) + wave * 128 + lane;
     // masks the scores of tile i and tells the pair their largest
     auto largest = [&](int i, int have, floatx16_v& x) {
       const int64_t key0 = (kt0 + i) * kTile;
@@ -288,16 +305,19 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams p
       for (int r = 2; r < 16; ++r) mx = fmaxf(mx, x[r]);
       const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
       top = fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
-      if (hi == 0) s_max[((i & 1) * kWaves + wave) * 32 + col] = top;
+      if (hi == 0) s_max[((i & (S::kPBufs - 1)) * kWaves + wave) * 32 + col] = top;
     };
     // Iteration i: the probabilities of tile i between the products of tile i - 1's values, then the scores of tile i + 1.
     constexpr int kValues = 4 * MT;  // products of a tile's values
     floatx16_v sc;
     auto iterate = [&](int i, auto has_scores, auto has_probs, auto has_values) {
-      if constexpr (has_scores) ask(kt0 + i + 2);
-      const unsigned char* vat = value_lane + ((i - 1) & (kValueBufs - 1)) * S::kTileBytes;
-      const float* vsc = s_vscale + ((i - 1) & (kValueBufs - 1)) * kRuns;
-      const uint4* pat = p_own + ((i - 1) & 1) * kWaves * 128 - (wave & 1) * 128;  // runs 0 and 1 are the first wave's of the pair
+      if constexpr (kWide && has_scores) {
+        offsets(kt0 + i + 2);
+        ask(own_pool, own);
+      }
+      const unsigned char* vat = value_lane + ((i - 1) & (S::kValueBufs - 1)) * S::kTileBytes;
+      const float* vsc = s_vscale + ((i - 1) & (S::kValueBufs - 1)) * kRuns;
+      const uint4* pat = p_own + ((i - 1) & (S::kPBufs - 1)) * kWaves * 128 - (wave & 1) * 128;  // runs 0 and 1 are the first wave's of the pair
       uint32_t vlo[2][MT], vup[2][MT];
       float vscale[2];
       bf16x8_v pv[2];
@@ -324,7 +344,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams p
       // ---- the reference points of tile i: both waves of a pair move their columns' alike
       float use = 0.f;
       if constexpr (has_probs) {
-        const float mx = fmaxf(top, s_max[((i & 1) * kWaves + (wave ^ 1)) * 32 + col]) * qk_scale;
+        const float mx = fmaxf(top, s_max[((i & (S::kPBufs - 1)) * kWaves + (wave ^ 1)) * 32 + col]) * qk_scale;
         corr = 1.f;
         if (__ballot(mx > m_run + kLazy) != 0) {
           const float m_new = fmaxf(m_run, mx);
@@ -337,7 +357,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams p
       // a wave in its value products goes ahead of its neighbour on the SIMD that is at its scores: 1034 us against 1048 without
       // priorities and 1052 the other way round, 2048 tokens behind 32000
       __builtin_amdgcn_s_setprio(1);
-      bf16x8_v pb;
+      bf16x8_v pb[2];
 #pragma unroll
       for (int f = 0; f < kValues; ++f) {
         if constexpr (has_values) {
@@ -350,14 +370,21 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams p
           for (int r = f * (16 / kValues); r < (f + 1) * (16 / kValues); ++r) {
             const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r], qk_scale, -use));
             l_run += pr;
-            pb[r & 7] = static_cast<__bf16>(pr);  // for the bf16 product; l_run has it unrounded
-            if ((r & 7) == 7) const_cast<uint4*>(p_own)[(i & 1) * kWaves * 128 + 64 * (r >> 3)] = __builtin_bit_cast(uint4, pb);
+            pb[r >> 3][r & 7] = static_cast<__bf16>(pr);  // for the bf16 product; l_run has it unrounded
+            if (kWide && (r & 7) == 7) p_own[(i & (S::kPBufs - 1)) * kWaves * 128 + 64 * (r >> 3)] = __builtin_bit_cast(uint4, pb[r >> 3]);
           }
         }
         __builtin_amdgcn_sched_barrier(0);
       }
+      if constexpr (!kWide && has_probs) {
+        if constexpr (has_scores) put(false, i + 1);
+        ask(vb, own_values);
+        lds_barrier();
+#pragma unroll
+        for (int r = 0; r < 2; ++r) p_own[64 * r] = __builtin_bit_cast(uint4, pb[r]);
+      }
       if constexpr (has_scores) {
-        const int kbuf = (i + 1) & (kKeyBufs - 1);
+        const int kbuf = (i + 1) & (S::kKeyBufs - 1);
         const unsigned char* kat = key_lane + kbuf * S::kTileBytes;
         const float kscale = s_kscale[kbuf * kRuns + 2 * (wave & 1) + (col >> 4)];
         uint4 kc[3];
@@ -373,9 +400,22 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams p
           sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(operand(u.z, u.w, kscale, kscale), q[2 * f + 1], sc, 0, 0, 0);
           __builtin_amdgcn_sched_barrier(0);
         }
+      }
+      if constexpr (!kWide && has_probs) {
+        put(true, i);
+      }
+      if constexpr (has_scores) {
         largest(i + 1, there_next, sc);
+        if constexpr (!kWide) {
+          own_values = own_keys;
+          offsets(kt0 + i + 2);
+          own_keys = own;
+          ask(kb, own);
+        }
         there_next = there;
-        put(kt0 + i + 2);
+        if constexpr (kWide) {
+          put(of_values, i + 2);
+        }
       }
       if constexpr (has_probs || has_scores) lds_barrier();
     };
@@ -444,19 +484,19 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams p
   float* s_l = s_max;  // [half][column]; then the reference points
   const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(l_run), __float_as_uint(l_run), false, false);
   if (hi == 0) {
-    s_l[(wave & 1) * kCols + 32 * pair + col] = __uint_as_float(both[0]) + __uint_as_float(both[1]);
-    s_l[2 * kCols + 32 * pair + col] = m_run;  // of either wave, the same
+    s_l[(wave & 1) * COLS + 32 * pair + col] = __uint_as_float(both[0]) + __uint_as_float(both[1]);
+    s_l[2 * COLS + 32 * pair + col] = m_run;  // of either wave, the same
   }
   constexpr int kRowFloats = D + 4;
-  static_assert(kCols / 2 * kRowFloats * 4 <= S::kP && 3 * kCols <= 2 * kWaves * 32, "half of the columns fit below the sums");
+  static_assert(COLS / 2 * kRowFloats * 4 <= S::kMax, "half of the columns fit below the sums");
   float* s_o = reinterpret_cast<float*>(smem);
 #pragma unroll
   for (int pass = 0; pass < 2; ++pass) {
     if (pass == 1) lds_barrier();  // the first columns have been read
-    if (pair >> 1 == pass) {
+    if (pair / (COLS / 64) == pass) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        float* row = s_o + (32 * (pair & 1) + col) * kRowFloats + 64 * (r >> 3) + 4 * (8 * (r >> 2 & 1) + 4 * hi + (r & 3));
+        float* row = s_o + (32 * (pair % (COLS / 64)) + col) * kRowFloats + 64 * (r >> 3) + 4 * (8 * (r >> 2 & 1) + 4 * hi + (r & 3));
         if constexpr (D == 256)
           *reinterpret_cast<floatx4_v*>(row + 128 * (wave & 1)) = floatx4_v{o[0][r], o[1][r], o[2][r], o[3][r]};
         else
@@ -471,10 +511,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams p
       const float* at = s_o + (tid / kLanes + i * kRowsAtOnce) * kRowFloats;
       const Place pl = place_of(late->c, x);
       const uint32_t row = pl.token * static_cast<uint32_t>(late->c.H) + pl.head;  // past row0
-      const float l = s_l[x] + s_l[kCols + x];
+      const float l = s_l[x] + s_l[COLS + x];
       if (parts > 1) {
         const int64_t part = (blockIdx.z * late->part_tokens + part_base(*late, b, tok0) - tok0) * late->c.H + row0 + row;
-        if (in_row == 0) *reinterpret_cast<float2*>(late->part_ml + part * 2) = make_float2(s_l[2 * kCols + x], l);
+        if (in_row == 0) *reinterpret_cast<float2*>(late->part_ml + part * 2) = make_float2(s_l[2 * COLS + x], l);
 #pragma unroll
         for (int k = 0; k < 2; ++k)
           *reinterpret_cast<floatx4_v*>(late->part_o + part * D + 4 * in_row + k * D / 2) = *reinterpret_cast<const floatx4_v*>(at + 4 * in_row + k * D / 2);
@@ -498,15 +538,26 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(PrefillParams p
   }
 }
 
-template <int D>
-static int launch(const PrefillParams& p, dim3 grid, hipStream_t stream) {
-  if (int rc = reserve_lds<&prefill_kernel<D>>("paged_attention_prefill_kv8", Smem<D>::kBytes)) return rc;
+template <int D, int COLS>
+static int launch(const PrefillParams& p, hipStream_t stream) {
+  using S = Smem<D, COLS>;
+  if (int rc = reserve_lds<&prefill_kernel<D, COLS>>("paged_attention_prefill_kv8", S::kBytes)) return rc;
   {
     KernelTimer timer_("prefill_kv8", stream);
-    hipLaunchKernelGGL(prefill_kernel<D>, grid, dim3(64 * kWaves), Smem<D>::kBytes, stream, p);
+    const dim3 grid(static_cast<unsigned>(ceil_div(p.max_new * p.c.G, COLS)), static_cast<unsigned>(p.c.B * p.c.Hkv), static_cast<unsigned>(p.splits));
+    hipLaunchKernelGGL((prefill_kernel<D, COLS>), grid, dim3(64 * S::kWaves), S::kBytes, stream, p);
   }
   if (int rc = check_launch("paged_attention_prefill_kv8")) return rc;
-  return join<D>(p, "paged_attention_prefill_kv8", "prefill_kv8_join", stream);
+  return join<D, COLS>(p, "paged_attention_prefill_kv8", "prefill_kv8_join", stream);
+}
+
+// Columns of a workgroup.  64, two workgroups a CU, end sooner where the keys are few, and start sooner; 128 read each key half as
+// often.  us with 64 / 128, D = 256, 16 heads, rows x new tokens behind cached ones: 1 x 64 behind none 12.4 / 17.0, 1 x 512 23.2 /
+// 29.1, 8 x 512 46.5 / 52.3, 2 x 256 behind 500 33.7 / 36.6, 64 x 8 behind 1000 35.8 / 43.3, 1 x 512 behind 2000 49.3 / 48.0 and behind
+// 8000 96.2 / 91.6, 16 x 128 behind 500 38.6 / 37.7 and behind 4000 158 / 147, 1 x 4096 behind 4096 433 / 405.  D = 128, 20 heads, 4 of
+// keys: 1 x 512 17.2 / 20.6, 16 x 128 behind 4000 175 / 181, 1 x 4096 behind 4096 393 / 393, 1 x 512 behind 8000 80.3 / 77.3.
+static int columns_of(int64_t batch, int kv_heads, int group, int64_t max_new, int head_dim, int64_t max_tokens) {
+  return head_dim == 128 || max_tokens <= 1024 || workgroups_of(batch, kv_heads, group, max_new, 128) <= 64 ? 64 : 128;
 }
 
 }  // namespace prefill8
@@ -514,7 +565,9 @@ static int launch(const PrefillParams& p, dim3 grid, hipStream_t stream) {
 
 extern "C" int64_t qa_paged_attention_prefill_kv8_workspace(int64_t total_new, int64_t batch, int64_t max_new, int32_t heads, int32_t kv_heads, int32_t head_dim,
                                                             int64_t max_tokens) {
-  return qa::attn::workspace_bytes_of(total_new, batch, max_new, heads, kv_heads, head_dim, max_tokens);
+  // of either number of columns, so that tables narrower than these need no more
+  return std::max(qa::attn::workspace_bytes_of(total_new, batch, max_new, heads, kv_heads, head_dim, max_tokens, 64),
+                  qa::attn::workspace_bytes_of(total_new, batch, max_new, heads, kv_heads, head_dim, max_tokens, 128));
 }
 
 extern "C" int qa_paged_attention_prefill_kv8(const void* query, int32_t q_dtype, int64_t q_stride_t, int64_t q_stride_h, int64_t total_new, const void* cu_seqlens,
@@ -528,8 +581,9 @@ extern "C" int qa_paged_attention_prefill_kv8(const void* query, int32_t q_dtype
   const Args a{"paged_attention_prefill_kv8", query, q_dtype, q_stride_t, q_stride_h, total_new, batch, heads, head_dim, kv, block_tables, table_dtype, table_stride, max_blocks,
                idx_dtype, block_size, scale, gate, gate_stride_t, gate_stride_h, output};
   if (int rc = fill(p.c, a)) return rc;
-  if (int rc = share_out(p, a, cu_seqlens, prefix_lens, max_new, workspace, workspace_bytes)) return rc;
+  const int cols = columns_of(batch, p.c.Hkv, p.c.G, std::min(max_new, total_new), head_dim, max_blocks * block_size);
+  if (int rc = share_out(p, a, cu_seqlens, prefix_lens, max_new, workspace, workspace_bytes, cols)) return rc;
   if (p.max_new == 0) return 0;
-  const dim3 grid(static_cast<unsigned>(ceil_div(p.max_new * p.c.G, kCols)), static_cast<unsigned>(batch * kv->kv_heads), static_cast<unsigned>(p.splits));
-  return head_dim == 256 ? launch<256>(p, grid, stream) : launch<128>(p, grid, stream);
+  if (head_dim == 128) return launch<128, 64>(p, stream);
+  return cols == 64 ? launch<256, 64>(p, stream) : launch<256, 128>(p, stream);
 }

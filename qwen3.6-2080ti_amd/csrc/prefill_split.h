@@ -1,4 +1,4 @@
-// The split of a prefill over a paged cache in runs of 16 tokens, whatever a run holds: workgroups of 128 columns and tiles of
+// The split of a prefill over a paged cache in runs of 16 tokens, whatever a run holds: workgroups of COLS columns and tiles of
 // 64 keys, the keys split over gridDim.z where the columns are few, and the launch that joins the parts.  One copy of it for
 // each kernel that uses it.
 #pragma once
@@ -25,8 +25,6 @@ struct PrefillParams {
 
 constexpr int kTile = 64;      // keys
 constexpr int kRuns = kTile / 16;
-constexpr int kWaves = 8;
-constexpr int kCols = kWaves * 16;
 constexpr int kMaxSplits = 64;
 // Batches up to this many rows start with the longest row, so that the launch ends on short ones: 60 rows of up to 300 new
 // tokens behind up to 4000 439 -> 403 us, 12 of up to 1500 behind up to 8000 738 -> 677; 64 equal rows of 16 64.5 -> 65.8.
@@ -61,7 +59,7 @@ __device__ __forceinline__ ParamsAgain params_again() {
 constexpr int kJoinAhead = 8;  // parts asked for at a time
 
 // Joins the parts of one (token, head): a wave each, lane l dims l D/64 ..
-template <int D>
+template <int D, int COLS>
 __global__ __launch_bounds__(256) void join_kernel(PrefillParams pp) {
   const Params& p = pp.c;
   constexpr int E = D / 64;
@@ -75,7 +73,7 @@ __global__ __launch_bounds__(256) void join_kernel(PrefillParams pp) {
   const uint32_t n = static_cast<uint32_t>(x) / static_cast<uint32_t>(p.H), h = static_cast<uint32_t>(x) - n * static_cast<uint32_t>(p.H);
   // the workgroups that had this column
   const int64_t column = static_cast<int64_t>(n) * p.G + (h - over_group(p, h) * static_cast<uint32_t>(p.G));
-  const int64_t last = min64(n_new * p.G, column / kCols * kCols + kCols) - 1;
+  const int64_t last = min64(n_new * p.G, column / COLS * COLS + COLS) - 1;
   const int parts = parts_of(pp, (keys_of(p, read_index(p.prefix, p.idx_i64, b), last) + kTile - 1) / kTile);
   if (parts == 1) return;  // written by the workgroup itself
   const int64_t row = part_base(pp, b, tok0) * p.H + x;
@@ -116,39 +114,43 @@ __global__ __launch_bounds__(256) void join_kernel(PrefillParams pp) {
 // us with 1, 2, 4, 8, 16 parts, D = 256, one row: 16 tokens (2 workgroups) over 32 tiles 65.6 41.9 29.2 23.3 22.1, 128 tokens
 // (16) over 17 tiles 42.3 31.9 27.7 30.8 35.4, 512 tokens (64) over 8 tiles 28.6 33.6 35.4 51.4 64.5, over 32 tiles 67.2
 // 52.8 45.3 64.9 105.
-constexpr double kPerTile = 30.0;
+// A workgroup of fewer columns has that much less of both, and more of them fit the chip.
+static double per_tile_of(int cols) { return 30.0 * 128 / cols; }
+static int slots_of(int cols) { return 256 * 128 / cols; }
 
-static int64_t workgroups_of(int64_t batch, int kv_heads, int group, int64_t max_new) { return batch * kv_heads * ceil_div(max_new * group, kCols); }
+static int64_t workgroups_of(int64_t batch, int kv_heads, int group, int64_t max_new, int cols) {
+  return batch * kv_heads * ceil_div(max_new * group, cols);
+}
 
 // What the launch has room for, from the longest row that the tables hold; each row's own number is parts_of its tiles.
-static int splits_of(int64_t batch, int kv_heads, int group, int64_t max_new, int64_t max_tokens) {
-  const int64_t wgs = workgroups_of(batch, kv_heads, group, max_new);
+static int splits_of(int64_t batch, int kv_heads, int group, int64_t max_new, int64_t max_tokens, int cols) {
+  const int64_t wgs = workgroups_of(batch, kv_heads, group, max_new, cols);
   const int64_t tiles = ceil_div(std::max<int64_t>(max_tokens, 1), kTile);
-  if (wgs >= 256) return 1;
-  const int64_t best = static_cast<int64_t>(std::sqrt(kPerTile * static_cast<double>(tiles) / static_cast<double>(wgs)));
-  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({kMaxSplits, 256 / wgs, tiles, best})));
+  if (wgs >= slots_of(cols)) return 1;
+  const int64_t best = static_cast<int64_t>(std::sqrt(per_tile_of(cols) * static_cast<double>(tiles) / static_cast<double>(wgs)));
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({kMaxSplits, slots_of(cols) / wgs, tiles, best})));
 }
 
 // Tokens that partial results are kept of: a query padded past its rows' bound is no reason for more.  With splits of at most
-// 256 / workgroups and a workgroup per 128 columns they are below 35 MB at any padding and any width of the tables.
+// 256 / workgroups of 128 columns they are below 35 MB at any padding and any width of the tables.
 static int64_t part_tokens_of(int64_t total, int64_t batch, int64_t max_new) { return std::min(total, batch * max_new); }
 
 static int64_t workspace_of(int splits, int64_t part_tokens, int heads, int head_dim) {
   return splits > 1 ? splits * part_tokens * heads * (static_cast<int64_t>(head_dim) + 2) * 4 : 0;
 }
 
-template <int D>
+template <int D, int COLS>
 static int join(const PrefillParams& p, const char* what, const char* label, hipStream_t stream) {
   if (p.splits > 1) {
     KernelTimer timer_(label, stream);
     const dim3 jgrid(static_cast<unsigned>(ceil_div(p.max_new * p.c.H, 4)), static_cast<unsigned>(p.c.B));
-    hipLaunchKernelGGL(join_kernel<D>, jgrid, dim3(256), 0, stream, p);
+    hipLaunchKernelGGL((join_kernel<D, COLS>), jgrid, dim3(256), 0, stream, p);
   }
   return check_launch(what);
 }
 
 // The launch's parts and workspace; p.max_new stays 0 where there is nothing to compute.
-static int share_out(PrefillParams& p, const Args& a, const void* cu_seqlens, const void* prefix_lens, int64_t max_new, void* workspace, int64_t workspace_bytes) {
+static int share_out(PrefillParams& p, const Args& a, const void* cu_seqlens, const void* prefix_lens, int64_t max_new, void* workspace, int64_t workspace_bytes, int cols) {
   QA_REQUIRE(a.q_rows >= 0 && a.q_rows <= 0x7fffffff && max_new >= 0 && max_new <= 0x7fffffff, "%s: token counts out of range", a.what);
   if (a.batch == 0 || max_new == 0 || a.q_rows == 0) return 0;
   QA_REQUIRE(cu_seqlens && prefix_lens, "%s: pointers must be non-null", a.what);
@@ -159,8 +161,8 @@ static int share_out(PrefillParams& p, const Args& a, const void* cu_seqlens, co
   p.c.prefix = prefix_lens;
   p.c.total = a.q_rows;
   p.max_new = max_new;
-  p.splits = splits_of(a.batch, a.kv->kv_heads, p.c.G, max_new, a.max_blocks * a.block_size);
-  p.per_tile = static_cast<float>(kPerTile / static_cast<double>(workgroups_of(a.batch, a.kv->kv_heads, p.c.G, max_new)));
+  p.splits = splits_of(a.batch, a.kv->kv_heads, p.c.G, max_new, a.max_blocks * a.block_size, cols);
+  p.per_tile = static_cast<float>(per_tile_of(cols) / static_cast<double>(workgroups_of(a.batch, a.kv->kv_heads, p.c.G, max_new, cols)));
   p.part_tokens = part_tokens_of(a.q_rows, a.batch, max_new);
   p.per_row = p.part_tokens < a.q_rows ? max_new : 0;
   const int64_t need = workspace_of(p.splits, p.part_tokens, a.heads, a.head_dim);
@@ -171,10 +173,10 @@ static int share_out(PrefillParams& p, const Args& a, const void* cu_seqlens, co
   return 0;
 }
 
-static int64_t workspace_bytes_of(int64_t total_new, int64_t batch, int64_t max_new, int heads, int kv_heads, int head_dim, int64_t max_tokens) {
+static int64_t workspace_bytes_of(int64_t total_new, int64_t batch, int64_t max_new, int heads, int kv_heads, int head_dim, int64_t max_tokens, int cols) {
   if (total_new <= 0 || batch <= 0 || max_new <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 || head_dim <= 0 || max_tokens < 0) return 0;
   max_new = std::min(max_new, total_new);
-  return workspace_of(splits_of(batch, kv_heads, heads / kv_heads, max_new, max_tokens), part_tokens_of(total_new, batch, max_new), heads, head_dim);
+  return workspace_of(splits_of(batch, kv_heads, heads / kv_heads, max_new, max_tokens, cols), part_tokens_of(total_new, batch, max_new), heads, head_dim);
 }
 
 }  // namespace

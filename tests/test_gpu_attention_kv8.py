@@ -255,6 +255,14 @@ def test_prefill_of_many_rows_and_of_a_long_one() -> None:
     _check_prefill(24, [333], [66_000], 4, 1, 128, 16)
 
 
+@pytest.mark.parametrize("new,prefix", [([300, 260, 1, 0, 41], [900, 0, 1200, 7, 64]), ([600], [600]), ([64, 64, 64, 64, 8, 100, 33, 64, 5], [1100, 63, 64, 65, 1, 0, 1000, 0, 15])])
+@pytest.mark.parametrize("holes", [False, True])
+def test_prefill_of_many_columns_behind_many_keys(new, prefix, holes) -> None:
+    """Workgroups of 128 columns, a row's last ones part of them."""
+    _check_prefill(29 + len(new), new, prefix, 16, 2, 256, 16, holes=holes, width=100, pad=2)
+    _check_prefill(39 + len(new), new, prefix, 16, 1, 256, 64, torch.int64, gated=False, holes=holes, width=30)
+
+
 def test_prefill_of_one_token_is_decode() -> None:
     query, cu, tables, pools, got, _ = _check_prefill(25, [1, 1, 1], [0, 77, 500], 16, 2, 256, 16, gated=False)
     one = hip_ops.paged_attention_decode_kv8(query.unsqueeze(2), tables, *pools, torch.tensor([1, 78, 501], device=DEV), 16)
@@ -299,16 +307,16 @@ def test_refusals_of_tensors() -> None:
             hip_ops.paged_attention_decode_kv8(*args)
 
 
-@pytest.mark.parametrize("dim,heads", [(256, 16), (128, 6)])
-def test_prefill_keeps_a_nan_to_the_tokens_that_see_it(dim, heads) -> None:
+@pytest.mark.parametrize("dim,heads,new,prefix,width", [(256, 16, 150, 70, None), (128, 6, 150, 70, None), (256, 16, 550, 70, 80)])
+def test_prefill_keeps_a_nan_to_the_tokens_that_see_it(dim, heads, new, prefix, width) -> None:
     gen = torch.Generator().manual_seed(29)
-    new, prefix, block = 150, 70, 16
-    tables, pools = _cache(gen, [new + prefix], 2, dim, block)
+    block = 16
+    tables, pools = _cache(gen, [new + prefix], 2, dim, block, width=width)
     query = torch.randn(new, heads, dim, generator=gen).to(torch.bfloat16).to(DEV)
     cu = torch.tensor([0, new], device=DEV)
     run = lambda: hip_ops.paged_attention_prefill_kv8(query, cu, torch.tensor([prefix], device=DEV), *pools, tables, block, max_new=new)  # noqa: E731
     group = heads // 2
-    for at in (219, 195, 130, 70, 30):
+    for at in (new + prefix - 1, new + prefix - 25, 130, 70, 30):
         saved = [p.clone() for p in pools]
         run0 = at // 16 * 16
         tokens = torch.arange(run0, min(run0 + 16, new + prefix), device=DEV)
