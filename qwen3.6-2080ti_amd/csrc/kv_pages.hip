@@ -487,15 +487,24 @@ __global__ __launch_bounds__(kListThreads) void compact_list_kernel(CompactParam
 
 constexpr int kPools = 32;  // of a launch
 
+// Not uint4: an array of those went to LDS, by an address for which each workgroup read its launch's size from the host's memory,
+// 12 us where the first workgroup of every CU did.
+typedef uint32_t uintx4_v __attribute__((ext_vector_type(4)));
+
+struct PoolOfPages {
+  uint8_t* base;
+  int64_t stride;  // bytes from page to page
+  int64_t bytes;   // of a page
+  int64_t count;   // pages
+};
+
 struct CopyParams {
-  uint8_t* base[kPools];
-  int64_t stride[kPools];  // bytes from page to page
-  int64_t bytes[kPools];   // of a page
-  int64_t count[kPools];   // pages
   const void* sources;
   const void* targets;
   int64_t n;
   int ids_i64;
+  uint32_t groups;  // gridDim.x
+  PoolOfPages pools[kPools];
 };
 
 constexpr int kCopyThreads = 256;
@@ -505,22 +514,32 @@ constexpr int64_t kCopyGroups = 4096;
 // UNIT: 16 or 4 bytes.  Workgroups take pieces of kCopyThreads * kInFlight units of the pages of pool blockIdx.y in turn.
 template <typename UNIT>
 __global__ __launch_bounds__(kCopyThreads) void copy_kernel(CopyParams p) {
-  const int pool = blockIdx.y;
-  const int64_t units = p.bytes[pool] / static_cast<int64_t>(sizeof(UNIT));
-  const int64_t pieces = (units + kCopyThreads * kInFlight - 1) / (kCopyThreads * kInFlight);
-  for (int64_t x = blockIdx.x; x < p.n * pieces; x += gridDim.x) {
-    const int64_t pair = x / pieces, piece = x - pair * pieces;
+  const PoolOfPages pool = p.pools[blockIdx.y];
+  const int64_t units = pool.bytes / static_cast<int64_t>(sizeof(UNIT));
+  const uint32_t pieces = static_cast<uint32_t>((units + kCopyThreads * kInFlight - 1) / (kCopyThreads * kInFlight));  // memory ends long before 2^32
+  if (pieces == 0) return;
+  const uint32_t pairs_ahead = p.groups / pieces, pieces_ahead = p.groups - pairs_ahead * pieces;
+  int64_t pair = blockIdx.x / pieces;
+  uint32_t piece = blockIdx.x - static_cast<uint32_t>(pair) * pieces;
+  while (pair < p.n) {
     const int64_t source = index_of(p.sources, p.ids_i64, pair), target = index_of(p.targets, p.ids_i64, pair);
-    if (source < 0 || target < 0 || source >= p.count[pool] || target >= p.count[pool]) continue;
-    const UNIT* from = reinterpret_cast<const UNIT*>(p.base[pool] + source * p.stride[pool]);
-    UNIT* to = reinterpret_cast<UNIT*>(p.base[pool] + target * p.stride[pool]);
-    const int64_t u0 = piece * (kCopyThreads * kInFlight) + threadIdx.x;
-    UNIT u[kInFlight];
+    if (source >= 0 && target >= 0 && source < pool.count && target < pool.count) {
+      const UNIT* from = reinterpret_cast<const UNIT*>(pool.base + source * pool.stride);
+      UNIT* to = reinterpret_cast<UNIT*>(pool.base + target * pool.stride);
+      const int64_t u0 = static_cast<int64_t>(piece) * (kCopyThreads * kInFlight) + threadIdx.x;
+      UNIT u[kInFlight];
 #pragma unroll
-    for (int i = 0; i < kInFlight; ++i) u[i] = from[min64(u0 + i * kCopyThreads, units - 1)];
+      for (int i = 0; i < kInFlight; ++i) u[i] = from[min64(u0 + i * kCopyThreads, units - 1)];
 #pragma unroll
-    for (int i = 0; i < kInFlight; ++i)
-      if (u0 + i * kCopyThreads < units) to[u0 + i * kCopyThreads] = u[i];
+      for (int i = 0; i < kInFlight; ++i)
+        if (u0 + i * kCopyThreads < units) to[u0 + i * kCopyThreads] = u[i];
+    }
+    pair += pairs_ahead;
+    piece += pieces_ahead;
+    if (piece >= pieces) {
+      piece -= pieces;
+      ++pair;
+    }
   }
 }
 
@@ -701,21 +720,19 @@ extern "C" int qa_paged_kv_copy(void* const* pools, const int64_t* page_strides,
     CopyParams p{};
     int64_t units = 0;
     for (int64_t i = 0; i < here; ++i) {
-      p.base[i] = reinterpret_cast<uint8_t*>(pools[i0 + i]);
-      p.stride[i] = page_strides[i0 + i];
-      p.bytes[i] = page_bytes[i0 + i];
-      p.count[i] = page_counts[i0 + i];
-      units = std::max(units, p.bytes[i] / (wide ? 16 : 4));
+      p.pools[i] = {reinterpret_cast<uint8_t*>(pools[i0 + i]), page_strides[i0 + i], page_bytes[i0 + i], page_counts[i0 + i]};
+      units = std::max(units, p.pools[i].bytes / (wide ? 16 : 4));
     }
     if (units == 0) continue;
     p.sources = sources;
     p.targets = targets;
     p.n = n;
     p.ids_i64 = ids_dtype == QA_I64;
-    const dim3 grid(static_cast<unsigned>(std::min<int64_t>(n * ceil_div(units, kCopyThreads * kInFlight), kCopyGroups)), static_cast<unsigned>(here));
+    p.groups = static_cast<uint32_t>(std::min<int64_t>(n * ceil_div(units, kCopyThreads * kInFlight), kCopyGroups));
+    const dim3 grid(p.groups, static_cast<unsigned>(here));
     KernelTimer timer_("kv_copy", stream);
     if (wide)
-      hipLaunchKernelGGL(copy_kernel<uint4>, grid, dim3(kCopyThreads), 0, stream, p);
+      hipLaunchKernelGGL(copy_kernel<uintx4_v>, grid, dim3(kCopyThreads), 0, stream, p);
     else
       hipLaunchKernelGGL(copy_kernel<uint32_t>, grid, dim3(kCopyThreads), 0, stream, p);
   }
