@@ -1664,22 +1664,20 @@ def paged_kv_copy(pools: Sequence[torch.Tensor], sources: torch.Tensor, targets:
     _index_dtype(sources, "sources")
     _require(sources.dtype is targets.dtype and sources.dim() == 1 and sources.shape == targets.shape, "sources and targets must be vectors of page ids, alike")
     n = len(pools)
-    bases, strides, sizes, counts = [], [], [], []
-    for pool in pools:
-        if pool.device != device:
-            _require_cuda(pool, "pools", device)
-        shape, each = pool.shape, pool.element_size()
-        if pool.is_contiguous() and len(shape) > 1 and shape[0]:
-            size = stride = pool.numel() // shape[0] * each
-        else:
-            _require(len(shape) > 1 and (pool.numel() == 0 or pool[0].is_contiguous()), "a pool's pages must be contiguous along its first axis")
-            size, stride = math.prod(shape[1:]) * each, pool.stride(0) * each
-        bases.append(pool.data_ptr())
-        strides.append(stride)
-        sizes.append(size)
-        counts.append(shape[0])
     longs = ctypes.c_int64 * n
-    bases, strides, sizes, counts = (ctypes.c_void_p * n)(*bases), longs(*strides), longs(*sizes), longs(*counts)
+    shape, dtype = pools[0].shape, pools[0].dtype
+    if len(shape) > 1 and shape[0] and all(p.shape == shape and p.dtype is dtype and p.is_contiguous() and p.device == device for p in pools):
+        sizes = strides = longs(*[pools[0].numel() // shape[0] * pools[0].element_size()] * n)
+        counts = longs(*[shape[0]] * n)
+    else:
+        for pool in pools:
+            if pool.device != device:
+                _require_cuda(pool, "pools", device)
+            _require(pool.dim() > 1 and (pool.numel() == 0 or pool[0].is_contiguous()), "a pool's pages must be contiguous along its first axis")
+        sizes = longs(*[math.prod(pool.shape[1:]) * pool.element_size() for pool in pools])
+        strides = longs(*[pool.stride(0) * pool.element_size() for pool in pools])
+        counts = longs(*[pool.shape[0] for pool in pools])
+    bases = (ctypes.c_void_p * n)(*[pool.data_ptr() for pool in pools])
     s, t = sources.contiguous(), targets.contiguous()
     code = _launch(device, lib.qa_paged_kv_copy, bases, strides, sizes, counts, n, s.data_ptr(), t.data_ptr(), _code(s), s.numel())
     L.check(lib, code, "paged_kv_copy")
