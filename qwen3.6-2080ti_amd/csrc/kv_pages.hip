@@ -262,15 +262,32 @@ struct ReleaseParams {
   int list_words;    // of a workgroup of the second launch
 };
 
-// Table entry e of a row loses its block.
-__device__ __forceinline__ void release_entry(const Books& k, int64_t row, int64_t e, uint32_t* bits) {
-  int32_t* entry = &k.tables[row * k.table_stride + e];
-  if (*entry == -1) return;
-  const int32_t id = atomicExch(entry, -1);  // a row named twice is freed once
-  if (id < 0 || id >= k.capacity) return;
-  if (atomicSub(&k.references[id], 1) > 0) return;
-  atomicAdd(&k.references[id], 1);
-  set_bit(bits, id);
+// The table entries first, first + step .. of a row lose their blocks, four at a time: each is a chain of a load and three atomics,
+// one after the other 10.4 us for 16 rows of 256, so 9.0.
+__device__ __forceinline__ void release_entries(const Books& k, int64_t row, int64_t first, int64_t step, uint32_t* bits) {
+  constexpr int kAtOnce = 4;
+  int32_t* entries = &k.tables[row * k.table_stride];
+  for (int64_t e = first; e < k.max_blocks; e += kAtOnce * step) {
+    int32_t id[kAtOnce], holders[kAtOnce];
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) id[j] = e + j * step < k.max_blocks ? entries[e + j * step] : -1;
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j)
+      if (id[j] != -1) id[j] = atomicExch(&entries[e + j * step], -1);  // a row named twice is freed once
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) {
+      holders[j] = 1;
+      if (static_cast<uint32_t>(id[j]) < static_cast<uint32_t>(k.capacity)) holders[j] = atomicSub(&k.references[id[j]], 1);
+    }
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) asm volatile("" : "+v"(holders[j]));  // all of them on their way before the first is looked at
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) {
+      if (holders[j] > 0) continue;
+      atomicAdd(&k.references[id[j]], 1);
+      set_bit(bits, id[j]);
+    }
+  }
 }
 
 // All of it in one workgroup.
@@ -289,7 +306,7 @@ __global__ __launch_bounds__(kSmallThreads) void release_small_kernel(ReleasePar
   for (int i = tid / 64; i < p.n; i += kSmallThreads / 64) {  // a wave a row
     const int64_t row = index_of(p.release_rows, p.rows_i64, i);
     if (row < 0 || row >= k.rows) continue;
-    for (int64_t e = tid % 64; e < k.max_blocks; e += 64) release_entry(k, row, e, s_bits);
+    release_entries(k, row, tid % 64, 64, s_bits);
     if (tid % 64 == 0) k.lengths[row] = 0;
   }
   __syncthreads();
@@ -315,7 +332,7 @@ __global__ __launch_bounds__(256) void release_kernel(ReleaseParams p) {
   }
   const int64_t row = index_of(p.release_rows, p.rows_i64, blockIdx.y);
   if (row < 0 || row >= k.rows) return;
-  for (int64_t e = first; e < k.max_blocks; e += step) release_entry(k, row, e, p.bits);
+  release_entries(k, row, first, step, p.bits);
   if (first == 0) k.lengths[row] = 0;
 }
 
