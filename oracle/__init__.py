@@ -11,8 +11,9 @@ Every function restates an algorithm of the reference runtime
 reference ``file:line`` it follows.  Integer and byte work (slot indexing, block
 tables, gathers) is bit-exact NumPy / plain Python; floating-point work uses
 PyTorch CPU kernels with the reference's dtype cast points, because PyTorch CPU
-is the arithmetic the reference itself runs on.  ``kv4`` restates operators that
-the reference does not have, by their definitions in 64 bits.
+is the arithmetic the reference itself runs on.  ``kv4``, ``kv8`` and
+``pages`` restate operators that the reference does not have, by their definitions
+in 64 bits.
 
 Pinning status (what checks each function against something other than its own
 formula) is recorded per function in the module docstrings and enforced by

@@ -78,6 +78,9 @@ def test_forks_releases_and_compactions_are_checked_on_the_host() -> None:
     states = LinearStatePool(2, 1, 4, 4, 8, 4)
     with pytest.raises(RuntimeError, match="exhausted"):
         states.fork(0, 3)
+    for slot, count, message in ((0, 0, "positive"), (0, 1, "holds no request"), (2, 1, "holds no request"), (-1, 1, "holds no request")):
+        with pytest.raises(ValueError, match=message):
+            states.fork(slot, count)
     assert states.free_slots == [0, 1]
 
 
