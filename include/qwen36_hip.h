@@ -355,7 +355,8 @@ int qa_paged_attention_prefill_kv4(const void* query, int32_t q_dtype, int64_t q
  * [-117, 120]; x / 2^e goes to the nearest code, ties to even, and what is not
  * finite is NaN.  Where the call does not write the run's first token, e is
  * not below the run's, and if it is above, the codes of the tokens before the
- * first new one are rounded to it.
+ * first new one are rounded to it.  The values of the tokens behind the last
+ * new one are lost.
  *   keys    codes  [slice of 64 dims][dim / 16 % 4][token][16 bytes]
  *   values  codes  [slice of 64 dims][token / 4][dim / 4 % 16][dim % 4][token % 4]
  * Every value held is exact in bfloat16.  A new pool's bytes may be anything.

@@ -199,6 +199,22 @@ __global__ __launch_bounds__(256) void append_kernel(AppendParams p) {
   auto of_lane = [&](int64_t v, int from) {
     return (static_cast<int64_t>(__shfl(static_cast<int>(v >> 32), from, 64)) << 32) | static_cast<uint32_t>(__shfl(static_cast<int>(v), from, 64));
   };
+  // Of the groups of 64 tokens n + 64 j, j from 0 (step 64) or 0 down (step -64), the first one, by its first token, that are not all
+  // skipped: a stretch of skipped tokens goes by 512 at a time (a call of 10 tokens with 8182 skipped ones behind them 39.5 -> 16.9 us; 1024 at a time 13.0, but 40
+  // registers more, with which a long prompt took 33.5 and not 31.6).
+  auto past_skipped = [&](int64_t n, int64_t step) {
+    constexpr int kGroups = 8;
+    while (n < p.tokens && n > -64) {
+      uint32_t some = 0;
+#pragma unroll
+      for (int j = 0; j < kGroups; ++j) some |= (run_of(n + step * j + lane) >= 0 ? 1u : 0u) << j;
+#pragma unroll
+      for (int off = 1; off < 64; off <<= 1) some |= __shfl_xor(some, off, 64);
+      if (some != 0) return n + step * (__ffs(static_cast<int>(some)) - 1);
+      n += step * kGroups;
+    }
+    return n;
+  };
   // Lane i has token n0 - 1 + i: the one before the window, the window, and those that may follow its last leader.  A token leads
   // its run where the last one before it that is not skipped belongs to another.
   const int64_t run = run_of(n0 - 1 + lane);
@@ -208,11 +224,10 @@ __global__ __launch_bounds__(256) void append_kernel(AppendParams p) {
   int64_t before = of_lane(run, below != 0 ? 63 - __clzll(static_cast<long long>(below)) : 0);
   if ((there & 1) == 0 && (there >> 1 & ((1ull << p.window) - 1)) != 0) {
     int64_t last = -1;  // of the tokens before those: the last that is not skipped
-    for (int64_t n = n0 - 1; n > 0 && last < 0; n -= 64) {
-      const int64_t earlier = run_of(n - 64 + lane);
-      const uint64_t some = __ballot(earlier >= 0);
-      if (some != 0) last = of_lane(earlier, 63 - __clzll(static_cast<long long>(some)));
-    }
+    const int64_t n = past_skipped(n0 - 65, -64);
+    const int64_t earlier = run_of(n + lane);
+    const uint64_t some = __ballot(earlier >= 0);
+    if (some != 0) last = of_lane(earlier, 63 - __clzll(static_cast<long long>(some)));
     if (below == 0) before = last;
   }
   uint64_t leaders = __ballot(run >= 0 && run != before && lane >= 1 && lane <= p.window);
@@ -238,6 +253,11 @@ __global__ __launch_bounds__(256) void append_kernel(AppendParams p) {
       n += 64;
       if (end < 64 || r.count == kRun || n >= p.tokens) break;
       mine = run_of(n + lane);
+      if (__ballot(mine >= 0) == 0) {
+        n = past_skipped(n + 64, 64);
+        if (n >= p.tokens) break;
+        mine = run_of(n + lane);
+      }
       its = at;
       from = 0;
     }

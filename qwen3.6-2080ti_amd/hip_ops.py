@@ -1469,7 +1469,7 @@ def paged_kv8_append(key: torch.Tensor, value: torch.Tensor, key_pool: torch.Ten
     The pools are float8_e4m3fn ``(P, H_kv, kv8_tile_bytes(D, block_size))``: E4M3 codes, and a power-of-two scale for each run of
     16 tokens of a block and head (the format and layout stand in ``qwen36_hip.h``).  A run's scale fits the values that the call
     writes to it; a call that goes on with a run never makes its scale smaller, and where it grows, rounds the codes of the
-    tokens before to it.  ``slots`` ``(tokens,)`` hold ``block id * block_size + position % block_size``
+    tokens before to it; values behind the call's last token of a run are lost.  ``slots`` ``(tokens,)`` hold ``block id * block_size + position % block_size``
     (:func:`paged_kv_plan`); those outside the pool, such as -1, are skipped.  They have to be distinct, and the tokens of a
     run have to follow one another, with none but skipped ones between them, as a plan's do.
     """

@@ -99,6 +99,17 @@ def test_a_batch_of_single_tokens_touches_their_runs_only() -> None:
         _append_both(pools, host, *(_rows(gen, 33, 2, 256, torch.bfloat16) for _ in range(2)), slots, 16)
 
 
+@pytest.mark.parametrize("gap", [130, 1100, 2300])
+@pytest.mark.parametrize("front,tail", [(0, 0), (1, 70), (64, 5000), (1500, 1)])
+def test_runs_with_long_stretches_of_skipped_tokens(gap, front, tail) -> None:
+    """Padded slot maps: a run goes on behind the stretch, another begins there, and nothing follows the last."""
+    gen = torch.Generator().manual_seed(gap + front)
+    skipped = lambda n: torch.full((n,), -1, dtype=torch.int64)  # noqa: E731
+    slots = torch.cat((skipped(front), torch.arange(3, 9), skipped(gap), torch.arange(9, 13), skipped(gap - 63), torch.tensor([13]), skipped(gap), torch.arange(32, 75), skipped(tail)))
+    pools = _pools(6, 1, 128, 16)
+    _append_both(pools, [_bytes(p) for p in pools], *(_rows(gen, slots.numel(), 1, 128, torch.bfloat16) for _ in range(2)), slots, 16)
+
+
 def test_append_reads_strided_rows_in_place() -> None:
     gen = torch.Generator().manual_seed(5)
     both = torch.randn(20, 2, 512, generator=gen).to(torch.bfloat16).to(DEV)
