@@ -17,14 +17,17 @@
 //
 // With few columns the keys are split over gridDim.z and a second launch joins the parts.
 //
-// What bounds it: issue.  A tile of 64 keys, D = 256, is 32 matrix instructions of 32 cycles a wave, two waves a SIMD, and
-// beside them 128 conversions, 16 exponentials and their shares of loads, masks and sums; a matrix instruction lets the other
-// wave's vector ones by half of its time, which would take 2984 cycles a tile, and it takes 4050 (matrix units busy 49 %).
+// What bounds it: power, and issue.  A tile of 64 keys, D = 256, is 32 matrix instructions of 32 cycles a wave, two waves a SIMD,
+// and beside them 128 conversions, 16 exponentials and their shares of loads, masks and sums.  It takes 4050 cycles, the
+// matrix units busy for half of them, at 1.95 to 2.1 GHz of 2.4: with fewer cycles the clock falls.  A copy of the kernel without its
+// tiles' writes to LDS had 11% fewer cycles and took 5% less time; zeros for data took 988 us at the longest size below.
 // Measured, 16 heads, 2 of keys, D = 256: 2048 new behind 32 000 1046 us (1108 Gflop, 1060 Tflop/s; a library's 8192 x 8192
 // x 8192 product 1268), 8 x 512 behind up to 8192 331 us (930 Tflop/s); 20 heads, 4 of keys, D = 128, five prompts of up to 700 25 us.
-// Values' products at a raised wave priority 1048 -> 1034, probabilities between them 1221 -> 1055.  Not kept: the two halves of
-// the workgroup half a tile apart 1040, two accumulators of scores 1049, three key buffers 1065, four waves of 64 columns with
-// 512 registers 1187, workgroups of 64 columns at that size 1130.
+// Values' products at a raised wave priority 1048 -> 1034, probabilities between them 1221 -> 1055.  Not kept, us at that size: the
+// two halves of the workgroup half a tile apart 1040, two accumulators of scores 1049, three key buffers 1065, four waves of 64
+// columns with 512 registers 1187, workgroups of 64 columns 1130; within 1% of the kernel, each against it on one card: four waves that
+// share 64 columns' values (96 conversions for 128), counters in LDS for the barrier, runs copied straight to LDS two or three
+// tiles ahead, a wave's own probabilities kept in registers and its first values asked for before the barrier.
 #include "attention_kv8.h"
 #include "prefill_split.h"
 
