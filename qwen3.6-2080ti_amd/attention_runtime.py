@@ -564,13 +564,18 @@ _COUNT_UP: dict[tuple[int, str], Any] = {}
 
 
 def _count_up(tokens: int, device: Any) -> Any:
-    """``[0, 1, .., tokens - 1]`` int64, a part of the next power of two, cached per (power, device) as ``_row_offsets`` is."""
+    """``[0, 1, .., tokens - 1]`` int64, a part of the next power of two, cached per (power, device).
+
+    What is cached came by a copy that had ended, so that every stream may read it; the first call of a power inside a capture
+    makes a tensor of the graph's own instead."""
     import torch
 
     key = (1 << max(tokens - 1, 0).bit_length(), str(device))
     cached = _COUNT_UP.get(key)
     if cached is None:
-        cached = torch.arange(key[0], dtype=torch.int64, device=device)
+        if torch.cuda.is_current_stream_capturing():
+            return torch.arange(tokens, dtype=torch.int64, device=device)
+        cached = torch.arange(key[0], dtype=torch.int64).to(device)
         _COUNT_UP[key] = cached
     return cached[:tokens]
 

@@ -622,7 +622,7 @@ class DeviceBatchPageTables:
         a fork for which the pool has no block raises and takes nothing."""
         import torch
 
-        if not self.active[row]:
+        if not 0 <= row < self.rows or not self.active[row]:
             raise ValueError(f"row {row} holds no request")
         if count <= 0:
             raise ValueError("count must be positive")

@@ -164,6 +164,20 @@ def test_a_running_batch(heads, kv_heads, dim, block, sections, interleaved) -> 
     assert runtime.paged_attention_stats.dense_fallbacks == 0
 
 
+def test_slots_of_a_step_whose_first_call_is_captured() -> None:
+    ar._COUNT_UP.clear()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        inside = ar._count_up(11, torch.device(DEV)) + 0
+    want = torch.arange(11, device=DEV)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        eager = [ar._count_up(n, torch.device(DEV)) + 0 for n in (11, 9, 16)]
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(inside, want) and torch.equal(eager[0], want) and torch.equal(eager[1], want[:9]) and eager[2].shape == (16,)
+
+
 def test_post_rotary_keys_and_values_on_an_8_bit_pool() -> None:
     heads, kv_heads, dim, block, rows = 16, 2, 256, 16, 3
     config, runtime = _config(heads, kv_heads, dim), ar.HotPathRuntime()

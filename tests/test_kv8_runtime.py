@@ -65,6 +65,7 @@ def test_forks_releases_and_compactions_are_checked_on_the_host() -> None:
     pools = [pool.key_blocks, pool.value_blocks]
     tables.add_request()
     for call, message in ((lambda: tables.fork_request(1, 1, pools), "holds no request"), (lambda: tables.fork_request(0, 0, pools), "positive"),
+                          (lambda: tables.fork_request(-3, 1, pools), "holds no request"), (lambda: tables.fork_request(3, 1, pools), "holds no request"),
                           (lambda: tables.fork_request(0, 1, []), "8 blocks each"), (lambda: tables.fork_request(0, 1, pools[:1]), "own pool"),
                           (lambda: tables.fork_request(0, 1, [*pools, torch.zeros(7, 2)]), "8 blocks each"), (lambda: tables.compact(pools[1:]), "own pool"),
                           (lambda: tables.compact(pools, max_moves=-1), "non-negative"), (lambda: tables.release_requests([0, 0]), "distinct"),
