@@ -209,6 +209,24 @@ def test_copies_of_pages_of_every_kind() -> None:
     hip_ops.paged_kv_copy(many, torch.zeros(0, dtype=torch.int32, device=DEV), torch.zeros(0, dtype=torch.int32, device=DEV))
 
 
+def test_copies_of_pages_of_more_pieces_than_a_launch_has_workgroups() -> None:
+    """Pages of 80 MB and of 64 bytes in one call, and so many small ones that a workgroup takes several."""
+    gen = torch.Generator(device=DEV).manual_seed(8)
+    for big in (20_000_003 // 4 * 4, 20_000_001):  # units of 16 and of 4 bytes
+        pools = [torch.randn(3, big, generator=gen, device=DEV), torch.randn(3, 16, generator=gen, device=DEV)]
+        want = [torch.stack((p[0], p[0], p[2])) for p in pools]
+        hip_ops.paged_kv_copy(pools, torch.tensor([0, 7], device=DEV), torch.tensor([1, 2], device=DEV))
+        assert all(torch.equal(p, w) for p, w in zip(pools, want))
+    pools = [torch.randn(20_000, 2, 9, generator=gen, device=DEV), torch.randn(20_000, 5000, generator=gen, device=DEV).to(torch.bfloat16)]
+    ids = torch.randperm(20_000, generator=gen, device=DEV)
+    sources, targets = ids[:9000], ids[10_000:19_000]
+    want = [p.clone() for p in pools]
+    for w in want:
+        w[targets] = w[sources]
+    hip_ops.paged_kv_copy(pools, sources, targets)
+    assert all(torch.equal(p, w) for p, w in zip(pools, want))
+
+
 def test_copies_past_four_gigabytes() -> None:
     pool = torch.empty(5 * 2**30 // 8192, 4096, dtype=torch.bfloat16, device=DEV)
     pool[0] = 1.5
