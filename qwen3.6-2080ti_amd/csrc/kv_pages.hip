@@ -173,7 +173,7 @@ constexpr int kListThreads = 256;
 constexpr int kListWords = 64;  // of a workgroup where the bitmap lies in the workspace, at most
 
 // One workgroup does a release or a compaction where the pool has up to so many blocks, the rows so many table entries, and a
-// compaction so many pairs.  us of a release and a compaction in one workgroup / in several: 8000 blocks 13 / 9 and 18 / 17, but a
+// compaction so many pairs.  us of a release and a compaction in one workgroup / in several: 8000 blocks 10 / 9 and 18 / 17, but a
 // fill and a launch more each, 8 us of the host; 470 blocks, a compaction 6 / 13; 32000 blocks 27 / 9 and 50 / 22.
 constexpr int kSmallThreads = 1024;  // each a word of the bitmap at most
 constexpr int64_t kSmallBlocks = 8192;
