@@ -412,6 +412,21 @@ def test_decode_in_one_stream_beside_another() -> None:
     assert all(torch.equal(out, cases[i % 2][3]) for i, out in enumerate(got))
 
 
+def test_prefill_in_one_stream_beside_another() -> None:
+    """Two calls at once, each with partial results of its own where the keys are split, and one of each number of columns."""
+    cases = [(*_check_prefill(60, [20, 3], [6000, 900], 16, 2, 256, 16), [6000, 900], 20), (*_check_prefill(61, [400, 300], [900, 1100], 16, 2, 256, 16), [900, 1100], 400)]
+    prefixes = [torch.tensor(case[6], dtype=torch.int32, device=DEV) for case in cases]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(5):
+        for stream, (query, cu, tables, pools, _out, gate, _p, most), prefix in zip(streams, cases, prefixes):
+            with torch.cuda.stream(stream):
+                got.append(hip_ops.paged_attention_prefill_kv8(query, cu, prefix, *pools, tables, 16, max_new=most, gate=gate))
+    torch.cuda.synchronize()
+    assert all(torch.equal(out, cases[i % 2][4]) for i, out in enumerate(got))
+
+
 @pytest.mark.parametrize("dim,kv_heads", [(256, 2), (128, 1)])
 def test_pools_past_four_gigabytes(dim, kv_heads) -> None:
     """The last blocks of a pool of 5 GB: offsets do not fit 32 bits."""
