@@ -633,6 +633,7 @@ class DeviceBatchPageTables:
         device = self.block_tables.device
         import hip_ops
 
+        pages = hip_ops.page_pools(pools)  # raises before the books change
         for lo in range(0, count, _FORKS):
             part = torch.tensor(targets[lo : lo + _FORKS], dtype=torch.int32, device=device)
             copies = self.allocator.fork(self.block_tables, self.sequence_lengths, torch.full_like(part, row), part, self.block_size)
@@ -642,7 +643,7 @@ class DeviceBatchPageTables:
                 if lo:
                     self.allocator.release_rows(self.block_tables, self.sequence_lengths, torch.tensor(targets[:lo], dtype=torch.int32, device=device))
                 raise
-            hip_ops.paged_kv_copy(pools, copies.sources, copies.targets)
+            hip_ops.paged_kv_copy(pages, copies.sources, copies.targets)
         for target in targets:
             self.active[target] = True
         self.step_counts[torch.tensor(targets, device=device)] = self.step_counts[row].clone()
@@ -675,8 +676,9 @@ class DeviceBatchPageTables:
         if max_moves is not None and max_moves < 0:
             raise ValueError("max_moves must be non-negative")
         self._check_pools(pools)
+        pages = hip_ops.page_pools(pools)  # raises before the books change
         copies = self.allocator.compact(self.block_tables, self.num_blocks // 2 if max_moves is None else min(max_moves, self.num_blocks // 2))
-        hip_ops.paged_kv_copy(pools, copies.sources, copies.targets)
+        hip_ops.paged_kv_copy(pages, copies.sources, copies.targets)
 
     def _check_pools(self, pools: Sequence[Any]) -> None:
         if not pools or any(int(pool.shape[0]) != self.num_blocks for pool in pools):

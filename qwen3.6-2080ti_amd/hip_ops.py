@@ -1647,7 +1647,56 @@ def paged_kv_compact(
     return PagedCopy(*pages.unbind())
 
 
-def paged_kv_copy(pools: Sequence[torch.Tensor], sources: torch.Tensor, targets: torch.Tensor) -> None:
+class PagePools(NamedTuple):
+    """Pools whose pages can be copied, checked once (:func:`page_pools`)."""
+
+    device: torch.device
+    bases: Any
+    strides: Any
+    sizes: Any
+    counts: Any
+    tensors: list[torch.Tensor]
+
+
+def page_pools(pools: Sequence[torch.Tensor]) -> PagePools:
+    """The pools as :func:`paged_kv_copy` takes them, or its ``RuntimeError`` for what it cannot copy: a caller whose books
+    change before the copy asks first."""
+    pools = list(pools)
+    _require(len(pools) > 0, "pools must name at least one tensor")
+    device = pools[0].device
+    if device.type != "cuda":
+        _require_cuda(pools[0], "pools")
+    n = len(pools)
+    longs = ctypes.c_int64 * n
+    addresses = [pool.data_ptr() for pool in pools]
+    shape, dtype = pools[0].shape, pools[0].dtype
+    if len(shape) > 1 and shape[0] and all(p.shape == shape and p.dtype is dtype and p.is_contiguous() and p.device == device for p in pools):
+        size = pools[0].numel() // shape[0] * pools[0].element_size()
+        units = size
+        sizes = strides = longs(*[size] * n)
+        counts = longs(*[shape[0]] * n)
+        _require(0 not in addresses, "pools must have memory")
+    else:
+        for pool in pools:
+            if pool.device != device:
+                _require_cuda(pool, "pools", device)
+            _require(pool.dim() > 1 and (pool.numel() == 0 or pool[0].is_contiguous()), "a pool's pages must be contiguous along its first axis")
+        size_of = [math.prod(pool.shape[1:]) * pool.element_size() for pool in pools]
+        stride_of = [pool.stride(0) * pool.element_size() for pool in pools]
+        units = 0
+        for pool, address, size, stride in zip(pools, addresses, size_of, stride_of):
+            _require(address != 0 or pool.shape[0] == 0, "pools must have memory")
+            _require(stride >= size or pool.shape[0] <= 1, "pages of a pool overlap")
+            units |= size | stride
+        sizes, strides = longs(*size_of), longs(*stride_of)
+        counts = longs(*[pool.shape[0] for pool in pools])
+    for address in addresses:
+        units |= address
+    _require(units & 3 == 0, "pages of pools must be of 4-byte units")
+    return PagePools(device, (ctypes.c_void_p * n)(*addresses), strides, sizes, counts, pools)
+
+
+def paged_kv_copy(pools: Sequence[torch.Tensor] | PagePools, sources: torch.Tensor, targets: torch.Tensor) -> None:
     """Copies page ``sources[i]`` to page ``targets[i]`` of every pool, in place.
 
     A pool is any tensor whose first axis counts pages of contiguous elements: ``(P, H_kv, bs, D)``, 4- or 8-bit tiles, states of
@@ -1656,30 +1705,15 @@ def paged_kv_copy(pools: Sequence[torch.Tensor], sources: torch.Tensor, targets:
     :func:`paged_kv_compact` are.
     """
     lib = L.load_library()
-    pools = list(pools)
-    _require(len(pools) > 0, "pools must name at least one tensor")
-    device = pools[0].device
-    if device.type != "cuda" or not (sources.device == targets.device == device):
-        _same_device(device, pools=pools[0], sources=sources, targets=targets)
+    if not isinstance(pools, PagePools):
+        pools = page_pools(pools)
+    device = pools.device
+    if not (sources.device == targets.device == device):
+        _same_device(device, sources=sources, targets=targets)
     _index_dtype(sources, "sources")
     _require(sources.dtype is targets.dtype and sources.dim() == 1 and sources.shape == targets.shape, "sources and targets must be vectors of page ids, alike")
-    n = len(pools)
-    longs = ctypes.c_int64 * n
-    shape, dtype = pools[0].shape, pools[0].dtype
-    if len(shape) > 1 and shape[0] and all(p.shape == shape and p.dtype is dtype and p.is_contiguous() and p.device == device for p in pools):
-        sizes = strides = longs(*[pools[0].numel() // shape[0] * pools[0].element_size()] * n)
-        counts = longs(*[shape[0]] * n)
-    else:
-        for pool in pools:
-            if pool.device != device:
-                _require_cuda(pool, "pools", device)
-            _require(pool.dim() > 1 and (pool.numel() == 0 or pool[0].is_contiguous()), "a pool's pages must be contiguous along its first axis")
-        sizes = longs(*[math.prod(pool.shape[1:]) * pool.element_size() for pool in pools])
-        strides = longs(*[pool.stride(0) * pool.element_size() for pool in pools])
-        counts = longs(*[pool.shape[0] for pool in pools])
-    bases = (ctypes.c_void_p * n)(*[pool.data_ptr() for pool in pools])
     s, t = sources.contiguous(), targets.contiguous()
-    code = _launch(device, lib.qa_paged_kv_copy, bases, strides, sizes, counts, n, s.data_ptr(), t.data_ptr(), _code(s), s.numel())
+    code = _launch(device, lib.qa_paged_kv_copy, pools.bases, pools.strides, pools.sizes, pools.counts, len(pools.tensors), s.data_ptr(), t.data_ptr(), _code(s), s.numel())
     L.check(lib, code, "paged_kv_copy")
 
 

@@ -1,0 +1,43 @@
+"""What the calls on a batch's shared pages leave behind when they refuse, without a GPU."""
+
+from __future__ import annotations
+
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+from decode_state import DeviceBatchPageTables, SharedKV8BlockPool
+
+
+class _Recorded:
+    """An allocator that notes which of the books' calls were reached."""
+
+    def __init__(self):
+        self.calls = []
+
+    def _note(self, call):
+        self.calls.append(call)
+        return SimpleNamespace(sources=torch.zeros(1, dtype=torch.int32), targets=torch.ones(1, dtype=torch.int32))
+
+    def fork(self, *args):
+        return self._note("fork")
+
+    def compact(self, *args):
+        return self._note("compact")
+
+    def check(self, *args):
+        pass
+
+
+def test_pools_are_checked_before_the_books_change() -> None:
+    """Host tensors are pools that no page can be copied in: neither call may get as far as the books."""
+    pool = SharedKV8BlockPool(8, kv_heads=2, head_dim=128)
+    tables = DeviceBatchPageTables(pool, rows=3, max_blocks=4)
+    tables.add_request()
+    tables.allocator = _Recorded()
+    pools = [pool.key_blocks, pool.value_blocks]
+    for call in (lambda: tables.fork_request(0, 1, pools), lambda: tables.compact(pools)):
+        with pytest.raises(RuntimeError, match="must be CUDA"):
+            call()
+    assert tables.allocator.calls == [] and tables.active == [True, False, False]
