@@ -1095,9 +1095,10 @@ class LinearStatePool:
             raise RuntimeError("linear state pool exhausted")
         if not 0 <= slot < int(self.state.shape[0]) or slot in self.free_slots:
             raise ValueError(f"slot {slot} holds no request")
-        taken, self.free_slots = self.free_slots[:count], self.free_slots[count:]
+        taken = self.free_slots[:count]
         targets = torch.tensor(taken, dtype=torch.int32, device=self.state.device)
         hip_ops.paged_kv_copy([self.state, self.conv], torch.full_like(targets, slot), targets)
+        self.free_slots = self.free_slots[count:]  # last: a copy that is refused takes no slot
         return taken
 
     def release(self, slot: int) -> None:

@@ -7,7 +7,7 @@ from types import SimpleNamespace
 import pytest
 import torch
 
-from decode_state import DeviceBatchPageTables, SharedKV8BlockPool
+from decode_state import DeviceBatchPageTables, LinearStatePool, SharedKV8BlockPool
 
 
 class _Recorded:
@@ -41,3 +41,13 @@ def test_pools_are_checked_before_the_books_change() -> None:
         with pytest.raises(RuntimeError, match="must be CUDA"):
             call()
     assert tables.allocator.calls == [] and tables.active == [True, False, False]
+
+
+def test_a_fork_of_states_that_cannot_be_copied_takes_no_slot() -> None:
+    states = LinearStatePool(6, 1, 4, 4, 8, 4)
+    slot = states.acquire()
+    for _ in range(2):
+        with pytest.raises(RuntimeError, match="must be CUDA"):
+            states.fork(slot, 3)
+        assert states.free_slots == [1, 2, 3, 4, 5]
+    assert states.acquire() == 1
