@@ -403,8 +403,10 @@ int qa_paged_attention_prefill_kv8(const void* query, int32_t q_dtype, int64_t q
  * (0 for a block that one row has).  status: 0, or 1 (no block left), 3 (a
  * cursor out of range), 4 (a length out of range), 6 (a row out of range, a
  * target that is not empty, named twice, or a source too); with a status other
- * than 0 nothing has changed and no page is to be copied.  The reference has no
- * shared blocks; its frees are host lists (src/decode_state.py:80-84).        */
+ * than 0 nothing has changed and no page is to be copied.  A word other than the
+ * reservations': a success writes 0 over what a refused step has left.  The
+ * reference has no shared blocks; its frees are host lists
+ * (src/decode_state.py:80-84).                                                */
 
 /* Row target_rows[i] becomes a copy of row source_rows[i] (n of them, at most
  * 1024; a source of -1: no fork).  It shares the full blocks and gets a block of

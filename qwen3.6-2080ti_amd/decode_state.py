@@ -338,7 +338,9 @@ class DeviceBlockAllocator:
         if ids:
             self.free_list[: len(ids)] = torch.tensor(ids, dtype=torch.int32, device=self.device)
         self.free_state = torch.tensor([0, len(ids)], dtype=torch.int32, device=self.device)
-        self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
+        # a word each: a refused step stays to be told whatever calls on pages run behind it
+        self._words = torch.zeros(4, dtype=torch.int32, device=self.device)
+        self.status, self.fork_status, self.release_status, self.compact_status = self._words.split(1)
         # holders of a block beyond its first (fork): 0 for all that one row has
         self.references = torch.zeros(num_blocks, dtype=torch.int32, device=self.device)
         self._last = "paged_kv_reserve"
@@ -370,28 +372,31 @@ class DeviceBlockAllocator:
         """Rows that share their sources' full blocks (``hip_ops.paged_kv_fork``): the ``PagedCopy`` that every layer's pools need."""
         import hip_ops
 
-        self._last = "paged_kv_fork"
-        return hip_ops.paged_kv_fork(block_tables, lengths, source_rows, target_rows, self.free_list, self.free_state, self.references, self.status, block_size)
+        return hip_ops.paged_kv_fork(block_tables, lengths, source_rows, target_rows, self.free_list, self.free_state, self.references, self.fork_status, block_size)
 
     def release_rows(self, block_tables: Any, lengths: Any, rows: Any) -> None:
         """Free the blocks of table rows on the device, without reading anything back (``hip_ops.paged_kv_release``)."""
         import hip_ops
 
-        self._last = "paged_kv_release"
-        hip_ops.paged_kv_release(block_tables, lengths, rows, self.free_list, self.free_state, self.references, self.status)
+        hip_ops.paged_kv_release(block_tables, lengths, rows, self.free_list, self.free_state, self.references, self.release_status)
 
     def compact(self, block_tables: Any, max_moves: int) -> Any:
         """Move the tables' blocks to the lowest ids (``hip_ops.paged_kv_compact``): the ``PagedCopy`` that every layer's pools need."""
         import hip_ops
 
-        self._last = "paged_kv_compact"
-        return hip_ops.paged_kv_compact(block_tables, self.free_list, self.free_state, self.references, self.status, max_moves=max_moves)
+        return hip_ops.paged_kv_compact(block_tables, self.free_list, self.free_state, self.references, self.compact_status, max_moves=max_moves)
 
-    def check(self) -> None:
-        """Raise ``RuntimeError`` if the last reservation failed (reads the status: a sync)."""
-        code = int(self.status.item())
-        if code != 0:
-            raise RuntimeError(f"{self._last} failed: {self._STATUS.get(code, f'status {code}')}")
+    def check(self, what: str | None = None) -> None:
+        """Raise ``RuntimeError`` if the last reservation, fork, release or compaction failed (reads their status words: a
+        sync); ``what`` names one of them, ``"paged_kv_fork"``, to ask for it alone.  A failed reservation is told until the next
+        one, a failed call on pages once."""
+        names = (self._last, "paged_kv_fork", "paged_kv_release", "paged_kv_compact")
+        for i, (name, code) in enumerate(zip(names, self._words.tolist())):
+            if code == 0 or what not in (None, name):
+                continue
+            if i > 0:
+                self._words[i].zero_()
+            raise RuntimeError(f"{name} failed: {self._STATUS.get(code, f'status {code}')}")
 
     def free_blocks(self) -> list[int]:
         head, count = (int(v) for v in self.free_state.tolist())
@@ -488,7 +493,7 @@ class DeviceBatchPageTables:
             counts = torch.zeros_like(self.step_counts)
             counts[row] = prompt_tokens
             self.allocator.reserve(self.block_tables, self.sequence_lengths, self.block_size, counts=counts, positions=self._admit_positions)
-            self.allocator.check()
+            self.allocator.check("paged_kv_reserve")
         self.step_counts[row] = 1
         return row
 
@@ -519,7 +524,7 @@ class DeviceBatchPageTables:
         device = self.block_tables.device
         index = torch.tensor(rows, dtype=torch.int64, device=device)
         plan = self.allocator.plan(self.block_tables, self.sequence_lengths, self.block_size, counts=torch.tensor(full, dtype=torch.int32, device=device), max_tokens=sum(counts))
-        self.allocator.check()
+        self.allocator.check("paged_kv_plan")
         return PrefillStep(
             rows=tuple(rows), counts=tuple(counts), index=index,
             # rows without tokens take no part, so the last row's end is the total
@@ -559,7 +564,7 @@ class DeviceBatchPageTables:
         full = torch.zeros_like(self.step_counts)
         full[index] = torch.tensor(counts, dtype=torch.int32, device=device)
         self.allocator.reserve(self.block_tables, self.sequence_lengths, self.block_size, counts=full, positions=self._admit_positions)
-        self.allocator.check()
+        self.allocator.check("paged_kv_reserve")
         cu = [0]
         for c in counts:
             cu.append(cu[-1] + c)
@@ -599,6 +604,7 @@ class DeviceBatchPageTables:
                                 counts=self.step_counts if counts is None else counts)
 
     def check(self) -> None:
+        """``DeviceBlockAllocator.check``: of the last step's reservation, and of the last fork, release and compaction."""
         self.allocator.check()
 
     def release_request(self, row: int) -> list[int]:
@@ -638,7 +644,7 @@ class DeviceBatchPageTables:
             part = torch.tensor(targets[lo : lo + _FORKS], dtype=torch.int32, device=device)
             copies = self.allocator.fork(self.block_tables, self.sequence_lengths, torch.full_like(part, row), part, self.block_size)
             try:
-                self.allocator.check()
+                self.allocator.check("paged_kv_fork")
             except RuntimeError:
                 if lo:
                     self.allocator.release_rows(self.block_tables, self.sequence_lengths, torch.tensor(targets[:lo], dtype=torch.int32, device=device))

@@ -1581,7 +1581,8 @@ def paged_kv_fork(
     and no sources; a source of -1 is no fork; at most 1024 a call.  Tables, lengths and ``free_state`` are those of
     :func:`paged_kv_plan`.  ``status`` becomes 0, or 1 (pool exhausted), 3 (corrupt free state), 4 (a length that the table does
     not hold), 6 (rows out of range, targets that are not empty or not distinct): then nothing is changed and no page is to be
-    copied.  Nothing is read back, so the call can be captured in a HIP graph.
+    copied; as for the other calls on pages it is a tensor other than the plan's, whose refusal a success would overwrite.
+    Nothing is read back, so the call can be captured in a HIP graph.
     """
     lib = L.load_library()
     device = block_tables.device

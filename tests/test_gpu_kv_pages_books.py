@@ -51,3 +51,32 @@ def test_pools_that_cannot_be_copied_leave_the_books_alone(bad, alike) -> None:
     assert tables.active == active and all(torch.equal(a, b) for a, b in zip(before, _books(tables)))
     tables.compact(pools[:2])
     assert tables.block_tables[1, :2].tolist() == [1, 0] and tables.fork_request(1, 1, pools[:2]) == [0]
+
+
+def test_a_refused_step_is_told_behind_releases_forks_and_compactions() -> None:
+    pool, tables = _batch(blocks=5, tokens=(32, 32))  # a step of both needs two blocks, and there is one
+    pools = [pool.key_blocks, pool.value_blocks]
+    tables.plan_step()
+    assert tables.fork_request(0, 1, pools) == [2]  # of full blocks alone
+    tables.compact(pools)
+    tables.release_requests([0, 2])
+    for _ in range(2):
+        with pytest.raises(RuntimeError, match="paged_kv_plan failed: shared KV pool exhausted"):
+            tables.check()
+    assert tables.sequence_lengths.tolist() == [0, 32, 0, 0]
+    plan = tables.plan_step()
+    tables.check()
+    assert tables.sequence_lengths.tolist() == [0, 33, 0, 0] and plan.slots.tolist()[1] >= 0
+
+
+def test_a_refused_fork_is_told_behind_a_step() -> None:
+    pool, tables = _batch(blocks=5, tokens=(40, 20))  # no block is left for a partly filled last one
+    a = tables.allocator
+    rows = torch.tensor([0, 2], dtype=torch.int32, device=DEV)
+    a.fork(tables.block_tables, tables.sequence_lengths, rows[:1], rows[1:], tables.block_size)
+    tables.release_requests([])
+    tables.plan_step()
+    with pytest.raises(RuntimeError, match="paged_kv_fork failed: shared KV pool exhausted"):
+        tables.check()
+    tables.check()
+    assert tables.sequence_lengths.tolist() == [41, 21, 0, 0]
