@@ -353,7 +353,8 @@ int qa_paged_attention_prefill_kv4(const void* query, int32_t q_dtype, int64_t q
  * its scale 2^e with 15 zeros: 16 D + 16 bytes.  Of the finite values that a
  * call writes to a run, e is the least integer with max|x| <= 448 2^e, within
  * [-117, 120]; x / 2^e goes to the nearest code, ties to even, and what is not
- * finite is NaN.  Where the call does not write the run's first token, e is
+ * finite is NaN; with e = 120 the code of 240 stands for that of 256, since 2^128
+ * is no bfloat16.  Where the call does not write the run's first token, e is
  * not below the run's, and if it is above, the codes of the tokens before the
  * first new one are rounded to it.  The values of the tokens behind the last
  * new one are lost.

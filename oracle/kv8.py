@@ -30,13 +30,15 @@ def scale_exponent(amax: float) -> int:
 
 
 def encode(x: np.ndarray, e: int) -> np.ndarray:
-    """The nearest code of x / 2^e, ties to the even one; a NaN where x is not finite."""
+    """The nearest code of x / 2^e, ties to the even one, but 240 for 256 at the largest scale; a NaN where x is not finite."""
     x = np.asarray(x, dtype=np.float64)
     ok = np.isfinite(x)
     a = np.where(ok, np.abs(x), 0.0) * 2.0**-e
     up = np.clip(np.searchsorted(GRID, a), 1, 126)  # GRID[up - 1] <= a <= GRID[up] within the range
     below, above = a - GRID[up - 1], GRID[up] - a
     code = np.where((below < above) | ((below == above) & (up % 2 == 1)), up - 1, up)
+    if e == 120:
+        code = np.minimum(code, 0x77)
     return np.where(ok, code + 128 * (np.signbit(x) & (code > 0)), 127).astype(np.uint8)
 
 

@@ -3,7 +3,7 @@
 // A run is 16 consecutive tokens of a block and one KV head, held as 16 D E4M3 codes and one scale 2^e (the byte e + 127).
 // Of the finite values that a call writes to the run, e is the least integer with max|x| <= 448 2^e, 448 being the largest
 // code; e is clamped to [-117, 120], so that a code times the scale is a normal bfloat16 or zero down to the least code, and
-// 448 2^120 is above the largest float.  A power of two costs no precision: a code has four significant bits wherever it lies
+// 448 2^120 is above the largest float; at that scale 256, which would be 2^128, is held as 240.  A power of two costs no precision: a code has four significant bits wherever it lies
 // between 2^-6 and 448, fifteen powers of two.  So reading the cache rounds nothing, and a run whose scale grows (a call that
 // does not write its first token and brings larger values) keeps its codes' values but for those that become subnormal.
 // An infinity or a NaN is held as a NaN, by itself: it has no part in the scale.
