@@ -413,15 +413,16 @@ class DeviceBlockAllocator:
         blocks = [int(b) for b in blocks]
         if not blocks:
             return []
-        free = self.free_blocks()
+        books = torch.cat((self.free_state, self.free_list, self.references)).cpu()
+        head, count = books[:2].tolist()
+        free = books[2 + head : 2 + head + count].tolist()
         if min(blocks) < 0 or max(blocks) >= self.capacity or len(set(blocks)) != len(blocks) or set(blocks) & set(free):
             raise ValueError("released block ids must be in range and not already free")
-        index = torch.tensor(blocks, dtype=torch.int64, device=self.device)
-        held = self.references[index]
-        shared = held.tolist()
-        if any(shared):
-            self.references[index] = (held - 1).clamp(min=0)
-        gone = [b for b, n in zip(blocks, shared) if n == 0]
+        beyond = books[2 + self.capacity :][torch.tensor(blocks)].tolist()
+        shared = [b for b, n in zip(blocks, beyond) if n > 0]
+        if shared:
+            self.references[torch.tensor(shared, dtype=torch.int64, device=self.device)] -= 1
+        gone = [b for b, n in zip(blocks, beyond) if n <= 0]
         merged = sorted(free + gone)
         self.free_list[: len(merged)] = torch.tensor(merged, dtype=torch.int32, device=self.device)
         self.free_state.copy_(torch.tensor([0, len(merged)], dtype=torch.int32))

@@ -130,3 +130,17 @@ def test_a_reservation_that_is_checked_at_once_answers_for_itself(monkeypatch) -
     tables.reserve_step()
     tables.check()  # the fork has been told
     assert tables.active == [True, True, False]
+
+
+def test_releases_on_the_host_behind_a_cursor() -> None:
+    """The list's front has been taken, and blocks have up to three holders."""
+    allocator = DeviceBlockAllocator(9, device="cpu")
+    allocator.free_state.copy_(torch.tensor([5, 4]))  # 0 to 4 are held
+    allocator.references[:5] = torch.tensor([0, 2, 1, 0, 0], dtype=torch.int32)
+    assert allocator.release([4, 1, 2]) == [4]
+    assert allocator.free_blocks() == [4, 5, 6, 7, 8] and allocator.references.tolist() == [0, 1, 0] + [0] * 6
+    assert allocator.release([2, 1, 0]) == [2, 0]
+    assert allocator.release([1]) == [1]
+    assert allocator.free_blocks() == [0, 1, 2, 4, 5, 6, 7, 8] and not allocator.references.any() and allocator.free_state.tolist() == [0, 8]
+    with pytest.raises(ValueError, match="not already free"):
+        allocator.release([3, 8])
