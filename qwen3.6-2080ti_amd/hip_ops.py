@@ -22,6 +22,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+from array import array
 from typing import Any, NamedTuple, Sequence
 
 import torch
@@ -1648,53 +1649,55 @@ def paged_kv_compact(
     return PagedCopy(*pages.unbind())
 
 
-class PagePools(NamedTuple):
+class PagePools:
     """Pools whose pages can be copied, checked once (:func:`page_pools`)."""
 
-    device: torch.device
-    bases: Any
-    strides: Any
-    sizes: Any
-    counts: Any
-    tensors: list[torch.Tensor]
+    __slots__ = ("device", "bases", "strides", "sizes", "counts", "tensors")
 
 
 def page_pools(pools: Sequence[torch.Tensor]) -> PagePools:
     """The pools as :func:`paged_kv_copy` takes them, or its ``RuntimeError`` for what it cannot copy: a caller whose books
     change before the copy asks first."""
     pools = list(pools)
-    _require(len(pools) > 0, "pools must name at least one tensor")
-    device = pools[0].device
-    if device.type != "cuda":
-        _require_cuda(pools[0], "pools")
     n = len(pools)
-    longs = ctypes.c_int64 * n
-    addresses = [pool.data_ptr() for pool in pools]
-    shape, dtype = pools[0].shape, pools[0].dtype
-    if len(shape) > 1 and shape[0] and all(p.shape == shape and p.dtype is dtype and p.is_contiguous() and p.device == device for p in pools):
-        size = pools[0].numel() // shape[0] * pools[0].element_size()
-        units = size
-        sizes = strides = longs(*[size] * n)
-        counts = longs(*[shape[0]] * n)
+    _require(n > 0, "pools must name at least one tensor")
+    first = pools[0]
+    device, shape, dtype = first.device, first.shape, first.dtype
+    if device.type != "cuda":
+        _require_cuda(first, "pools")
+    described = PagePools()
+    described.tensors, described.device = pools, device
+    index = first.get_device()
+    addresses, bits = [], 0
+    alike = len(shape) > 1 and shape[0] > 0
+    for pool in pools:
+        at = pool.data_ptr()
+        addresses.append(at)
+        bits |= at
+        if alike and not (pool.is_contiguous() and pool.shape == shape and pool.dtype is dtype and pool.get_device() == index):
+            alike = False
+    if alike:
+        size = first.numel() // shape[0] * first.element_size()
+        bits |= size
+        described.sizes = described.strides = array("q", (size,)) * n
+        described.counts = array("q", (shape[0],)) * n
         _require(0 not in addresses, "pools must have memory")
     else:
         for pool in pools:
             if pool.device != device:
                 _require_cuda(pool, "pools", device)
             _require(pool.dim() > 1 and (pool.numel() == 0 or pool[0].is_contiguous()), "a pool's pages must be contiguous along its first axis")
-        size_of = [math.prod(pool.shape[1:]) * pool.element_size() for pool in pools]
-        stride_of = [pool.stride(0) * pool.element_size() for pool in pools]
-        units = 0
-        for pool, address, size, stride in zip(pools, addresses, size_of, stride_of):
-            _require(address != 0 or pool.shape[0] == 0, "pools must have memory")
+        sizes = [math.prod(pool.shape[1:]) * pool.element_size() for pool in pools]
+        strides = [pool.stride(0) * pool.element_size() for pool in pools]
+        for pool, at, size, stride in zip(pools, addresses, sizes, strides):
+            _require(at != 0 or pool.shape[0] == 0, "pools must have memory")
             _require(stride >= size or pool.shape[0] <= 1, "pages of a pool overlap")
-            units |= size | stride
-        sizes, strides = longs(*size_of), longs(*stride_of)
-        counts = longs(*[pool.shape[0] for pool in pools])
-    for address in addresses:
-        units |= address
-    _require(units & 3 == 0, "pages of pools must be of 4-byte units")
-    return PagePools(device, (ctypes.c_void_p * n)(*addresses), strides, sizes, counts, pools)
+            bits |= size | stride
+        described.sizes, described.strides = array("q", sizes), array("q", strides)
+        described.counts = array("q", [pool.shape[0] for pool in pools])
+    _require(bits & 3 == 0, "pages of pools must be of 4-byte units")
+    described.bases = array("Q", addresses)
+    return described
 
 
 def paged_kv_copy(pools: Sequence[torch.Tensor] | PagePools, sources: torch.Tensor, targets: torch.Tensor) -> None:
@@ -1714,7 +1717,10 @@ def paged_kv_copy(pools: Sequence[torch.Tensor] | PagePools, sources: torch.Tens
     _index_dtype(sources, "sources")
     _require(sources.dtype is targets.dtype and sources.dim() == 1 and sources.shape == targets.shape, "sources and targets must be vectors of page ids, alike")
     s, t = sources.contiguous(), targets.contiguous()
-    code = _launch(device, lib.qa_paged_kv_copy, pools.bases, pools.strides, pools.sizes, pools.counts, len(pools.tensors), s.data_ptr(), t.data_ptr(), _code(s), s.numel())
+    code = _launch(
+        device, lib.qa_paged_kv_copy, pools.bases.buffer_info()[0], pools.strides.buffer_info()[0], pools.sizes.buffer_info()[0], pools.counts.buffer_info()[0],
+        len(pools.tensors), s.data_ptr(), t.data_ptr(), _code(s), s.numel(),
+    )
     L.check(lib, code, "paged_kv_copy")
 
 
