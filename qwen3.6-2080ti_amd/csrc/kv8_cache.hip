@@ -5,8 +5,8 @@
 // run that the call brings, so one wave holds them all in registers and reads them once, and no two waves write to one run.
 // Tokens of a run follow one another in the slot map, with none but skipped ones between them; the first of them leads, and the waves
 // look for leaders among `window` tokens each.
-// Four prompts of 6003 tokens, two heads of 256, 74 MB each way: append 15.2 us, gather 13.5; a token for each of seven rows 5.2, and
-// their dense view of 428 tokens 4.1.
+// Four prompts of 6003 tokens, two heads of 256, 74 MB each way: append 18.0 to 18.6 us (16.5 where the caches still hold the rows),
+// gather 14.0; a token for each of seven rows 5.7 to 6.0, and their dense view of 428 tokens 4.2.
 #include "kv8.h"
 
 namespace qa {
@@ -383,8 +383,8 @@ static void launch_gather(const GatherParams& p, bool t64, dim3 grid, hipStream_
 }
 
 // Tokens among which a wave looks for leaders: one where there are few, so that every run has a wave at once; more where waves
-// that lead nothing would be too many.  us with windows of 1, 4, 16, two heads of 256: 128 rows of a token 5.1 13.3 41.9, 512 rows 6.6
-// 13.2 42.4, 2000 rows 16.5 18.9 44.7; prompts of 500 tokens 4.5 4.3 4.8, of 1000 4.8 4.4 4.8, 4000 13.5 5.8 5.3, 24000 61 19.8 16.2.
+// that lead nothing would be too many.  us with windows of 1, 4, 16, two heads of 256: 128 rows of a token 5.0 14.3 45.0, 512 rows 6.5
+// 13.7 46.6, 2000 rows 16.7 19.8 48.0; prompts of 500 tokens 4.3 4.2 4.6, of 1000 4.6 4.3 4.7, 4000 14.0 5.9 5.1, 24000 66 20.6 16.5.
 static int window_of(int64_t tokens) { return tokens <= 1024 ? 1 : tokens <= 4096 ? 4 : 16; }
 
 static int shift_of(int32_t block_size) { return __builtin_ctz(static_cast<unsigned>(block_size)); }

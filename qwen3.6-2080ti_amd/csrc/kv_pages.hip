@@ -41,7 +41,7 @@ __device__ __forceinline__ bool corrupt(const Books& k) {
   return head < 0 || count < 0 || head + count > k.capacity;
 }
 
-// Inclusive sum over the workgroup of 64 kThreads / 64 waves; total: of all.
+// Inclusive sum over a workgroup of THREADS / 64 waves; total: of all.
 template <int THREADS>
 __device__ __forceinline__ int32_t block_scan(int32_t v, int32_t* s_wave, int32_t& total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -263,7 +263,7 @@ struct ReleaseParams {
 };
 
 // The table entries first, first + step .. of a row lose their blocks, four at a time: each is a chain of a load and three atomics,
-// one after the other 10.4 us for 16 rows of 256, so 9.0.
+// one after the other 10.4 us for 16 rows of 256, so 8.8 to 9.0.
 __device__ __forceinline__ void release_entries(const Books& k, int64_t row, int64_t first, int64_t step, uint32_t* bits) {
   constexpr int kAtOnce = 4;
   int32_t* entries = &k.tables[row * k.table_stride];

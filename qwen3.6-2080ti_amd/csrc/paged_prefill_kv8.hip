@@ -22,7 +22,9 @@
 // matrix units busy for half of them, at 1.95 to 2.1 GHz of 2.4: with fewer cycles the clock falls.  A copy of the kernel without its
 // tiles' writes to LDS had 11% fewer cycles and took 5% less time; zeros for data took 988 us at the longest size below.
 // Measured, 16 heads, 2 of keys, D = 256: 2048 new behind 32 000 1046 us (1108 Gflop, 1060 Tflop/s; a library's 8192 x 8192
-// x 8192 product 1268), 8 x 512 behind up to 8192 331 us (930 Tflop/s); 20 heads, 4 of keys, D = 128, five prompts of up to 700 25 us.
+// x 8192 product 1268), 8 x 512 behind up to 8192 333 us (925 Tflop/s; 512 workgroups of up to 129 tiles, one a CU:
+// the last ends after 157 tiles where the mean is 145, so 8% of it is the launch's tail); 20 heads, 4 of keys, D = 128, five prompts of up
+// to 700 25.7 us.
 // Values' products at a raised wave priority 1048 -> 1034, probabilities between them 1221 -> 1055.  Not kept, us at that size: the
 // two halves of the workgroup half a tile apart 1040, two accumulators of scores 1049, three key buffers 1065, four waves of 64
 // columns with 512 registers 1187, workgroups of 64 columns 1130; within 1% of the kernel, each against it on one card: four waves that

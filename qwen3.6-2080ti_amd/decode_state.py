@@ -676,8 +676,8 @@ class DeviceBatchPageTables:
 
     def compact(self, pools: Sequence[Any], *, max_moves: int | None = None) -> None:
         """Move the requests' blocks to the pool's lowest ids, their pages in ``pools`` (as in :meth:`fork_request`) with them,
-        at most ``max_moves`` in a call: then the pools' ends are free, to be saved or given back.  Between steps; nothing is
-        read back.  Blocks in use that these tables do not hold stay where they are."""
+        at most ``max_moves`` in a call: then the pools' ends are free, and a slice of the pools' fronts holds the cache for a
+        caller that saves it or goes on with less.  Between steps; nothing is read back.  Blocks in use that these tables do not hold stay where they are."""
         import hip_ops
 
         if max_moves is not None and max_moves < 0:
